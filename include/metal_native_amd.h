@@ -250,6 +250,86 @@ MQ_API int mq_argmax_embed_f16(const void* logits, int64_t vocab, const void* em
                                int64_t* token, int64_t* pos, void* x, void* workspace, int64_t workspace_bytes,
                                void* stream);
 
+/* ---- serving from a paged key/value cache (no reference counterpart) ----
+ *
+ * k, v: [pages, kv_heads, page_size, head_dim], fp16 or bf16, unit stride along
+ * head_dim, the other strides (elements) multiples of 8, 16-byte aligned;
+ * page_size a power of two from 8, head_dim 64 or 128.  Sequence s keeps slot j
+ * (its token at position j) in page table[s * ld_table + j / page_size].  lens[s]
+ * is the number of its slots, those of the tokens of this call among them.
+ *
+ * The call's tokens are packed: sequence s has tokens cu_q[s] .. cu_q[s + 1]
+ * (NULL: one token each), the newest of its slots, so token i of n stands at
+ * position lens[s] - n + i.
+ *
+ * table, lens, cu_q and prefix_lens are device memory that the host does not
+ * look at.  A slot whose page number is outside [0, pages) does not exist: it
+ * is not read, not written and not attended to.  Lengths past the table's
+ * width, chunks past the last row and positions past the rotary tables are cut
+ * to what exists.  Nothing here allocates or synchronises. */
+enum mq_paged_dtype { MQ_PAGED_F16 = 0, MQ_PAGED_BF16 = 1 };
+typedef struct mq_paged_cache {
+  void *k, *v;
+  int64_t k_page, k_head, k_slot, v_page, v_head, v_slot;
+  int64_t pages;
+  int32_t kv_heads, page_size, head_dim, dtype;
+  const int32_t* table;
+  int64_t ld_table, width, batch;
+  const int32_t* lens;
+} mq_paged_cache;
+
+/* Scores x = scale * q . k, then softcap * tanh(x / softcap) (softcap 0: none),
+ * then - slopes[head] * |position - slot| (NULL: none).  A row at position p
+ * sees slot j where j <= p and, with window > 0, j > p - window, or where j <
+ * prefix_lens[s] (NULL: 0).  max_q: the longest chunk; it sizes launches only. */
+typedef struct mq_paged_mask {
+  float scale, softcap;
+  const float* slopes;
+  int64_t window;
+  const int32_t* prefix_lens;
+  const int32_t* cu_q;
+  int64_t max_q;
+} mq_paged_mask;
+
+/* Rotary positions of q and k from fused rows qkv [rows, (heads + 2 kv_heads) *
+ * head_dim]: q goes to q_out [rows, heads, head_dim], k and v into the pages of
+ * their tokens.  Frequency f turns (x[f], x[f + head_dim / 2]) by the cosine and
+ * sine at row pos[a * ld_pos + token], column f of the tables, a the axis whose
+ * section of the frequencies holds f (sections add up to head_dim / 2; at most
+ * eight axes). */
+MQ_API int mq_paged_rope_kv(const mq_paged_cache* cache, const void* qkv, int64_t ld_qkv, const float* cos_table,
+                            int64_t ld_cos, const float* sin_table, int64_t ld_sin, int64_t table_rows,
+                            const int64_t* pos, int64_t ld_pos, int32_t axes, const int32_t* sections,
+                            const int32_t* cu_q, int64_t rows, int32_t heads, void* q_out, void* stream);
+
+/* Softmax attention of q [rows, heads, head_dim] (strides q_token, q_head) over
+ * the cache: out [rows, heads, head_dim], and with lse [rows, heads] the log of
+ * each row's sum of exp(x).  A row that sees nothing gives zeros and -inf. */
+MQ_API int64_t mq_paged_attention_workspace_size(const mq_paged_cache* cache, const mq_paged_mask* mask, int64_t rows,
+                                                 int32_t heads);
+MQ_API int mq_paged_attention(const mq_paged_cache* cache, const mq_paged_mask* mask, const void* q, int64_t q_token,
+                              int64_t q_head, int64_t rows, int32_t heads, void* out, float* lse, void* workspace,
+                              int64_t workspace_bytes, void* stream);
+
+/* mass [batch, kv_heads, width * page_size]: the sum over the call's tokens and
+ * the query heads of a key/value head of exp(x - lse), zero past lens.  Rows of
+ * lse -inf add nothing.  v is not read. */
+MQ_API int64_t mq_paged_attention_mass_workspace_size(const mq_paged_cache* cache, const mq_paged_mask* mask,
+                                                      int64_t rows, int32_t heads);
+MQ_API int mq_paged_attention_mass(const mq_paged_cache* cache, const mq_paged_mask* mask, const void* q,
+                                   int64_t q_token, int64_t q_head, int64_t rows, int32_t heads, const float* lse,
+                                   float* mass, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Cuts every sequence to `budget` slots per key/value head: its newest `recent`
+ * (at most budget) and those of largest mass before them (NaN above all, ties to
+ * the lowest slot), in order, moved to the pages of to [batch, to_width], which
+ * must not be pages of table.  kept [batch, kv_heads, budget]: the slots that
+ * stay, -1 past new_lens [batch]; left [batch, kv_heads, to_width * page_size]:
+ * their mass, zero past them.  A sequence within the budget moves whole. */
+MQ_API int mq_paged_evict(const mq_paged_cache* cache, const float* mass, int64_t mass_batch, int64_t mass_head,
+                          const int32_t* to, int64_t ld_to, int64_t to_width, int64_t budget, int64_t recent,
+                          int32_t* kept, int32_t* new_lens, float* left, void* stream);
+
 /* Read probe: a measurement aid with no reference counterpart.  Reads the
  * `bytes` (< 2^31) bytes at p once, in one launch, the fastest way found on
  * gfx950 (one 12-wave workgroup per CU, 4-deep rings of 16-byte

@@ -22,7 +22,9 @@ LIB_NAME = "libmetal_native_amd.so"
 FRONT_NAME = "_mq_torch.so"
 BUILD_DIR = os.path.join(HERE, "_build")
 
-SOURCES = ["mq_capi.cpp", "mq_gemv.hip", "mq_rows.hip", "mq_rstream.hip", "mq_gemmw.hip", "mq_gemm16.hip", "mq_gemmn.hip", "mq_tiled.hip", "mq_misc.hip", "mq_quant.hip", "mq_glue.hip", "mq_vecmat32.hip"]
+SOURCES = ["mq_capi.cpp", "mq_gemv.hip", "mq_rows.hip", "mq_rstream.hip", "mq_gemmw.hip", "mq_gemm16.hip", "mq_gemmn.hip", "mq_tiled.hip", "mq_misc.hip", "mq_quant.hip", "mq_glue.hip", "mq_vecmat32.hip",
+           "mq_paged_capi.cpp", "mq_pattn.hip", "mq_pmass.hip", "mq_pcache.hip"]
+FRONT_SOURCES = ["mq_torch.cpp", "mq_torch_paged.cpp"]
 
 HIP_FLAGS = [
     "-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950",
@@ -59,8 +61,8 @@ def _compile(src: str, hipcc: str) -> str:
     return obj
 
 
-def _compile_front() -> str:
-    """The object of csrc/mq_torch.cpp: host code against torch's headers.
+def _compile_front(src: str) -> str:
+    """The object of one of the front's sources: host code against torch's headers.
 
     NDEBUG leaves out pybind11's per-thread reference counter, the front's only
     thread-local variable: a library with thread-local storage that is loaded
@@ -71,11 +73,11 @@ def _compile_front() -> str:
     import torch  # noqa: PLC0415
 
     inc = os.path.join(os.path.dirname(torch.__file__), "include")
-    obj = os.path.join(BUILD_DIR, "mq_torch.o")
+    obj = os.path.join(BUILD_DIR, os.path.splitext(src)[0] + ".o")
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-DNDEBUG",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            f"-I{inc}", f"-I{os.path.join(inc, 'torch', 'csrc', 'api', 'include')}",
-           f"-I{sysconfig.get_paths()['include']}", "-c", os.path.join(CSRC, "mq_torch.cpp"), "-o", obj]
+           f"-I{sysconfig.get_paths()['include']}", "-c", os.path.join(CSRC, src), "-o", obj]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
@@ -93,7 +95,7 @@ def build(verbose: bool = False) -> str:
     os.makedirs(BUILD_DIR, exist_ok=True)
     hipcc = _hipcc()
     with cf.ThreadPoolExecutor(max_workers=min(8, len(SOURCES))) as ex:
-        front = ex.submit(_compile_front)
+        front = [ex.submit(_compile_front, s) for s in FRONT_SOURCES]
         objs = list(ex.map(lambda s: _compile(s, hipcc), SOURCES))
     tlib = _torch_lib_dir()
     out = os.path.join(OUT_DIR, LIB_NAME)
@@ -103,7 +105,7 @@ def build(verbose: bool = False) -> str:
     _link(cmd, tmp, out)
     fout = os.path.join(OUT_DIR, FRONT_NAME)
     ftmp = fout + ".tmp"
-    _link(["g++", "-shared", "-o", ftmp, front.result(), f"-L{OUT_DIR}", "-lmetal_native_amd", f"-L{tlib}",
+    _link(["g++", "-shared", "-o", ftmp, *[f.result() for f in front], f"-L{OUT_DIR}", "-lmetal_native_amd", f"-L{tlib}",
            "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{tlib}"], ftmp, fout)
     if verbose:
         print(f"built {out}, {fout}")

@@ -445,6 +445,12 @@ hipError_t allow_dynamic_lds(const void* kernel, int bytes) {
 
 }  // namespace mq
 
+namespace mq {
+int fail_with(int code, const char* msg) { return fail(code, msg); }
+int hip_fail_with(hipError_t e, const char* what) { return hip_fail(e, what); }
+int current_num_cus() { return num_cus_current(); }
+}  // namespace mq
+
 extern "C" {
 
 static int dequant_matmul_impl(bool noalloc, const void* activations, int64_t lda, const void* weights_packed,

@@ -7,6 +7,12 @@
 
 namespace mq {
 
+// Status with a message for mq_last_error, and the current device's CU count
+// (mq_capi.cpp).
+int fail_with(int code, const char* msg);
+int hip_fail_with(hipError_t e, const char* what);
+int current_num_cus();
+
 enum Fmt { FMT_INT4 = 0, FMT_INT8 = 1, FMT_F16 = 2 };
 // Epilogues, numbered like the reference's MatmulEpilogue
 // (include/metal_native/ops/fused_matmul.h:18-24), plus SwiGLU.  The first

@@ -1,0 +1,107 @@
+// Device-side building blocks of the paged-cache kernels (gfx950 only).
+#pragma once
+#include "mq_paged.hpp"
+#include "mq_device.hpp"
+
+namespace mq {
+namespace {
+
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef short s8v __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+
+struct F16 {
+  typedef _Float16 e;
+  static __device__ __forceinline__ f16v mfma(u4 a, u4 b, f16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+  }
+};
+struct BF16 {
+  typedef __bf16 e;
+  static __device__ __forceinline__ f16v mfma(u4 a, u4 b, f16v c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+  }
+};
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  typedef typename T::e e2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){a, b}, e2));
+}
+
+__device__ __forceinline__ float swap32(float v) {   // v of lane ^ 32
+  const int x = __float_as_int(v);
+  const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return __int_as_float((threadIdx.x & 32) ? (int)r[0] : (int)r[1]);
+}
+__device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uni64(int64_t v) {
+  return ((int64_t)uni((int)(v >> 32)) << 32) | (uint32_t)uni((int)v);
+}
+
+__device__ __forceinline__ PagedSeq load_seq(const PagedArgs& p, int s) {
+  return paged_seq(s, p.cu ? p.cu[s] : 0, p.cu ? p.cu[s + 1] : 0, p.cu != nullptr, p.lens[s],
+                   p.prefix ? p.prefix[s] : 0, p.rows, p.cap);
+}
+__device__ __forceinline__ int64_t wave_scan(int64_t v) {   // inclusive
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t t = __shfl_up(v, o);
+    if (lane >= o) v += t;
+  }
+  return v;
+}
+
+// Where a cache's slots lie for one key/value head, and the lane's part of a
+// 1024-byte load: LDS is written in lane order, rows of D elements one after
+// the other, and the 16-byte pieces of a row are permuted on their way (piece
+// c of slot j at c ^ swizzle(j)) so that the reads below meet no bank twice.
+template <int D> struct Lay {
+  static constexpr int ROW = D / 8;           // 16-byte pieces of a slot
+  static constexpr int GS = 64 / ROW;         // slots per load: 4 (D = 128) or 8 (64)
+  static __device__ __forceinline__ int swz_k(int j) { return D == 128 ? j & 15 : (j >> 1) & 7; }
+  static __device__ __forceinline__ int swz_v(int j) { return D == 128 ? 2 * (j & 7) : 2 * ((j >> 1) & 3); }
+};
+
+#if defined(__HIP_DEVICE_COMPILE__)
+// 64 lanes' 16 bytes each at base + voff (zeros where voff + 16 > bytes) into
+// 1024 bytes of LDS in lane order; base, bytes and lds are wave-uniform.  In
+// asm, without an output: the builtin's load counts as a write that any later
+// LDS read may depend on, and the compiler waits for the next tile's loads
+// before it reads this tile.  Whoever reads the LDS waits for vmcnt itself;
+// the compiler's own vmcnt waits only become stricter by loads it does not
+// know of.  s_nop: M0 and descriptors written by v_readlane need up to five
+// wait states before the load.
+__device__ __forceinline__ void lds_load16(const void* base, uint32_t bytes, uint32_t voff, void* lds) {
+  typedef uint32_t u4_ __attribute__((ext_vector_type(4)));
+  const uint64_t a = (uint64_t)base;
+  const u4_ r = {(uint32_t)a, (uint32_t)(a >> 32) & 0xffffu, bytes, 0x00020000u};
+  const uint32_t l = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds;
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(l), "v"(voff), "s"(r)
+               : "memory", "m0");
+}
+#else
+__device__ inline void lds_load16(const void*, uint32_t, uint32_t, void*) {}
+#endif
+
+struct Base {   // wave-uniform
+  const char* ptr;      // of the key/value head
+  int64_t page;         // bytes
+  uint32_t slot;        // bytes
+};
+__device__ __forceinline__ Base cache_base(const PagedCache& c, int kv) {
+  return {(const char*)c.ptr + 2 * kv * c.head, 2 * c.page, 2u * (uint32_t)c.slot};
+}
+// Slots j .. j + GS of page `page` (one page: page sizes are multiples of GS),
+// of which the first nv exist.
+__device__ __forceinline__ void load_group(const Base& c, int page, int in_page, int nv, uint32_t voff, u4* lds) {
+  const char* at = c.ptr + (page < 0 ? 0 : page) * c.page + (int64_t)in_page * c.slot;
+  lds_load16(at, page < 0 ? 0u : (uint32_t)nv * c.slot, voff, lds);
+}
+
+
+}  // namespace
+}  // namespace mq

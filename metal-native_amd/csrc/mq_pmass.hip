@@ -1,0 +1,224 @@
+// Attention weight that every cached key got:
+//   mass[s][kv][j] = sum over the chunk's tokens and the query heads of kv of
+//                    exp(x_rj - lse_r),
+// x_rj the masked score of attention (mq_pattn.hip) and lse_r the log sum that
+// attention left for the row, so a row's weights over its slots sum to one.  A
+// row that saw nothing (lse -inf) adds nothing.
+//
+// A workgroup takes 256 slots, each wave 64 of them, whose keys stay in
+// registers as the matrix instruction's second operand; the rows stream
+// through LDS in blocks of 64, read once per workgroup.  With rows as the
+// result's rows a lane's 16 results all belong to its own slot: the sum over
+// rows needs no exchange but the last one between two lanes, and every output
+// is written once, in a fixed order of additions.  Sums run over 16 rows, then
+// 16 blocks, then all: fp32 throughout.
+#include "mq_paged_dev.hpp"
+
+#include <algorithm>
+
+namespace mq {
+namespace {
+
+constexpr int kSlotsM = 256, kRowsM = 64;
+
+template <typename T, int D, bool EXTRA>
+__global__ __launch_bounds__(256, 2) void paged_mass_kernel(PagedArgs p, float* out, int parts) {
+  constexpr int ROW = Lay<D>::ROW, GS = Lay<D>::GS, NG = kRowsM / GS / 4;
+  __shared__ u4 qs[2][kRowsM * ROW];
+  __shared__ float nl[2][kRowsM], sl[2][kRowsM];
+  __shared__ int ps[2][kRowsM];
+  const int tid = threadIdx.x, lane = tid & 63, w = uni(tid >> 6), col = lane & 31, h = lane >> 5;
+  const int slots = p.width << p.shift;
+  const int part = blockIdx.x % parts, kv = (blockIdx.x / parts) % p.KVH, blk = blockIdx.x / parts / p.KVH, s = blockIdx.y;
+  const PagedSeq sq0 = load_seq(p, s);
+  const PagedSeq sq = {uni(sq0.start), uni(sq0.n), uni(sq0.len), uni(sq0.prefix)};
+  const int j0 = blk * kSlotsM, off = sq.len - sq.n, total = sq.n * p.g;
+  // tokens that see a slot of the block
+  int ta = 0, tb = sq.n;
+  if (j0 >= sq.len) tb = 0;
+  if (j0 >= sq.prefix) {
+    ta = max(0, j0 - off);
+    if (p.window > 0) tb = (int)min((int64_t)tb, max((int64_t)0, (int64_t)j0 + kSlotsM - 1 + p.window - off));
+  }
+  const int ra = (int)((int64_t)ta * p.g) / kRowsM * kRowsM, rb = tb * p.g;
+  const int blocks = rb > ra ? (rb - ra + kRowsM - 1) / kRowsM : 0;
+  const int b0 = (int)((int64_t)blocks * part / parts), b1 = (int)((int64_t)blocks * (part + 1) / parts);
+
+  u4 kr[2][D / 16];
+  bool have[2];
+#pragma unroll
+  for (int nb = 0; nb < 2; ++nb) {
+    const int j = j0 + 64 * w + 32 * nb + col;
+    const int page = b1 > b0 ? paged_page(p.table + (int64_t)s * p.ld_table, j, sq.len, p.shift, p.pages) : -1;
+    have[nb] = page >= 0;
+    const u4* src = (const u4*)((const uint16_t*)p.k.ptr + page * p.k.page + kv * p.k.head +
+                                (int64_t)(j & ((1 << p.shift) - 1)) * p.k.slot) + h;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) kr[nb][ks] = have[nb] ? src[2 * ks] : (u4){0u, 0u, 0u, 0u};
+  }
+
+  const int gl = lane / ROW, piece = lane % ROW;
+  auto load = [&](int b, u4* dst) {
+    const int r0 = ra + b * kRowsM, tok0 = uni((int)p.gdiv.div(r0));
+    const uint16_t* base = (const uint16_t*)p.q + (int64_t)(sq.start + tok0) * p.q_t + (int64_t)kv * p.g * p.q_h;
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+      const int gi = 4 * n + w, rl = gi * GS + gl, r = r0 + rl, i = (int)p.gdiv.div(r);
+      const uint32_t off = 2u * ((uint32_t)(i - tok0) * (uint32_t)p.q_t + (uint32_t)(r - i * p.g) * (uint32_t)p.q_h) +
+                           16u * (piece ^ Lay<D>::swz_k(rl));
+      lds_load16(base, r0 + gi * GS < total ? 0x7fffffffu : 0u, r < total ? off : kOob, dst + 64 * gi);
+    }
+  };
+  // lse, position and slope of row tid of a block
+  float my_lse = 0.f, my_slope = 0.f;
+  int my_pos = 0;
+  auto row_info = [&](int b) {
+    const int r = ra + b * kRowsM + tid;
+    if (tid < kRowsM) {
+      const int i = (int)p.gdiv.div(r), a = kv * p.g + r - i * p.g;
+      my_pos = off + i;
+      my_lse = r < total ? p.lse[(int64_t)(sq.start + i) * p.H + a] : -INFINITY;
+      my_slope = EXTRA && p.slopes && r < total ? p.slopes[a] : 0.f;
+    }
+  };
+  const int jw = j0 + 64 * w;
+  float sum[2] = {0.f, 0.f}, mid[2] = {0.f, 0.f};
+  auto step = [&](int b, int x) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (tid < kRowsM) {
+      nl[x][tid] = my_lse == -INFINITY ? -INFINITY : -my_lse * kLog2e;
+      ps[x][tid] = my_pos;
+      sl[x][tid] = my_slope * kLog2e;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (b + 1 < b1) {
+      load(b + 1, qs[x ^ 1]);
+      row_info(b + 1);
+    }
+    const int r0 = ra + b * kRowsM;
+    const int first = off + (int)p.gdiv.div(r0), last = off + (int)p.gdiv.div(min(r0 + kRowsM, total) - 1);
+    const bool masked = jw + 63 > first || (p.window > 0 && (int64_t)jw <= (int64_t)last - p.window);
+#pragma unroll
+    for (int rb2 = 0; rb2 < 2; ++rb2) {
+      if (r0 + 32 * rb2 >= total) break;
+      const int swz = Lay<D>::swz_k(col) ^ h;
+      const u4* qt = qs[x] + (32 * rb2 + col) * ROW;
+      f16v sc[2] = {};
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        const u4 a = qt[swz ^ (2 * ks)];
+#pragma unroll
+        for (int nb = 0; nb < 2; ++nb) sc[nb] = T::mfma(a, kr[nb][ks], sc[nb]);
+      }
+      const float c = p.scale * kLog2e;
+#pragma unroll
+      for (int nb = 0; nb < 2; ++nb) {
+        const int j = jw + 32 * nb + col;
+        float t4[4];
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+          const int at = 32 * rb2 + 8 * q4 + 4 * h;
+          const f4 n4 = *(const f4*)&nl[x][at];
+          f4 v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float z = sc[nb][4 * q4 + e];
+            if constexpr (EXTRA) {
+              float y = z * p.scale;
+              if (p.softcap != 0.f) {
+                const float ex = __builtin_amdgcn_exp2f(y * (2.f * kLog2e / p.softcap));
+                y = p.softcap - 2.f * p.softcap * __builtin_amdgcn_rcpf(ex + 1.f);
+              }
+              z = y * kLog2e - sl[x][at + e] * fabsf((float)(ps[x][at + e] - j)) + n4[e];
+            } else {
+              z = __builtin_fmaf(z, c, n4[e]);
+            }
+            v[e] = z;
+          }
+          if (masked) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int pos = ps[x][at + e];
+              const bool see = (j <= pos && (p.window <= 0 || (int64_t)j > (int64_t)pos - p.window)) || j < sq.prefix;
+              v[e] = see ? v[e] : -INFINITY;
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = __builtin_amdgcn_exp2f(v[e]);
+          t4[q4] = (v[0] + v[1]) + (v[2] + v[3]);
+        }
+        mid[nb] += (t4[0] + t4[1]) + (t4[2] + t4[3]);
+      }
+    }
+    if ((b & 15) == 15) {
+#pragma unroll
+      for (int nb = 0; nb < 2; ++nb) {
+        sum[nb] += mid[nb];
+        mid[nb] = 0.f;
+      }
+    }
+  };
+  if (b0 < b1) {
+    load(b0, qs[b0 & 1]);
+    row_info(b0);
+#pragma unroll
+    for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) asm volatile("" : "+v"(kr[nb][ks]));
+    for (int b = b0; b < b1; ++b) step(b, b & 1);
+  }
+  float* dst = out + ((int64_t)part * p.b * p.KVH + (int64_t)s * p.KVH + kv) * slots;
+#pragma unroll
+  for (int nb = 0; nb < 2; ++nb) {
+    float t = sum[nb] + mid[nb];
+    t += swap32(t);
+    const int j = jw + 32 * nb + col;
+    if (h == 0 && j < slots) dst[j] = have[nb] ? t : 0.f;
+  }
+}
+
+__global__ __launch_bounds__(256) void paged_mass_sum_kernel(const float* in, float* out, int64_t n, int parts) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  float t = 0.f;
+  for (int x = 0; x < parts; ++x) t += in[x * n + i];
+  out[i] = t;
+}
+
+// Workgroups per 256 slots and key/value head: as many as bring the launch to
+// two per CU, of at least four row blocks each.
+int mass_parts(const PagedArgs& a, int num_cus) {
+  const int64_t slots = (int64_t)a.width << a.shift;
+  const int64_t wgs = (slots + kSlotsM - 1) / kSlotsM * a.KVH * a.b;
+  const int64_t blocks = ((int64_t)a.max_q * a.g + kRowsM - 1) / kRowsM;
+  return (int)std::max<int64_t>(1, std::min(2 * num_cus / std::max<int64_t>(wgs, 1), blocks / 4));
+}
+
+template <typename T, int D> hipError_t launch(const PagedArgs& a, int num_cus, void* ws, hipStream_t s) {
+  const int parts = mass_parts(a, num_cus);
+  const int64_t slots = (int64_t)a.width << a.shift, n = slots * a.KVH * a.b;
+  const int64_t gx = (slots + kSlotsM - 1) / kSlotsM * a.KVH * parts;
+  if (gx > 0x7fffffff || a.b > 65535) return hipErrorInvalidValue;
+  float* out = parts > 1 ? (float*)ws : a.mass;
+  const dim3 grid((int)gx, a.b);
+  if (a.extra()) paged_mass_kernel<T, D, true><<<grid, 256, 0, s>>>(a, out, parts);
+  else paged_mass_kernel<T, D, false><<<grid, 256, 0, s>>>(a, out, parts);
+  if (parts > 1) paged_mass_sum_kernel<<<(int)((n + 255) / 256), 256, 0, s>>>(out, a.mass, n, parts);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+size_t pmass_workspace(const PagedArgs& a, int num_cus) {
+  const int parts = mass_parts(a, num_cus);
+  return parts > 1 ? sizeof(float) * parts * (((size_t)a.width << a.shift) * a.KVH * a.b) : 0;
+}
+
+hipError_t pmass_launch(const PagedArgs& a, int num_cus, void* ws, hipStream_t s) {
+  if (a.D == 128) return a.bf16 ? launch<BF16, 128>(a, num_cus, ws, s) : launch<F16, 128>(a, num_cus, ws, s);
+  return a.bf16 ? launch<BF16, 64>(a, num_cus, ws, s) : launch<F16, 64>(a, num_cus, ws, s);
+}
+
+}  // namespace mq

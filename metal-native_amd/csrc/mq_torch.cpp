@@ -24,8 +24,9 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/metal_native_amd.h"
+#include "mq_torch.hpp"
 
-namespace {
+namespace mq_front {
 
 bool modes_set() { return c10::impl::TorchDispatchModeTLS::any_modes_set() || at::impl::torch_function_mode_enabled(); }
 
@@ -39,13 +40,17 @@ const at::Tensor* plain(PyObject* o) {
   return &t;
 }
 
+}  // namespace mq_front
+
+namespace {
+
+using namespace mq_front;
+
 // 2-D, rows of unit stride that do not overlap
 bool rowmajor(const at::Tensor& t) {
   return t.dim() == 2 && (t.size(1) <= 1 || t.stride(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1));
 }
 int64_t ld(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
-
-PyObject* decline() { Py_RETURN_NONE; }
 
 // (activations, weights, scales, zeros, group_size, is_int4, epilogue code, bias | None, residual | None, stream)
 PyObject* dequant_matmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -143,6 +148,10 @@ PyObject* vecmat(PyObject*, PyObject* const* p, Py_ssize_t n) {
 PyMethodDef kMethods[] = {
     {"dequant_matmul", (PyCFunction)(void (*)(void))dequant_matmul, METH_FASTCALL, nullptr},
     {"vecmat", (PyCFunction)(void (*)(void))vecmat, METH_FASTCALL, nullptr},
+    {"paged_rope_kv", (PyCFunction)(void (*)(void))mq_front::paged_rope_kv, METH_FASTCALL, nullptr},
+    {"paged_attention", (PyCFunction)(void (*)(void))mq_front::paged_attention, METH_FASTCALL, nullptr},
+    {"paged_attention_mass", (PyCFunction)(void (*)(void))mq_front::paged_attention_mass, METH_FASTCALL, nullptr},
+    {"paged_evict", (PyCFunction)(void (*)(void))mq_front::paged_evict, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_mq_torch", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

@@ -80,6 +80,17 @@ SIGNATURES = {
                                                   _c_void_p, _i32, _i32, _i32, _i64, ctypes.c_float, _c_void_p]),
     "mq_attention_parts_dequant_matmul": (_i32, [_c_void_p, _i32, _i32, _c_void_p, _i64, _c_void_p, _c_void_p,
                                                  _c_void_p, _i64, _i32, _i32, _c_void_p]),
+    # struct mq_paged_cache and struct mq_paged_mask go by address
+    "mq_paged_rope_kv": (_i32, [_c_void_p, _c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64, _i64, _c_void_p, _i64, _i32,
+                                _c_void_p, _c_void_p, _i64, _i32, _c_void_p, _c_void_p]),
+    "mq_paged_attention_workspace_size": (_i64, [_c_void_p, _c_void_p, _i64, _i32]),
+    "mq_paged_attention": (_i32, [_c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i64, _i32, _c_void_p, _c_void_p,
+                                  _c_void_p, _i64, _c_void_p]),
+    "mq_paged_attention_mass_workspace_size": (_i64, [_c_void_p, _c_void_p, _i64, _i32]),
+    "mq_paged_attention_mass": (_i32, [_c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i64, _i32, _c_void_p, _c_void_p,
+                                       _c_void_p, _i64, _c_void_p]),
+    "mq_paged_evict": (_i32, [_c_void_p, _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _i64, _i64, _c_void_p,
+                              _c_void_p, _c_void_p, _c_void_p]),
     "mq_release_workspaces": (_i32, []),
     "mq_set_option": (_i32, [ctypes.c_char_p, _i64]),
     "mq_last_path": (_i32, []),
