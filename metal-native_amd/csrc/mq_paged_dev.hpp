@@ -15,12 +15,14 @@ constexpr float kLn2 = 0.69314718055994530942f;
 
 struct F16 {
   typedef _Float16 e;
+  static constexpr uint32_t kExp = 0x7C007C00u, kExpLow = 0x04000400u;   // exponent fields of two values, their lowest bits
   static __device__ __forceinline__ f16v mfma(u4 a, u4 b, f16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
   }
 };
 struct BF16 {
   typedef __bf16 e;
+  static constexpr uint32_t kExp = 0x7F807F80u, kExpLow = 0x00800080u;
   static __device__ __forceinline__ f16v mfma(u4 a, u4 b, f16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
   }

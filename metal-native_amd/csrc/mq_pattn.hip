@@ -51,6 +51,29 @@ template <int D> struct Acc {
   }
 };
 
+// Whether any of n 16-byte pieces in LDS holds an infinity or NaN (n a
+// multiple of 64; wave-uniform): an exponent of ones carries into the sign's place.
+template <typename T> __device__ __forceinline__ bool not_finite(const u4* at, int n) {
+  uint32_t any = 0;
+#pragma unroll 4
+  for (int i = threadIdx.x & 63; i < n; i += 64) {
+    const u4 v = at[i];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) any |= (v[e] & T::kExp) + T::kExpLow;
+  }
+  return __any((any & 0x80008000u) != 0);
+}
+
+// The values with zeros for infinities and NaN.
+template <typename T> __device__ __forceinline__ u4 finite(u4 v) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t bad = ((v[e] & T::kExp) + T::kExpLow) & 0x80008000u;   // the sign bits' places
+    v[e] &= ~((bad >> 15) * 0xFFFFu);
+  }
+  return v;
+}
+
 // One tile of 32 * NB slots from tile0 for the wave's rows.  vm: bit per slot,
 // set where it exists.
 template <typename T, int D, int NB, bool EXTRA>
@@ -87,7 +110,8 @@ __device__ __forceinline__ void tile(const PagedArgs& p, const Rows& rw, const P
   }
   constexpr uint64_t kAll = NB == 2 ? ~0ull : 0xFFFFFFFFull;
   const int end = tile0 + 32 * NB - 1;
-  if (vm != kAll || end > rw.first || (p.window > 0 && (int64_t)tile0 <= (int64_t)rw.last - p.window)) {
+  const bool masked = vm != kAll || end > rw.first || (p.window > 0 && (int64_t)tile0 <= (int64_t)rw.last - p.window);
+  if (masked) {
     const int64_t lo64 = p.window > 0 ? (int64_t)rw.pos - p.window + 1 : -0x7fffffff;
     const int hi = rw.pos - tile0 - 4 * h, lo = (int)(lo64 < -0x7fffffff ? -0x7fffffff : lo64), pre = sq.prefix - tile0 - 4 * h;
     const int lor = lo < 0 ? -0x7fffffff : lo - tile0 - 4 * h;
@@ -129,18 +153,52 @@ __device__ __forceinline__ void tile(const PagedArgs& p, const Rows& rw, const P
   const int i = lane & 15, key0 = 4 * h + (i >> 2), low = 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
   const s4* vp = (const s4*)vt + key0 * (D / 4) + (i & 1);
   const int sv = Lay<D>::swz_v(key0);
-#pragma unroll
-  for (int u = 0; u < 2 * NB; ++u) {
+  auto weights = [&](int u) {
     u4 pr;
 #pragma unroll
     for (int e = 0; e < 4; ++e) pr[e] = pack2<T>(s[u / 2][8 * (u & 1) + 2 * e], s[u / 2][8 * (u & 1) + 2 * e + 1]);
+    return pr;
+  };
+  auto values = [&](int u, int db) {
+    const s4* a = vp + 16 * u * (D / 4) + 2 * ((4 * db + low) ^ sv);
+    const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)a);
+    const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(a + 8 * (D / 4)));
+    return __builtin_bit_cast(u4, (s8v)__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+  if (masked && not_finite<T>(vt, 32 * NB * Lay<D>::ROW)) {
+    // A hidden slot's infinity or NaN times its weight of zero would be NaN:
+    // the product takes zeros for them all, and each is then added to the
+    // rows that see its slot (times any weight it is itself, or NaN).
 #pragma unroll
-    for (int db = 0; db < D / 32; ++db) {
-      const s4* a = vp + 16 * u * (D / 4) + 2 * ((4 * db + low) ^ sv);
-      const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)a);
-      const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(a + 8 * (D / 4)));
-      ac.o[db] = T::mfma(__builtin_bit_cast(u4, (s8v)__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7)), pr, ac.o[db]);
+    for (int u = 0; u < 2 * NB; ++u) {
+      const u4 pr = weights(u);
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db) ac.o[db] = T::mfma(finite<T>(values(u, db)), pr, ac.o[db]);
     }
+#pragma unroll 1
+    for (int kk = 0; kk < 32 * NB; ++kk) {
+      const bool see = paged_visible(rw.pos, tile0 + kk, sq.len, sq.prefix, p.window) && ((vm >> kk) & 1);
+      const uint2* row = (const uint2*)(vt + kk * Lay<D>::ROW);
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint2 raw = row[2 * ((4 * db + e) ^ Lay<D>::swz_v(kk)) + h];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const uint32_t bits = (x < 2 ? raw.x : raw.y) >> (16 * (x & 1)) & 0xFFFFu;
+            if (see && (bits & (T::kExp & 0xFFFFu)) == (T::kExp & 0xFFFFu))
+              ac.o[db][4 * e + x] += (float)__builtin_bit_cast(typename T::e, (uint16_t)bits);
+          }
+        }
+    }
+    return;
+  }
+#pragma unroll
+  for (int u = 0; u < 2 * NB; ++u) {
+    const u4 pr = weights(u);
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db) ac.o[db] = T::mfma(values(u, db), pr, ac.o[db]);
   }
 }
 
