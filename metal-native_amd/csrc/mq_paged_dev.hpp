@@ -19,12 +19,26 @@ struct F16 {
   static __device__ __forceinline__ f16v mfma(u4 a, u4 b, f16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
   }
+  // c += a b in c's own registers: from the builtin the result goes to others
+  // wherever c also lives on another path.  The compiler does not see the
+  // latency: operands that a vector instruction writes are written two
+  // instructions before, and c is not touched but by such products for 20.
+  static __device__ __forceinline__ void add(f16v& c, u4 a, u4 b) {
+    asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
+  }
 };
 struct BF16 {
   typedef __bf16 e;
   static constexpr uint32_t kExp = 0x7F807F80u, kExpLow = 0x00800080u;
   static __device__ __forceinline__ f16v mfma(u4 a, u4 b, f16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+  }
+  // c += a b in c's own registers: from the builtin the result goes to others
+  // wherever c also lives on another path.  The compiler does not see the
+  // latency: operands that a vector instruction writes are written two
+  // instructions before, and c is not touched but by such products for 20.
+  static __device__ __forceinline__ void add(f16v& c, u4 a, u4 b) {
+    asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
   }
 };
 template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -75,17 +89,27 @@ template <int D> struct Lay {
 // LDS read may depend on, and the compiler waits for the next tile's loads
 // before it reads this tile.  Whoever reads the LDS waits for vmcnt itself;
 // the compiler's own vmcnt waits only become stricter by loads it does not
-// know of.  s_nop: M0 and descriptors written by v_readlane need up to five
-// wait states before the load.
-__device__ __forceinline__ void lds_load16(const void* base, uint32_t bytes, uint32_t voff, void* lds) {
-  typedef uint32_t u4_ __attribute__((ext_vector_type(4)));
+// know of.  s_nop: M0, and a descriptor that v_readlane wrote (FRESH), need
+// one and up to five wait states before the load.
+typedef uint32_t desc_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ desc_t make_desc(const void* base, uint32_t bytes) {
   const uint64_t a = (uint64_t)base;
-  const u4_ r = {(uint32_t)a, (uint32_t)(a >> 32) & 0xffffu, bytes, 0x00020000u};
+  return (desc_t){(uint32_t)uni((int)a), (uint32_t)uni((int)(a >> 32)) & 0xffffu, (uint32_t)uni((int)bytes), 0x00020000u};
+}
+template <bool FRESH> __device__ __forceinline__ void lds_load16(desc_t r, uint32_t voff, void* lds) {
   const uint32_t l = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds;
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(l), "v"(voff), "s"(r)
-               : "memory", "m0");
+  if constexpr (FRESH)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(l), "v"(voff), "s"(r) : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(l), "v"(voff), "s"(r) : "memory");
+}
+__device__ __forceinline__ void lds_load16(const void* base, uint32_t bytes, uint32_t voff, void* lds) {
+  lds_load16<true>(make_desc(base, bytes), voff, lds);
 }
 #else
+typedef uint32_t desc_t __attribute__((ext_vector_type(4)));
+__device__ inline desc_t make_desc(const void*, uint32_t) { return {}; }
+template <bool FRESH> __device__ inline void lds_load16(desc_t, uint32_t, void*) {}
 __device__ inline void lds_load16(const void*, uint32_t, uint32_t, void*) {}
 #endif
 

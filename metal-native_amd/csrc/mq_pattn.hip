@@ -42,12 +42,16 @@ struct Rows {
 
 template <int D> struct Acc {
   f16v o[D / 32];
-  float m, l;
+  float m, l[2];
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) o[i] = (f16v){};
     m = -3.0e38f;
-    l = 0.f;
+    l[0] = l[1] = 0.f;
+  }
+  __device__ __forceinline__ float sum() const {   // of both lanes of a row
+    const float t = l[0] + l[1];
+    return t + swap32(t);
   }
 };
 
@@ -74,58 +78,140 @@ template <typename T> __device__ __forceinline__ u4 finite(u4 v) {
   return v;
 }
 
+// Cap and distance bias, in units of log 2: scores of 32 * NB slots from tile0.
+template <int NB>
+__device__ __forceinline__ void cap_and_bias(const PagedArgs& p, const Rows& rw, f16v (&s)[NB], int tile0) {
+  const int h = (threadIdx.x & 63) >> 5;
+  const float cap = p.softcap;
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      float x = s[nb][j] * p.scale;
+      if (cap != 0.f) {
+        const float e = __builtin_amdgcn_exp2f(x * (2.f * kLog2e / cap));   // tanh y = 1 - 2 / (e^2y + 1)
+        x = cap - 2.f * cap * __builtin_amdgcn_rcpf(e + 1.f);
+      }
+      const int away = rw.pos - (tile0 + 32 * nb + 8 * (j / 4) + 4 * h + j % 4);
+      s[nb][j] = x * kLog2e - rw.slope2 * fabsf((float)away);
+    }
+}
+
+// Bits 0 .. n - 1, n clamped to 0 .. 64.
+__device__ __forceinline__ uint64_t low_bits(int n) { return n <= 0 ? 0 : (n >= 64 ? ~0ull : (1ull << n) - 1); }
+
+// -inf for what the lane's row does not see.  vm: bit per slot, set where it
+// exists.  By a bit per slot, spread over the word, rather than by a condition
+// per slot: those would all be kept in scalar registers at once.
+template <int NB>
+__device__ __forceinline__ void hide(const PagedArgs& p, const Rows& rw, const PagedSeq& sq, f16v (&s)[NB], int tile0, uint64_t vm) {
+  const int h = (threadIdx.x & 63) >> 5;
+  const int64_t before = p.window > 0 ? (int64_t)rw.pos - p.window + 1 - tile0 : 0;   // slots of the tile past the window
+  uint64_t vis = low_bits(rw.pos - tile0 + 1) & ~low_bits(before > 64 ? 64 : (int)max(before, (int64_t)0));
+  vis = ((vis | low_bits(sq.prefix - tile0)) & vm) >> (4 * h);
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    const uint32_t bits = (uint32_t)(vis >> (32 * nb));
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const uint32_t see = (uint32_t)((int32_t)(bits << (31 - (8 * (j / 4) + j % 4))) >> 31);
+      s[nb][j] = __uint_as_float((__float_as_uint(s[nb][j]) & see) | (0xFF800000u & ~see));
+    }
+  }
+}
+
+// Infinities and NaN among the values, of a tile that some row does not see
+// all of: a hidden slot's would still be NaN times its weight of zero, so the
+// products take zeros for them all, and the outputs that they reach are kept
+// as bits (of the lane's D / 2 outputs of one row) and written at the end: up
+// where a slot that the row sees holds +inf or NaN, down where -inf or NaN.
+template <int D> struct Odd {
+  uint64_t up, down;
+  __device__ __forceinline__ void clear() { up = down = 0; }
+  template <typename T>
+  __device__ __forceinline__ void mark(const PagedArgs& p, const Rows& rw, const PagedSeq& sq, const u4* vt, int slots, int tile0,
+                                       uint64_t vm) {
+    const int h = (threadIdx.x & 63) >> 5;
+    constexpr uint32_t kExp = T::kExp & 0xFFFFu;
+#pragma unroll 1
+    for (int kk = 0; kk < slots; ++kk) {
+      const bool see = paged_visible(rw.pos, tile0 + kk, sq.len, sq.prefix, p.window) && ((vm >> kk) & 1);
+      const uint16_t* row = (const uint16_t*)(vt + kk * Lay<D>::ROW);
+#pragma unroll 1
+      for (int i = 0; i < D / 2; ++i) {   // output i of the lane is 32 (i / 16) + 8 (i / 4 % 4) + 4 h + i % 4
+        const uint32_t bits = row[8 * ((i >> 2) ^ Lay<D>::swz_v(kk)) + 4 * h + (i & 3)];
+        const bool hit = see && (bits & kExp) == kExp, nan = (bits & 0x7FFFu) != kExp;
+        up |= (uint64_t)(hit && (nan || !(bits & 0x8000u))) << i;
+        down |= (uint64_t)(hit && (nan || (bits & 0x8000u))) << i;
+      }
+    }
+  }
+  __device__ __forceinline__ float fix(float v, int i) const {   // output i of the lane
+    const bool a = (up >> i) & 1, b = (down >> i) & 1;
+    return a ? (b ? __builtin_nanf("") : v + INFINITY) : (b ? v - INFINITY : v);
+  }
+};
+
 // One tile of 32 * NB slots from tile0 for the wave's rows.  vm: bit per slot,
-// set where it exists.
-template <typename T, int D, int NB, bool EXTRA>
+// set where it exists.  MASKED: some row may not see some slot of it.
+//
+// One wave's instructions issue in order, so both products read their LDS
+// operands a few instructions ahead (kf, vf): with a wait for LDS before each
+// step the 4096-token chunk behind 28672 slots took 2.0 ms.
+template <typename T, int D, int NB, bool EXTRA, bool MASKED>
 __device__ __forceinline__ void tile(const PagedArgs& p, const Rows& rw, const PagedSeq& sq, const u4 (&q)[D / 16],
-                                     Acc<D>& ac, const u4* kt, const u4* vt, int tile0, uint64_t vm) {
-  constexpr int ROW = Lay<D>::ROW;
+                                     Acc<D>& ac, Odd<D>& odd, const u4* kt, const u4* vt, int tile0, uint64_t vm) {
+  constexpr int ROW = Lay<D>::ROW, KS = D / 16, DB = D / 32;
   const int lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5;
   f16v s[NB];
   {
     const int swz = Lay<D>::swz_k(col) ^ h;
+    const u4* kp = kt + col * ROW;
+    constexpr int AHEAD = 3;   // steps of keys in flight
+    u4 kf[AHEAD][NB];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) s[nb] = (f16v){};
 #pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks)
+    for (int ks = 0; ks < AHEAD; ++ks)
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) s[nb] = T::mfma(kt[(32 * nb + col) * ROW + (swz ^ (2 * ks))], q[ks], s[nb]);
-  }
-  float c = p.scale * kLog2e;
-  if constexpr (EXTRA) {
-    const float cap = p.softcap;
+      for (int nb = 0; nb < NB; ++nb) kf[ks][nb] = kp[32 * nb * ROW + (swz ^ (2 * ks))];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
+    for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        float x = s[nb][j] * p.scale;
-        if (cap != 0.f) {
-          const float e = __builtin_amdgcn_exp2f(x * (2.f * kLog2e / cap));   // tanh y = 1 - 2 / (e^2y + 1)
-          x = cap - 2.f * cap * __builtin_amdgcn_rcpf(e + 1.f);
-        }
-        const int away = rw.pos - (tile0 + 32 * nb + 8 * (j / 4) + 4 * h + j % 4);
-        s[nb][j] = x * kLog2e - rw.slope2 * fabsf((float)away);
-      }
-    c = 1.f;
-  }
-  constexpr uint64_t kAll = NB == 2 ? ~0ull : 0xFFFFFFFFull;
-  const int end = tile0 + 32 * NB - 1;
-  const bool masked = vm != kAll || end > rw.first || (p.window > 0 && (int64_t)tile0 <= (int64_t)rw.last - p.window);
-  if (masked) {
-    const int64_t lo64 = p.window > 0 ? (int64_t)rw.pos - p.window + 1 : -0x7fffffff;
-    const int hi = rw.pos - tile0 - 4 * h, lo = (int)(lo64 < -0x7fffffff ? -0x7fffffff : lo64), pre = sq.prefix - tile0 - 4 * h;
-    const int lor = lo < 0 ? -0x7fffffff : lo - tile0 - 4 * h;
+      for (int nb = 0; nb < NB; ++nb) s[nb] = T::mfma(kf[ks % AHEAD][nb], q[ks], s[nb]);
+      if (ks + AHEAD < KS) {
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      const uint32_t bits = (uint32_t)(vm >> (32 * nb)) >> (4 * h);
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const int kk = 8 * (j / 4) + j % 4, jj = 32 * nb + kk;
-        const bool see = ((jj <= hi && jj >= lor) || jj < pre) && ((bits >> kk) & 1);
-        s[nb][j] = see ? s[nb][j] : -INFINITY;
+        for (int nb = 0; nb < NB; ++nb) kf[ks % AHEAD][nb] = kp[32 * nb * ROW + (swz ^ (2 * (ks + AHEAD)))];
       }
     }
+    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * NB, 0);   // LDS reads
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      __builtin_amdgcn_sched_group_barrier(0x008, NB, 0);         // MFMAs
+      if (ks + AHEAD < KS) __builtin_amdgcn_sched_group_barrier(0x100, NB, 0);
+    }
   }
+  const int i = lane & 15, key0 = 4 * h + (i >> 2), low = 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+  const s4* vp = (const s4*)vt + key0 * (D / 4) + (i & 1);
+  const int sv = Lay<D>::swz_v(key0);
+  auto values = [&](int u, int db) {
+    const s4* a = vp + 16 * u * (D / 4) + 2 * ((4 * db + low) ^ sv);
+    const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)a);
+    const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(a + 8 * (D / 4)));
+    return __builtin_bit_cast(u4, (s8v)__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+  constexpr int VF = DB;   // the first step's values: on their way during the softmax
+  u4 vf[VF];
+#pragma unroll
+  for (int x = 0; x < VF; ++x) vf[x] = values(x / DB, x % DB);
+  asm volatile("" ::: "memory");   // not moved down to their use
+
+  float c = p.scale * kLog2e;
+  if constexpr (EXTRA) {
+    cap_and_bias(p, rw, s, tile0);
+    c = 1.f;
+  }
+  if constexpr (MASKED) hide(p, rw, sq, s, tile0, vm);
   float t = s[0][0];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb)
@@ -136,70 +222,66 @@ __device__ __forceinline__ void tile(const PagedArgs& p, const Rows& rw, const P
     const float m2 = t > ac.m + kAbove ? t - kBelow : ac.m;
     const float f = __builtin_amdgcn_exp2f(ac.m - m2);
     ac.m = m2;
-    ac.l *= f;
+    ac.l[0] *= f;
+    ac.l[1] *= f;
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) ac.o[i] *= f;
+    for (int i = 0; i < DB; ++i) ac.o[i] *= f;
   }
   const float nm = -ac.m;
-  float l = 0.f;
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      s[nb][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[nb][j], c, nm));
-      l += s[nb][j];
-    }
-  ac.l += l;
-  const int i = lane & 15, key0 = 4 * h + (i >> 2), low = 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
-  const s4* vp = (const s4*)vt + key0 * (D / 4) + (i & 1);
-  const int sv = Lay<D>::swz_v(key0);
+  float(&l)[2] = ac.l;
   auto weights = [&](int u) {
     u4 pr;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) pr[e] = pack2<T>(s[u / 2][8 * (u & 1) + 2 * e], s[u / 2][8 * (u & 1) + 2 * e + 1]);
+    for (int e = 0; e < 4; ++e) {
+      const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u / 2][8 * (u & 1) + 2 * e], c, nm));
+      const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u / 2][8 * (u & 1) + 2 * e + 1], c, nm));
+      l[0] += x;
+      l[1] += y;
+      pr[e] = pack2<T>(x, y);
+    }
     return pr;
   };
-  auto values = [&](int u, int db) {
-    const s4* a = vp + 16 * u * (D / 4) + 2 * ((4 * db + low) ^ sv);
-    const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)a);
-    const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(a + 8 * (D / 4)));
-    return __builtin_bit_cast(u4, (s8v)__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
-  };
-  if (masked && not_finite<T>(vt, 32 * NB * Lay<D>::ROW)) {
-    // A hidden slot's infinity or NaN times its weight of zero would be NaN:
-    // the product takes zeros for them all, and each is then added to the
-    // rows that see its slot (times any weight it is itself, or NaN).
+  if (MASKED && not_finite<T>(vt, 32 * NB * ROW)) {
+    odd.template mark<T>(p, rw, sq, vt, 32 * NB, tile0, vm);
 #pragma unroll
     for (int u = 0; u < 2 * NB; ++u) {
       const u4 pr = weights(u);
 #pragma unroll
-      for (int db = 0; db < D / 32; ++db) ac.o[db] = T::mfma(finite<T>(values(u, db)), pr, ac.o[db]);
-    }
-#pragma unroll 1
-    for (int kk = 0; kk < 32 * NB; ++kk) {
-      const bool see = paged_visible(rw.pos, tile0 + kk, sq.len, sq.prefix, p.window) && ((vm >> kk) & 1);
-      const uint2* row = (const uint2*)(vt + kk * Lay<D>::ROW);
-#pragma unroll
-      for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint2 raw = row[2 * ((4 * db + e) ^ Lay<D>::swz_v(kk)) + h];
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const uint32_t bits = (x < 2 ? raw.x : raw.y) >> (16 * (x & 1)) & 0xFFFFu;
-            if (see && (bits & (T::kExp & 0xFFFFu)) == (T::kExp & 0xFFFFu))
-              ac.o[db][4 * e + x] += (float)__builtin_bit_cast(typename T::e, (uint16_t)bits);
-          }
-        }
+      for (int db = 0; db < DB; ++db) ac.o[db] = T::mfma(finite<T>(values(u, db)), pr, ac.o[db]);
     }
     return;
   }
+  u4 pr = weights(0);
 #pragma unroll
   for (int u = 0; u < 2 * NB; ++u) {
-    const u4 pr = weights(u);
 #pragma unroll
-    for (int db = 0; db < D / 32; ++db) ac.o[db] = T::mfma(values(u, db), pr, ac.o[db]);
+    for (int db = 0; db < DB; ++db) {
+      ac.o[db] = T::mfma(vf[db], pr, ac.o[db]);
+      if (u + 1 < 2 * NB) vf[db] = values(u + 1, db);
+    }
+    if (u + 1 < 2 * NB) pr = weights(u + 1);
   }
+#pragma unroll
+  for (int u = 0; u < 2 * NB; ++u)
+#pragma unroll
+    for (int db = 0; db < DB; ++db) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      if (u + 1 < 2 * NB) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 28 / DB, 0);
+      }
+    }
+}
+
+// tile, as the slots that the wave's rows see ask for.
+template <typename T, int D, int NB, bool EXTRA>
+__device__ __forceinline__ void any_tile(const PagedArgs& p, const Rows& rw, const PagedSeq& sq, const u4 (&q)[D / 16],
+                                         Acc<D>& ac, Odd<D>& odd, const u4* kt, const u4* vt, int tile0, uint64_t vm) {
+  constexpr uint64_t kAll = NB == 2 ? ~0ull : 0xFFFFFFFFull;
+  if (vm != kAll || tile0 + 32 * NB - 1 > rw.first || (p.window > 0 && (int64_t)tile0 <= (int64_t)rw.last - p.window))
+    tile<T, D, NB, EXTRA, true>(p, rw, sq, q, ac, odd, kt, vt, tile0, vm);
+  else
+    tile<T, D, NB, EXTRA, false>(p, rw, sq, q, ac, odd, kt, vt, tile0, vm);
 }
 
 // The wave's rows r0 .. r0 + 32 of a sequence and key/value head, and their
@@ -235,15 +317,29 @@ __device__ __forceinline__ float log_sum(float m, float l) {
   return l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
-// ---- many rows: one workgroup per 128 rows, whose four waves share the tiles ----
+// ---- many rows: one workgroup of eight waves per 256 rows ----
+//
+// Per tile of 64 slots a wave has D / 4 MFMAs (output of the tile before,
+// scores of this one) and a softmax of about as many cycles.  One wave issues
+// an instruction every five cycles at most, so one per SIMD cannot keep both
+// units busy; two can, if one multiplies while the other takes the softmax.
+// Waves 0..3 and 4..7 (one of each per SIMD) therefore stand half a tile apart
+// and change places at a barrier: phase 2t is waves 0..3's products of tile t,
+// phase 2t + 1 their softmax, and waves 4..7 are one phase behind.
+//
+// Tiles lie in four LDS slots.  A wave asks for its eight slots of a tile two
+// (waves 4..7: three) tiles ahead at the start of a softmax, and waits for them
+// at the start of the next one.
 
-constexpr int kRowsP = 128;
+constexpr int kRowsP = 256;
 
 template <typename T, int D, bool EXTRA>
-__global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedArgs p) {
-  constexpr int TK = 64, ROW = Lay<D>::ROW, GS = Lay<D>::GS, NG = TK / GS / 4;
-  __shared__ u4 k0[TK * ROW], k1[TK * ROW], v0[TK * ROW], v1[TK * ROW];
-  const int lane = threadIdx.x & 63, w = uni(threadIdx.x >> 6);
+__global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p) {
+  constexpr int TK = 64, ROW = Lay<D>::ROW, GS = Lay<D>::GS, NG = 8 / GS, NM = D / 8, DB = D / 32, KS = D / 16, AHEAD = 6;
+  constexpr int SLOT = TK * ROW;
+  __shared__ u4 kbuf[4 * SLOT], vbuf[4 * SLOT];
+  const int lane = threadIdx.x & 63, w = uni(threadIdx.x >> 6), behind = w >> 2;
+  const int col = lane & 31, h = lane >> 5;
   const int kv = blockIdx.x % p.KVH;
   int item = blockIdx.x / p.KVH, seq = -1;
   PagedSeq sq{};
@@ -270,80 +366,206 @@ __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedArgs p) {
   if (seq < 0) return;
 
   const int r0 = item * kRowsP, total = sq.n * p.g, off = sq.len - sq.n;
-  u4 q[D / 16];
+  u4 q[KS];
   const Rows rw = load_rows<D>(p, sq, kv, r0 + 32 * w, q);
-  const bool busy = r0 + 32 * w < total;
   const int rl = r0 + kRowsP < total ? r0 + kRowsP - 1 : total - 1;
-  const PagedSpan span = paged_span(off + (int)p.gdiv.div(r0), off + (int)p.gdiv.div(rl), sq.len, sq.prefix, p.window, TK);
-  const int count = span.count();
+  const int first = uni(off + (int)p.gdiv.div(r0)), last = uni(off + (int)p.gdiv.div(rl));
+  const PagedSpan span = paged_span(first, last, sq.len, sq.prefix, p.window, TK);
+  const int count = uni(span.count());
 
+  // the wave's slots of a tile: 8 w .. 8 w + 8, in one page
   const Base kb = cache_base(p.k, kv), vb = cache_base(p.v, kv);
-  const int gl = lane / ROW, piece = lane % ROW;
-  const uint32_t koff = gl * kb.slot + 16u * (piece ^ Lay<D>::swz_k(GS * w + gl));
-  const uint32_t voff = gl * vb.slot + 16u * (piece ^ Lay<D>::swz_v(GS * w + gl));
+  uint32_t koff[NG], voff[NG];
+#pragma unroll
+  for (int n = 0; n < NG; ++n) {
+    const int j = GS * n + lane / ROW, piece = lane % ROW;
+    koff[n] = j * kb.slot + 16u * (piece ^ Lay<D>::swz_k(8 * w + j));
+    voff[n] = j * vb.slot + 16u * (piece ^ Lay<D>::swz_v(8 * w + j));
+  }
   const int32_t* row = p.table + (int64_t)seq * p.ld_table;
   const int mask = (1 << p.shift) - 1;
-  // the table's entry for the lane's slot in tile i, checked when it is used:
-  // a check here would wait for the loads before it
+  // the table's entry for them in tile i, checked when it is used: a check
+  // here would wait for the loads before it
+  auto slot_of = [&](int i) { return span.tile(i < count ? i : count - 1) * TK + 8 * w; };
   auto entry_of = [&](int i) {
-    const int j = span.tile(i < count ? i : count - 1) * TK + lane;
+    const int j = slot_of(i);
     return row[(j < sq.len ? j : sq.len - 1) >> p.shift];
   };
-  auto page_of = [&](int i, int id) {
-    return i < count && span.tile(i) * TK + lane < sq.len && id >= 0 && id < p.pages ? id : -1;
-  };
-  auto load = [&](int i, int pg, uint64_t vm, u4* kd, u4* vd) {
+  auto load = [&](int i, int entry) {   // past the last tile: zeros that nobody reads
+    const int j = slot_of(i), id = uni(entry);
+    const bool ok = i < count && id >= 0 && id < p.pages;
+    const int64_t page = ok ? id : 0;
+    int n = ok ? sq.len - j : 0;
+    n = n < 0 ? 0 : (n > 8 ? 8 : n);
+    const desc_t kd = make_desc(kb.ptr + page * kb.page + (int64_t)(j & mask) * kb.slot, n * kb.slot);
+    const desc_t vd = make_desc(vb.ptr + page * vb.page + (int64_t)(j & mask) * vb.slot, n * vb.slot);
+    const int at = (i & 3) * SLOT + 64 * NG * w;
 #pragma unroll
-    for (int n = 0; n < NG; ++n) {
-      const int gi = 4 * n + w, j = gi * GS;
-      const int page = __builtin_amdgcn_readlane(pg, j), nv = __popcll((vm >> j) & ((1u << GS) - 1));
-      const int in = (span.tile(i) * TK + j) & mask;
-      load_group(kb, page, in, nv, koff, kd + 64 * gi);
-      load_group(vb, page, in, nv, voff, vd + 64 * gi);
+    for (int x = 0; x < NG; ++x) {
+      if (x == 0) lds_load16<true>(kd, koff[0], kbuf + at);
+      else lds_load16<false>(kd, koff[x], kbuf + at + 64 * x);
+      lds_load16<false>(vd, voff[x], vbuf + at + 64 * x);
     }
+  };
+  // whether some page in reach is not one of the cache
+  bool gaps = false;
+  for (int part = 0; part < 2; ++part) {
+    const int from = part ? span.lo * TK : 0, to = min(part ? span.hi * TK : span.pre * TK, sq.len);
+    for (int x = (from >> p.shift) + threadIdx.x; (int64_t)x << p.shift < to; x += 512) gaps |= row[x] < 0 || row[x] >= p.pages;
+  }
+  gaps = uni(__syncthreads_or(gaps));
+  auto exist = [&](int t0) -> uint64_t {   // bit per slot of a tile
+    if (gaps) return __ballot(paged_page(row, t0 + lane, sq.len, p.shift, p.pages) >= 0);
+    const int n = sq.len - t0;
+    return n >= TK ? ~0ull : (1ull << n) - 1;
+  };
+
+  int entry = 0;   // of the tile that is loaded next
+  if (count > 0) {
+    for (int i = 0; i < 2 + behind; ++i) load(i, entry_of(i));
+    entry = entry_of(2 + behind);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+
+  // operands of MFMA m: keys (step m / 2, block m % 2), values (step m / DB, columns m % DB)
+  const int kswz = Lay<D>::swz_k(col) ^ h, klow = col * ROW;
+  const int li = lane & 15, key0 = 4 * h + (li >> 2), vlow = key0 * (D / 4) + (li & 1);
+  const int vswz = Lay<D>::swz_v(key0) ^ (2 * ((lane >> 4) & 1) + ((li & 3) >> 1));
+  auto key = [&](int t, int m) { return kbuf[(t & 3) * SLOT + klow + 32 * (m & 1) * ROW + (kswz ^ (2 * (m >> 1)))]; };
+  auto value = [&](int t, int m) {
+    const s4* a = (const s4*)(vbuf + (t & 3) * SLOT) + vlow + 16 * (m / DB) * (D / 4) + 2 * ((4 * (m % DB)) ^ vswz);
+    const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)a);
+    const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(a + 8 * (D / 4)));
+    return __builtin_bit_cast(u4, (s8v)__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
   };
 
   Acc<D> ac;
   ac.clear();
-  int id = 0;
-  uint64_t vm = 0;
-  if (count > 0) {
-    const int pg = page_of(0, entry_of(0));
-    vm = __ballot(pg >= 0);
-    load(0, pg, vm, k0, v0);
-    id = entry_of(1);
-  }
-  auto step = [&](int i, const u4* kt, const u4* vt, u4* kn, u4* vn) {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();   // tile i is in LDS, and no wave reads tile i - 1 any more
+  f16v s[2];
+  uint32_t wt[16] = {};   // the tile's weights, two to a word; none before the first
+  u4 frag[AHEAD];
+  bool strange = false;   // some tile holds infinities or NaN that not every row sees
+  const float c = EXTRA ? 1.f : p.scale * kLog2e;
+  auto change = [] {
+    __builtin_amdgcn_sched_barrier(0);
     asm volatile("" ::: "memory");
-    const int pg = page_of(i + 1, id);
-    const uint64_t vm1 = __ballot(pg >= 0);
-    if (i + 1 < count) {
-      load(i + 1, pg, vm1, kn, vn);
-      id = entry_of(i + 2);
-    }
-    const int t0 = span.tile(i) * TK;
-    if (busy && (t0 <= rw.last || t0 < sq.prefix)) tile<T, D, 2, EXTRA>(p, rw, sq, q, ac, kt, vt, t0, vm);
-    vm = vm1;
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
   };
-  for (int i = 0; i < count; i += 2) {
-    step(i, k0, v0, k1, v1);
-    if (i + 1 < count) step(i + 1, k1, v1, k0, v0);
+  // O += V P of tile t; frag: its first operands, on return the first of K in tile tk
+  auto outputs = [&](int t, int tk) {
+    auto weight = [&](int m) {
+      const int u = m / DB;
+      return (u4){wt[4 * u], wt[4 * u + 1], wt[4 * u + 2], wt[4 * u + 3]};
+    };
+#pragma unroll
+    for (int m = 0; m < NM; ++m) {
+      T::add(ac.o[m % DB], frag[m % AHEAD], weight(m));
+      frag[m % AHEAD] = m + AHEAD < NM ? value(t, m + AHEAD) : key(tk, (m + AHEAD) % NM);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    u4 f[AHEAD];
+#pragma unroll
+    for (int m = 0; m < AHEAD; ++m) f[m] = frag[(m + NM) % AHEAD];
+#pragma unroll
+    for (int m = 0; m < AHEAD; ++m) frag[m] = f[m];
+  };
+  auto scores = [&](int t) {
+#pragma unroll
+    for (int m = 0; m < NM; ++m) {
+      s[m & 1] = T::mfma(frag[m % AHEAD], q[m >> 1], m < 2 ? (f16v){} : s[m & 1]);
+      if (m + AHEAD < NM) frag[m % AHEAD] = key(t, m + AHEAD);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  auto softmax = [&](int t) {
+    const int t0 = span.tile(t) * TK;
+    const uint64_t vm = exist(t0);
+    if constexpr (EXTRA) cap_and_bias(p, rw, s, t0);
+    if (vm != ~0ull || t0 + TK - 1 > rw.first || (p.window > 0 && (int64_t)t0 <= (int64_t)rw.last - p.window)) {
+      hide(p, rw, sq, s, t0, vm);
+      strange |= not_finite<T>(vbuf + (t & 3) * SLOT, SLOT);
+    }
+    float top = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+    for (int j = 1; j < 16; ++j) top = fmaxf(fmaxf(top, s[0][j]), s[1][j]);
+    top = fmaxf(top, swap32(top)) * c;
+    if (__any(top > ac.m + kAbove)) {
+      const float m2 = top > ac.m + kAbove ? top - kBelow : ac.m;
+      const float f = __builtin_amdgcn_exp2f(ac.m - m2);
+      ac.m = m2;
+      ac.l[0] *= f;
+      ac.l[1] *= f;
+#pragma unroll
+      for (int i = 0; i < DB; ++i) ac.o[i] *= f;
+    }
+    const float nm = -ac.m;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k / 8][2 * (k % 8)], c, nm));
+      const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k / 8][2 * (k % 8) + 1], c, nm));
+      ac.l[0] += x;
+      ac.l[1] += y;
+      wt[k] = pack2<T>(x, y);
+    }
+#pragma unroll
+    for (int k = 0; k < 16; ++k) asm volatile("" : "+v"(wt[k]));   // in this phase, not where they are used
+#pragma unroll
+    for (int m = 0; m < AHEAD; ++m) frag[m] = value(t, m);   // landed long ago
+  };
+
+  change();
+  if (behind) change();
+#pragma unroll
+  for (int m = 0; m < AHEAD; ++m) frag[m] = value(0, m);
+#pragma unroll 1
+  for (int t = 0; t < count; ++t) {
+    outputs(t > 0 ? t - 1 : 0, t);
+    scores(t);
+    change();
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    load(t + 2 + behind, entry);
+    entry = entry_of(t + 3 + behind);
+    softmax(t);
+    change();
   }
-  if (!busy) return;
-  const int r = r0 + 32 * w + (lane & 31), h = lane >> 5;
+  if (count > 0) outputs(count - 1, count);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no load into LDS outlives the workgroup
+  if (!behind) change();
+  asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");   // the last products have arrived
+#pragma unroll
+  for (int i = 0; i < DB; ++i) asm volatile("" : "+v"(ac.o[i]));
+  Odd<D> odd;
+  odd.clear();
+  if (uni(__syncthreads_or(strange))) {
+    // once more, a tile at a time, with what hides the hidden values
+    ac.clear();
+#pragma unroll 1
+    for (int t = 0; t < count; ++t) {
+      const int t0 = span.tile(t) * TK;
+      load(t, entry_of(t));
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      tile<T, D, 2, EXTRA, true>(p, rw, sq, q, ac, odd, kbuf + (t & 3) * SLOT, vbuf + (t & 3) * SLOT, t0, exist(t0));
+      __syncthreads();
+    }
+  }
+
+  const int r = r0 + 32 * w + col;
+  const float l = ac.sum();
   if (r >= total) return;
-  const float l = ac.l + swap32(ac.l), f = inverse(l);
+  const float f = inverse(l);
   const int tok = (int)p.gdiv.div(r), a = kv * p.g + r - tok * p.g;
   const int64_t at = (int64_t)(sq.start + tok) * p.H + a;
 #pragma unroll
-  for (int db = 0; db < D / 32; ++db)
+  for (int db = 0; db < DB; ++db)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const f16v& o = ac.o[db];
-      store4<T>(p.out, at * D + 32 * db + 8 * e + 4 * h,
-                (f4){o[4 * e] * f, o[4 * e + 1] * f, o[4 * e + 2] * f, o[4 * e + 3] * f});
+      f4 v;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) v[x] = odd.fix(ac.o[db][4 * e + x] * f, 16 * db + 4 * e + x);
+      store4<T>(p.out, at * D + 32 * db + 8 * e + 4 * h, v);
     }
   if (p.lse && h == 0) p.lse[at] = log_sum(ac.m, l);
 }
@@ -380,7 +602,7 @@ constexpr int record_floats(int D) { return kRowsS * (D + 2); }
 template <typename T, int D, bool EXTRA>
 __global__ __launch_bounds__(256, 1) void paged_split_kernel(PagedArgs p, float* ws, int wgs) {
   constexpr int TK = kTileS, ROW = Lay<D>::ROW, GS = Lay<D>::GS, NG = TK / GS;
-  __shared__ u4 k0[4 * TK * ROW], k1[4 * TK * ROW], v0[4 * TK * ROW], v1[4 * TK * ROW];
+  __shared__ u4 kbuf[4][2 * TK * ROW], vbuf[4][2 * TK * ROW];
   __shared__ float ml[4][kRowsS][2];
   const int tid = threadIdx.x, lane = tid & 63, w = uni(tid >> 6);
   const int64_t units = all_units(p), per = units_per(units, p.KVH, wgs);
@@ -388,8 +610,7 @@ __global__ __launch_bounds__(256, 1) void paged_split_kernel(PagedArgs p, float*
   const int64_t u_end = u_begin + per < u_all ? u_begin + per : u_all;
   const int gl = lane / ROW, piece = lane % ROW;
   const int mask = (1 << p.shift) - 1;
-  u4* const kw[2] = {k0 + w * TK * ROW, k1 + w * TK * ROW};
-  u4* const vw[2] = {v0 + w * TK * ROW, v1 + w * TK * ROW};
+  u4 *const kw = kbuf[w], *const vw = vbuf[w];
 
   for (int64_t u = u_begin; u < u_end;) {
     const int kv = uni((int)(u / units));
@@ -450,36 +671,35 @@ __global__ __launch_bounds__(256, 1) void paged_split_kernel(PagedArgs p, float*
     };
     Acc<D> ac;
     ac.clear();
+    Odd<D> odd;
+    odd.clear();
     int i = t_begin + w;
     int id = 0;
     uint64_t vm = 0;
     if (i < last) {
       const int pg = page_of(i, entry_of(i));
       vm = __ballot(pg >= 0);
-      load(i, pg, vm, kw[0], vw[0]);
+      load(i, pg, vm, kw, vw);
       id = entry_of(i + 4);
     }
-    auto step = [&](int n, const u4* kt, const u4* vt, u4* kn, u4* vn) {
+#pragma unroll 1
+    for (int at = 0; i < last; i += 4, at ^= TK * ROW) {
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   // the wave's own tile is in LDS
-      const int pg = page_of(n + 4, id);
+      const int pg = page_of(i + 4, id);
       const uint64_t vm1 = __ballot(pg >= 0);
-      if (n + 4 < last) {
-        load(n + 4, pg, vm1, kn, vn);
-        id = entry_of(n + 8);
+      if (i + 4 < last) {
+        load(i + 4, pg, vm1, kw + (at ^ (TK * ROW)), vw + (at ^ (TK * ROW)));
+        id = entry_of(i + 8);
       }
-      tile<T, D, 1, EXTRA>(p, rw, sq, q, ac, kt, vt, span.tile(n) * TK, vm);
+      any_tile<T, D, 1, EXTRA>(p, rw, sq, q, ac, odd, kw + at, vw + at, span.tile(i) * TK, vm);
       vm = vm1;
-    };
-    for (; i < last; i += 8) {
-      step(i, kw[0], vw[0], kw[1], vw[1]);
-      if (i + 4 < last) step(i + 4, kw[1], vw[1], kw[0], vw[0]);
     }
 
     // ---- the four waves' sums meet in LDS: f4 piece d / 4 of row r at [d / 4][r] ----
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     {
       const int r = lane & 31, h = lane >> 5;
-      const float l = ac.l + swap32(ac.l);
+      const float l = ac.sum();
       if (h == 0) {
         ml[w][r][0] = ac.m;
         ml[w][r][1] = l;
@@ -488,8 +708,12 @@ __global__ __launch_bounds__(256, 1) void paged_split_kernel(PagedArgs p, float*
       for (int db = 0; db < D / 32; ++db)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          f4* at = (f4*)(db < D / 64 ? kw[0] : kw[1]) + ((db % (D / 64)) * 8 + 2 * e + h) * kRowsS + r;
-          *at = (f4){ac.o[db][4 * e], ac.o[db][4 * e + 1], ac.o[db][4 * e + 2], ac.o[db][4 * e + 3]};
+          {
+            f4 v;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) v[x] = odd.fix(ac.o[db][4 * e + x], 16 * db + 4 * e + x);
+            ((f4*)kw)[(db * 8 + 2 * e + h) * kRowsS + r] = v;
+          }
         }
     }
     __syncthreads();
@@ -516,7 +740,7 @@ __global__ __launch_bounds__(256, 1) void paged_split_kernel(PagedArgs p, float*
         if (have) {
 #pragma unroll
           for (int x = 0; x < 4; ++x)
-            v += f[x] * ((const f4*)((n < D / 64 ? k0 : k1) + x * TK * ROW))[(d4 % (D / 8)) * kRowsS + r];
+            v += f[x] * ((const f4*)kbuf[x])[d4 * kRowsS + r];
           if (whole) store4<T>(p.out, at * D + 4 * d4, v * inv);
           else *(f4*)(rec + 4 * (d4 * kRowsS + r)) = v;
         }
@@ -612,8 +836,8 @@ hipError_t launch(const PagedArgs& a, int num_cus, void* ws, hipStream_t s) {
   if (many_rows(a, num_cus)) {
     const int64_t grid = row_blocks(a, kRowsP) * a.KVH;
     if (grid > 0x7fffffff) return hipErrorInvalidValue;
-    if (a.extra()) paged_rows_kernel<T, D, true><<<(int)grid, 256, 0, s>>>(a);
-    else paged_rows_kernel<T, D, false><<<(int)grid, 256, 0, s>>>(a);
+    if (a.extra()) paged_rows_kernel<T, D, true><<<(int)grid, 512, 0, s>>>(a);
+    else paged_rows_kernel<T, D, false><<<(int)grid, 512, 0, s>>>(a);
     return hipGetLastError();
   }
   if (a.extra()) paged_split_kernel<T, D, true><<<num_cus, 256, 0, s>>>(a, (float*)ws, num_cus);
