@@ -33,7 +33,8 @@ const char* bad_cache(const mq_paged_cache* c, bool with_v) {
   for (int i = 0; i < (with_v ? 2 : 1); ++i) {
     const int64_t page = i ? c->v_page : c->k_page, head = i ? c->v_head : c->k_head, slot = i ? c->v_slot : c->k_slot;
     if (!aligned16(i ? c->v : c->k) || page % 8 || head % 8 || slot % 8) return "the cache must be 16-byte aligned, its strides multiples of 8";
-    if (slot < c->head_dim || slot > (1 << 26) || page < 0 || head < 0) return "strides of the cache out of range";
+    if (slot < c->head_dim || slot > (1 << 26) || head < 0 || page < 0 || page >= (int64_t)1 << 31 ||
+        (c->page_size - 1) * slot + c->head_dim >= (int64_t)1 << 31) return "strides of the cache out of range";
   }
   return nullptr;
 }

@@ -79,7 +79,8 @@ template <int D> struct Lay {
   static constexpr int ROW = D / 8;           // 16-byte pieces of a slot
   static constexpr int GS = 64 / ROW;         // slots per load: 4 (D = 128) or 8 (64)
   static __device__ __forceinline__ int swz_k(int j) { return D == 128 ? j & 15 : (j >> 1) & 7; }
-  static __device__ __forceinline__ int swz_v(int j) { return D == 128 ? 2 * (j & 7) : 2 * ((j >> 1) & 3); }
+  // four pieces (32 lanes' 8 bytes) of four slots at a time
+  static __device__ __forceinline__ int swz_v(int j) { return D == 128 ? 4 * (j & 3) : 4 * ((j >> 1) & 1); }
 };
 
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -115,17 +116,18 @@ __device__ inline void lds_load16(const void*, uint32_t, uint32_t, void*) {}
 
 struct Base {   // wave-uniform
   const char* ptr;      // of the key/value head
-  int64_t page;         // bytes
-  uint32_t slot;        // bytes
+  uint32_t page, slot;  // bytes: below 2^32 each, and a page's slots together
+  __device__ __forceinline__ const char* at(uint32_t id, uint32_t in_page) const {
+    return ptr + ((uint64_t)id * page + in_page * slot);
+  }
 };
 __device__ __forceinline__ Base cache_base(const PagedCache& c, int kv) {
-  return {(const char*)c.ptr + 2 * kv * c.head, 2 * c.page, 2u * (uint32_t)c.slot};
+  return {(const char*)c.ptr + 2 * kv * c.head, 2u * (uint32_t)c.page, 2u * (uint32_t)c.slot};
 }
 // Slots j .. j + GS of page `page` (one page: page sizes are multiples of GS),
 // of which the first nv exist.
 __device__ __forceinline__ void load_group(const Base& c, int page, int in_page, int nv, uint32_t voff, u4* lds) {
-  const char* at = c.ptr + (page < 0 ? 0 : page) * c.page + (int64_t)in_page * c.slot;
-  lds_load16(at, page < 0 ? 0u : (uint32_t)nv * c.slot, voff, lds);
+  lds_load16(c.at(page < 0 ? 0 : page, in_page), page < 0 ? 0u : (uint32_t)nv * c.slot, voff, lds);
 }
 
 

@@ -327,9 +327,10 @@ __device__ __forceinline__ float log_sum(float m, float l) {
 // and change places at a barrier: phase 2t is waves 0..3's products of tile t,
 // phase 2t + 1 their softmax, and waves 4..7 are one phase behind.
 //
-// Tiles lie in four LDS slots.  A wave asks for its eight slots of a tile two
-// (waves 4..7: three) tiles ahead at the start of a softmax, and waits for them
-// at the start of the next one.
+// Tiles lie in four LDS slots.  A wave asks for its eight slots of tile t + 2
+// among its products of tile t, whose issue slots are free (beside the softmax
+// the loads' address arithmetic took 230 of 1900 cycles), and waits for them
+// before its products of tile t + 1.
 
 constexpr int kRowsP = 256;
 
@@ -393,12 +394,11 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p) {
   };
   auto load = [&](int i, int entry) {   // past the last tile: zeros that nobody reads
     const int j = slot_of(i), id = uni(entry);
-    const bool ok = i < count && id >= 0 && id < p.pages;
-    const int64_t page = ok ? id : 0;
+    const bool ok = i < count && (uint32_t)id < (uint32_t)p.pages;
+    const uint32_t page = ok ? id : 0, in = j & mask;
     int n = ok ? sq.len - j : 0;
     n = n < 0 ? 0 : (n > 8 ? 8 : n);
-    const desc_t kd = make_desc(kb.ptr + page * kb.page + (int64_t)(j & mask) * kb.slot, n * kb.slot);
-    const desc_t vd = make_desc(vb.ptr + page * vb.page + (int64_t)(j & mask) * vb.slot, n * vb.slot);
+    const desc_t kd = make_desc(kb.at(page, in), n * kb.slot), vd = make_desc(vb.at(page, in), n * vb.slot);
     const int at = (i & 3) * SLOT + 64 * NG * w;
 #pragma unroll
     for (int x = 0; x < NG; ++x) {
@@ -422,8 +422,9 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p) {
 
   int entry = 0;   // of the tile that is loaded next
   if (count > 0) {
-    for (int i = 0; i < 2 + behind; ++i) load(i, entry_of(i));
-    entry = entry_of(2 + behind);
+    load(0, entry_of(0));
+    load(1, entry_of(1));
+    entry = entry_of(2);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
@@ -445,7 +446,7 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p) {
   uint32_t wt[16] = {};   // the tile's weights, two to a word; none before the first
   u4 frag[AHEAD];
   bool strange = false;   // some tile holds infinities or NaN that not every row sees
-  const float c = EXTRA ? 1.f : p.scale * kLog2e;
+  const float c = __int_as_float(uni(__float_as_int(EXTRA ? 1.f : p.scale * kLog2e)));
   auto change = [] {
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("" ::: "memory");
@@ -459,10 +460,13 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p) {
       const int u = m / DB;
       return (u4){wt[4 * u], wt[4 * u + 1], wt[4 * u + 2], wt[4 * u + 3]};
     };
+    // two at a time, the later operand first: one wait for both
 #pragma unroll
-    for (int m = 0; m < NM; ++m) {
+    for (int m = 0; m < NM; m += 2) {
+      T::add(ac.o[(m + 1) % DB], frag[(m + 1) % AHEAD], weight(m + 1));
       T::add(ac.o[m % DB], frag[m % AHEAD], weight(m));
-      frag[m % AHEAD] = m + AHEAD < NM ? value(t, m + AHEAD) : key(tk, (m + AHEAD) % NM);
+#pragma unroll
+      for (int x = m; x < m + 2; ++x) frag[x % AHEAD] = x + AHEAD < NM ? value(t, x + AHEAD) : key(tk, (x + AHEAD) % NM);
       __builtin_amdgcn_sched_barrier(0);
     }
     u4 f[AHEAD];
@@ -473,42 +477,71 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p) {
   };
   auto scores = [&](int t) {
 #pragma unroll
-    for (int m = 0; m < NM; ++m) {
-      s[m & 1] = T::mfma(frag[m % AHEAD], q[m >> 1], m < 2 ? (f16v){} : s[m & 1]);
-      if (m + AHEAD < NM) frag[m % AHEAD] = key(t, m + AHEAD);
+    for (int m = 0; m < NM; m += 2) {
+      s[1] = T::mfma(frag[(m + 1) % AHEAD], q[m >> 1], m < 2 ? (f16v){} : s[1]);
+      s[0] = T::mfma(frag[m % AHEAD], q[m >> 1], m < 2 ? (f16v){} : s[0]);
+#pragma unroll
+      for (int x = m; x < m + 2; ++x)
+        if (x + AHEAD < NM) frag[x % AHEAD] = key(t, x + AHEAD);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
+  // Weights of tile t.  No maximum beforehand: where a lane's 32 weights add up
+  // to more than kMost (one may be too large for fp16, or the first tile has no
+  // reference yet), the reference moves to kBelow under the largest score and
+  // they are taken again, once.
+  constexpr float kMost = 32768.f;
+  // tiles [clean0, clean1) are seen whole by all the wave's rows
+  int clean0 = count, clean1 = count;
+  if (!gaps) {
+    auto clean = [&](int i) {
+      const int t0 = span.tile(i) * TK;
+      return t0 + TK - 1 <= rw.first && t0 + TK <= sq.len && (p.window <= 0 || (int64_t)t0 > (int64_t)rw.last - p.window);
+    };
+    // one run of tiles: before it lie those of the prefix and the window's edge,
+    // after it those past the wave's first row or the sequence
+    while (clean1 > 0 && !clean(clean1 - 1)) --clean1;
+    clean0 = 0;
+    while (clean0 < clean1 && !clean(clean0)) ++clean0;
+  }
   auto softmax = [&](int t) {
-    const int t0 = span.tile(t) * TK;
-    const uint64_t vm = exist(t0);
-    if constexpr (EXTRA) cap_and_bias(p, rw, s, t0);
-    if (vm != ~0ull || t0 + TK - 1 > rw.first || (p.window > 0 && (int64_t)t0 <= (int64_t)rw.last - p.window)) {
-      hide(p, rw, sq, s, t0, vm);
+    if constexpr (EXTRA) cap_and_bias(p, rw, s, span.tile(t) * TK);
+    if (t < clean0 || t >= clean1) {
+      const int t0 = span.tile(t) * TK;
+      hide(p, rw, sq, s, t0, exist(t0));
       strange |= not_finite<T>(vbuf + (t & 3) * SLOT, SLOT);
     }
-    float top = fmaxf(s[0][0], s[1][0]);
+    float l[2];
+    auto weigh = [&] {
+      const float nm = -ac.m;
+      l[0] = l[1] = 0.f;
 #pragma unroll
-    for (int j = 1; j < 16; ++j) top = fmaxf(fmaxf(top, s[0][j]), s[1][j]);
-    top = fmaxf(top, swap32(top)) * c;
-    if (__any(top > ac.m + kAbove)) {
-      const float m2 = top > ac.m + kAbove ? top - kBelow : ac.m;
+      for (int k = 0; k < 16; ++k) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k / 8][2 * (k % 8)], c, nm));
+        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k / 8][2 * (k % 8) + 1], c, nm));
+        l[0] += x;
+        l[1] += y;
+        wt[k] = pack2<T>(x, y);
+      }
+    };
+    weigh();
+    const float sum = l[0] + l[1];
+    if (__builtin_expect(__any(sum > kMost), 0)) {
+      float top = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+      for (int j = 1; j < 16; ++j) top = fmaxf(fmaxf(top, s[0][j]), s[1][j]);
+      top = fmaxf(top, swap32(top)) * c;
+      const float m2 = fmaxf(sum, swap32(sum)) > kMost ? top - kBelow : ac.m;
       const float f = __builtin_amdgcn_exp2f(ac.m - m2);
       ac.m = m2;
       ac.l[0] *= f;
       ac.l[1] *= f;
 #pragma unroll
       for (int i = 0; i < DB; ++i) ac.o[i] *= f;
+      weigh();
     }
-    const float nm = -ac.m;
-#pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k / 8][2 * (k % 8)], c, nm));
-      const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k / 8][2 * (k % 8) + 1], c, nm));
-      ac.l[0] += x;
-      ac.l[1] += y;
-      wt[k] = pack2<T>(x, y);
-    }
+    ac.l[0] += l[0];
+    ac.l[1] += l[1];
 #pragma unroll
     for (int k = 0; k < 16; ++k) asm volatile("" : "+v"(wt[k]));   // in this phase, not where they are used
 #pragma unroll
@@ -521,12 +554,12 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p) {
   for (int m = 0; m < AHEAD; ++m) frag[m] = value(0, m);
 #pragma unroll 1
   for (int t = 0; t < count; ++t) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // tile t + 1
     outputs(t > 0 ? t - 1 : 0, t);
+    load(t + 2, entry);
+    entry = entry_of(t + 3);
     scores(t);
     change();
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    load(t + 2 + behind, entry);
-    entry = entry_of(t + 3 + behind);
     softmax(t);
     change();
   }
