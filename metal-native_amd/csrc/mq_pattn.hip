@@ -327,10 +327,10 @@ __device__ __forceinline__ float log_sum(float m, float l) {
 // and change places at a barrier: phase 2t is waves 0..3's products of tile t,
 // phase 2t + 1 their softmax, and waves 4..7 are one phase behind.
 //
-// Tiles lie in four LDS slots.  A wave asks for its eight slots of tile t + 2
-// among its products of tile t, whose issue slots are free (beside the softmax
-// the loads' address arithmetic took 230 of 1900 cycles), and waits for them
-// before its products of tile t + 1.
+// Tiles of keys lie in four LDS slots, of values (read a tile later) in five.  A
+// wave asks for its eight slots of tile t + 3 among its products of tile t, whose
+// issue slots are free (beside the softmax the loads' address arithmetic took 230
+// of 1900 cycles), and waits for them before its products of tile t + 2.
 
 constexpr int kRowsP = 256;
 
@@ -338,7 +338,7 @@ template <typename T, int D, bool EXTRA>
 __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p) {
   constexpr int TK = 64, ROW = Lay<D>::ROW, GS = Lay<D>::GS, NG = 8 / GS, NM = D / 8, DB = D / 32, KS = D / 16, AHEAD = 6;
   constexpr int SLOT = TK * ROW;
-  __shared__ u4 kbuf[4 * SLOT], vbuf[4 * SLOT];
+  __shared__ u4 kbuf[4 * SLOT], vbuf[5 * SLOT];
   const int lane = threadIdx.x & 63, w = uni(threadIdx.x >> 6), behind = w >> 2;
   const int col = lane & 31, h = lane >> 5;
   const int kv = blockIdx.x % p.KVH;
@@ -385,27 +385,45 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p) {
   }
   const int32_t* row = p.table + (int64_t)seq * p.ld_table;
   const int mask = (1 << p.shift) - 1;
-  // the table's entry for them in tile i, checked when it is used: a check
-  // here would wait for the loads before it
   auto slot_of = [&](int i) { return span.tile(i < count ? i : count - 1) * TK + 8 * w; };
-  auto entry_of = [&](int i) {
-    const int j = slot_of(i);
-    return row[(j < sq.len ? j : sq.len - 1) >> p.shift];
-  };
-  auto load = [&](int i, int entry) {   // past the last tile: zeros that nobody reads
-    const int j = slot_of(i), id = uni(entry);
-    const bool ok = i < count && (uint32_t)id < (uint32_t)p.pages;
-    const uint32_t page = ok ? id : 0, in = j & mask;
-    int n = ok ? sq.len - j : 0;
-    n = n < 0 ? 0 : (n > 8 ? 8 : n);
-    const desc_t kd = make_desc(kb.at(page, in), n * kb.slot), vd = make_desc(vb.at(page, in), n * vb.slot);
-    const int at = (i & 3) * SLOT + 64 * NG * w;
-#pragma unroll
-    for (int x = 0; x < NG; ++x) {
-      if (x == 0) lds_load16<true>(kd, koff[0], kbuf + at);
-      else lds_load16<false>(kd, koff[x], kbuf + at + 64 * x);
-      lds_load16<false>(vd, voff[x], vbuf + at + 64 * x);
+  int entries = 0;   // lane i: the table's entry for them in tile number i modulo 64
+  // in steps, to be taken between MFMAs (past the last tile: zeros that nobody reads)
+  struct {
+    int j, n;
+    uint32_t page, in;
+    desc_t kd, vd;
+  } ld;
+  constexpr int LOAD_STEPS = 4 + NG;
+  auto load_step = [&](int x, int i, int vslot) {
+    if (x == 0) {
+      ld.j = slot_of(i);
+      const int id = __builtin_amdgcn_readlane(entries, i & 63);
+      const bool ok = i < count && (uint32_t)id < (uint32_t)p.pages;
+      ld.page = ok ? id : 0;
+      ld.n = ok ? sq.len - ld.j : 0;
+    } else if (x == 1) {
+      ld.in = ld.j & mask;
+      ld.n = ld.n < 0 ? 0 : (ld.n > 8 ? 8 : ld.n);
+    } else if (x == 2) {
+      ld.kd = make_desc(kb.at(ld.page, ld.in), ld.n * kb.slot);
+    } else if (x == 3) {
+      ld.vd = make_desc(vb.at(ld.page, ld.in), ld.n * vb.slot);
+    } else {
+      const int n = x - 4;
+      lds_load16<true>(ld.kd, koff[n], kbuf + (i & 3) * SLOT + 64 * (NG * w + n));
+      lds_load16<false>(ld.vd, voff[n], vbuf + vslot * SLOT + 64 * (NG * w + n));
     }
+  };
+  auto next_entries = [&](int i) {
+    if ((i & 63) == 0 && i < count) {
+      const int j = slot_of(i + lane);
+      entries = row[(j < sq.len ? j : sq.len - 1) >> p.shift];
+    }
+  };
+  auto load = [&](int i, int vslot) {
+    next_entries(i);
+#pragma unroll
+    for (int x = 0; x < LOAD_STEPS; ++x) load_step(x, i, vslot);
   };
   // whether some page in reach is not one of the cache
   bool gaps = false;
@@ -420,12 +438,8 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p) {
     return n >= TK ? ~0ull : (1ull << n) - 1;
   };
 
-  int entry = 0;   // of the tile that is loaded next
-  if (count > 0) {
-    load(0, entry_of(0));
-    load(1, entry_of(1));
-    entry = entry_of(2);
-  }
+  if (count > 0)
+    for (int i = 0; i < 3; ++i) load(i, i);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
   // operands of MFMA m: keys (step m / 2, block m % 2), values (step m / DB, columns m % DB)
@@ -433,8 +447,8 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p) {
   const int li = lane & 15, key0 = 4 * h + (li >> 2), vlow = key0 * (D / 4) + (li & 1);
   const int vswz = Lay<D>::swz_v(key0) ^ (2 * ((lane >> 4) & 1) + ((li & 3) >> 1));
   auto key = [&](int t, int m) { return kbuf[(t & 3) * SLOT + klow + 32 * (m & 1) * ROW + (kswz ^ (2 * (m >> 1)))]; };
-  auto value = [&](int t, int m) {
-    const s4* a = (const s4*)(vbuf + (t & 3) * SLOT) + vlow + 16 * (m / DB) * (D / 4) + 2 * ((4 * (m % DB)) ^ vswz);
+  auto value = [&](int vslot, int m) {
+    const s4* a = (const s4*)(vbuf + vslot * SLOT) + vlow + 16 * (m / DB) * (D / 4) + 2 * ((4 * (m % DB)) ^ vswz);
     const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)a);
     const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(a + 8 * (D / 4)));
     return __builtin_bit_cast(u4, (s8v)__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -454,8 +468,8 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p) {
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
   };
-  // O += V P of tile t; frag: its first operands, on return the first of K in tile tk
-  auto outputs = [&](int t, int tk) {
+  // O += V P of the values in slot vs; frag: its first operands, on return the first of K in tile tk
+  auto outputs = [&](int vs, int tk) {
     auto weight = [&](int m) {
       const int u = m / DB;
       return (u4){wt[4 * u], wt[4 * u + 1], wt[4 * u + 2], wt[4 * u + 3]};
@@ -466,7 +480,7 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p) {
       T::add(ac.o[(m + 1) % DB], frag[(m + 1) % AHEAD], weight(m + 1));
       T::add(ac.o[m % DB], frag[m % AHEAD], weight(m));
 #pragma unroll
-      for (int x = m; x < m + 2; ++x) frag[x % AHEAD] = x + AHEAD < NM ? value(t, x + AHEAD) : key(tk, (x + AHEAD) % NM);
+      for (int x = m; x < m + 2; ++x) frag[x % AHEAD] = x + AHEAD < NM ? value(vs, x + AHEAD) : key(tk, (x + AHEAD) % NM);
       __builtin_amdgcn_sched_barrier(0);
     }
     u4 f[AHEAD];
@@ -475,7 +489,8 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p) {
 #pragma unroll
     for (int m = 0; m < AHEAD; ++m) frag[m] = f[m];
   };
-  auto scores = [&](int t) {
+  // S of tile t, and the loads of tile t + 3 between its products
+  auto scores = [&](int t, int vslot) {
 #pragma unroll
     for (int m = 0; m < NM; m += 2) {
       s[1] = T::mfma(frag[(m + 1) % AHEAD], q[m >> 1], m < 2 ? (f16v){} : s[1]);
@@ -483,6 +498,8 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p) {
 #pragma unroll
       for (int x = m; x < m + 2; ++x)
         if (x + AHEAD < NM) frag[x % AHEAD] = key(t, x + AHEAD);
+#pragma unroll
+      for (int x = m * LOAD_STEPS / NM; x < (m + 2) * LOAD_STEPS / NM; ++x) load_step(x, t + 3, vslot);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -504,12 +521,12 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p) {
     clean0 = 0;
     while (clean0 < clean1 && !clean(clean0)) ++clean0;
   }
-  auto softmax = [&](int t) {
+  auto softmax = [&](int t, int vs) {
     if constexpr (EXTRA) cap_and_bias(p, rw, s, span.tile(t) * TK);
     if (t < clean0 || t >= clean1) {
       const int t0 = span.tile(t) * TK;
       hide(p, rw, sq, s, t0, exist(t0));
-      strange |= not_finite<T>(vbuf + (t & 3) * SLOT, SLOT);
+      strange |= not_finite<T>(vbuf + vs * SLOT, SLOT);
     }
     float l[2];
     auto weigh = [&] {
@@ -545,25 +562,28 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p) {
 #pragma unroll
     for (int k = 0; k < 16; ++k) asm volatile("" : "+v"(wt[k]));   // in this phase, not where they are used
 #pragma unroll
-    for (int m = 0; m < AHEAD; ++m) frag[m] = value(t, m);   // landed long ago
+    for (int m = 0; m < AHEAD; ++m) frag[m] = value(vs, m);   // landed long ago
   };
 
   change();
   if (behind) change();
 #pragma unroll
   for (int m = 0; m < AHEAD; ++m) frag[m] = value(0, m);
+  int vprev = 0, vcur = 0, vload = 3;   // slots of the values of tiles t - 1 (tile 0: its own, times weights of zero), t, t + 3
 #pragma unroll 1
   for (int t = 0; t < count; ++t) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // tile t + 1
-    outputs(t > 0 ? t - 1 : 0, t);
-    load(t + 2, entry);
-    entry = entry_of(t + 3);
-    scores(t);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NG) : "memory");   // tile t + 1 has landed; t + 2 may be on its way
+    outputs(vprev, t);
+    next_entries(t + 3);
+    scores(t, vload);
+    vload = vload == 4 ? 0 : vload + 1;
     change();
-    softmax(t);
+    softmax(t, vcur);
+    vprev = vcur;
+    vcur = vcur == 4 ? 0 : vcur + 1;
     change();
   }
-  if (count > 0) outputs(count - 1, count);
+  if (count > 0) outputs(vprev, count);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no load into LDS outlives the workgroup
   if (!behind) change();
   asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");   // the last products have arrived
@@ -577,10 +597,10 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p) {
 #pragma unroll 1
     for (int t = 0; t < count; ++t) {
       const int t0 = span.tile(t) * TK;
-      load(t, entry_of(t));
+      load(t, 0);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
-      tile<T, D, 2, EXTRA, true>(p, rw, sq, q, ac, odd, kbuf + (t & 3) * SLOT, vbuf + (t & 3) * SLOT, t0, exist(t0));
+      tile<T, D, 2, EXTRA, true>(p, rw, sq, q, ac, odd, kbuf + (t & 3) * SLOT, vbuf, t0, exist(t0));
       __syncthreads();
     }
   }
