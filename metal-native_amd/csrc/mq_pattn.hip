@@ -158,9 +158,12 @@ template <int D> struct Odd {
 // One wave's instructions issue in order, so both products read their LDS
 // operands a few instructions ahead (kf, vf): with a wait for LDS before each
 // step the 4096-token chunk behind 28672 slots took 2.0 ms.
-template <typename T, int D, int NB, bool EXTRA, bool MASKED>
+// keys_done() follows the last read of the keys, values_ready() comes before the
+// first read of the values.
+template <typename T, int D, int NB, bool EXTRA, bool MASKED, typename F, typename G>
 __device__ __forceinline__ void tile(const PagedArgs& p, const Rows& rw, const PagedSeq& sq, const u4 (&q)[D / 16],
-                                     Acc<D>& ac, Odd<D>& odd, const u4* kt, const u4* vt, int tile0, uint64_t vm) {
+                                     Acc<D>& ac, Odd<D>& odd, const u4* kt, const u4* vt, int tile0, uint64_t vm,
+                                     F&& keys_done, G&& values_ready) {
   constexpr int ROW = Lay<D>::ROW, KS = D / 16, DB = D / 32;
   const int lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5;
   f16v s[NB];
@@ -200,6 +203,8 @@ __device__ __forceinline__ void tile(const PagedArgs& p, const Rows& rw, const P
     const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(a + 8 * (D / 4)));
     return __builtin_bit_cast(u4, (s8v)__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
   };
+  keys_done();
+  values_ready();
   constexpr int VF = DB;   // the first step's values: on their way during the softmax
   u4 vf[VF];
 #pragma unroll
@@ -273,17 +278,6 @@ __device__ __forceinline__ void tile(const PagedArgs& p, const Rows& rw, const P
     }
 }
 
-// tile, as the slots that the wave's rows see ask for.
-template <typename T, int D, int NB, bool EXTRA>
-__device__ __forceinline__ void any_tile(const PagedArgs& p, const Rows& rw, const PagedSeq& sq, const u4 (&q)[D / 16],
-                                         Acc<D>& ac, Odd<D>& odd, const u4* kt, const u4* vt, int tile0, uint64_t vm) {
-  constexpr uint64_t kAll = NB == 2 ? ~0ull : 0xFFFFFFFFull;
-  if (vm != kAll || tile0 + 32 * NB - 1 > rw.first || (p.window > 0 && (int64_t)tile0 <= (int64_t)rw.last - p.window))
-    tile<T, D, NB, EXTRA, true>(p, rw, sq, q, ac, odd, kt, vt, tile0, vm);
-  else
-    tile<T, D, NB, EXTRA, false>(p, rw, sq, q, ac, odd, kt, vt, tile0, vm);
-}
-
 // The wave's rows r0 .. r0 + 32 of a sequence and key/value head, and their
 // queries (zeros for padding rows).
 template <int D>
@@ -300,11 +294,13 @@ __device__ __forceinline__ Rows load_rows(const PagedArgs& p, const PagedSeq& sq
   const u4* src = (const u4*)((const uint16_t*)p.q + (int64_t)(sq.start + i) * p.q_t + (int64_t)a * p.q_h) + h;
 #pragma unroll
   for (int ks = 0; ks < D / 16; ++ks) q[ks] = have ? src[2 * ks] : (u4){0u, 0u, 0u, 0u};
-  // waited for here: the compiler would otherwise wait in the loop over the
-  // tiles, where the wait takes in the loads of the next tile
-#pragma unroll
-  for (int ks = 0; ks < D / 16; ++ks) asm volatile("" : "+v"(q[ks]));
   return rw;
+}
+// Waits for them: the compiler would otherwise wait in the loop over the tiles,
+// where the wait takes in the loads of the next tile.
+template <int N> __device__ __forceinline__ void have_queries(u4 (&q)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(q[i]));
 }
 
 template <typename T>
@@ -369,6 +365,7 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p) {
   const int r0 = item * kRowsP, total = sq.n * p.g, off = sq.len - sq.n;
   u4 q[KS];
   const Rows rw = load_rows<D>(p, sq, kv, r0 + 32 * w, q);
+  have_queries(q);
   const int rl = r0 + kRowsP < total ? r0 + kRowsP - 1 : total - 1;
   const int first = uni(off + (int)p.gdiv.div(r0)), last = uni(off + (int)p.gdiv.div(rl));
   const PagedSpan span = paged_span(first, last, sq.len, sq.prefix, p.window, TK);
@@ -600,7 +597,7 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p) {
       load(t, 0);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
-      tile<T, D, 2, EXTRA, true>(p, rw, sq, q, ac, odd, kbuf + (t & 3) * SLOT, vbuf, t0, exist(t0));
+      tile<T, D, 2, EXTRA, true>(p, rw, sq, q, ac, odd, kbuf + (t & 3) * SLOT, vbuf, t0, exist(t0), [] {}, [] {});
       __syncthreads();
     }
   }
@@ -623,253 +620,259 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p) {
   if (p.lse && h == 0) p.lse[at] = log_sum(ac.m, l);
 }
 
-// ---- few rows: every workgroup takes an equal run of (row block, key tile)
-// units, its four waves the run's tiles in turn ----
+// ---- few rows: one workgroup per 32 rows and a part of their tiles of 32 slots,
+// which its four waves take in turn ----
+//
+// Reading the cache is all the work there is, so what counts is that many
+// loads are on their way: 16 KiB per wave in one buffer for keys and one for
+// values, each filled again as soon as its products have read it, two
+// workgroups per CU.  Workgroups past a sequence's end return at once: the host
+// does not know the lengths and launches for the longest that the table can
+// hold.
 
 constexpr int kRowsS = 32, kTileS = 32;
 
-__device__ __forceinline__ int64_t split_units(const PagedArgs& p, const PagedSeq& q, int* blocks, PagedSpan* span) {
-  *blocks = (int)(((int64_t)q.n * p.g + kRowsS - 1) / kRowsS);
-  *span = paged_span(q.len - q.n, q.len - 1, q.len, q.prefix, p.window, kTileS);
-  const int c = span->count();
-  return (int64_t)*blocks * (c > 0 ? c : 1);   // a row that sees nothing is written too
-}
-__device__ __forceinline__ int64_t all_units(const PagedArgs& p) {
+// Row block `item` of the call: its sequence (-1: there is none) and number.
+__device__ __forceinline__ int find_block(const PagedArgs& p, int item, int rows, PagedSeq& sq, int& block) {
+  if (!p.cu) {   // as many blocks for every sequence
+    const int per = (p.g + rows - 1) / rows, s = uni(item / per);
+    block = item - s * per;
+    if (s >= p.b) return -1;
+    const PagedSeq q = load_seq(p, s);
+    sq = {uni(q.start), uni(q.n), uni(q.len), uni(q.prefix)};
+    return block * rows < sq.n * p.g ? s : -1;
+  }
   const int lane = threadIdx.x & 63;
-  int64_t total = 0;
   for (int s0 = 0; s0 < p.b; s0 += 64) {
-    int blocks;
-    PagedSpan span;
-    const int64_t u = s0 + lane < p.b ? split_units(p, load_seq(p, s0 + lane), &blocks, &span) : 0;
-    total += uni64(__shfl(wave_scan(u), 63));
-  }
-  return total;
-}
-// units per workgroup: at least one tile per wave
-__device__ __forceinline__ int64_t units_per(int64_t units, int kvh, int wgs) {
-  const int64_t per = (units * kvh + wgs - 1) / wgs;
-  return per < 4 ? 4 : per;
-}
-constexpr int record_floats(int D) { return kRowsS * (D + 2); }
-
-template <typename T, int D, bool EXTRA>
-__global__ __launch_bounds__(256, 1) void paged_split_kernel(PagedArgs p, float* ws, int wgs) {
-  constexpr int TK = kTileS, ROW = Lay<D>::ROW, GS = Lay<D>::GS, NG = TK / GS;
-  __shared__ u4 kbuf[4][2 * TK * ROW], vbuf[4][2 * TK * ROW];
-  __shared__ float ml[4][kRowsS][2];
-  const int tid = threadIdx.x, lane = tid & 63, w = uni(tid >> 6);
-  const int64_t units = all_units(p), per = units_per(units, p.KVH, wgs);
-  const int64_t u_begin = per * blockIdx.x, u_all = units * p.KVH;
-  const int64_t u_end = u_begin + per < u_all ? u_begin + per : u_all;
-  const int gl = lane / ROW, piece = lane % ROW;
-  const int mask = (1 << p.shift) - 1;
-  u4 *const kw = kbuf[w], *const vw = vbuf[w];
-
-  for (int64_t u = u_begin; u < u_end;) {
-    const int kv = uni((int)(u / units));
-    int64_t left = u - kv * units;
-    int seq = -1, blocks = 0;
-    PagedSeq sq{};
-    PagedSpan span{};
-    for (int s0 = 0; s0 < p.b && seq < 0; s0 += 64) {
-      PagedSeq mine{};
-      int64_t n = 0;
-      if (s0 + lane < p.b) {
-        mine = load_seq(p, s0 + lane);
-        n = split_units(p, mine, &blocks, &span);
-      }
-      const int64_t sum = wave_scan(n);
-      const uint64_t past = __ballot(sum > left);
-      if (past) {
-        const int at = __ffsll((unsigned long long)past) - 1;
-        left -= uni64(__shfl(sum - n, at));
-        seq = s0 + at;
-        sq.start = __builtin_amdgcn_readlane(mine.start, at);
-        sq.n = __builtin_amdgcn_readlane(mine.n, at);
-        sq.len = __builtin_amdgcn_readlane(mine.len, at);
-        sq.prefix = __builtin_amdgcn_readlane(mine.prefix, at);
-      } else {
-        left -= uni64(__shfl(sum, 63));
-      }
-    }
-    if (seq < 0) return;   // not reached: u < u_all
-    split_units(p, sq, &blocks, &span);
-    const int count = span.count(), cost = count > 0 ? count : 1;
-    const int block = uni((int)(left / cost)), t_begin = uni((int)(left - (int64_t)block * cost));
-    const int t_end = uni((int)(cost - t_begin < u_end - u ? cost : t_begin + (u_end - u)));
-    const bool whole = t_begin == 0 && t_end == cost;
-
-    u4 q[D / 16];
-    const int r0 = block * kRowsS, total = sq.n * p.g;
-    const Rows rw = load_rows<D>(p, sq, kv, r0, q);
-    const Base kb = cache_base(p.k, kv), vb = cache_base(p.v, kv);
-    const int32_t* row = p.table + (int64_t)seq * p.ld_table;
-    const int last = t_end < count ? t_end : count;
-    auto entry_of = [&](int i) {
-      const int j = span.tile(i < last ? i : last - 1) * TK + (lane & 31);
-      return row[(j < sq.len ? j : sq.len - 1) >> p.shift];
-    };
-    auto page_of = [&](int i, int id) {
-      return i < last && lane < TK && span.tile(i) * TK + lane < sq.len && id >= 0 && id < p.pages ? id : -1;
-    };
-    auto load = [&](int i, int pg, uint64_t vm, u4* kd, u4* vd) {
-#pragma unroll
-      for (int gi = 0; gi < NG; ++gi) {
-        const int j = gi * GS;
-        const int page = __builtin_amdgcn_readlane(pg, j), nv = __popcll((vm >> j) & ((1u << GS) - 1));
-        const int in = (span.tile(i) * TK + j) & mask;
-        load_group(kb, page, in, nv, gl * kb.slot + 16u * (piece ^ Lay<D>::swz_k(j + gl)), kd + 64 * gi);
-        load_group(vb, page, in, nv, gl * vb.slot + 16u * (piece ^ Lay<D>::swz_v(j + gl)), vd + 64 * gi);
-      }
-    };
-    Acc<D> ac;
-    ac.clear();
-    Odd<D> odd;
-    odd.clear();
-    int i = t_begin + w;
-    int id = 0;
-    uint64_t vm = 0;
-    if (i < last) {
-      const int pg = page_of(i, entry_of(i));
-      vm = __ballot(pg >= 0);
-      load(i, pg, vm, kw, vw);
-      id = entry_of(i + 4);
-    }
-#pragma unroll 1
-    for (int at = 0; i < last; i += 4, at ^= TK * ROW) {
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   // the wave's own tile is in LDS
-      const int pg = page_of(i + 4, id);
-      const uint64_t vm1 = __ballot(pg >= 0);
-      if (i + 4 < last) {
-        load(i + 4, pg, vm1, kw + (at ^ (TK * ROW)), vw + (at ^ (TK * ROW)));
-        id = entry_of(i + 8);
-      }
-      any_tile<T, D, 1, EXTRA>(p, rw, sq, q, ac, odd, kw + at, vw + at, span.tile(i) * TK, vm);
-      vm = vm1;
-    }
-
-    // ---- the four waves' sums meet in LDS: f4 piece d / 4 of row r at [d / 4][r] ----
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    {
-      const int r = lane & 31, h = lane >> 5;
-      const float l = ac.sum();
-      if (h == 0) {
-        ml[w][r][0] = ac.m;
-        ml[w][r][1] = l;
-      }
-#pragma unroll
-      for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          {
-            f4 v;
-#pragma unroll
-            for (int x = 0; x < 4; ++x) v[x] = odd.fix(ac.o[db][4 * e + x], 16 * db + 4 * e + x);
-            ((f4*)kw)[(db * 8 + 2 * e + h) * kRowsS + r] = v;
-          }
-        }
-    }
-    __syncthreads();
-    {
-      const int r = tid & 31;
-      float m = ml[0][r][0];
-#pragma unroll
-      for (int x = 1; x < 4; ++x) m = fmaxf(m, ml[x][r][0]);
-      float f[4], l = 0.f;
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        f[x] = __builtin_amdgcn_exp2f(ml[x][r][0] - m);
-        l += ml[x][r][1] * f[x];
-      }
-      const float inv = inverse(l);
-      float* rec = ws + ((int64_t)2 * blockIdx.x + (u == u_begin ? 0 : 1)) * record_floats(D);
-      const int tok = (int)p.gdiv.div(r0 + r), a = kv * p.g + r0 + r - tok * p.g;
-      const int64_t at = (int64_t)(sq.start + tok) * p.H + a;
-      const bool have = r0 + r < total;
-#pragma unroll
-      for (int n = 0; n < D / 32; ++n) {
-        const int d4 = (tid >> 5) + 8 * n;
-        f4 v = {};
-        if (have) {
-#pragma unroll
-          for (int x = 0; x < 4; ++x)
-            v += f[x] * ((const f4*)kbuf[x])[d4 * kRowsS + r];
-          if (whole) store4<T>(p.out, at * D + 4 * d4, v * inv);
-          else *(f4*)(rec + 4 * (d4 * kRowsS + r)) = v;
-        }
-      }
-      if (have && tid < kRowsS) {
-        if (!whole) {
-          rec[kRowsS * D + 2 * r] = m;
-          rec[kRowsS * D + 2 * r + 1] = l;
-        } else if (p.lse) {
-          p.lse[at] = log_sum(m, l);
-        }
-      }
-    }
-    __syncthreads();
-    u += t_end - t_begin;
-  }
-}
-
-// Adds up the records of the row blocks that more than one workgroup worked
-// on, in the workgroups' order.  blockIdx.x: row block and key/value head;
-// blockIdx.y: 32 of the output's columns.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs p, const float* ws, int wgs) {
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int64_t units = all_units(p), per = units_per(units, p.KVH, wgs);
-  const int kv = blockIdx.x % p.KVH;
-  int item = blockIdx.x / p.KVH, seq = -1, blocks = 0;
-  int64_t u0 = kv * units;
-  PagedSeq sq{};
-  PagedSpan span{};
-  for (int s0 = 0; s0 < p.b && seq < 0; s0 += 64) {
+    const int s = s0 + lane;
     PagedSeq mine{};
-    int64_t n = 0;
-    int nb = 0;
-    if (s0 + lane < p.b) {
-      mine = load_seq(p, s0 + lane);
-      n = split_units(p, mine, &nb, &span);
+    if (s < p.b) mine = load_seq(p, s);
+    const int blocks = (int)(((int64_t)mine.n * p.g + rows - 1) / rows);
+    int sum = blocks;   // at most rows * heads / 32 + b: an int
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int t = __shfl_up(sum, o);
+      if (lane >= o) sum += t;
     }
-    const int64_t sum = wave_scan(nb), usum = wave_scan(n);
     const uint64_t past = __ballot(sum > item);
-    const int at = past ? __ffsll((unsigned long long)past) - 1 : 63;
     if (past) {
-      item -= uni((int)__shfl(sum - nb, at));
-      u0 += uni64(__shfl(usum - n, at));
-      seq = s0 + at;
+      const int at = __ffsll((unsigned long long)past) - 1;
       sq.start = __builtin_amdgcn_readlane(mine.start, at);
       sq.n = __builtin_amdgcn_readlane(mine.n, at);
       sq.len = __builtin_amdgcn_readlane(mine.len, at);
       sq.prefix = __builtin_amdgcn_readlane(mine.prefix, at);
+      block = item - (__builtin_amdgcn_readlane(sum, at) - __builtin_amdgcn_readlane(blocks, at));
+      return s0 + at;
+    }
+    item -= __builtin_amdgcn_readlane(sum, 63);
+  }
+  return -1;
+}
+__device__ __forceinline__ PagedSpan block_span(const PagedArgs& p, const PagedSeq& sq, int r0) {
+  const int total = sq.n * p.g, off = sq.len - sq.n, rl = r0 + kRowsS < total ? r0 + kRowsS - 1 : total - 1;
+  return paged_span(off + (int)p.gdiv.div(r0), off + (int)p.gdiv.div(rl), sq.len, sq.prefix, p.window, kTileS);
+}
+
+// Tiles per part of a row block that sees `count`: parts_max parts, but of
+// per_min tiles at least.
+__device__ __forceinline__ int tiles_per_part(int count, int parts_max, int per_min) {
+  const int per = ((count + parts_max - 1) / parts_max + 3) & ~3;
+  return uni(per < per_min ? per_min : per);
+}
+
+// Partial sums of a part: R rows (the call's most rows per block, a multiple of
+// eight) of D outputs, then R (m, l) pairs.
+__device__ __host__ constexpr int record_floats(int D, int R) { return R * (D + 2); }
+
+template <typename T, int D, bool EXTRA>
+__global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs p, float* ws, int per_min, int R) {
+  constexpr int TK = kTileS, ROW = Lay<D>::ROW, GS = Lay<D>::GS, NG = TK / GS;
+  __shared__ u4 buf[4][2 * TK * ROW];   // a wave's keys, then values; its sums at the end
+  __shared__ float ml[4][kRowsS][2];
+  const int tid = threadIdx.x, lane = tid & 63, w = uni(tid >> 6);
+  PagedSeq sq;
+  int block;
+  const int seq = find_block(p, blockIdx.z, kRowsS, sq, block), kv = blockIdx.y;
+  if (seq < 0) return;
+  const int r0 = block * kRowsS, total = sq.n * p.g;
+  const PagedSpan span = block_span(p, sq, r0);
+  const int count = uni(span.count()), per = tiles_per_part(count, gridDim.x, per_min), begin = blockIdx.x * per;
+  if (begin >= count && begin > 0) return;   // a row block that sees nothing is written by its first part
+  const int last = begin + per < count ? begin + per : count;
+  const bool whole = count <= per;
+
+  u4 *const kt = buf[w], *const vt = kt + TK * ROW;
+  const int gl = lane / ROW, piece = lane % ROW, mask = (1 << p.shift) - 1;
+  const Base kb = cache_base(p.k, kv), vb = cache_base(p.v, kv);
+  uint32_t koff[D == 128 ? 4 : 2], voff[D == 128 ? 1 : 1];
+#pragma unroll
+  for (int n = 0; n < (D == 128 ? 4 : 2); ++n) koff[n] = gl * kb.slot + 16u * (piece ^ Lay<D>::swz_k(n * GS + gl));
+  voff[0] = gl * vb.slot + 16u * (piece ^ Lay<D>::swz_v(gl));
+  const int32_t* row = p.table + (int64_t)seq * p.ld_table;
+  int base = 0, entries = 0;   // lane x: the table's entry for page number base + x of the sequence
+  bool filled = false;
+  struct {
+    int t0, page[NG], n[NG];
+    uint64_t vm;
+  } nx;   // the tile that is loaded next
+  auto look_up = [&](int i) {
+    nx.t0 = span.tile(i) * TK;
+    const int p0 = nx.t0 >> p.shift;
+    if (!filled || p0 < base || ((nx.t0 + TK - 1) >> p.shift) >= base + 64) {
+      filled = true;
+      base = p0;
+      const int top = (sq.len - 1) >> p.shift;   // a tile of the span begins before sq.len, or a page is not looked at
+      entries = row[base + lane < top ? base + lane : top];
+    }
+    nx.vm = 0;
+#pragma unroll
+    for (int gi = 0; gi < NG; ++gi) {
+      const int j = nx.t0 + gi * GS, id = __builtin_amdgcn_readlane(entries, (j >> p.shift) - base);
+      const bool ok = j < sq.len && (uint32_t)id < (uint32_t)p.pages;
+      nx.page[gi] = ok ? id : 0;
+      nx.n[gi] = ok ? (sq.len - j < GS ? sq.len - j : GS) : 0;
+      nx.vm |= (uint64_t)((1u << nx.n[gi]) - 1) << (gi * GS);
+    }
+  };
+  auto load = [&](const Base& c, const uint32_t* off, int noff, u4* dst) {
+#pragma unroll
+    for (int gi = 0; gi < NG; ++gi)
+      lds_load16(c.at(nx.page[gi], (nx.t0 + gi * GS) & mask), nx.n[gi] * c.slot, off[gi % noff], dst + 64 * gi);
+  };
+  constexpr int KO = D == 128 ? 4 : 2;
+  u4 q[D / 16];
+  const Rows rw = load_rows<D>(p, sq, kv, r0, q);
+  int i = begin + w;
+  if (i < last) look_up(i);
+  have_queries(q);
+  uint64_t vm = nx.vm;
+  if (i < last) {
+    load(kb, koff, KO, kt);
+    load(vb, voff, 1, vt);
+  }
+  Acc<D> ac;
+  ac.clear();
+  Odd<D> odd;
+  odd.clear();
+#pragma unroll 1
+  for (; i < last; i += 4) {
+    // in order: keys i, values i, keys i + 4, values i + 4
+    const int t0 = span.tile(i) * TK;
+    const bool more = i + 4 < last;
+    if (more) look_up(i + 4);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NG) : "memory");
+    auto keys_done = [&] {
+      if (more) load(kb, koff, KO, kt);
+    };
+    auto values_ready = [&] {
+      if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NG) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    };
+    if (vm != 0xFFFFFFFFull || t0 + TK - 1 > rw.first || (p.window > 0 && (int64_t)t0 <= (int64_t)rw.last - p.window))
+      tile<T, D, 1, EXTRA, true>(p, rw, sq, q, ac, odd, kt, vt, t0, vm, keys_done, values_ready);
+    else
+      tile<T, D, 1, EXTRA, false>(p, rw, sq, q, ac, odd, kt, vt, t0, vm, keys_done, values_ready);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the values are read
+    if (more) load(vb, voff, 1, vt);
+    vm = nx.vm;
+  }
+
+  // ---- the four waves' sums meet in LDS: piece d of row r (four outputs) at
+  // [r][d ^ r], so that neither side meets a bank twice ----
+  constexpr int P4 = D / 4;
+  {
+    const int r = lane & 31, h = lane >> 5;
+    const float l = ac.sum();
+    if (h == 0) {
+      ml[w][r][0] = ac.m;
+      ml[w][r][1] = l;
+    }
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        f4 v;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) v[x] = odd.fix(ac.o[db][4 * e + x], 16 * db + 4 * e + x);
+        ((f4*)kt)[r * P4 + ((db * 8 + 2 * e + h) ^ (r & (P4 - 1)))] = v;
+      }
+  }
+  __syncthreads();
+  float* rec = ws + (((int64_t)blockIdx.z * p.KVH + kv) * gridDim.x + blockIdx.x) * record_floats(D, R);
+  const int d4 = tid % P4, rows = total - r0 < kRowsS ? total - r0 : kRowsS;
+  for (int r = tid / P4; r < rows; r += 256 / P4) {
+    float m = ml[0][r][0], l = 0.f;
+#pragma unroll
+    for (int x = 1; x < 4; ++x) m = fmaxf(m, ml[x][r][0]);
+    f4 v = {};
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const float f = __builtin_amdgcn_exp2f(ml[x][r][0] - m);
+      l += ml[x][r][1] * f;
+      v += f * ((const f4*)buf[x])[r * P4 + (d4 ^ (r & (P4 - 1)))];
+    }
+    if (!whole) {
+      *(f4*)(rec + r * D + 4 * d4) = v;
+      if (d4 == 0) {
+        rec[R * D + 2 * r] = m;
+        rec[R * D + 2 * r + 1] = l;
+      }
     } else {
-      item -= uni((int)__shfl(sum, 63));
-      u0 += uni64(__shfl(usum, 63));
+      const int tok = (int)p.gdiv.div(r0 + r), a = kv * p.g + r0 + r - tok * p.g;
+      const int64_t at = (int64_t)(sq.start + tok) * p.H + a;
+      store4<T>(p.out, at * D + 4 * d4, v * inverse(l));
+      if (p.lse && d4 == 0) p.lse[at] = log_sum(m, l);
     }
   }
+}
+
+// Adds up a row block's parts.  SHARES = 1: a thread takes a piece of four
+// outputs of its row through all parts, several rows to a workgroup; else each
+// of SHARES threads takes every SHARES-th part, one row to a workgroup, and the
+// shares are added up in their order.
+template <typename T, int D, int SHARES>
+__global__ __launch_bounds__(SHARES == 1 ? 256 : D / 4 * SHARES) void paged_join_kernel(PagedArgs p, const float* ws, int parts_max,
+                                                                                     int per_min, int R) {
+  constexpr int P4 = D / 4;   // pieces of a row
+  PagedSeq sq;
+  int block;
+  const int seq = find_block(p, blockIdx.z, kRowsS, sq, block), kv = blockIdx.y;
   if (seq < 0) return;
-  split_units(p, sq, &blocks, &span);
-  const int cost = span.count() > 0 ? span.count() : 1;
-  u0 += (int64_t)item * cost;
-  const int64_t u1 = u0 + cost;
-  const int64_t w0 = u0 / per, w1 = (u1 - 1) / per;
-  if (w0 == w1) return;
-  const int r = tid & 31, r0 = item * kRowsS, d4 = blockIdx.y * 8 + (tid >> 5);
-  if (r0 + r >= sq.n * p.g) return;
-  auto record = [&](int64_t w) {   // the workgroup's first segment, but where the block starts inside its run
-    return ws + (2 * w + (w == w0 && w * per != u0 ? 1 : 0)) * record_floats(D);
-  };
-  float m = -3.0e38f;
-  for (int64_t w = w0; w <= w1; ++w) m = fmaxf(m, record(w)[kRowsS * D + 2 * r]);
+  const int r0 = block * kRowsS;
+  const int count = block_span(p, sq, r0).count(), per = tiles_per_part(count, parts_max, per_min);
+  const int parts = (count + per - 1) / per;
+  const int d4 = threadIdx.x % P4, share = SHARES == 1 ? 0 : threadIdx.x / P4;
+  const int r = SHARES == 1 ? blockIdx.x * (256 / P4) + threadIdx.x / P4 : blockIdx.x;
+  if (parts <= 1) return;   // written by its only part
+  const bool have = r < R && r0 + r < sq.n * p.g;
+  if (!have && SHARES == 1) return;
+  const float* base = ws + ((int64_t)blockIdx.z * p.KVH + kv) * parts_max * record_floats(D, R);
+  float m = -3.0e38f, l = 0.f;
   f4 v = {};
-  float l = 0.f;
-#pragma unroll 4
-  for (int64_t w = w0; w <= w1; ++w) {
-    const float* rec = record(w);
-    const float f = __builtin_amdgcn_exp2f(rec[kRowsS * D + 2 * r] - m);
-    l += rec[kRowsS * D + 2 * r + 1] * f;
-    v += f * *(const f4*)(rec + 4 * (d4 * kRowsS + r));
+  auto take = [&](float m1, float l1, f4 v1) {
+    const float m2 = fmaxf(m, m1), f = __builtin_amdgcn_exp2f(m - m2), f1 = __builtin_amdgcn_exp2f(m1 - m2);
+    m = m2;
+    l = l * f + l1 * f1;
+    v = v * f + v1 * f1;
+  };
+  if (have) {
+#pragma unroll 8
+    for (int x = share; x < parts; x += SHARES) {
+      const float* rec = base + (int64_t)x * record_floats(D, R);
+      take(rec[R * D + 2 * r], rec[R * D + 2 * r + 1], *(const f4*)(rec + r * D + 4 * d4));
+    }
+  }
+  if constexpr (SHARES > 1) {
+    __shared__ f4 part[SHARES][P4];
+    __shared__ float pm[SHARES], pl[SHARES];
+    part[share][d4] = v;
+    if (d4 == 0) {
+      pm[share] = m;
+      pl[share] = l;
+    }
+    __syncthreads();
+    if (share || !have) return;
+    for (int x = 1; x < SHARES; ++x) take(pm[x], pl[x], part[x][d4]);
   }
   const int tok = (int)p.gdiv.div(r0 + r), a = kv * p.g + r0 + r - tok * p.g;
   const int64_t at = (int64_t)(sq.start + tok) * p.H + a;
@@ -881,7 +884,31 @@ int64_t row_blocks(const PagedArgs& a, int rows) {   // at most, over all sequen
   return ((int64_t)a.rows * a.g + rows - 1) / rows + (a.cu ? a.b : (int64_t)a.rows * ((a.g + rows - 1) / rows));
 }
 bool many_rows(const PagedArgs& a, int num_cus) {
-  return ((int64_t)a.rows * a.g / kRowsP) * a.KVH >= num_cus;
+  return ((int64_t)a.rows * a.g / 128) * a.KVH >= num_cus;
+}
+
+// The parts of a few-row call: as many for every row block, for sequences as
+// long as the table (or the window) can hold; so many that the longest sequence
+// of a ragged batch does not decide when the call ends, but of at least per_min
+// tiles, more where there are row blocks enough to fill the chip.
+struct SplitPlan {
+  int64_t blocks, parts;
+  int per_min, R;
+  size_t ws_bytes;
+};
+SplitPlan split_plan(const PagedArgs& a, int num_cus) {
+  SplitPlan s;
+  s.blocks = row_blocks(a, kRowsS);
+  int64_t slots = a.cap;
+  if (a.window > 0 && !a.prefix) slots = std::min<int64_t>(slots, (int64_t)a.window + kRowsS + 2 * kTileS);
+  const int64_t tiles = (slots + kTileS - 1) / kTileS, lanes = std::max<int64_t>(s.blocks * a.KVH, 1);
+  s.per_min = lanes >= num_cus ? 16 : (4 * lanes >= num_cus ? 8 : 4);
+  const int64_t want = std::max<int64_t>(1, (lanes >= num_cus ? 16 : 8) * (int64_t)num_cus / lanes);   // parts per row block and head
+  s.parts = std::max<int64_t>(1, std::min(want, (tiles + s.per_min - 1) / s.per_min));
+  const int64_t most = std::min<int64_t>(kRowsS, (a.cu ? (int64_t)a.rows : 1) * a.g);
+  s.R = (int)((most + 7) / 8 * 8);
+  s.ws_bytes = s.parts > 1 ? (size_t)(s.blocks * a.KVH * s.parts) * record_floats(a.D, s.R) * sizeof(float) : 0;
+  return s;
 }
 
 template <typename T, int D>
@@ -893,18 +920,22 @@ hipError_t launch(const PagedArgs& a, int num_cus, void* ws, hipStream_t s) {
     else paged_rows_kernel<T, D, false><<<(int)grid, 512, 0, s>>>(a);
     return hipGetLastError();
   }
-  if (a.extra()) paged_split_kernel<T, D, true><<<num_cus, 256, 0, s>>>(a, (float*)ws, num_cus);
-  else paged_split_kernel<T, D, false><<<num_cus, 256, 0, s>>>(a, (float*)ws, num_cus);
-  const int64_t grid = row_blocks(a, kRowsS) * a.KVH;
-  if (grid > 0x7fffffff) return hipErrorInvalidValue;
-  paged_join_kernel<T, D><<<dim3((int)grid, D / 32), 256, 0, s>>>(a, (const float*)ws, num_cus);
+  const SplitPlan sp = split_plan(a, num_cus);
+  if (sp.blocks > 65535 || a.KVH > 65535) return hipErrorInvalidValue;
+  const dim3 grid((unsigned)sp.parts, a.KVH, (unsigned)sp.blocks);
+  if (a.extra()) paged_split_kernel<T, D, true><<<grid, 256, 0, s>>>(a, (float*)ws, sp.per_min, sp.R);
+  else paged_split_kernel<T, D, false><<<grid, 256, 0, s>>>(a, (float*)ws, sp.per_min, sp.R);
+  if (sp.parts > 16)
+    paged_join_kernel<T, D, 16><<<dim3(sp.R, a.KVH, (unsigned)sp.blocks), D / 4 * 16, 0, s>>>(a, (const float*)ws, (int)sp.parts, sp.per_min, sp.R);
+  else if (sp.parts > 1)
+    paged_join_kernel<T, D, 1><<<dim3((sp.R + 1024 / D - 1) / (1024 / D), a.KVH, (unsigned)sp.blocks), 256, 0, s>>>(a, (const float*)ws, (int)sp.parts, sp.per_min, sp.R);
   return hipGetLastError();
 }
 
 }  // namespace
 
 size_t pattn_workspace(const PagedArgs& a, int num_cus) {
-  return many_rows(a, num_cus) ? 0 : (size_t)2 * num_cus * record_floats(a.D) * sizeof(float);
+  return many_rows(a, num_cus) ? 0 : split_plan(a, num_cus).ws_bytes;
 }
 
 hipError_t pattn_launch(const PagedArgs& a, int num_cus, void* ws, hipStream_t s) {
