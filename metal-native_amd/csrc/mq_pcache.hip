@@ -115,11 +115,15 @@ __device__ __forceinline__ uint32_t order_key(float v) {   // NaN above all, -0 
 struct EvictShared {
   uint32_t hist[4][2048];
   int list[kEvictList];
-  int gt[kEvictWaves], eq[kEvictWaves];
+  uint32_t count[32 * kEvictWaves];   // per 1024 slots and wave: above the threshold | equal to it << 16
+  uint32_t wave_sum[kEvictWaves];
   uint32_t digit;
   int above, zeros;
 };
 
+// E: weights per thread, kept in registers from the first look to the last (a
+// head of at most 1024 E slots); 0: any number, read again each time.
+template <int E>
 __global__ __launch_bounds__(kEvictThreads) void paged_evict_kernel(PagedEvictArgs p, int parts, int per) {
   __shared__ EvictShared sh;
   const int tid = threadIdx.x, lane = tid & 63, w = uni(tid >> 6);
@@ -134,54 +138,73 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_kernel(PagedEvictAr
   const int from_old = cut ? p.budget - (len - old) : 0;   // how many of the old slots stay
 
   if (cut && from_old > 0 && r_begin < from_old) {
+    constexpr uint32_t kZero = 0x80000000u;
+    constexpr int N = E > 0 ? E : 1;
+    uint32_t key[N];
+    if constexpr (E > 0) {
+      float m[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) m[i] = tid + i * kEvictThreads < old ? mass[tid + i * kEvictThreads] : 0.f;
+#pragma unroll
+      for (int i = 0; i < N; ++i) key[i] = order_key(m[i]);
+    }
+    auto each = [&](auto&& f) {   // f(slot, key) of the thread's slots
+      if constexpr (E > 0) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (tid + i * kEvictThreads < old) f(tid + i * kEvictThreads, key[i]);
+      } else {
+#pragma unroll 4
+        for (int j = tid; j < old; j += kEvictThreads) f(j, order_key(mass[j]));
+      }
+    };
     uint32_t prefix = 0, done = 0;   // digits found so far, and their bits
     int need = from_old;             // how many stay among the slots that match them
-    constexpr uint32_t kZero = 0x80000000u;
 #pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
       const int bits = pass == 2 ? 10 : 11, shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
-      for (int i = tid; i < 4 * 2048; i += kEvictThreads) (&sh.hist[0][0])[i] = 0;
+      for (int i = tid; i < 4 * 2048 / 4; i += kEvictThreads) ((u4*)&sh.hist[0][0])[i] = (u4){0u, 0u, 0u, 0u};
       if (tid == 0) sh.zeros = 0;
       __syncthreads();
       int zeros = 0;
       // weights that are exactly zero are many: counted apart, not one by one in one histogram cell
-#pragma unroll 4
-      for (int j = tid; j < old; j += kEvictThreads) {
-        const uint32_t k = order_key(mass[j]);
+      each([&](int, uint32_t k) {
         if (k == kZero) ++zeros;
         else if ((k & done) == prefix) atomicAdd(&sh.hist[w & 3][(k >> shift) & ((1u << bits) - 1)], 1u);
-      }
+      });
       if ((kZero & done) == prefix) {
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) zeros += __shfl_xor(zeros, o);
-        if (lane == 0) atomicAdd(&sh.zeros, zeros);
+        if (lane == 0 && zeros) atomicAdd(&sh.zeros, zeros);
       }
       __syncthreads();
-      if (w == 0) {   // lane l: cells 32 l .. 32 l + 31, from the top
-        if (lane == 0) sh.hist[0][(kZero >> shift) & ((1u << bits) - 1)] += sh.zeros;
-        const int per_lane = (1 << bits) / 64, top = (1 << bits) - 1 - lane * per_lane;
-        int mine = 0;
-        for (int i = 0; i < per_lane; ++i)
-          mine += sh.hist[0][top - i] + sh.hist[1][top - i] + sh.hist[2][top - i] + sh.hist[3][top - i];
-        int sum = mine;
+      // thread t: cells top - 2 t and top - 2 t - 1, summed from the top
+      const int top = (1 << bits) - 1 - 2 * tid, zc = (kZero >> shift) & ((1u << bits) - 1);
+      int c0 = 0, c1 = 0;
+      if (top > 0) {
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-          const int x = __shfl_up(sum, o);
-          if (lane >= o) sum += x;
+        for (int x = 0; x < 4; ++x) {
+          const uint2 h2v = *(const uint2*)&sh.hist[x][top - 1];
+          c1 += h2v.x;
+          c0 += h2v.y;
         }
-        const uint64_t past = __ballot(sum >= need);
-        if (past && lane == __ffsll((unsigned long long)past) - 1) {
-          int before = sum - mine;
-          for (int i = 0; i < per_lane; ++i) {
-            const int x = sh.hist[0][top - i] + sh.hist[1][top - i] + sh.hist[2][top - i] + sh.hist[3][top - i];
-            if (before + x >= need) {
-              sh.digit = (uint32_t)(top - i);
-              sh.above = before;
-              break;
-            }
-            before += x;
-          }
-        }
+        if (zc == top) c0 += sh.zeros;
+        if (zc == top - 1) c1 += sh.zeros;
+      }
+      int sum = c0 + c1;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int x = __shfl_up(sum, o);
+        if (lane >= o) sum += x;
+      }
+      if (lane == 63) sh.wave_sum[w] = sum;
+      __syncthreads();
+      int before = sum - c0 - c1;
+      for (int x = 0; x < w; ++x) before += sh.wave_sum[x];
+      if (before < need && before + c0 + c1 >= need) {
+        const bool first = before + c0 >= need;
+        sh.digit = (uint32_t)(first ? top : top - 1);
+        sh.above = first ? before : before + c0;
       }
       __syncthreads();
       prefix |= sh.digit << shift;
@@ -189,37 +212,76 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_kernel(PagedEvictAr
       need -= sh.above;
       __syncthreads();
     }
-    // waves take contiguous runs of slots; selected: key > prefix, and the first `need` of key == prefix
-    const int run = ((old + kEvictWaves - 1) / kEvictWaves + 63) & ~63;
-    const int a = min(w * run, old), b = min(a + run, old);
-    int gt = 0, eq = 0;
-#pragma unroll 4
-    for (int j = a; j < b; j += 64) {
-      const uint32_t k = j + lane < b ? order_key(mass[j + lane]) : 0u;   // 0: below every key but a NaN's of other sign
-      gt += __popcll(__ballot(j + lane < b && k > prefix));
-      eq += __popcll(__ballot(j + lane < b && k == prefix));
-    }
-    if (lane == 0) {
-      sh.gt[w] = gt;
-      sh.eq[w] = eq;
-    }
-    __syncthreads();
-    gt = eq = 0;
-    for (int x = 0; x < w; ++x) {
-      gt += sh.gt[x];
-      eq += sh.eq[x];
-    }
+    // stays: key > prefix, and the first `need` of key == prefix
     const uint64_t below = (1ull << lane) - 1;
+    if constexpr (E > 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const bool in = tid + i * kEvictThreads < old;
+        const uint64_t mg = __ballot(in && key[i] > prefix), me = __ballot(in && key[i] == prefix);
+        if (lane == 0) sh.count[i * kEvictWaves + w] = (uint32_t)__popcll(mg) | (uint32_t)__popcll(me) << 16;
+      }
+      __syncthreads();
+      if (w == 0) {   // sums of all before, in the slots' order (both fields at most 1024 E <= 32768)
+        constexpr int C = N * kEvictWaves / 64 > 0 ? N * kEvictWaves / 64 : 1;
+        uint32_t mine = 0;
+        for (int x = 0; x < C; ++x) mine += lane * C + x < N * kEvictWaves ? sh.count[lane * C + x] : 0u;
+        uint32_t sum = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+          const uint32_t x = __shfl_up(sum, o);
+          if (lane >= o) sum += x;
+        }
+        uint32_t before = sum - mine;
+        for (int x = 0; x < C; ++x)
+          if (lane * C + x < N * kEvictWaves) {
+            const uint32_t c = sh.count[lane * C + x];
+            sh.count[lane * C + x] = before;
+            before += c;
+          }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int j = tid + i * kEvictThreads;
+        const bool in = j < old, gt = in && key[i] > prefix, eq = in && key[i] == prefix;
+        const uint64_t mg = __ballot(gt), me = __ballot(eq);
+        const uint32_t c = sh.count[i * kEvictWaves + w];
+        const int e = (int)(c >> 16) + __popcll(me & below), r = (int)(c & 0xFFFFu) + __popcll(mg & below) + min(e, need);
+        if ((gt || (eq && e < need)) && r >= r_begin && r < r_end) sh.list[r - r_begin] = j;
+      }
+    } else {
+      // waves take contiguous runs of slots
+      const int run = ((old + kEvictWaves - 1) / kEvictWaves + 63) & ~63;
+      const int a = min(w * run, old), b = min(a + run, old);
+      int gt = 0, eq = 0;
 #pragma unroll 4
-    for (int j = a; j < b; j += 64) {
-      const bool in = j + lane < b;
-      const uint32_t k = in ? order_key(mass[j + lane]) : 0u;
-      const uint64_t mg = __ballot(in && k > prefix), me = __ballot(in && k == prefix);
-      const int e = eq + __popcll(me & below), r = gt + __popcll(mg & below) + min(e, need);
-      const bool sel = in && (k > prefix || (k == prefix && e < need));
-      if (sel && r >= r_begin && r < r_end) sh.list[r - r_begin] = j + lane;
-      gt += __popcll(mg);
-      eq += __popcll(me);
+      for (int j = a; j < b; j += 64) {
+        const uint32_t k = j + lane < b ? order_key(mass[j + lane]) : 0u;
+        gt += __popcll(__ballot(j + lane < b && k > prefix));
+        eq += __popcll(__ballot(j + lane < b && k == prefix));
+      }
+      if (lane == 0) {
+        sh.count[w] = gt;
+        sh.count[kEvictWaves + w] = eq;
+      }
+      __syncthreads();
+      gt = eq = 0;
+      for (int x = 0; x < w; ++x) {
+        gt += sh.count[x];
+        eq += sh.count[kEvictWaves + x];
+      }
+#pragma unroll 4
+      for (int j = a; j < b; j += 64) {
+        const bool in = j + lane < b;
+        const uint32_t k = in ? order_key(mass[j + lane]) : 0u;
+        const uint64_t mg = __ballot(in && k > prefix), me = __ballot(in && k == prefix);
+        const int e = eq + __popcll(me & below), r = gt + __popcll(mg & below) + min(e, need);
+        const bool sel = in && (k > prefix || (k == prefix && e < need));
+        if (sel && r >= r_begin && r < r_end) sh.list[r - r_begin] = j + lane;
+        gt += __popcll(mg);
+        eq += __popcll(me);
+      }
     }
     __syncthreads();
   }
@@ -278,7 +340,10 @@ hipError_t pevict_launch(const PagedEvictArgs& a, int num_cus, hipStream_t s) {
   if (parts < 1) parts = 1;
   const int per = (int)((a.budget + parts - 1) / parts);
   if (rows * parts > 0x7fffffff) return hipErrorInvalidValue;
-  paged_evict_kernel<<<(int)(rows * parts), kEvictThreads, 0, s>>>(a, (int)parts, per);
+  const int grid = (int)(rows * parts);
+  if (a.cap <= 4 * kEvictThreads) paged_evict_kernel<4><<<grid, kEvictThreads, 0, s>>>(a, (int)parts, per);
+  else if (a.cap <= 32 * kEvictThreads) paged_evict_kernel<32><<<grid, kEvictThreads, 0, s>>>(a, (int)parts, per);
+  else paged_evict_kernel<0><<<grid, kEvictThreads, 0, s>>>(a, (int)parts, per);
   return hipGetLastError();
 }
 
