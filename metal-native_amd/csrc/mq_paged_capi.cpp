@@ -105,7 +105,7 @@ const char* query(mq::PagedArgs& a, const void* q, int64_t q_token, int64_t q_he
   if (!aligned16(q) || q_token % 8 || q_head % 8 || q_token < 0 || q_head < 0)
     return "queries must be 16-byte aligned, their strides multiples of 8";
   // a block of rows is addressed by 32-bit offsets from its first token
-  if (66 * q_token + a.g * q_head + a.D > (int64_t)1 << 29) return "strides of the queries out of range";
+  if (66 * q_token + a.g * q_head + a.D > (int64_t)1 << 29 || a.g > 1 << 16) return "strides of the queries out of range";
   a.q = q;
   a.q_t = q_token;
   a.q_h = (int)q_head;

@@ -98,7 +98,7 @@ __device__ __forceinline__ desc_t make_desc(const void* base, uint32_t bytes) {
   return (desc_t){(uint32_t)uni((int)a), (uint32_t)uni((int)(a >> 32)) & 0xffffu, (uint32_t)uni((int)bytes), 0x00020000u};
 }
 template <bool FRESH> __device__ __forceinline__ void lds_load16(desc_t r, uint32_t voff, void* lds) {
-  const uint32_t l = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds;
+  const uint32_t l = (uint32_t)uni((int)(uintptr_t)(__attribute__((address_space(3))) void*)lds);
   if constexpr (FRESH)
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(l), "v"(voff), "s"(r) : "memory");
   else
