@@ -254,7 +254,10 @@ MQ_API int mq_argmax_embed_f16(const void* logits, int64_t vocab, const void* em
  *
  * k, v: [pages, kv_heads, page_size, head_dim], fp16 or bf16, unit stride along
  * head_dim, the other strides (elements) multiples of 8, 16-byte aligned;
- * page_size a power of two from 8, head_dim 64 or 128.  Sequence s keeps slot j
+ * page_size a power of two from 8 to 65536, head_dim 64 or 128.  A page's stride
+ * is below 2^31 elements, a head's slots of one page span less than that; kv_heads
+ * and batch are at most 65535, heads to a kv_head 65536, width * page_size and
+ * rows * heads below 2^31.  Sequence s keeps slot j
  * (its token at position j) in page table[s * ld_table + j / page_size].  lens[s]
  * is the number of its slots, those of the tokens of this call among them.
  *

@@ -151,7 +151,6 @@ struct PagedEvictArgs {
   const int32_t* lens;
   const float* mass;      // [b, KVH, slots], strides
   int64_t mass_b, mass_h;
-  int slots;
   const int32_t* to;      // [b, to_width]
   int64_t ld_to;
   int to_width, budget, recent;

@@ -26,10 +26,10 @@ const char* bad_cache(const mq_paged_cache* c, bool with_v) {
   if (c->dtype != MQ_PAGED_F16 && c->dtype != MQ_PAGED_BF16) return "unknown dtype";
   if (c->page_size < 8 || c->page_size > 65536 || (c->page_size & (c->page_size - 1)))
     return "page_size must be a power of two from 8 to 65536";
-  if (c->kv_heads < 1 || c->pages < 1 || c->pages > INT_MAX || c->batch < 1 || c->batch > 65535 || c->width < 1)
-    return "kv_heads, pages, batch (at most 65535) and the table's width must be positive";
+  if (c->kv_heads < 1 || c->kv_heads > 65535 || c->pages < 1 || c->pages > INT_MAX || c->batch < 1 || c->batch > 65535 || c->width < 1)
+    return "kv_heads and batch (at most 65535 each), pages and the table's width must be positive";
   if (c->width > INT_MAX / c->page_size) return "the table names 2^31 slots or more";
-  if (c->width > 1 && c->batch > 1 && c->ld_table < c->width) return "the table's rows overlap";
+  if (c->batch > 1 && (c->ld_table < 0 || (c->width > 1 && c->ld_table < c->width))) return "the table's rows overlap";
   for (int i = 0; i < (with_v ? 2 : 1); ++i) {
     const int64_t page = i ? c->v_page : c->k_page, head = i ? c->v_head : c->k_head, slot = i ? c->v_slot : c->k_slot;
     if (!aligned16(i ? c->v : c->k) || page % 8 || head % 8 || slot % 8) return "the cache must be 16-byte aligned, its strides multiples of 8";
@@ -75,7 +75,7 @@ const char* attn_args(mq::PagedArgs& a, const mq_paged_cache* c, const mq_paged_
   if (const char* bad = bad_cache(c, with_v)) return bad;
   if (!m) return "null mask";
   if (rows < 0 || heads < 1 || heads % c->kv_heads) return "heads must be a multiple of kv_heads";
-  if (rows * (int64_t)heads > INT_MAX) return "rows * heads must be below 2^31";
+  if (rows > INT_MAX || rows * (int64_t)heads > INT_MAX) return "rows * heads must be below 2^31";
   if (!(m->scale > 0.f) || !std::isfinite(m->scale)) return "scale must be positive and finite";
   if (!(m->softcap >= 0.f) || !std::isfinite(m->softcap)) return "softcap must be zero or positive, and finite";
   if (m->window < 0) return "window must not be negative";
@@ -105,7 +105,8 @@ const char* query(mq::PagedArgs& a, const void* q, int64_t q_token, int64_t q_he
   if (!aligned16(q) || q_token % 8 || q_head % 8 || q_token < 0 || q_head < 0)
     return "queries must be 16-byte aligned, their strides multiples of 8";
   // a block of rows is addressed by 32-bit offsets from its first token
-  if (66 * q_token + a.g * q_head + a.D > (int64_t)1 << 29 || a.g > 1 << 16) return "strides of the queries out of range";
+  const int64_t most = (int64_t)1 << 29;
+  if (q_token > most || q_head > most || a.g > 1 << 16 || 66 * q_token + a.g * q_head + a.D > most) return "strides of the queries out of range";
   a.q = q;
   a.q_t = q_token;
   a.q_h = (int)q_head;
@@ -129,9 +130,10 @@ MQ_API int mq_paged_rope_kv(const mq_paged_cache* c, const void* qkv, int64_t ld
   if (!cu_q && rows != c->batch) return refuse(op, "without cu_q there must be one row per sequence");
   if (!aligned16(qkv) || ld_qkv % 8 || (rows > 1 && ld_qkv < cols) || !aligned16(q_out))
     return refuse(op, "qkv rows must be 16-byte aligned");
-  if (table_rows < 1 || !aligned16(cos_t) || !aligned16(sin_t) || ld_cos % 4 || ld_sin % 4)
+  if (table_rows < 1 || !aligned16(cos_t) || !aligned16(sin_t) || ld_cos % 4 || ld_sin % 4 || ld_cos < 0 || ld_sin < 0)
     return refuse(op, "rotary tables must be 16-byte aligned and not empty");
   if (axes < 1 || axes > 8) return refuse(op, "one to eight axes");
+  if (axes > 1 && ld_pos < 0) return refuse(op, "stride of the positions out of range");
   mq::PagedRopeArgs a{};
   int end = 0;
   for (int i = 0; i < 8; ++i) {
@@ -230,13 +232,12 @@ MQ_API int mq_paged_evict(const mq_paged_cache* c, const float* mass, int64_t ma
   if (budget < 1 || budget > INT_MAX || recent < 0 || recent > budget) return refuse(op, "recent must be 0 .. budget, budget positive");
   if (to_width < 1 || to_width > INT_MAX / c->page_size || to_width * c->page_size < budget)
     return refuse(op, "the target pages must hold the budget");
-  if (mass_batch < 0 || mass_head < 0) return refuse(op, "strides of mass out of range");
+  if (mass_batch < 0 || mass_head < 0 || (c->batch > 1 && ld_to < to_width)) return refuse(op, "strides of mass or of the targets out of range");
   mq::PagedEvictArgs a{};
   fill_cache(a, c);
   a.mass = mass;
   a.mass_b = mass_batch;
   a.mass_h = mass_head;
-  a.slots = a.cap;
   a.to = to;
   a.ld_to = ld_to;
   a.to_width = (int)to_width;

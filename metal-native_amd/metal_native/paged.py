@@ -34,11 +34,11 @@ from .ops import _check, _invalid, _mq_torch, _raw_stream, _require_cuda
 __all__ = ["rope_kv", "attention", "attention_mass", "evict"]
 
 
-def _cache(op, k, v, table, lens):
+def _cache(op, k, v, table, lens, keys_only=False):
     """Raises for what no kernel takes; returns table and lens as the kernels
     read them.  The caches themselves are never copied."""
     for t, what in ((k, "k_cache"), (v, "v_cache"), (table, "table"), (lens, "lens")):
-        if t is None and what == "v_cache":
+        if keys_only and what == "v_cache":
             continue
         _require_cuda(t, what, op)
         if t.device != k.device:
@@ -106,7 +106,6 @@ def rope_kv(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: torch.
                                     _raw_stream(qkv.get_device()))
         if r is not None:
             return _finish(op, r)
-    _require_cuda(k_cache, "k_cache", op)
     table, lens = _cache(op, k_cache, v_cache, table, lens)
     kvh, d = k_cache.shape[1], k_cache.shape[3]
     for t, what in ((qkv, "qkv"), (cos, "cos"), (sin, "sin"), (pos, "pos")):
@@ -172,7 +171,7 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, tab
     """
     op = "paged.attention"
     if scale is None:
-        scale = k_cache.shape[-1] ** -0.5
+        scale = q.shape[-1] ** -0.5 if isinstance(q, torch.Tensor) and q.dim() and q.shape[-1] else 1.0
     if max_q is None:
         max_q = 0
     if type(q) is torch.Tensor and q.is_cuda:
@@ -180,7 +179,6 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, tab
                                       max_q, return_lse, _raw_stream(q.get_device()))
         if r is not None:
             return _finish(op, r)
-    _require_cuda(k_cache, "k_cache", op)
     table, lens = _cache(op, k_cache, v_cache, table, lens)
     q, *how = _mask(op, q, k_cache, table, cu, scale, softcap, slopes, window, prefix_lens, max_q)
     with torch.cuda.device(q.device):
@@ -202,7 +200,7 @@ def attention_mass(q: torch.Tensor, k_cache: torch.Tensor, table: torch.Tensor, 
     """
     op = "paged.attention_mass"
     if scale is None:
-        scale = k_cache.shape[-1] ** -0.5
+        scale = q.shape[-1] ** -0.5 if isinstance(q, torch.Tensor) and q.dim() and q.shape[-1] else 1.0
     if max_q is None:
         max_q = 0
     if type(q) is torch.Tensor and q.is_cuda:
@@ -210,8 +208,7 @@ def attention_mass(q: torch.Tensor, k_cache: torch.Tensor, table: torch.Tensor, 
                                            max_q, _raw_stream(q.get_device()))
         if r is not None:
             return _finish(op, r)
-    _require_cuda(k_cache, "k_cache", op)
-    table, lens = _cache(op, k_cache, None, table, lens)
+    table, lens = _cache(op, k_cache, None, table, lens, keys_only=True)
     q, *how = _mask(op, q, k_cache, table, cu, scale, softcap, slopes, window, prefix_lens, max_q)
     _require_cuda(lse, "lse", op)
     if lse.dtype != torch.float32 or tuple(lse.shape) != tuple(q.shape[:2]) or lse.device != q.device:
@@ -244,7 +241,6 @@ def evict(k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor, len
                                   _raw_stream(k_cache.get_device()))
         if r is not None:
             return _finish(op, r)
-    _require_cuda(k_cache, "k_cache", op)
     table, lens = _cache(op, k_cache, v_cache, table, lens)
     b, kvh, ps = table.shape[0], k_cache.shape[1], k_cache.shape[2]
     for t, what in ((mass, "mass"), (to, "to")):

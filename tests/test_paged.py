@@ -429,3 +429,44 @@ def test_graph_of_a_step(gpu):
         torch.cuda.synchronize()
         for a, b in zip(got, want):
             assert torch.equal(a, b) or bool(((a == b) | (torch.isnan(a) & torch.isnan(b))).all())
+
+
+def test_many_sequences(gpu):
+    """Chunks found among more sequences than a wavefront has lanes, some of no tokens."""
+    n = 150
+    new = [(7 * i) % 5 for i in range(n)]
+    lens = [x + (11 * i) % 40 for i, x in enumerate(new)]
+    check_mass(build(gpu, torch.float16, 6, 2, 64, 8, lens, new, seed=12), max_q=4)
+    check_attention(build(gpu, torch.bfloat16, 28, 4, 128, 16, lens, new, seed=13))
+    check_attention(build(gpu, torch.float16, 32, 8, 128, 16, [x + 20 for x in lens] * 7, seed=14))   # single tokens
+
+
+@pytest.mark.parametrize("ps", [8, 64, 128])
+def test_many_rows_of_other_pages_and_masks(gpu, ps):
+    c = build(gpu, torch.float16, 32, 8, 64, ps, [900, 640, 129], [700, 500, 129], seed=ps)
+    check_attention(c)
+    pre = torch.tensor([65, 200, 0], dtype=torch.int32, device=gpu)   # a gap between the prefix and the window
+    check_attention(c, window=70, prefix=pre)
+    check_attention(c, window=1)
+
+
+@pytest.mark.parametrize("max_q", [1, 2, 64])
+def test_a_longest_chunk_that_is_understated(gpu, max_q):
+    check_mass(build(gpu, torch.float16, 14, 2, 64, 16, [400, 65], [300, 65], seed=15), max_q=max_q)
+
+
+def test_a_table_far_wider_than_the_sequences(gpu):
+    c = build(gpu, torch.float16, 8, 2, 64, 16, [700, 0, 33], seed=16, width=5000)
+    check_mass(c)
+    check_mass(c, window=40)
+    c = build(gpu, torch.float16, 8, 2, 64, 16, [700, 0, 33], [50, 0, 33], seed=17, width=5000)
+    check_mass(c)
+
+
+@pytest.mark.parametrize("lens,width", [([9000, 20, 5001], 80), ([40000, 3, 33000], None), ([700, 0, 90], 500)])
+@pytest.mark.parametrize("budget,recent", [(3000, 64), (64, 0)])
+def test_evict_from_long_tables(gpu, lens, width, budget, recent):
+    """Tables of 10240, 40064 and 64000 slots: weights kept in registers, and read again each time."""
+    c = build(gpu, torch.bfloat16, 4, 1, 64, 128, lens, seed=18, extra=3 * 24, width=width, junk=2.0)
+    u = torch.rand(3, 1, c["table"].shape[1] * 128, device=gpu, generator=c["gen"])
+    check_evict(c, torch.where(u < 0.3, torch.zeros_like(u), (40 * u).floor() + u * (u > 0.7)), budget, recent, 1, 128, lens)
