@@ -881,10 +881,14 @@ __global__ __launch_bounds__(SHARES == 1 ? 256 : D / 4 * SHARES) void paged_join
 }
 
 int64_t row_blocks(const PagedArgs& a, int rows) {   // at most, over all sequences
-  return ((int64_t)a.rows * a.g + rows - 1) / rows + (a.cu ? a.b : (int64_t)a.rows * ((a.g + rows - 1) / rows));
+  return a.cu ? ((int64_t)a.rows * a.g + rows - 1) / rows + a.b : (int64_t)a.rows * ((a.g + rows - 1) / rows);
 }
+// Rows past each sequence's first token that fill the chip by themselves.  Single
+// tokens never count, however many sequences there are: a block of 256 rows would
+// hold the g rows of one (1280 tokens of 32 heads over 8, 500 slots: 1150 us, in
+// blocks of 32 rows 440; 4096 of 28 over 4, 130 slots: 1945 and 315).
 bool many_rows(const PagedArgs& a, int num_cus) {
-  return ((int64_t)a.rows * a.g / 128) * a.KVH >= num_cus;
+  return ((int64_t)(a.rows - a.b) * a.g / 128) * a.KVH >= num_cus || row_blocks(a, kRowsS) > 65535;   // the grid's z
 }
 
 // The parts of a few-row call: as many for every row block, for sequences as
@@ -921,7 +925,6 @@ hipError_t launch(const PagedArgs& a, int num_cus, void* ws, hipStream_t s) {
     return hipGetLastError();
   }
   const SplitPlan sp = split_plan(a, num_cus);
-  if (sp.blocks > 65535 || a.KVH > 65535) return hipErrorInvalidValue;
   const dim3 grid((unsigned)sp.parts, a.KVH, (unsigned)sp.blocks);
   if (a.extra()) paged_split_kernel<T, D, true><<<grid, 256, 0, s>>>(a, (float*)ws, sp.per_min, sp.R);
   else paged_split_kernel<T, D, false><<<grid, 256, 0, s>>>(a, (float*)ws, sp.per_min, sp.R);

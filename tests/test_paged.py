@@ -470,3 +470,19 @@ def test_evict_from_long_tables(gpu, lens, width, budget, recent):
     c = build(gpu, torch.bfloat16, 4, 1, 64, 128, lens, seed=18, extra=3 * 24, width=width, junk=2.0)
     u = torch.rand(3, 1, c["table"].shape[1] * 128, device=gpu, generator=c["gen"])
     check_evict(c, torch.where(u < 0.3, torch.zeros_like(u), (40 * u).floor() + u * (u > 0.7)), budget, recent, 1, 128, lens)
+
+
+def test_single_tokens_of_very_many_sequences(gpu):
+    """More row blocks than a grid holds along z, and many rows that are all single tokens."""
+    from metal_native import paged
+
+    for n, H, KVH in ((1500, 32, 8), (40000, 64, 1)):
+        c = build(gpu, torch.float16, H, KVH, 64, 8, [3, 17, 40], seed=n)
+        rows = torch.arange(n, device=gpu) % 3
+        q = torch.randn(3, H, 64, device=gpu).half()
+        table, lens = c["table"][rows], c["lens"][rows]
+        out, lse = paged.attention(q[rows], c["k"], c["v"], table, lens, return_lse=True)
+        o, l, ob, lb = ref.attention(q, c["k"], c["v"], c["table"], c["lens"], scale=0.125)
+        at = rows.cpu()
+        assert bool(((out.double().cpu() - o[at]).abs() <= ob[at]).all())
+        assert bool(((lse.double().cpu() - l[at]).abs() <= lb[at]).all())
