@@ -7,10 +7,11 @@
 //   out = sum_j exp(x_j) v_j / sum_j exp(x_j),   lse = log sum_j exp(x_j)
 // in one pass over the slots: with a reference M, the sums of exp2(x_j - M)
 // v_j and exp2(x_j - M) (x in units of log 2) are multiplied by exp2(M - M')
-// where M moves to M'.  M moves only when a score passes it by kAbove: then to
-// kBelow under the row's largest score, so that weights reach from 2^15 down,
-// far enough into fp16's range that 2^17 weights which round to zero together
-// stay below an output's rounding step.  Weights are rounded to the cache's type for
+// where M moves to M'.  M moves only where weights would grow past 2^15 (few
+// rows: a score more than kAbove over it; many rows: a lane's weights of a tile
+// that add up to more): then to kBelow under the row's largest score, so that
+// weights reach from 2^15 down, far enough into fp16's range that 2^17 weights
+// which round to zero together stay below an output's rounding step.  Weights are rounded to the cache's type for
 // the product with v (the matrix instruction takes no other); their sum, the
 // output's sum and M are fp32.
 //
@@ -156,8 +157,7 @@ template <int D> struct Odd {
 // set where it exists.  MASKED: some row may not see some slot of it.
 //
 // One wave's instructions issue in order, so both products read their LDS
-// operands a few instructions ahead (kf, vf): with a wait for LDS before each
-// step the 4096-token chunk behind 28672 slots took 2.0 ms.
+// operands a few instructions ahead (kf, vf).
 // keys_done() follows the last read of the keys, values_ready() comes before the
 // first read of the values.
 template <typename T, int D, int NB, bool EXTRA, bool MASKED, typename F, typename G>
@@ -327,6 +327,14 @@ __device__ __forceinline__ float log_sum(float m, float l) {
 // wave asks for its eight slots of tile t + 3 among its products of tile t, whose
 // issue slots are free (beside the softmax the loads' address arithmetic took 230
 // of 1900 cycles), and waits for them before its products of tile t + 2.
+//
+// 4096 tokens of 28 heads over 4, 128 wide, fp16, behind 28672 slots: 1.63-1.71 ms,
+// 1.05-1.11 PFLOP/s where a large matrix product reaches 1.35.  On the way: four
+// waves of 32 rows with two tiles in flight 2.30 ms; eight in two groups 1.79;
+// no maximum beforehand 1.69; three tiles ahead 1.63.  What bounds it then is the
+// count of workgroups: 448 on 256 CUs, one each, are two rounds of which the
+// second is three quarters full.  Seven prompts of 300 to 2048 tokens: 77 us for
+// 48 GFLOP, of which the longest workgroup's 32 tiles take 55.
 
 constexpr int kRowsP = 256;
 
@@ -629,6 +637,13 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p) {
 // workgroups per CU.  Workgroups past a sequence's end return at once: the host
 // does not know the lengths and launches for the longest that the table can
 // hold.
+//
+// Measured (kernel, then join): four sequences of 90-131 thousand slots, 28 heads
+// over 4, fp16, 961 MB: 172 + 10 us, 5.3 TB/s (a large copy 4.95; 191 with a
+// wave to each part); 48 ragged sequences of up to 8000 slots, 191 MB: 42 + 5 us,
+// bound by start-up and tail (124 with parts as long as the longest
+// sequence asks for);
+// one token behind 513 slots: 7.6 + 3.8, both mostly the launch (20.9 unsplit).
 
 constexpr int kRowsS = 32, kTileS = 32;
 
@@ -829,7 +844,8 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs p, float*
 // Adds up a row block's parts.  SHARES = 1: a thread takes a piece of four
 // outputs of its row through all parts, several rows to a workgroup; else each
 // of SHARES threads takes every SHARES-th part, one row to a workgroup, and the
-// shares are added up in their order.
+// shares are added up in their order.  16 shares take 10 us for the 128 parts of
+// 28 heads and four long sequences; a call of one part has no join at all.
 template <typename T, int D, int SHARES>
 __global__ __launch_bounds__(SHARES == 1 ? 256 : D / 4 * SHARES) void paged_join_kernel(PagedArgs p, const float* ws, int parts_max,
                                                                                      int per_min, int R) {

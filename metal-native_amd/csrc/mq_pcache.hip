@@ -15,6 +15,8 @@ namespace {
 // fp32, one rounding.  A thread takes eight frequencies of one token and walks
 // over heads with their cosines and sines in registers: one 16-byte load per
 // half head, and the tables are read once per thread instead of once per head.
+// Bound by memory: 6700 tokens of 28 heads over 4, bf16, three axes, 100 MB: 18.6 us
+// (5.4 TB/s; a large copy 4.95), 22 with the launch; one token 3 us, the launch.
 template <typename T> struct V8 { typedef typename T::e v __attribute__((ext_vector_type(8))); };
 typedef float f8 __attribute__((ext_vector_type(8)));
 
@@ -104,6 +106,10 @@ __global__ __launch_bounds__(256) void paged_rope_kernel(PagedRopeArgs p, int sp
 // head's workgroups does this for itself (a head's weights are at most some
 // hundred KiB, in L2) and then moves its own part of the slots: one launch and
 // nothing passed between workgroups.
+// Eight sequences of 20-32 thousand slots to 8192, 8 heads, 547 MB moved: 143 us
+// (110 at the copy rate; the looks at up to 128 KiB of weights come before anything
+// moves); 1100 slots to 512: 10.9 us.  Without all threads summing the histograms
+// and weights kept in registers 212 and 21.7; with two workgroups per CU 159.
 constexpr int kEvictThreads = 1024, kEvictWaves = kEvictThreads / 64, kEvictList = 2048;
 
 __device__ __forceinline__ uint32_t order_key(float v) {   // NaN above all, -0 like +0
