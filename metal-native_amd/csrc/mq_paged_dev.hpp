@@ -53,9 +53,6 @@ __device__ __forceinline__ float swap32(float v) {   // v of lane ^ 32
   return __int_as_float((threadIdx.x & 32) ? (int)r[0] : (int)r[1]);
 }
 __device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
-__device__ __forceinline__ int64_t uni64(int64_t v) {
-  return ((int64_t)uni((int)(v >> 32)) << 32) | (uint32_t)uni((int)v);
-}
 
 __device__ __forceinline__ PagedSeq load_seq(const PagedArgs& p, int s) {
   return paged_seq(s, p.cu ? p.cu[s] : 0, p.cu ? p.cu[s + 1] : 0, p.cu != nullptr, p.lens[s],
@@ -124,12 +121,6 @@ struct Base {   // wave-uniform
 __device__ __forceinline__ Base cache_base(const PagedCache& c, int kv) {
   return {(const char*)c.ptr + 2 * kv * c.head, 2u * (uint32_t)c.page, 2u * (uint32_t)c.slot};
 }
-// Slots j .. j + GS of page `page` (one page: page sizes are multiples of GS),
-// of which the first nv exist.
-__device__ __forceinline__ void load_group(const Base& c, int page, int in_page, int nv, uint32_t voff, u4* lds) {
-  lds_load16(c.at(page < 0 ? 0 : page, in_page), page < 0 ? 0u : (uint32_t)nv * c.slot, voff, lds);
-}
-
 
 }  // namespace
 }  // namespace mq

@@ -11,9 +11,9 @@
 // rows: a score more than kAbove over it; many rows: a lane's weights of a tile
 // that add up to more): then to kBelow under the row's largest score, so that
 // weights reach from 2^15 down, far enough into fp16's range that 2^17 weights
-// which round to zero together stay below an output's rounding step.  Weights are rounded to the cache's type for
-// the product with v (the matrix instruction takes no other); their sum, the
-// output's sum and M are fp32.
+// which round to zero together stay below an output's rounding step.  Weights
+// are rounded to the cache's type for the product with v (the matrix instruction
+// takes no other); their sum, the output's sum and M are fp32.
 //
 // Both products are v_mfma_f32_32x32x16 with keys (then value columns) as the
 // result's rows and 32 query rows as its columns: S^T = K Q^T leaves lane l the
