@@ -333,20 +333,31 @@ __device__ __forceinline__ float log_sum(float m, float l) {
 // waves of 32 rows with two tiles in flight 2.30 ms; eight in two groups 1.79;
 // no maximum beforehand 1.69; three tiles ahead 1.63.  What bounds it then is the
 // count of workgroups: 448 on 256 CUs, one each, are two rounds of which the
-// second is three quarters full.  Seven prompts of 300 to 2048 tokens: 77 us for
+// second is three quarters full (rows_plan says why they are not split).  Seven prompts of 300 to 2048 tokens: 77 us for
 // 48 GFLOP, of which the longest workgroup's 32 tiles take 55.
 
-constexpr int kRowsP = 256;
+constexpr int kRowsP = 256, kTileP = 64, kPerMinP = 8;   // kPerMinP: fewest tiles of a part
+
+// Tiles per part of a row block that sees `count`: parts_max parts, but of
+// per_min tiles at least.
+__device__ __forceinline__ int tiles_per_part(int count, int parts_max, int per_min) {
+  const int per = ((count + parts_max - 1) / parts_max + 3) & ~3;
+  return uni(per < per_min ? per_min : per);
+}
+
+// Partial sums of a part: R rows (the call's most rows per block, a multiple of
+// eight) of D outputs, then R (m, l) pairs.
+__device__ __host__ constexpr int record_floats(int D, int R) { return R * (D + 2); }
 
 template <typename T, int D, bool EXTRA>
-__global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p) {
-  constexpr int TK = 64, ROW = Lay<D>::ROW, GS = Lay<D>::GS, NG = 8 / GS, NM = D / 8, DB = D / 32, KS = D / 16, AHEAD = 6;
+__global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p, float* ws, int parts) {
+  constexpr int TK = kTileP, ROW = Lay<D>::ROW, GS = Lay<D>::GS, NG = 8 / GS, NM = D / 8, DB = D / 32, KS = D / 16, AHEAD = 6;
   constexpr int SLOT = TK * ROW;
   __shared__ u4 kbuf[4 * SLOT], vbuf[5 * SLOT];
   const int lane = threadIdx.x & 63, w = uni(threadIdx.x >> 6), behind = w >> 2;
   const int col = lane & 31, h = lane >> 5;
-  const int kv = blockIdx.x % p.KVH;
-  int item = blockIdx.x / p.KVH, seq = -1;
+  const int kv = blockIdx.x % p.KVH, part = blockIdx.x / p.KVH % parts;
+  int item = blockIdx.x / p.KVH / parts, seq = -1;
   PagedSeq sq{};
   for (int s0 = 0; s0 < p.b && seq < 0; s0 += 64) {
     const int s = s0 + lane;
@@ -377,7 +388,12 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p) {
   const int rl = r0 + kRowsP < total ? r0 + kRowsP - 1 : total - 1;
   const int first = uni(off + (int)p.gdiv.div(r0)), last = uni(off + (int)p.gdiv.div(rl));
   const PagedSpan span = paged_span(first, last, sq.len, sq.prefix, p.window, TK);
-  const int count = uni(span.count());
+  // the part's tiles: begin .. begin + count
+  const int all = uni(span.count()), per = tiles_per_part(all, parts, kPerMinP), begin = part * per;
+  if (begin >= all && begin > 0) return;   // a row block that sees nothing is written by its first part
+  const int count = all - begin < per ? all - begin : per;
+  const bool whole = all <= per;
+  auto tile_at = [&](int i) { return span.tile(begin + i); };
 
   // the wave's slots of a tile: 8 w .. 8 w + 8, in one page
   const Base kb = cache_base(p.k, kv), vb = cache_base(p.v, kv);
@@ -390,7 +406,7 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p) {
   }
   const int32_t* row = p.table + (int64_t)seq * p.ld_table;
   const int mask = (1 << p.shift) - 1;
-  auto slot_of = [&](int i) { return span.tile(i < count ? i : count - 1) * TK + 8 * w; };
+  auto slot_of = [&](int i) { return tile_at(i < count ? i : count - 1) * TK + 8 * w; };
   int entries = 0;   // lane i: the table's entry for them in tile number i modulo 64
   // in steps, to be taken between MFMAs (past the last tile: zeros that nobody reads)
   struct {
@@ -432,8 +448,8 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p) {
   };
   // whether some page in reach is not one of the cache
   bool gaps = false;
-  for (int part = 0; part < 2; ++part) {
-    const int from = part ? span.lo * TK : 0, to = min(part ? span.hi * TK : span.pre * TK, sq.len);
+  for (int range = 0; range < 2; ++range) {
+    const int from = range ? span.lo * TK : 0, to = min(range ? span.hi * TK : span.pre * TK, sq.len);
     for (int x = (from >> p.shift) + threadIdx.x; (int64_t)x << p.shift < to; x += 512) gaps |= row[x] < 0 || row[x] >= p.pages;
   }
   gaps = uni(__syncthreads_or(gaps));
@@ -517,7 +533,7 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p) {
   int clean0 = count, clean1 = count;
   if (!gaps) {
     auto clean = [&](int i) {
-      const int t0 = span.tile(i) * TK;
+      const int t0 = tile_at(i) * TK;
       return t0 + TK - 1 <= rw.first && t0 + TK <= sq.len && (p.window <= 0 || (int64_t)t0 > (int64_t)rw.last - p.window);
     };
     // one run of tiles: before it lie those of the prefix and the window's edge,
@@ -527,9 +543,9 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p) {
     while (clean0 < clean1 && !clean(clean0)) ++clean0;
   }
   auto softmax = [&](int t, int vs) {
-    if constexpr (EXTRA) cap_and_bias(p, rw, s, span.tile(t) * TK);
+    if constexpr (EXTRA) cap_and_bias(p, rw, s, tile_at(t) * TK);
     if (t < clean0 || t >= clean1) {
-      const int t0 = span.tile(t) * TK;
+      const int t0 = tile_at(t) * TK;
       hide(p, rw, sq, s, t0, exist(t0));
       strange |= not_finite<T>(vbuf + vs * SLOT, SLOT);
     }
@@ -601,7 +617,7 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p) {
     ac.clear();
 #pragma unroll 1
     for (int t = 0; t < count; ++t) {
-      const int t0 = span.tile(t) * TK;
+      const int t0 = tile_at(t) * TK;
       load(t, 0);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
@@ -613,6 +629,24 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p) {
   const int r = r0 + 32 * w + col;
   const float l = ac.sum();
   if (r >= total) return;
+  if (!whole) {
+    float* rec = ws + (((int64_t)(blockIdx.x / p.KVH / parts) * p.KVH + kv) * parts + part) * record_floats(D, kRowsP);
+    const int i = 32 * w + col;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        f4 v;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) v[x] = odd.fix(ac.o[db][4 * e + x], 16 * db + 4 * e + x);
+        *(f4*)(rec + i * D + 32 * db + 8 * e + 4 * h) = v;
+      }
+    if (h == 0) {
+      rec[kRowsP * D + 2 * i] = ac.m;
+      rec[kRowsP * D + 2 * i + 1] = l;
+    }
+    return;
+  }
   const float f = inverse(l);
   const int tok = (int)p.gdiv.div(r), a = kv * p.g + r - tok * p.g;
   const int64_t at = (int64_t)(sq.start + tok) * p.H + a;
@@ -683,21 +717,10 @@ __device__ __forceinline__ int find_block(const PagedArgs& p, int item, int rows
   }
   return -1;
 }
-__device__ __forceinline__ PagedSpan block_span(const PagedArgs& p, const PagedSeq& sq, int r0) {
-  const int total = sq.n * p.g, off = sq.len - sq.n, rl = r0 + kRowsS < total ? r0 + kRowsS - 1 : total - 1;
-  return paged_span(off + (int)p.gdiv.div(r0), off + (int)p.gdiv.div(rl), sq.len, sq.prefix, p.window, kTileS);
+__device__ __forceinline__ PagedSpan block_span(const PagedArgs& p, const PagedSeq& sq, int r0, int rows, int tk) {
+  const int total = sq.n * p.g, off = sq.len - sq.n, rl = r0 + rows < total ? r0 + rows - 1 : total - 1;
+  return paged_span(off + (int)p.gdiv.div(r0), off + (int)p.gdiv.div(rl), sq.len, sq.prefix, p.window, tk);
 }
-
-// Tiles per part of a row block that sees `count`: parts_max parts, but of
-// per_min tiles at least.
-__device__ __forceinline__ int tiles_per_part(int count, int parts_max, int per_min) {
-  const int per = ((count + parts_max - 1) / parts_max + 3) & ~3;
-  return uni(per < per_min ? per_min : per);
-}
-
-// Partial sums of a part: R rows (the call's most rows per block, a multiple of
-// eight) of D outputs, then R (m, l) pairs.
-__device__ __host__ constexpr int record_floats(int D, int R) { return R * (D + 2); }
 
 template <typename T, int D, bool EXTRA>
 __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs p, float* ws, int per_min, int R) {
@@ -710,7 +733,7 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs p, float*
   const int seq = find_block(p, blockIdx.z, kRowsS, sq, block), kv = blockIdx.y;
   if (seq < 0) return;
   const int r0 = block * kRowsS, total = sq.n * p.g;
-  const PagedSpan span = block_span(p, sq, r0);
+  const PagedSpan span = block_span(p, sq, r0, kRowsS, kTileS);
   const int count = uni(span.count()), per = tiles_per_part(count, gridDim.x, per_min), begin = blockIdx.x * per;
   if (begin >= count && begin > 0) return;   // a row block that sees nothing is written by its first part
   const int last = begin + per < count ? begin + per : count;
@@ -841,21 +864,23 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs p, float*
   }
 }
 
-// Adds up a row block's parts.  SHARES = 1: a thread takes a piece of four
+// Adds up the parts of a row block, of 32 rows or (MANY) of 256.  SHARES = 1: a thread takes a piece of four
 // outputs of its row through all parts, several rows to a workgroup; else each
 // of SHARES threads takes every SHARES-th part, one row to a workgroup, and the
 // shares are added up in their order.  16 shares take 10 us for the 128 parts of
 // 28 heads and four long sequences; a call of one part has no join at all.
-template <typename T, int D, int SHARES>
+template <typename T, int D, int SHARES, bool MANY>
 __global__ __launch_bounds__(SHARES == 1 ? 256 : D / 4 * SHARES) void paged_join_kernel(PagedArgs p, const float* ws, int parts_max,
                                                                                      int per_min, int R) {
   constexpr int P4 = D / 4;   // pieces of a row
   PagedSeq sq;
   int block;
-  const int seq = find_block(p, blockIdx.z, kRowsS, sq, block), kv = blockIdx.y;
+  constexpr int ROWS = MANY ? kRowsP : kRowsS;
+  const int seq = find_block(p, blockIdx.z, ROWS, sq, block), kv = blockIdx.y;
   if (seq < 0) return;
-  const int r0 = block * kRowsS;
-  const int count = block_span(p, sq, r0).count(), per = tiles_per_part(count, parts_max, per_min);
+  if (MANY) block = (int)(((int64_t)sq.n * p.g + ROWS - 1) / ROWS) - 1 - block;   // that kernel takes the last rows first
+  const int r0 = block * ROWS;
+  const int count = block_span(p, sq, r0, ROWS, MANY ? kTileP : kTileS).count(), per = tiles_per_part(count, parts_max, per_min);
   const int parts = (count + per - 1) / per;
   const int d4 = threadIdx.x % P4, share = SHARES == 1 ? 0 : threadIdx.x / P4;
   const int r = SHARES == 1 ? blockIdx.x * (256 / P4) + threadIdx.x / P4 : blockIdx.x;
@@ -899,12 +924,56 @@ __global__ __launch_bounds__(SHARES == 1 ? 256 : D / 4 * SHARES) void paged_join
 int64_t row_blocks(const PagedArgs& a, int rows) {   // at most, over all sequences
   return a.cu ? ((int64_t)a.rows * a.g + rows - 1) / rows + a.b : (int64_t)a.rows * ((a.g + rows - 1) / rows);
 }
-// Rows past each sequence's first token that fill the chip by themselves.  Single
-// tokens never count, however many sequences there are: a block of 256 rows would
-// hold the g rows of one (1280 tokens of 32 heads over 8, 500 slots: 1150 us, in
-// blocks of 32 rows 440; 4096 of 28 over 4, 130 slots: 1945 and 315).
-bool many_rows(const PagedArgs& a, int num_cus) {
-  return ((int64_t)(a.rows - a.b) * a.g / 128) * a.KVH >= num_cus || row_blocks(a, kRowsS) > 65535;   // the grid's z
+int64_t most_slots(const PagedArgs& a, int rows, int tk) {   // that a row block can see
+  if (a.window > 0 && !a.prefix) return std::min<int64_t>(a.cap, (int64_t)a.window + rows + 2 * tk);
+  return a.cap;
+}
+// Whether the sequences' chunks fill half a block of 256 rows on average, and
+// there is work (rows by slots) enough for its longer start-up.  Single tokens
+// never do: a block would hold the g rows of one (1280 tokens of 32 heads over 8,
+// 500 slots: 1150 us, in blocks of 32 rows 440).  28 heads over 4, 128 wide, few-row
+// kernel and this one, us: 40 tokens over 600 slots (0.7 M) 15 and 27; 20 over 8192
+// (4.6 M) 34 and 33; 64 over 8192 59 and 35; 512 over 8192 191 and 77.  With caps and
+// biases, whose softmax weighs more here: 4 chunks of 160 over 1000 slots (18 M) 65 and
+// 70, 800 over 1000 (22 M) 70 and 71, 128 over 8192 (29 M) 110 and 67.
+constexpr int64_t kWork = 4 << 20, kWorkExtra = 24 << 20;
+bool many_rows(const PagedArgs& a) {
+  const int64_t slots = a.window > 0 ? std::min<int64_t>(a.cap, a.window + kRowsP) : a.cap;
+  return ((int64_t)(a.rows - a.b) * a.g >= 128 * (int64_t)a.b && (int64_t)a.rows * a.H * slots >= (a.extra() ? kWorkExtra : kWork)) ||
+         row_blocks(a, kRowsS) > 65535;   // the grid's z
+}
+// The parts of a many-row call.  A workgroup takes a CU, so the time is rounds of
+// workgroups: parts fill the chip where there are few row blocks and round off
+// the last round where there are many.  Microseconds: 1.7 per tile of 128-wide
+// heads, 6 until the first tile has landed, a part's record written and read
+// again at the copy rate, 8 for the second launch; a tenth must be gained (4096
+// tokens behind 28672 slots in four parts, 1.75 rounds for 2: 1690 us for 1665, the
+// clock falls when all CUs work).  8192 slots, 28 heads over 4, one part and these:
+// 512 tokens 191 and 77 us, 1100 tokens 186 and 138.
+struct RowsPlan {
+  int64_t blocks, parts;
+  size_t ws_bytes;
+};
+RowsPlan rows_plan(const PagedArgs& a, int num_cus) {
+  RowsPlan s;
+  s.blocks = row_blocks(a, kRowsP);
+  s.parts = 1;
+  if (a.cu && s.blocks <= 65535) {
+    const int64_t units = (((int64_t)a.rows * a.g + kRowsP - 1) / kRowsP + (a.b - 1) / 2) * a.KVH;   // half of each chunk's last block
+    const int64_t tiles = (most_slots(a, kRowsP, kTileP) + kTileP - 1) / kTileP;
+    const double record = (double)units * kRowsP * (a.D + 2) * sizeof(float) * 2 / 4.9e6, tile = 1.7 * a.D / 128;
+    double least = 0;
+    for (int parts = 1; parts <= 16 && (parts == 1 || parts * kPerMinP <= tiles); ++parts) {
+      const int64_t rounds = (units * parts + num_cus - 1) / num_cus;
+      const double t = (double)rounds * ((double)tiles / parts * tile + 6) + (parts > 1 ? 8 + parts * record : 0);
+      if (parts == 1 || t < 0.9 * least) {
+        least = t;
+        s.parts = parts;
+      }
+    }
+  }
+  s.ws_bytes = s.parts > 1 ? (size_t)(s.blocks * a.KVH * s.parts) * record_floats(a.D, kRowsP) * sizeof(float) : 0;
+  return s;
 }
 
 // The parts of a few-row call: as many for every row block, for sequences as
@@ -919,8 +988,7 @@ struct SplitPlan {
 SplitPlan split_plan(const PagedArgs& a, int num_cus) {
   SplitPlan s;
   s.blocks = row_blocks(a, kRowsS);
-  int64_t slots = a.cap;
-  if (a.window > 0 && !a.prefix) slots = std::min<int64_t>(slots, (int64_t)a.window + kRowsS + 2 * kTileS);
+  const int64_t slots = most_slots(a, kRowsS, kTileS);
   const int64_t tiles = (slots + kTileS - 1) / kTileS, lanes = std::max<int64_t>(s.blocks * a.KVH, 1);
   s.per_min = lanes >= num_cus ? 16 : (4 * lanes >= num_cus ? 8 : 4);
   const int64_t want = std::max<int64_t>(1, (lanes >= num_cus ? 16 : 8) * (int64_t)num_cus / lanes);   // parts per row block and head
@@ -933,11 +1001,14 @@ SplitPlan split_plan(const PagedArgs& a, int num_cus) {
 
 template <typename T, int D>
 hipError_t launch(const PagedArgs& a, int num_cus, void* ws, hipStream_t s) {
-  if (many_rows(a, num_cus)) {
-    const int64_t grid = row_blocks(a, kRowsP) * a.KVH;
+  if (many_rows(a)) {
+    const RowsPlan rp = rows_plan(a, num_cus);
+    const int64_t grid = rp.blocks * a.KVH * rp.parts;
     if (grid > 0x7fffffff) return hipErrorInvalidValue;
-    if (a.extra()) paged_rows_kernel<T, D, true><<<(int)grid, 512, 0, s>>>(a);
-    else paged_rows_kernel<T, D, false><<<(int)grid, 512, 0, s>>>(a);
+    if (a.extra()) paged_rows_kernel<T, D, true><<<(int)grid, 512, 0, s>>>(a, (float*)ws, (int)rp.parts);
+    else paged_rows_kernel<T, D, false><<<(int)grid, 512, 0, s>>>(a, (float*)ws, (int)rp.parts);
+    if (rp.parts > 1)
+      paged_join_kernel<T, D, 1, true><<<dim3(kRowsP * D / 1024, a.KVH, (unsigned)rp.blocks), 256, 0, s>>>(a, (const float*)ws, (int)rp.parts, kPerMinP, kRowsP);
     return hipGetLastError();
   }
   const SplitPlan sp = split_plan(a, num_cus);
@@ -945,16 +1016,16 @@ hipError_t launch(const PagedArgs& a, int num_cus, void* ws, hipStream_t s) {
   if (a.extra()) paged_split_kernel<T, D, true><<<grid, 256, 0, s>>>(a, (float*)ws, sp.per_min, sp.R);
   else paged_split_kernel<T, D, false><<<grid, 256, 0, s>>>(a, (float*)ws, sp.per_min, sp.R);
   if (sp.parts > 16)
-    paged_join_kernel<T, D, 16><<<dim3(sp.R, a.KVH, (unsigned)sp.blocks), D / 4 * 16, 0, s>>>(a, (const float*)ws, (int)sp.parts, sp.per_min, sp.R);
+    paged_join_kernel<T, D, 16, false><<<dim3(sp.R, a.KVH, (unsigned)sp.blocks), D / 4 * 16, 0, s>>>(a, (const float*)ws, (int)sp.parts, sp.per_min, sp.R);
   else if (sp.parts > 1)
-    paged_join_kernel<T, D, 1><<<dim3((sp.R + 1024 / D - 1) / (1024 / D), a.KVH, (unsigned)sp.blocks), 256, 0, s>>>(a, (const float*)ws, (int)sp.parts, sp.per_min, sp.R);
+    paged_join_kernel<T, D, 1, false><<<dim3((sp.R + 1024 / D - 1) / (1024 / D), a.KVH, (unsigned)sp.blocks), 256, 0, s>>>(a, (const float*)ws, (int)sp.parts, sp.per_min, sp.R);
   return hipGetLastError();
 }
 
 }  // namespace
 
 size_t pattn_workspace(const PagedArgs& a, int num_cus) {
-  return many_rows(a, num_cus) ? 0 : split_plan(a, num_cus).ws_bytes;
+  return many_rows(a) ? rows_plan(a, num_cus).ws_bytes : split_plan(a, num_cus).ws_bytes;
 }
 
 hipError_t pattn_launch(const PagedArgs& a, int num_cus, void* ws, hipStream_t s) {

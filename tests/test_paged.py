@@ -486,3 +486,31 @@ def test_single_tokens_of_very_many_sequences(gpu):
         at = rows.cpu()
         assert bool(((out.double().cpu() - o[at]).abs() <= ob[at]).all())
         assert bool(((lse.double().cpu() - l[at]).abs() <= lb[at]).all())
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("H,KVH,D", [(14, 2, 128), (14, 2, 64)])
+@pytest.mark.parametrize("masked", [False, True])
+def test_chunks_behind_long_caches(gpu, dtype, H, KVH, D, masked):
+    """Many rows whose slots are dealt out to several workgroups, sequences of fewer parts among them."""
+    c = build(gpu, DT[dtype], H, KVH, D, 16, [3200, 40, 1000, 0], [600, 40, 33, 0], seed=D)
+    how = {}
+    if masked:
+        how = dict(softcap=15.0, slopes=torch.rand(H, device=gpu) * 0.01, window=2500,
+                   prefix=torch.tensor([90, 3, 0, 0], dtype=torch.int32, device=gpu))
+    check_attention(c, **how)
+    first = c["table"][0]
+    first[3], first[100] = -1, 10**6
+    c["v"][first[150].long(), :, 5] = float("nan")   # slot 2405: seen by all rows; 3195: by the last few
+    c["v"][first[199].long(), 0, 11] = float("inf")
+    check_attention(c, **how)
+
+
+def test_chunks_behind_long_caches_repeat(gpu):
+    from metal_native import paged
+
+    c = build(gpu, torch.float16, 28, 4, 128, 16, [5000, 3000], [300, 200], seed=3)
+    a, la = paged.attention(c["q"], c["k"], c["v"], c["table"], c["lens"], c["cu"], return_lse=True)
+    for _ in range(3):
+        b, lb = paged.attention(c["q"], c["k"], c["v"], c["table"], c["lens"], c["cu"], return_lse=True)
+        assert torch.equal(a, b) and torch.equal(la, lb)
