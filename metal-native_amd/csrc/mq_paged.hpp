@@ -77,6 +77,26 @@ MQ_HD bool paged_visible(int p, int j, int len, int prefix, int window) {
   return j >= 0 && j < len && ((j <= p && (window <= 0 || (int64_t)j > (int64_t)p - window)) || j < prefix);
 }
 
+// Rows of a sequence's chunk (g per token) whose tokens may see a slot of j0 ..
+// j0 + slots - 1; none where the slots lie past the sequence.  Tokens are cut to
+// the chunk's before they are multiplied: a table may name far more slots than
+// the sequence has, and 2^31 rows' worth of them.
+struct PagedRange {
+  int begin, end;   // 0 <= begin <= end <= n * g
+};
+MQ_HD PagedRange paged_rows(int j0, int slots, const PagedSeq& s, int window, int g) {
+  if (j0 >= s.len) return {0, 0};
+  int64_t a = 0, b = s.n;
+  if (j0 >= s.prefix) {
+    const int64_t off = (int64_t)s.len - s.n;   // position of the chunk's first token
+    a = (int64_t)j0 - off;
+    a = a < 0 ? 0 : (a > s.n ? s.n : a);
+    const int64_t end = (int64_t)j0 + slots - 1 + window - off;
+    if (window > 0 && end < b) b = end;
+  }
+  return a < b ? PagedRange{(int)(a * g), (int)(b * g)} : PagedRange{0, 0};
+}
+
 // Page that holds slot j, or -1 where there is none.
 MQ_HD int paged_page(const int32_t* row, int j, int len, int shift, int pages) {
   if (j < 0 || j >= len) return -1;

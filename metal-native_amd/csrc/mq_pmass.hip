@@ -42,15 +42,10 @@ __global__ __launch_bounds__(256, 2) void paged_mass_kernel(PagedArgs p, float* 
   const PagedSeq sq0 = load_seq(p, s);
   const PagedSeq sq = {uni(sq0.start), uni(sq0.n), uni(sq0.len), uni(sq0.prefix)};
   const int j0 = blk * kSlotsM, off = sq.len - sq.n, total = sq.n * p.g;
-  // tokens that see a slot of the block
-  int ta = 0, tb = sq.n;
-  if (j0 >= sq.len) tb = 0;
-  if (j0 >= sq.prefix) {
-    ta = max(0, j0 - off);
-    if (p.window > 0) tb = (int)min((int64_t)tb, max((int64_t)0, (int64_t)j0 + kSlotsM - 1 + p.window - off));
-  }
-  const int ra = (int)((int64_t)ta * p.g) / kRowsM * kRowsM, rb = tb * p.g;
-  const int blocks = rb > ra ? (rb - ra + kRowsM - 1) / kRowsM : 0;
+  // rows that see a slot of the block, in blocks of kRowsM
+  const PagedRange rr = paged_rows(j0, kSlotsM, sq, p.window, p.g);
+  const int ra = rr.begin / kRowsM * kRowsM;
+  const int blocks = rr.end > rr.begin ? (rr.end - ra - 1) / kRowsM + 1 : 0;
   const int b0 = (int)((int64_t)blocks * part / parts), b1 = (int)((int64_t)blocks * (part + 1) / parts);
 
   u4 kr[2][D / 16];

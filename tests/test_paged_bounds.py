@@ -1,0 +1,49 @@
+"""Paged-cache operators where values, masks or tables stand at their ends."""
+
+import math
+import os
+import shutil
+import subprocess
+
+import pytest
+import torch
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="needs g++")
+def test_rows_of_a_block_of_slots(tmp_path):
+    """Built with a host compiler from the kernels' own header, undefined behaviour and bounds trapped."""
+    exe = tmp_path / "paged_rows_check"
+    cmd = ["g++", "-O1", "-std=c++17", "-fsanitize=undefined,address", "-fno-sanitize-recover=all",
+           f"-I{os.path.join(ROOT, 'metal-native_amd', 'csrc')}",
+           os.path.join(ROOT, "tests", "native", "paged_rows_check.cpp"), "-o", str(exe)]
+    subprocess.run(cmd, check=True, capture_output=True, timeout=300)
+    out = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300, env={k: v for k, v in os.environ.items() if k != "LD_PRELOAD"})
+    assert out.returncode == 0 and "bad 0" in out.stdout, out.stdout + out.stderr
+
+
+@pytest.mark.gpu
+def test_mass_of_short_sequences_in_a_table_of_far_more_slots(gpu):
+    """128 heads and a table of 2^24 + 128 slots: rows numbered by the table's slots would pass 32 bits."""
+    from metal_native import paged
+
+    H, D, ps, width = 128, 64, 128, (1 << 17) + 1
+    g = torch.Generator(device=gpu)
+    g.manual_seed(1)
+    k, v = (torch.randn(8, 1, ps, D, device=gpu, generator=g).half() for _ in range(2))
+    wide = torch.full((2, width), -1, dtype=torch.int32, device=gpu)
+    wide[0, :3] = torch.tensor([5, 1, 7])
+    wide[1, 0] = 2
+    lens = torch.tensor([300, 9], dtype=torch.int32, device=gpu)
+    for cu, rows in ((None, 2), (torch.tensor([0, 4, 9], dtype=torch.int32, device=gpu), 9)):
+        q = torch.randn(rows, H, D, device=gpu, generator=g).half()
+        near = wide[:, :3].contiguous()
+        _, lse = paged.attention(q, k, v, near, lens, cu, return_lse=True)
+        want = paged.attention_mass(q, k, near, lens, lse, cu)
+        got = paged.attention_mass(q, k, wide, lens, lse, cu)
+        assert got.shape == (2, 1, width * ps)
+        # the far table's call may add the rows up in other parts: two sums of weights, each within 2 (r^1/2 + 40) e
+        r = rows * H
+        assert bool(((got[..., :3 * ps] - want).abs() <= want * 4 * (math.sqrt(r) + 40) * 2.0**-24).all())
+        assert float(got[..., 3 * ps:].abs().max()) == 0
