@@ -452,6 +452,9 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p, float* 
     const int from = range ? span.lo * TK : 0, to = min(range ? span.hi * TK : span.pre * TK, sq.len);
     for (int x = (from >> p.shift) + threadIdx.x; (int64_t)x << p.shift < to; x += 512) gaps |= row[x] < 0 || row[x] >= p.pages;
   }
+  // values of "tile -1", which tile 0's first phase multiplies by weights of zero:
+  // zeros themselves, as tile 0's own could be infinite (tile 4 takes their slot)
+  for (int x = threadIdx.x; x < SLOT; x += 512) vbuf[4 * SLOT + x] = (u4){0u, 0u, 0u, 0u};
   gaps = uni(__syncthreads_or(gaps));
   auto exist = [&](int t0) -> uint64_t {   // bit per slot of a tile
     if (gaps) return __ballot(paged_page(row, t0 + lane, sq.len, p.shift, p.pages) >= 0);
@@ -589,8 +592,8 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p, float* 
   change();
   if (behind) change();
 #pragma unroll
-  for (int m = 0; m < AHEAD; ++m) frag[m] = value(0, m);
-  int vprev = 0, vcur = 0, vload = 3;   // slots of the values of tiles t - 1 (tile 0: its own, times weights of zero), t, t + 3
+  for (int m = 0; m < AHEAD; ++m) frag[m] = value(4, m);
+  int vprev = 4, vcur = 0, vload = 3;   // slots of the values of tiles t - 1 (before tile 0: zeros), t, t + 3
 #pragma unroll 1
   for (int t = 0; t < count; ++t) {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NG) : "memory");   // tile t + 1 has landed; t + 2 may be on its way

@@ -8,6 +8,8 @@ import subprocess
 import pytest
 import torch
 
+from test_paged import DT, build, check_attention
+
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
@@ -47,3 +49,25 @@ def test_mass_of_short_sequences_in_a_table_of_far_more_slots(gpu):
         r = rows * H
         assert bool(((got[..., :3 * ps] - want).abs() <= want * 4 * (math.sqrt(r) + 40) * 2.0**-24).all())
         assert float(got[..., 3 * ps:].abs().max()) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("parts", [False, True])
+def test_infinite_values_that_every_row_sees(gpu, dtype, D, parts):
+    """Blocks of 256 rows, their slots in one part or several: an infinity in each tile of 64 slots, the first of a
+    block and of a part among them, and both signs in one column."""
+    H, KVH, lens, new = (14, 2, [3200, 40], [600, 40]) if parts else (32, 8, [900, 300], [512, 300])
+    c = build(gpu, DT[dtype], H, KVH, D, 16, lens, new, seed=D)
+    seen = (lens[0] - new[0]) // 64   # tiles that every row of the first sequence sees whole
+    assert seen >= 6
+    for t in range(seen):
+        slot = 64 * t + 5 * t % 64
+        c["v"][c["table"][0, slot // 16].long(), :, slot % 16, t] = float("inf") if t % 2 else -float("inf")
+    last = c["table"][0, (64 * seen - 1) // 16].long()
+    c["v"][last, :, 15, 1] = -float("inf")   # +inf stands in tile 1: NaN
+    out, _, _ = check_attention(c)
+    first = out[:new[0]].float()
+    assert bool(first[..., 1].isnan().all()) and bool((first[..., 3:seen:2] == float("inf")).all())
+    assert bool((first[..., 0:seen:2] == -float("inf")).all()) and bool(first[..., seen:].isfinite().all())
