@@ -802,7 +802,8 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs p, float*
     const bool more = i + 4 < last;
     if (more) look_up(i + 4);
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NG) : "memory");
-    auto keys_done = [&] {
+    auto keys_done = [&] {   // the last of them read, whatever order the products were put in
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       if (more) load(kb, koff, KO, kt);
     };
     auto values_ready = [&] {

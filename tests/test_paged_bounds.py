@@ -2,6 +2,7 @@
 
 import math
 import os
+import re
 import shutil
 import subprocess
 
@@ -71,3 +72,37 @@ def test_infinite_values_that_every_row_sees(gpu, dtype, D, parts):
     first = out[:new[0]].float()
     assert bool(first[..., 1].isnan().all()) and bool((first[..., 3:seen:2] == float("inf")).all())
     assert bool((first[..., 0:seen:2] == -float("inf")).all()) and bool(first[..., seen:].isfinite().all())
+
+
+def test_refilled_buffers_have_been_read(tmp_path):
+    """The few-row kernel fills a wave's key and value buffers again as soon as its products have read them: in its
+    assembly no LDS read is outstanding where a load into LDS starts."""
+    import importlib.util
+
+    spec = importlib.util.spec_from_file_location("mq_build", os.path.join(ROOT, "metal-native_amd", "build.py"))
+    b = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(b)
+    try:
+        hipcc = b._hipcc()
+    except RuntimeError:
+        pytest.skip("needs hipcc")
+    src, asm = "mq_pattn.hip", tmp_path / "pattn.s"
+    subprocess.run([hipcc, *b.HIP_FLAGS, *b.SOURCE_FLAGS[src], "-x", "hip", "-S", "--cuda-device-only", os.path.join(b.CSRC, src),
+                    "-o", str(asm)], check=True, capture_output=True, timeout=600)
+    loads, name, reads = {}, "", 0
+    for line in asm.read_text().splitlines():
+        label = re.match(r"(_Z\w+):", line)
+        if label:
+            name, reads = label.group(1), 0
+        if "paged_split_kernel" not in name:
+            continue
+        line = line.strip()
+        wait = re.search(r"s_waitcnt.*lgkmcnt\((\d+)\)", line)
+        if line.startswith(("ds_", "s_load")):
+            reads += 1
+        elif wait:
+            reads = min(reads, int(wait.group(1)))
+        elif line.startswith("buffer_load_dwordx4") and line.endswith("lds"):
+            loads[name] = loads.get(name, 0) + 1
+            assert reads == 0, (name, line)
+    assert len(loads) == 8 and min(loads.values()) >= 8, loads   # two types, two widths, with and without caps and biases
