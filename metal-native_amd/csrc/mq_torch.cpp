@@ -30,11 +30,14 @@ namespace mq_front {
 
 bool modes_set() { return c10::impl::TorchDispatchModeTLS::any_modes_set() || at::impl::torch_function_mode_enabled(); }
 
-// a strided GPU tensor with memory of its own and nothing pending on it
+// a strided GPU tensor with memory of its own and nothing pending on it (by its
+// own keys: isTensorSubclassLike holds for every tensor under a dispatch mode,
+// which modes_set asks for)
 const at::Tensor* plain(PyObject* o) {
   if (!THPVariable_CheckExact(o)) return nullptr;
   const at::Tensor& t = THPVariable_Unpack(o);
-  if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || at::isTensorSubclassLike(t) || t.is_neg() ||
+  if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided ||
+      t.key_set().has_any(at::kTensorSubclassLike) || t.is_neg() ||
       t._is_zerotensor() || !t.has_storage())
     return nullptr;
   return &t;

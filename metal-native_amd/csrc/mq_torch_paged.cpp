@@ -1,13 +1,16 @@
 // Native front of the paged-cache operators: checks, allocation and launch as
 // one CPython call.  Every function returns None for what it does not take as
 // it is (paged.py then names the fault, or copies and calls again), an int for
-// a status of the library, else the outputs.
+// a status of the library, else the outputs.  Function and dispatch modes (a
+// default device is one) make no difference: nothing here is theirs to change,
+// and the outputs are allocated below them.
 #include "mq_torch.hpp"
 
 #include <algorithm>
 #include <utility>
 
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -143,6 +146,15 @@ bool mask(PyObject* const* a, const Cache& k, const Query& q, mq_paged_mask* m) 
   return as_int(a[6], &m->max_q);
 }
 
+// Device of a call, and dispatch below Python's modes: what is allocated here
+// is launched on at once and has to be memory.
+struct Call {
+  c10::DeviceGuard device;
+  c10::impl::ExcludeDispatchKeyGuard modes;
+  explicit Call(c10::Device d)
+      : device(d), modes(c10::DispatchKeySet({c10::DispatchKey::Python, c10::DispatchKey::PythonTLSSnapshot})) {}
+};
+
 PyObject* status(int rc) { return PyLong_FromLong(rc); }
 PyObject* wrong_count(const char* what) {
   PyErr_SetString(PyExc_TypeError, what);
@@ -154,7 +166,6 @@ PyObject* wrong_count(const char* what) {
 // (qkv, cos, sin, pos, k, v, table, lens, cu, sections tuple | None, stream)
 PyObject* paged_rope_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 11) return wrong_count("paged_rope_kv: 11 arguments");
-  if (modes_set()) return decline();
   Cache k;
   const at::Tensor *x = plain(a[0]), *co = plain(a[1]), *si = plain(a[2]), *pos = plain(a[3]);
   if (!x || !co || !si || !pos || !k.take(a[4], a[5], a[6], a[7], true)) return decline();
@@ -189,7 +200,7 @@ PyObject* paged_rope_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
   void* stream = PyLong_AsVoidPtr(a[10]);
   if (PyErr_Occurred()) return nullptr;
   HANDLE_TH_ERRORS
-  const c10::DeviceGuard guard(k.dev);
+  const Call guard(k.dev);
   at::Tensor out = at::empty({rows, heads, D}, x->options());
   if (rows == 0) return THPVariable_Wrap(std::move(out));
   int rc;
@@ -205,7 +216,6 @@ PyObject* paged_rope_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // (q, k, v, table, lens, cu, scale, softcap, slopes, window, prefix_lens, max_q, return_lse, stream)
 PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 14) return wrong_count("paged_attention: 14 arguments");
-  if (modes_set()) return decline();
   Cache k;
   Query q;
   mq_paged_mask m{};
@@ -214,7 +224,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   void* stream = PyLong_AsVoidPtr(a[13]);
   if (PyErr_Occurred()) return nullptr;
   HANDLE_TH_ERRORS
-  const c10::DeviceGuard guard(k.dev);
+  const Call guard(k.dev);
   const int64_t wsb = mq_paged_attention_workspace_size(&k.c, &m, q.rows, (int32_t)q.heads);
   if (wsb < 0) return status(MQ_INVALID_ARGUMENT);
   at::Tensor out = at::empty({q.rows, q.heads, q.t->size(2)}, q.t->options());
@@ -245,7 +255,6 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // (q, k, table, lens, lse, cu, scale, softcap, slopes, window, prefix_lens, max_q, stream)
 PyObject* paged_attention_mass(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 13) return wrong_count("paged_attention_mass: 13 arguments");
-  if (modes_set()) return decline();
   Cache k;
   Query q;
   mq_paged_mask m{};
@@ -257,7 +266,7 @@ PyObject* paged_attention_mass(PyObject*, PyObject* const* a, Py_ssize_t n) {
   void* stream = PyLong_AsVoidPtr(a[12]);
   if (PyErr_Occurred()) return nullptr;
   HANDLE_TH_ERRORS
-  const c10::DeviceGuard guard(k.dev);
+  const Call guard(k.dev);
   const int64_t wsb = mq_paged_attention_mass_workspace_size(&k.c, &m, q.rows, (int32_t)q.heads);
   if (wsb < 0) return status(MQ_INVALID_ARGUMENT);
   at::Tensor mass = at::empty({k.c.batch, k.c.kv_heads, k.c.width * k.c.page_size}, lse->options());
@@ -276,7 +285,6 @@ PyObject* paged_attention_mass(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // (k, v, table, lens, mass, to, budget, recent, stream)
 PyObject* paged_evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 9) return wrong_count("paged_evict: 9 arguments");
-  if (modes_set()) return decline();
   Cache k;
   const at::Tensor *mass = plain(a[4]), *to = plain(a[5]);
   int64_t budget, recent;
@@ -290,7 +298,7 @@ PyObject* paged_evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
   void* stream = PyLong_AsVoidPtr(a[8]);
   if (PyErr_Occurred()) return nullptr;
   HANDLE_TH_ERRORS
-  const c10::DeviceGuard guard(k.dev);
+  const Call guard(k.dev);
   const auto ints = mass->options().dtype(at::kInt);
   at::Tensor kept = at::empty({k.c.batch, k.c.kv_heads, budget}, ints), lens = at::empty({k.c.batch}, ints);
   at::Tensor left = at::empty({k.c.batch, k.c.kv_heads, to->size(1) * k.c.page_size}, mass->options());

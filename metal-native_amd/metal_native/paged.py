@@ -34,6 +34,15 @@ from .ops import _check, _invalid, _mq_torch, _raw_stream, _require_cuda
 __all__ = ["rope_kv", "attention", "attention_mass", "evict"]
 
 
+def _plain(*tensors):
+    """Tensors of other classes as ordinary ones over the same memory; anything else as it is."""
+    odd = [isinstance(t, torch.Tensor) and type(t) not in (torch.Tensor, torch.nn.Parameter) for t in tensors]
+    if not any(odd):
+        return tensors
+    with torch._C.DisableTorchFunctionSubclass():
+        return tuple(t.as_subclass(torch.Tensor) if o else t for t, o in zip(tensors, odd))
+
+
 def _cache(op, k, v, table, lens, keys_only=False):
     """Raises for what no kernel takes; returns table and lens as the kernels
     read them.  The caches themselves are never copied."""
@@ -79,7 +88,7 @@ def _chunks(op, cu, table, rows):
 
 def _finish(op, r):
     if r is None:
-        _invalid(f"{op}: arguments not supported (memory overlaps, or strides out of range)")
+        _invalid(f"{op}: arguments not supported (memory overlaps, strides out of range, or a tensor without memory of its own)")
     if type(r) is int:
         _check(r)
     return r
@@ -106,6 +115,7 @@ def rope_kv(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: torch.
                                     _raw_stream(qkv.get_device()))
         if r is not None:
             return _finish(op, r)
+    qkv, cos, sin, pos, k_cache, v_cache, table, lens, cu = _plain(qkv, cos, sin, pos, k_cache, v_cache, table, lens, cu)
     table, lens = _cache(op, k_cache, v_cache, table, lens)
     kvh, d = k_cache.shape[1], k_cache.shape[3]
     for t, what in ((qkv, "qkv"), (cos, "cos"), (sin, "sin"), (pos, "pos")):
@@ -179,6 +189,7 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, tab
                                       max_q, return_lse, _raw_stream(q.get_device()))
         if r is not None:
             return _finish(op, r)
+    q, k_cache, v_cache, table, lens, cu, slopes, prefix_lens = _plain(q, k_cache, v_cache, table, lens, cu, slopes, prefix_lens)
     table, lens = _cache(op, k_cache, v_cache, table, lens)
     q, *how = _mask(op, q, k_cache, table, cu, scale, softcap, slopes, window, prefix_lens, max_q)
     with torch.cuda.device(q.device):
@@ -208,6 +219,7 @@ def attention_mass(q: torch.Tensor, k_cache: torch.Tensor, table: torch.Tensor, 
                                            max_q, _raw_stream(q.get_device()))
         if r is not None:
             return _finish(op, r)
+    q, k_cache, table, lens, lse, cu, slopes, prefix_lens = _plain(q, k_cache, table, lens, lse, cu, slopes, prefix_lens)
     table, lens = _cache(op, k_cache, None, table, lens, keys_only=True)
     q, *how = _mask(op, q, k_cache, table, cu, scale, softcap, slopes, window, prefix_lens, max_q)
     _require_cuda(lse, "lse", op)
@@ -241,6 +253,7 @@ def evict(k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor, len
                                   _raw_stream(k_cache.get_device()))
         if r is not None:
             return _finish(op, r)
+    k_cache, v_cache, table, lens, mass, to = _plain(k_cache, v_cache, table, lens, mass, to)
     table, lens = _cache(op, k_cache, v_cache, table, lens)
     b, kvh, ps = table.shape[0], k_cache.shape[1], k_cache.shape[2]
     for t, what in ((mass, "mass"), (to, "to")):

@@ -166,9 +166,9 @@ def serve_tokens_per_second(model: SyntheticDecoder, batch: int = 8, prompt: int
     the prompts and of the steps."""
     room = -(-(prompt + tokens) // page_size) + (0 if budget is None else -(-budget // page_size))
     server = PagedServer(model, batch * room, batch, page_size=page_size, budget=budget)
-    gen = torch.Generator()
+    gen = torch.Generator("cpu")
     gen.manual_seed(0)
-    asked = torch.randint(0, model.cfg.vocab, (batch, prompt), generator=gen).tolist()
+    asked = torch.randint(0, model.cfg.vocab, (batch, prompt), generator=gen, device="cpu").tolist()
     t = [torch.cuda.Event(enable_timing=True) for _ in range(3)]
     for timed in (False, True):
         for s in list(server.last):

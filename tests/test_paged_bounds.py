@@ -106,3 +106,72 @@ def test_refilled_buffers_have_been_read(tmp_path):
             loads[name] = loads.get(name, 0) + 1
             assert reads == 0, (name, line)
     assert len(loads) == 8 and min(loads.values()) >= 8, loads   # two types, two widths, with and without caps and biases
+
+
+class Marked(torch.Tensor):
+    pass
+
+
+def step_of(gpu):
+    """The four operators on inputs of their own: the same outputs each time."""
+    from metal_native import paged
+
+    def run(form=lambda t: t):
+        c = build(gpu, torch.float16, 8, 2, 64, 16, [40, 100], [3, 1], seed=21, extra=12, junk=1.0)
+        qkv = torch.randn(4, 12 * 64, device=gpu, generator=c["gen"]).half()
+        ang = torch.rand(128, 64, device=gpu, generator=c["gen"])
+        pos = torch.tensor([37, 38, 39, 99], device=gpu)
+        k, v, table, lens, cu = (form(c[n]) for n in ("k", "v", "table", "lens", "cu"))
+        q = paged.rope_kv(form(qkv), form(ang.cos()), form(ang.sin()), form(pos), k, v, table, lens, cu)
+        slopes, prefix = form(torch.full((8,), 0.01, device=gpu)), form(torch.tensor([2, 0], dtype=torch.int32, device=gpu))
+        how = dict(slopes=slopes, prefix_lens=prefix, window=50)
+        out, lse = paged.attention(form(q), k, v, table, lens, cu, return_lse=True, **how)
+        m = paged.attention_mass(form(q), k, table, lens, form(lse), cu, **how)
+        to = form(c["free"][:4].reshape(2, 2).contiguous())
+        return [torch.Tensor(x) if type(x) is Marked else x for x in
+                (q, out, lse, m, *paged.evict(k, v, table, lens, form(m), to, 32, recent=4), k, v)]
+
+    return run
+
+
+@pytest.mark.gpu
+def test_modes_and_tensor_subclasses_make_no_difference(gpu):
+    """A default device is a function mode; profilers and counters are dispatch modes."""
+    from torch.overrides import TorchFunctionMode
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Function(TorchFunctionMode):
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    class Dispatch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    run = step_of(gpu)
+    want = run()
+
+    def same(got):
+        assert len(got) == len(want) and all(type(b) is torch.Tensor and torch.equal(a, b) for a, b in zip(want, got))
+
+    for mode in (torch.device("cuda"), torch.device("cpu"), Function(), Dispatch(), torch.inference_mode(), torch.no_grad()):
+        with mode:
+            same(run())
+    same(run(lambda t: t.as_subclass(Marked)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("device", ["cuda", "cpu"])
+def test_serving_under_a_default_device(gpu, device):
+    from metal_native.serving import PagedServer
+    from test_serving import PROMPTS, model_of
+
+    m = model_of(gpu)
+
+    def run():
+        server = PagedServer(m, 24, 4, chunk=24, budget=20, recent=6, slack=5)
+        return [server.start(PROMPTS)] + [server.step() for _ in range(8)]
+
+    want = run()
+    with torch.device(device):
+        assert run() == want
