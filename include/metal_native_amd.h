@@ -263,7 +263,9 @@ MQ_API int mq_argmax_embed_f16(const void* logits, int64_t vocab, const void* em
  *
  * The call's tokens are packed: sequence s has tokens cu_q[s] .. cu_q[s + 1]
  * (NULL: one token each), the newest of its slots, so token i of n stands at
- * position lens[s] - n + i.
+ * position lens[s] - n + i.  cu_q must not decrease; rows before cu_q[0] and
+ * from cu_q[batch] on belong to no sequence (attention writes zeros and -inf
+ * there).
  *
  * table, lens, cu_q and prefix_lens are device memory that the host does not
  * look at.  A slot whose page number is outside [0, pages) does not exist: it

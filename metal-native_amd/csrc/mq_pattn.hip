@@ -313,6 +313,33 @@ __device__ __forceinline__ float log_sum(float m, float l) {
   return l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
+// Tokens of no chunk (before the first one, past the last) give what a row that
+// sees nothing gives.  A call with chunk offsets launches for more blocks of ROWS
+// rows than there can be: b more than all its rows fill, of which b chunks waste
+// less than b.  So the workgroups that find no block are enough to take ROWS rows
+// of these tokens each, this one the at-th.
+template <int D, int ROWS>
+__device__ __forceinline__ void clear_unused(int kv, int at) {
+  // the arguments (a kernel's first) once more from where they lie: kept in
+  // registers for this they cost the 64-wide few-row kernel one of its three
+  // waves (five masked chunks 42.0 us, 47.2 so)
+  uint64_t args = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(args));
+  const PagedArgs& p = *(const PagedArgs*)args;
+  if (!p.cu) return;
+  const int lo = min(max(p.cu[0], 0), p.rows), skip = min(max(p.cu[p.b], lo), p.rows) - lo;
+  const int per = (ROWS + p.g - 1) / p.g;
+#pragma unroll 1
+  for (int o = at * per; o < (at + 1) * per && o < p.rows - skip; ++o) {
+    const int64_t head = (int64_t)(o < lo ? o : o + skip) * p.H + kv * p.g;
+#pragma unroll 1
+    for (int c = threadIdx.x; c < p.g * (D / 8); c += blockDim.x) {   // 16 bytes each
+      *(u4*)((uint16_t*)p.out + head * D + 8 * c) = (u4){0u, 0u, 0u, 0u};
+      if (p.lse && c < p.g) p.lse[head + c] = -INFINITY;
+    }
+  }
+}
+
 // ---- many rows: one workgroup of eight waves per 256 rows ----
 //
 // Per tile of 64 slots a wave has D / 4 MFMAs (output of the tile before,
@@ -379,7 +406,10 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p, float* 
       item -= __builtin_amdgcn_readlane((int)sum, 63);
     }
   }
-  if (seq < 0) return;
+  if (__builtin_expect(seq < 0, 0)) {   // item: what is left of the block's number after all sequences' blocks
+    if (part == 0) clear_unused<D, kRowsP>(kv, item);
+    return;
+  }
 
   const int r0 = item * kRowsP, total = sq.n * p.g, off = sq.len - sq.n;
   u4 q[KS];
@@ -684,7 +714,8 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p, float* 
 
 constexpr int kRowsS = 32, kTileS = 32;
 
-// Row block `item` of the call: its sequence (-1: there is none) and number.
+// Row block `item` of the call: its sequence and number (-1: there is none; of
+// chunks, how many blocks lie past the last).
 __device__ __forceinline__ int find_block(const PagedArgs& p, int item, int rows, PagedSeq& sq, int& block) {
   if (!p.cu) {   // as many blocks for every sequence
     const int per = (p.g + rows - 1) / rows, s = uni(item / per);
@@ -718,6 +749,7 @@ __device__ __forceinline__ int find_block(const PagedArgs& p, int item, int rows
     }
     item -= __builtin_amdgcn_readlane(sum, 63);
   }
+  block = item;
   return -1;
 }
 __device__ __forceinline__ PagedSpan block_span(const PagedArgs& p, const PagedSeq& sq, int r0, int rows, int tk) {
@@ -734,7 +766,10 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs p, float*
   PagedSeq sq;
   int block;
   const int seq = find_block(p, blockIdx.z, kRowsS, sq, block), kv = blockIdx.y;
-  if (seq < 0) return;
+  if (__builtin_expect(seq < 0, 0)) {
+    if (blockIdx.x == 0) clear_unused<D, kRowsS>(kv, block);
+    return;
+  }
   const int r0 = block * kRowsS, total = sq.n * p.g;
   const PagedSpan span = block_span(p, sq, r0, kRowsS, kTileS);
   const int count = uni(span.count()), per = tiles_per_part(count, gridDim.x, per_min), begin = blockIdx.x * per;
@@ -925,7 +960,8 @@ __global__ __launch_bounds__(SHARES == 1 ? 256 : D / 4 * SHARES) void paged_join
   if (p.lse && d4 == 0) p.lse[at] = log_sum(m, l);
 }
 
-int64_t row_blocks(const PagedArgs& a, int rows) {   // at most, over all sequences
+// At most, over all sequences; with chunk offsets more than enough (clear_unused).
+int64_t row_blocks(const PagedArgs& a, int rows) {
   return a.cu ? ((int64_t)a.rows * a.g + rows - 1) / rows + a.b : (int64_t)a.rows * ((a.g + rows - 1) / rows);
 }
 int64_t most_slots(const PagedArgs& a, int rows, int tk) {   // that a row block can see

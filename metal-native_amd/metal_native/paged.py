@@ -11,8 +11,11 @@ Shapes, for all four operators:
   position ``j``) lies in page ``table[s, j // page_size]``;
 * ``lens`` int32 ``[batch]``: slots per sequence, those of this call's tokens
   among them;
-* ``cu`` int32 ``[batch + 1]``: the call's packed tokens ``cu[s]:cu[s + 1]`` are
-  the newest of sequence ``s``; ``None``: one token per sequence.
+* ``cu`` int32 ``[batch + 1]``, not decreasing: the call's packed tokens
+  ``cu[s]:cu[s + 1]`` are the newest of sequence ``s``; ``None``: one token per
+  sequence.  Tokens before ``cu[0]`` or past ``cu[batch]`` (a batch padded for a
+  graph) belong to no sequence: ``rope_kv`` turns their queries and writes no
+  slot, ``attention`` gives zeros and -inf, ``attention_mass`` counts none.
 
 The index tensors are device memory that no call looks at on the host, so a
 step of a decode loop is capturable in a graph.  Whatever they hold, no kernel

@@ -9,6 +9,7 @@ import subprocess
 import pytest
 import torch
 
+import paged_ref as ref
 from test_paged import DT, build, check_attention
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -175,3 +176,30 @@ def test_serving_under_a_default_device(gpu, device):
     want = run()
     with torch.device(device):
         assert run() == want
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("H,KVH,D", [(14, 2, 64), (28, 4, 128), (6, 6, 64)])
+@pytest.mark.parametrize("lens,new,before,after", [
+    ([40, 9, 100], [3, 0, 17], 0, 1), ([40, 9, 100], [3, 9, 1], 5, 70), ([40, 9], [0, 0], 0, 40), ([900, 700], [700, 600], 3, 600)])
+def test_rows_of_no_chunk(gpu, dtype, H, KVH, D, lens, new, before, after):
+    """Rows before the first chunk and past the last, as a batch padded for a graph has them: zeros and -inf, the others
+    as without them.  The last case fills blocks of 256 rows."""
+    from metal_native import paged
+
+    c = build(gpu, DT[dtype], H, KVH, D, 16, lens, new, seed=before + after)
+    rows = before + sum(new) + after
+    q = torch.randn(rows, H, D, device=gpu, generator=c["gen"]).to(DT[dtype])
+    q[before:before + sum(new)] = c["q"]
+    for _ in range(2):   # what the outputs' memory held before
+        junk = [torch.full((rows, H, D), float("nan"), dtype=DT[dtype], device=gpu), torch.full((rows, H), float("nan"), device=gpu)]
+    del junk
+    out, lse = paged.attention(q, c["k"], c["v"], c["table"], c["lens"], c["cu"] + before, return_lse=True)
+    want, wl, ob, lb = ref.attention(q, c["k"], c["v"], c["table"], c["lens"], c["cu"] + before, scale=D**-0.5)
+    unused = torch.ones(rows, dtype=torch.bool)
+    unused[before:before + sum(new)] = False
+    assert bool((out[unused.to(gpu)] == 0).all()) and bool((lse[unused.to(gpu)] == -float("inf")).all())
+    assert bool(((out.double().cpu() - want).abs() <= ob).all())
+    gl = lse.double().cpu()
+    assert bool(((gl == wl) | ((gl - wl).abs() <= lb)).all())
