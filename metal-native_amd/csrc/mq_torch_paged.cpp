@@ -7,9 +7,11 @@
 #include "mq_torch.hpp"
 
 #include <algorithm>
+#include <initializer_list>
 #include <utility>
 
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/GradMode.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -155,6 +157,20 @@ struct Call {
       : device(d), modes(c10::DispatchKeySet({c10::DispatchKey::Python, c10::DispatchKey::PythonTLSSnapshot})) {}
 };
 
+// whether autograd follows one of them (null: not given); paged.py then marks
+// the outputs as having no gradient
+bool tracked(std::initializer_list<const at::Tensor*> ts) {
+  if (!c10::GradMode::is_enabled()) return false;
+  for (const at::Tensor* t : ts)
+    if (t && t->requires_grad()) return true;
+  return false;
+}
+// a cache that the call wrote
+void written(PyObject* o) {
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 PyObject* status(int rc) { return PyLong_FromLong(rc); }
 PyObject* wrong_count(const char* what) {
   PyErr_SetString(PyExc_TypeError, what);
@@ -168,7 +184,8 @@ PyObject* paged_rope_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 11) return wrong_count("paged_rope_kv: 11 arguments");
   Cache k;
   const at::Tensor *x = plain(a[0]), *co = plain(a[1]), *si = plain(a[2]), *pos = plain(a[3]);
-  if (!x || !co || !si || !pos || !k.take(a[4], a[5], a[6], a[7], true)) return decline();
+  if (!x || !co || !si || !pos || !k.take(a[4], a[5], a[6], a[7], true) || tracked({x, co, si, plain(a[4]), plain(a[5])}))
+    return decline();
   const int64_t D = k.c.head_dim, KVH = k.c.kv_heads;
   if (x->dim() != 2 || x->device() != k.dev || x->scalar_type() != k.ty || x->size(1) % D || x->size(1) / D <= 2 * KVH ||
       x->size(1) / D > INT32_MAX || x->stride(1) != 1)
@@ -209,6 +226,7 @@ PyObject* paged_rope_kv(PyObject*, PyObject* const* a, Py_ssize_t n) {
                         si->const_data_ptr<float>(), si->stride(0), co->size(0), pos->const_data_ptr<int64_t>(), ld_pos,
                         axes, a[9] == Py_None ? nullptr : sec, cu, rows, (int32_t)heads, out.mutable_data_ptr(), stream);
   Py_END_ALLOW_THREADS
+  if (rc == MQ_SUCCESS) written(a[4]), written(a[5]);
   return rc == MQ_SUCCESS ? THPVariable_Wrap(std::move(out)) : status(rc);
   END_HANDLE_TH_ERRORS
 }
@@ -219,7 +237,9 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Cache k;
   Query q;
   mq_paged_mask m{};
-  if (!k.take(a[1], a[2], a[3], a[4], false) || !q.take(a[0], k) || !mask(a + 5, k, q, &m)) return decline();
+  if (!k.take(a[1], a[2], a[3], a[4], false) || !q.take(a[0], k) || !mask(a + 5, k, q, &m) ||
+      tracked({q.t, plain(a[1]), plain(a[2]), plain(a[8])}))
+    return decline();
   const bool want_lse = a[12] == Py_True;
   void* stream = PyLong_AsVoidPtr(a[13]);
   if (PyErr_Occurred()) return nullptr;
@@ -259,7 +279,9 @@ PyObject* paged_attention_mass(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Query q;
   mq_paged_mask m{};
   const at::Tensor* lse = plain(a[4]);
-  if (!lse || !k.take(a[1], nullptr, a[2], a[3], false) || !q.take(a[0], k) || !mask(a + 5, k, q, &m)) return decline();
+  if (!lse || !k.take(a[1], nullptr, a[2], a[3], false) || !q.take(a[0], k) || !mask(a + 5, k, q, &m) ||
+      tracked({q.t, plain(a[1]), lse, plain(a[8])}))
+    return decline();
   if (lse->device() != k.dev || lse->scalar_type() != at::kFloat || lse->dim() != 2 || lse->size(0) != q.rows ||
       lse->size(1) != q.heads || !lse->is_contiguous())
     return decline();
@@ -289,7 +311,7 @@ PyObject* paged_evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const at::Tensor *mass = plain(a[4]), *to = plain(a[5]);
   int64_t budget, recent;
   if (!mass || !to || !k.take(a[0], a[1], a[2], a[3], true) || !index_rows(*to, k.dev) || to->size(0) != k.c.batch ||
-      to->size(1) < 1 || !as_int(a[6], &budget) || !as_int(a[7], &recent))
+      to->size(1) < 1 || !as_int(a[6], &budget) || !as_int(a[7], &recent) || tracked({plain(a[0]), plain(a[1]), mass}))
     return decline();
   if (mass->device() != k.dev || mass->scalar_type() != at::kFloat || mass->dim() != 3 || mass->size(0) != k.c.batch ||
       mass->size(1) != k.c.kv_heads || mass->size(2) != k.c.width * k.c.page_size || mass->stride(2) != 1)
@@ -310,6 +332,7 @@ PyObject* paged_evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
                       stream);
   Py_END_ALLOW_THREADS
   if (rc != MQ_SUCCESS) return status(rc);
+  written(a[0]), written(a[1]);
   PyObject* o[3] = {THPVariable_Wrap(std::move(kept)), THPVariable_Wrap(std::move(lens)), THPVariable_Wrap(std::move(left))};
   PyObject* r = o[0] && o[1] && o[2] ? PyTuple_Pack(3, o[0], o[1], o[2]) : nullptr;
   for (PyObject* x : o) Py_XDECREF(x);

@@ -25,7 +25,9 @@ width are cut to it, positions past the rotary tables to their last row.
 
 Every call launches HIP kernels of libmetal_native_amd.so on the current stream
 and returns without synchronising; workspaces come from torch's allocator on
-that stream.
+that stream.  None has a backward pass: where autograd follows an input, going
+back through the outputs raises, and a cache that is written may not require a
+gradient.
 """
 
 from __future__ import annotations
@@ -89,12 +91,35 @@ def _chunks(op, cu, table, rows):
     return cu.contiguous()
 
 
-def _finish(op, r):
+class _NoGradient(torch.autograd.Function):
+    """Outputs that autograd refuses to go back through."""
+
+    @staticmethod
+    def forward(ctx, op, out, *inputs):
+        ctx.op = op
+        return out
+
+    @staticmethod
+    def backward(ctx, *grads):
+        _invalid(f"{ctx.op}: has no backward pass (call it under torch.no_grad(), or detach what goes in)")
+
+
+def _tracked(op, read, written=()):
+    """The inputs that autograd follows; raises where one of them is written."""
+    if not torch.is_grad_enabled():
+        return []
+    for t in written:
+        if t.requires_grad:
+            _invalid(f"{op}: a cache that requires a gradient is written in place (call it under torch.no_grad())")
+    return [t for t in read if isinstance(t, torch.Tensor) and t.requires_grad]
+
+
+def _finish(op, r, tracked=()):
     if r is None:
         _invalid(f"{op}: arguments not supported (memory overlaps, strides out of range, or a tensor without memory of its own)")
     if type(r) is int:
         _check(r)
-    return r
+    return _NoGradient.apply(op, r, *tracked) if tracked else r
 
 
 def rope_kv(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: torch.Tensor, k_cache: torch.Tensor,
@@ -137,12 +162,16 @@ def rope_kv(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: torch.
     if pos.dtype != torch.int64 or tuple(pos.shape) not in (((axes, rows), (rows,)) if axes == 1 else ((axes, rows),)):
         _invalid(f"{op}: pos must be Int64 [rows], or [axes, rows] with sections")
     cu = _chunks(op, cu, table, rows)
-    fresh = torch.contiguous_format
-    qkv, cos, sin, pos = (t.clone(memory_format=fresh) for t in (qkv, cos, sin, pos))
-    with torch.cuda.device(qkv.device):
-        r = _mq_torch.paged_rope_kv(qkv, cos, sin, pos, k_cache, v_cache, table, lens, cu, sections,
-                                    _raw_stream(qkv.get_device()))
-    return _finish(op, r)
+    tracked = _tracked(op, (qkv, cos, sin), (k_cache, v_cache))
+    with torch.no_grad(), torch.cuda.device(qkv.device):
+        for copied in (False, True):   # as they are, then laid out anew
+            if copied:
+                qkv, cos, sin, pos = (t.clone(memory_format=torch.contiguous_format) for t in (qkv, cos, sin, pos))
+            r = _mq_torch.paged_rope_kv(qkv, cos, sin, pos, k_cache, v_cache, table, lens, cu, sections,
+                                        _raw_stream(qkv.get_device()))
+            if r is not None:
+                break
+    return _finish(op, r, tracked)
 
 
 def _mask(op, q, k_cache, table, cu, scale, softcap, slopes, window, prefix_lens, max_q):
@@ -163,7 +192,7 @@ def _mask(op, q, k_cache, table, cu, scale, softcap, slopes, window, prefix_lens
         if prefix_lens.dtype != torch.int32 or tuple(prefix_lens.shape) != (table.shape[0],) or prefix_lens.device != q.device:
             _invalid(f"{op}: prefix_lens must be Int32 [batch] = [{table.shape[0]}]")
         prefix_lens = prefix_lens.contiguous()
-    return q.clone(memory_format=torch.contiguous_format), cu, float(scale), float(softcap), slopes, int(window), prefix_lens, int(max_q)
+    return cu, float(scale), float(softcap), slopes, int(window), prefix_lens, int(max_q)
 
 
 def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
@@ -194,11 +223,15 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, tab
             return _finish(op, r)
     q, k_cache, v_cache, table, lens, cu, slopes, prefix_lens = _plain(q, k_cache, v_cache, table, lens, cu, slopes, prefix_lens)
     table, lens = _cache(op, k_cache, v_cache, table, lens)
-    q, *how = _mask(op, q, k_cache, table, cu, scale, softcap, slopes, window, prefix_lens, max_q)
-    with torch.cuda.device(q.device):
-        r = _mq_torch.paged_attention(q, k_cache, v_cache, table, lens, *how, bool(return_lse),
-                                      _raw_stream(q.get_device()))
-    return _finish(op, r)
+    tracked = _tracked(op, (q, k_cache, v_cache, slopes))
+    how = _mask(op, q, k_cache, table, cu, scale, softcap, slopes, window, prefix_lens, max_q)
+    with torch.no_grad(), torch.cuda.device(q.device):
+        for copied in (False, True):   # as it is, then laid out anew
+            r = _mq_torch.paged_attention(q.clone(memory_format=torch.contiguous_format) if copied else q, k_cache, v_cache,
+                                          table, lens, *how, bool(return_lse), _raw_stream(q.get_device()))
+            if r is not None:
+                break
+    return _finish(op, r, tracked)
 
 
 def attention_mass(q: torch.Tensor, k_cache: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, lse: torch.Tensor,
@@ -224,14 +257,18 @@ def attention_mass(q: torch.Tensor, k_cache: torch.Tensor, table: torch.Tensor, 
             return _finish(op, r)
     q, k_cache, table, lens, lse, cu, slopes, prefix_lens = _plain(q, k_cache, table, lens, lse, cu, slopes, prefix_lens)
     table, lens = _cache(op, k_cache, None, table, lens, keys_only=True)
-    q, *how = _mask(op, q, k_cache, table, cu, scale, softcap, slopes, window, prefix_lens, max_q)
+    tracked = _tracked(op, (q, k_cache, lse, slopes))
+    how = _mask(op, q, k_cache, table, cu, scale, softcap, slopes, window, prefix_lens, max_q)
     _require_cuda(lse, "lse", op)
     if lse.dtype != torch.float32 or tuple(lse.shape) != tuple(q.shape[:2]) or lse.device != q.device:
         _invalid(f"{op}: lse must be Float32 [rows, heads] = {list(q.shape[:2])}")
-    with torch.cuda.device(q.device):
-        r = _mq_torch.paged_attention_mass(q, k_cache, table, lens, lse.contiguous(), *how,
-                                           _raw_stream(q.get_device()))
-    return _finish(op, r)
+    with torch.no_grad(), torch.cuda.device(q.device):
+        for copied in (False, True):
+            r = _mq_torch.paged_attention_mass(q.clone(memory_format=torch.contiguous_format) if copied else q, k_cache, table, lens,
+                                               lse.contiguous(), *how, _raw_stream(q.get_device()))
+            if r is not None:
+                break
+    return _finish(op, r, tracked)
 
 
 def evict(k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, mass: torch.Tensor,
@@ -272,7 +309,8 @@ def evict(k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor, len
         _invalid(f"{op}: budget must be positive and recent 0 .. budget, got {budget} and {recent}")
     if to.shape[1] * ps < budget:
         _invalid(f"{op}: {to.shape[1]} pages of {ps} slots cannot hold {budget}")
-    with torch.cuda.device(k_cache.device):
+    tracked = _tracked(op, (mass,), (k_cache, v_cache))
+    with torch.no_grad(), torch.cuda.device(k_cache.device):
         r = _mq_torch.paged_evict(k_cache, v_cache, table, lens, mass.contiguous(), to.contiguous(), budget, recent,
                                   _raw_stream(k_cache.get_device()))
-    return _finish(op, r)
+    return _finish(op, r, tracked)

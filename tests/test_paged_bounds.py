@@ -203,3 +203,77 @@ def test_rows_of_no_chunk(gpu, dtype, H, KVH, D, lens, new, before, after):
     assert bool(((out.double().cpu() - want).abs() <= ob).all())
     gl = lse.double().cpu()
     assert bool(((gl == wl) | ((gl - wl).abs() <= lb)).all())
+
+
+@pytest.mark.parametrize("op", ["rope_kv", "evict"])
+@pytest.mark.parametrize("name", ["k_cache", "v_cache"])
+def test_written_caches_may_not_require_gradients(op, name, monkeypatch):
+    from metal_native import MetalNativeError, paged
+    from test_paged_host import arguments
+
+    monkeypatch.setattr(paged, "_require_cuda", lambda *a: None)
+    kw = arguments(torch.device("cpu"))[op]
+    kw[name].requires_grad_()
+    with pytest.raises(MetalNativeError, match="written in place"):
+        getattr(paged, op)(**kw)
+
+
+@pytest.mark.gpu
+def test_gradients_are_refused_not_lost(gpu):
+    from metal_native import MetalNativeError, paged
+    from test_paged_host import arguments
+
+    floats = {"rope_kv": ("qkv", "cos", "sin"), "attention": ("q", "k_cache", "v_cache", "slopes"),
+              "attention_mass": ("q", "k_cache", "lse", "slopes"), "evict": ("mass",)}
+    for op, names in floats.items():
+        def call(**other):
+            kw = arguments(gpu)[op]
+            if "q" in kw:
+                kw["q"] = torch.randn(kw["q"].shape, device=gpu, generator=torch.Generator(gpu).manual_seed(1)).half()
+                kw["slopes"] = torch.full((kw["q"].shape[1],), 0.1, device=gpu)
+            kw.update({n: form(kw[n]) for n, form in other.items()})
+            r = getattr(paged, op)(**kw)
+            return r if isinstance(r, tuple) else (r,)
+
+        want = call()
+        assert not any(x.requires_grad for x in want)
+        for name in names:
+            got = call(**{name: lambda t: t.detach().clone().requires_grad_()})
+            assert len(got) == len(want) and all(torch.equal(a, b) for a, b in zip(want, got))
+            out = [x for x in got if x.is_floating_point()]
+            assert all(x.requires_grad for x in out)
+            for x in out:
+                with pytest.raises(MetalNativeError, match=f"paged.{op}: has no backward pass"):
+                    x.float().sum().backward()
+            with torch.no_grad():
+                assert not any(x.requires_grad for x in call(**{name: lambda t: t.detach().clone().requires_grad_()}))
+        if op in ("rope_kv", "evict"):
+            for name in ("k_cache", "v_cache"):
+                with pytest.raises(MetalNativeError, match="written in place"):
+                    call(**{name: lambda t: t.requires_grad_()})
+                with torch.no_grad():
+                    call(**{name: lambda t: t.requires_grad_()})
+
+
+@pytest.mark.gpu
+def test_autograd_sees_that_caches_were_written(gpu):
+    """A product that saved a cache for its own gradient notices the write; caches of inference mode have no counter."""
+    from metal_native import paged
+    from test_paged_host import arguments
+
+    for op, other in (("rope_kv", {}), ("evict", {})):
+        kw = arguments(gpu)[op]
+        w = torch.ones((), device=gpu, dtype=torch.float16, requires_grad=True)
+        before = (kw["k_cache"]._version, kw["v_cache"]._version)
+        y = (kw["k_cache"] * w).sum()
+        getattr(paged, op)(**kw)
+        assert kw["k_cache"]._version > before[0] and kw["v_cache"]._version > before[1]
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+        with torch.inference_mode():
+            kw = arguments(gpu)[op]
+        getattr(paged, op)(**kw)
+    for op in ("attention", "attention_mass"):   # only read
+        kw = arguments(gpu)[op]
+        getattr(paged, op)(**kw)
+        assert kw["k_cache"]._version == 0
