@@ -240,7 +240,8 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!k.take(a[1], a[2], a[3], a[4], false) || !q.take(a[0], k) || !mask(a + 5, k, q, &m) ||
       tracked({q.t, plain(a[1]), plain(a[2]), plain(a[8])}))
     return decline();
-  const bool want_lse = a[12] == Py_True;
+  const int want_lse = PyObject_IsTrue(a[12]);
+  if (want_lse < 0) return nullptr;
   void* stream = PyLong_AsVoidPtr(a[13]);
   if (PyErr_Occurred()) return nullptr;
   HANDLE_TH_ERRORS

@@ -277,3 +277,13 @@ def test_autograd_sees_that_caches_were_written(gpu):
         kw = arguments(gpu)[op]
         getattr(paged, op)(**kw)
         assert kw["k_cache"]._version == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("flag", [True, 1, "yes", False, 0, None])
+def test_return_lse_is_a_truth_value(gpu, flag):
+    from metal_native import paged
+    from test_paged_host import arguments
+
+    r = paged.attention(**arguments(gpu)["attention"], return_lse=flag)
+    assert (isinstance(r, tuple) and len(r) == 2) if flag else isinstance(r, torch.Tensor)
