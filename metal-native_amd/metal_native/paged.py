@@ -136,8 +136,10 @@ def rope_kv(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, pos: torch.
     frequencies that each axis (time, height, width) turns, in order.
     """
     op = "paged.rope_kv"
-    if sections is not None and type(sections) is not tuple:
-        sections = tuple(int(n) for n in sections)
+    if sections is not None and (type(sections) is not tuple or any(type(n) is not int for n in sections)):
+        given, sections = tuple(sections), tuple(int(n) for n in sections)
+        if given != sections:
+            _invalid(f"{op}: sections must be whole numbers, got {given}")
     if type(qkv) is torch.Tensor and qkv.is_cuda:
         r = _mq_torch.paged_rope_kv(qkv, cos, sin, pos, k_cache, v_cache, table, lens, cu, sections,
                                     _raw_stream(qkv.get_device()))

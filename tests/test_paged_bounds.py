@@ -287,3 +287,28 @@ def test_return_lse_is_a_truth_value(gpu, flag):
 
     r = paged.attention(**arguments(gpu)["attention"], return_lse=flag)
     assert (isinstance(r, tuple) and len(r) == 2) if flag else isinstance(r, torch.Tensor)
+
+
+def test_sections_that_are_not_whole_numbers(monkeypatch):
+    from metal_native import MetalNativeError, paged
+    from test_paged_host import arguments
+
+    monkeypatch.setattr(paged, "_require_cuda", lambda *a: None)
+    kw = arguments(torch.device("cpu"))["rope_kv"]
+    kw["pos"] = kw["pos"].expand(2, -1)
+    for sections in ((16.5, 15.5), [16.5, 16.5]):
+        with pytest.raises(MetalNativeError, match="whole numbers"):
+            paged.rope_kv(**{**kw, "sections": sections})
+
+
+@pytest.mark.gpu
+def test_sections_of_any_integer_type(gpu):
+    import numpy as np
+
+    from metal_native import paged
+    from test_paged_host import arguments
+
+    for sections in ((20, 12), [20, 12], (np.int64(20), np.int32(12)), np.array([20, 12]), torch.tensor([20, 12]), (20.0, 12)):
+        kw = arguments(gpu)["rope_kv"]
+        kw["pos"] = kw["pos"].expand(2, -1).contiguous()
+        assert paged.rope_kv(**{**kw, "sections": sections}).shape == (5, 8, 64)
