@@ -129,6 +129,7 @@ struct PagedArgs {
   const int32_t *lens, *cu, *prefix;
   const float* slopes;    // [heads] or null
   float scale, softcap;   // softcap 0: none
+  float inv_cap;          // 1 / softcap, finite
   int window;             // 0: none
   int b, rows, H, KVH, g, D, bf16;
   int max_q;              // the longest chunk, as far as the host knows it

@@ -1,6 +1,8 @@
 // C entries of the paged-cache operators: argument checks and launch.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+#include <cfloat>
 #include <climits>
 #include <cmath>
 #include <cstdio>
@@ -86,6 +88,7 @@ const char* attn_args(mq::PagedArgs& a, const mq_paged_cache* c, const mq_paged_
   a.slopes = m->slopes;
   a.scale = m->scale;
   a.softcap = m->softcap;
+  a.inv_cap = m->softcap > 0.f ? std::min(1.f / m->softcap, FLT_MAX) : 0.f;
   a.window = m->window > INT_MAX ? 0 : (int)m->window;   // wider than any sequence
   a.rows = (int)rows;
   a.H = heads;

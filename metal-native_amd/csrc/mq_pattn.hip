@@ -83,18 +83,18 @@ template <typename T> __device__ __forceinline__ u4 finite(u4 v) {
 template <int NB>
 __device__ __forceinline__ void cap_and_bias(const PagedArgs& p, const Rows& rw, f16v (&s)[NB], int tile0) {
   const int h = (threadIdx.x & 63) >> 5;
-  const float cap = p.softcap;
+  float scale = p.scale;
+  if (p.softcap != 0.f) {
+    cap_scores<true>(s, p);
+    scale = 1.f;
+  }
+  scale *= kLog2e;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
-      float x = s[nb][j] * p.scale;
-      if (cap != 0.f) {
-        const float e = __builtin_amdgcn_exp2f(x * (2.f * kLog2e / cap));   // tanh y = 1 - 2 / (e^2y + 1)
-        x = cap - 2.f * cap * __builtin_amdgcn_rcpf(e + 1.f);
-      }
       const int away = rw.pos - (tile0 + 32 * nb + 8 * (j / 4) + 4 * h + j % 4);
-      s[nb][j] = x * kLog2e - rw.slope2 * fabsf((float)away);
+      s[nb][j] = s[nb][j] * scale - rw.slope2 * fabsf((float)away);
     }
 }
 

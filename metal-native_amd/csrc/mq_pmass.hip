@@ -116,7 +116,11 @@ __global__ __launch_bounds__(256, 2) void paged_mass_kernel(PagedArgs p, float* 
 #pragma unroll
         for (int nb = 0; nb < 2; ++nb) sc[nb] = T::mfma(a, kr[nb][ks], sc[nb]);
       }
-      const float c = p.scale * kLog2e;
+      float c = p.scale * kLog2e;
+      if (EXTRA && p.softcap != 0.f) {
+        cap_scores<false>(sc, p);   // a lane's are of 16 rows
+        c = kLog2e;
+      }
 #pragma unroll
       for (int nb = 0; nb < 2; ++nb) {
         const int j = jw + 32 * nb + col;
@@ -129,16 +133,8 @@ __global__ __launch_bounds__(256, 2) void paged_mass_kernel(PagedArgs p, float* 
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             float z = sc[nb][4 * q4 + e];
-            if constexpr (EXTRA) {
-              float y = z * p.scale;
-              if (p.softcap != 0.f) {
-                const float ex = __builtin_amdgcn_exp2f(y * (2.f * kLog2e / p.softcap));
-                y = p.softcap - 2.f * p.softcap * __builtin_amdgcn_rcpf(ex + 1.f);
-              }
-              z = y * kLog2e - sl[x][at + e] * fabsf((float)(ps[x][at + e] - j)) + n4[e];
-            } else {
-              z = __builtin_fmaf(z, c, n4[e]);
-            }
+            if constexpr (EXTRA) z = z * c - sl[x][at + e] * fabsf((float)(ps[x][at + e] - j)) + n4[e];
+            else z = __builtin_fmaf(z, c, n4[e]);
             v[e] = z;
           }
           if (masked) {

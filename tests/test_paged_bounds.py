@@ -312,3 +312,52 @@ def test_sections_of_any_integer_type(gpu):
         kw = arguments(gpu)["rope_kv"]
         kw["pos"] = kw["pos"].expand(2, -1).contiguous()
         assert paged.rope_kv(**{**kw, "sections": sections}).shape == (5, 8, 64)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("cap", [1e-40, 0.5, 8.0, 50.0, 1e4, 1e6, 3e38])
+def test_caps_of_every_size(gpu, cap, many):
+    """A cap far above the scores leaves them as they are.  Bounds: with S = scale max sum |q k| and X the largest score
+    in size, dx = (D + 4) e S + 32 e X + 4 e X (a product of D terms; the cap, 22 e at most; units of log 2): a weight is
+    off by 2 dx of itself, by u where it is rounded, an output by u again; the log sum by dx + (n + 8) e + 2 e of itself."""
+    from metal_native import paged
+
+    H, KVH, D, ps = 14, 2, 64, 16
+    lens, new = ([2000, 40, 1700], [1100, 40, 900]) if many else ([300, 1, 77, 130], [1, 1, 20, 130])
+    c = build(gpu, torch.float16, H, KVH, D, ps, lens, new, seed=3, amp=1.5)
+    cap = float(torch.tensor(cap, dtype=torch.float32))
+    how = dict(scale=0.2, softcap=cap)
+    out, lse = paged.attention(c["q"], c["k"], c["v"], c["table"], c["lens"], c["cu"], return_lse=True, **how)
+    m = paged.attention_mass(c["q"], c["k"], c["table"], c["lens"], lse, c["cu"], **how)
+    E, n = ref.E, max(lens)
+    at = torch.zeros(3 if many else 4, KVH, c["table"].shape[1] * ps, dtype=torch.float64)
+    for s in range(len(lens)):
+        for kv in range(KVH):
+            x, _, see, (start, n_new, total) = ref.seq_scores(c["q"], c["k"], c["table"], c["lens"], c["cu"], s, kv, **how)
+            plain, _, _, _ = ref.seq_scores(c["q"], c["k"], c["table"], c["lens"], c["cu"], s, kv, scale=0.2)
+            kk, _ = ref.gather(c["k"], c["table"][s], total, kv)
+            vv, _ = ref.gather(c["v"], c["table"][s], total, kv)
+            qq = c["q"][start:start + n_new, 7 * kv:7 * kv + 7].double().cpu()
+            S = 0.2 * float(torch.matmul(qq.abs(), kk.abs().t()).max())
+            X = float(torch.where(see, plain, torch.zeros_like(plain)).abs().max())
+            dx = (D + 4) * E * S + 36 * E * X
+            l = torch.logsumexp(x, -1)
+            w = torch.exp(x - l[..., None])
+            o = torch.matmul(w, vv)
+            a = torch.matmul(w, vv.abs())
+            u = ref.half_step(torch.float16)
+            ob = u * (a + o.abs()) + (2 * dx + 2 * (total + 8) * E) * a + total * 2.0**-32 * float(vv.abs().max()) + 2.0**-25
+            rows, hs = slice(start, start + n_new), slice(7 * kv, 7 * kv + 7)
+            err = (out[rows, hs].double().cpu().transpose(0, 1) - o).abs()
+            assert bool((err <= ob).all()), float((err / ob).max())
+            err, lb = (lse[rows, hs].double().cpu().t() - l).abs(), dx + (total + 8) * E + 2 * E * l.abs()
+            assert bool((err <= lb).all()), float((err / lb).max())
+            # the mass against the log sums that the call was given: dx + 4 e (1 + |lse|) a weight, and the sums
+            given = lse[rows, hs].double().cpu().t()
+            t = torch.where(see, torch.exp(x - given[..., None]), torch.zeros_like(x)).sum((0, 1))
+            at[s, kv, :total] = t
+            mb = t * (dx + (4 * (1 + float(given.abs().max())) + 4 * (n_new * 7) ** 0.5 + 80) * E) + 2.0**-120
+            err = (m[s, kv, :total].double().cpu() - t).abs()
+            assert bool((err <= mb).all()), float((err / mb).max())
+    assert float(m.double().cpu().sub(at).abs().max()) < 1   # and nothing past the sequences
