@@ -30,6 +30,45 @@ namespace {
 
 constexpr int kSlotsM = 256, kRowsM = 64;
 
+// The weight that slot j got from rows r0 .. r1 of sequence s's chunk, on all
+// lanes of the wave: a row to a lane, in plain arithmetic, until it is NaN.  For
+// slots whose sum above is NaN, which an infinite key makes of a row of zeros.
+// The arguments (the kernel's first) are read once more from where they lie, so
+// that none is kept in registers for this.
+template <typename T, int D>
+__device__ __forceinline__ float weight_of_slot(int s, int kv, int j, int r0, int64_t r1) {
+  uint64_t args = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(args));
+  const PagedArgs& p = *(const PagedArgs*)args;
+  const PagedSeq sq = load_seq(p, s);
+  const int page = paged_page(p.table + (int64_t)s * p.ld_table, j, sq.len, p.shift, p.pages);
+  if (page < 0) return 0.f;
+  typedef typename T::e e8 __attribute__((ext_vector_type(8)));
+  const e8* k = (const e8*)((const uint16_t*)p.k.ptr + page * p.k.page + kv * p.k.head + (int64_t)(j & ((1 << p.shift) - 1)) * p.k.slot);
+  float t = 0.f;
+#pragma unroll 1
+  for (int64_t r = r0 + (int64_t)(threadIdx.x & 63); r < r1; r += 64) {
+    const int i = (int)p.gdiv.div((uint32_t)r), a = kv * p.g + (int)r - i * p.g, pos = sq.len - sq.n + i;
+    const float lse = p.lse[(int64_t)(sq.start + i) * p.H + a];
+    const e8* q = (const e8*)((const uint16_t*)p.q + (int64_t)(sq.start + i) * p.q_t + (int64_t)a * p.q_h);
+    float x = 0.f;
+#pragma unroll 4
+    for (int d = 0; d < D / 8; ++d) {
+      const e8 y = q[d], z = k[d];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x += (float)y[e] * (float)z[e];
+    }
+    x *= p.scale;
+    if (p.softcap != 0.f) x = p.softcap * (1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * p.inv_cap * (2.f * kLog2e)) + 1.f));
+    if (p.slopes) x -= p.slopes[a] * fabsf((float)(pos - j));
+    if (lse != -INFINITY && paged_visible(pos, j, sq.len, sq.prefix, p.window)) t += __builtin_amdgcn_exp2f((x - lse) * kLog2e);
+    if (__any(t != t)) break;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o);
+  return t;
+}
+
 template <typename T, int D, bool EXTRA>
 __global__ __launch_bounds__(256, 2) void paged_mass_kernel(PagedArgs p, float* out, int parts) {
   constexpr int ROW = Lay<D>::ROW, GS = Lay<D>::GS, NG = kRowsM / GS / 4;
@@ -73,17 +112,15 @@ __global__ __launch_bounds__(256, 2) void paged_mass_kernel(PagedArgs p, float* 
       lds_load16(base, r0 + gi * GS < total ? 0x7fffffffu : 0u, r < total ? off : kOob, dst + 64 * gi);
     }
   };
-  // lse, position and slope of row tid of a block
+  // lse of row `lane` of a block, and in wave 0 its position and slope
   float my_lse = 0.f, my_slope = 0.f;
   int my_pos = 0;
   auto row_info = [&](int b) {
-    const int r = ra + b * kRowsM + tid;
-    if (tid < kRowsM) {
-      const int i = (int)p.gdiv.div(r), a = kv * p.g + r - i * p.g;
-      my_pos = off + i;
-      my_lse = r < total ? p.lse[(int64_t)(sq.start + i) * p.H + a] : -INFINITY;
-      my_slope = EXTRA && p.slopes && r < total ? p.slopes[a] : 0.f;
-    }
+    const int r = ra + b * kRowsM + lane;
+    const int i = (int)p.gdiv.div(r), a = kv * p.g + r - i * p.g;
+    my_pos = off + i;
+    my_lse = r < total ? p.lse[(int64_t)(sq.start + i) * p.H + a] : -INFINITY;
+    if (tid < kRowsM) my_slope = EXTRA && p.slopes && r < total ? p.slopes[a] : 0.f;
   };
   const int jw = j0 + 64 * w;
   float sum[2] = {0.f, 0.f}, mid[2] = {0.f, 0.f};
@@ -93,6 +130,16 @@ __global__ __launch_bounds__(256, 2) void paged_mass_kernel(PagedArgs p, float* 
       nl[x][tid] = my_lse == -INFINITY ? -INFINITY : -my_lse * kLog2e;
       ps[x][tid] = my_pos;
       sl[x][tid] = my_slope * kLog2e;
+    }
+    // rows of lse -inf add nothing, whatever their queries hold: each wave clears
+    // those that it loaded (past the last row there are zeros already)
+    const uint64_t none = __ballot(my_lse == -INFINITY && ra + b * kRowsM + lane < total);
+    if (__builtin_expect(none != 0, 0)) {
+      int l = lane;
+      asm volatile("" : "+v"(l));   // nothing of this is kept over the blocks: it would cost a wave per SIMD
+#pragma unroll 1
+      for (int gi = w; gi < kRowsM / GS; gi += 4)
+        if ((none >> (gi * GS + l / ROW)) & 1) qs[x][64 * gi + l] = (u4){0u, 0u, 0u, 0u};
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
@@ -175,6 +222,14 @@ __global__ __launch_bounds__(256, 2) void paged_mass_kernel(PagedArgs p, float* 
     float t = sum[nb] + mid[nb];
     t += swap32(t);
     const int j = jw + 32 * nb + col;
+    if (__builtin_expect(__any(t != t), 0)) {
+      uint64_t again = __ballot(t != t) & 0xFFFFFFFFull;   // both halves hold t
+      for (; again; again &= again - 1) {
+        const int at = __ffsll((unsigned long long)again) - 1;
+        const float v = weight_of_slot<T, D>(s, kv, jw + 32 * nb + at, ra + b0 * kRowsM, min(ra + (int64_t)b1 * kRowsM, (int64_t)total));
+        if (col == at) t = v;
+      }
+    }
     if (h == 0 && j < slots) dst[j] = have[nb] ? t : 0.f;
   }
 }

@@ -361,3 +361,33 @@ def test_caps_of_every_size(gpu, cap, many):
             err = (m[s, kv, :total].double().cpu() - t).abs()
             assert bool((err <= mb).all()), float((err / mb).max())
     assert float(m.double().cpu().sub(at).abs().max()) < 1   # and nothing past the sequences
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("chunk", [False, True])
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+def test_mass_of_infinite_keys_and_rows_left_out(gpu, dtype, chunk, cap):
+    """A key of -inf under positive queries has no weight, also where a block of rows is not full; rows whose log sum is
+    -inf add nothing, whatever their queries hold."""
+    from metal_native import paged
+
+    lens, new = [300, 70, 200], ([40, 1, 130] if chunk else None)
+    c = build(gpu, DT[dtype], 8, 2, 64, 16, lens, new, seed=5)
+    c["q"][..., 3] = c["q"][..., 3].abs() + 0.5
+    for s, slot in ((0, 17), (0, 150), (1, 69), (2, 0)):
+        c["k"][c["table"][s, slot // 16].long(), :, slot % 16, 3] = -float("inf")
+    how = dict(softcap=cap)
+    if not cap:   # with a cap an infinite score is a weight like others
+        _, lse, scale = check_attention(c)
+        got = paged.attention_mass(c["q"], c["k"], c["table"], c["lens"], lse, c["cu"], scale=scale)
+        want, bound = ref.mass(c["q"], c["k"], c["table"], c["lens"], lse, c["cu"], scale=scale)
+        assert bool(((got.double().cpu() - want).abs() <= bound).all())
+        assert float(got[0, :, 17].abs().max()) == 0 and float(got[1, :, 69].abs().max()) == 0
+    c = build(gpu, DT[dtype], 8, 2, 64, 16, lens, new, seed=6)
+    _, lse = paged.attention(c["q"], c["k"], c["v"], c["table"], c["lens"], c["cu"], return_lse=True, **how)
+    out = torch.rand(lse.shape, device=gpu, generator=c["gen"]) < 0.3
+    want = paged.attention_mass(c["q"], c["k"], c["table"], c["lens"], lse.masked_fill(out, -float("inf")), c["cu"], **how)
+    for junk in (float("nan"), float("inf")):
+        q = c["q"].masked_fill(out[..., None], junk)
+        assert torch.equal(want, paged.attention_mass(q, c["k"], c["table"], c["lens"], lse.masked_fill(out, -float("inf")), c["cu"], **how))
