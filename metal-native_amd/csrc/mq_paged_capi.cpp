@@ -89,7 +89,7 @@ const char* attn_args(mq::PagedArgs& a, const mq_paged_cache* c, const mq_paged_
   a.scale = m->scale;
   a.softcap = m->softcap;
   a.inv_cap = m->softcap > 0.f ? std::min(1.f / m->softcap, FLT_MAX) : 0.f;
-  a.window = m->window > INT_MAX ? 0 : (int)m->window;   // wider than any sequence
+  a.window = m->window >= a.cap ? 0 : (int)m->window;   // as wide as any sequence: hides nothing
   a.rows = (int)rows;
   a.H = heads;
   a.g = heads / c->kv_heads;

@@ -978,7 +978,7 @@ int64_t most_slots(const PagedArgs& a, int rows, int tk) {   // that a row block
 // 70, 800 over 1000 (22 M) 70 and 71, 128 over 8192 (29 M) 110 and 67.
 constexpr int64_t kWork = 4 << 20, kWorkExtra = 24 << 20;
 bool many_rows(const PagedArgs& a) {
-  const int64_t slots = a.window > 0 ? std::min<int64_t>(a.cap, a.window + kRowsP) : a.cap;
+  const int64_t slots = a.window > 0 ? std::min<int64_t>(a.cap, (int64_t)a.window + kRowsP) : a.cap;
   return ((int64_t)(a.rows - a.b) * a.g >= 128 * (int64_t)a.b && (int64_t)a.rows * a.H * slots >= (a.extra() ? kWorkExtra : kWork)) ||
          row_blocks(a, kRowsS) > 65535;   // the grid's z
 }

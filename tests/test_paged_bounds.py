@@ -391,3 +391,39 @@ def test_mass_of_infinite_keys_and_rows_left_out(gpu, dtype, chunk, cap):
     for junk in (float("nan"), float("inf")):
         q = c["q"].masked_fill(out[..., None], junk)
         assert torch.equal(want, paged.attention_mass(q, c["k"], c["table"], c["lens"], lse.masked_fill(out, -float("inf")), c["cu"], **how))
+
+
+@pytest.mark.parametrize("op", ["attention", "attention_mass"])
+def test_a_window_past_the_table_is_no_window(op):
+    """The same plan (its workspace) as without one, up to the largest number."""
+    import ctypes
+
+    from metal_native import _lib
+    from test_paged_host import Cache, Mask
+
+    size = getattr(_lib.load(), f"mq_paged_{op}_workspace_size")
+    for rows, width in ((4096, 512), (64, 512), (512, 512), (1, 4096)):
+        c = Cache(k=4096, v=4096, k_page=8192, k_head=2048, k_slot=128, v_page=8192, v_head=2048, v_slot=128, pages=600, kv_heads=4,
+                  page_size=16, head_dim=128, dtype=0, table=4096, ld_table=width, width=width, batch=1, lens=4096)
+
+        def need(window):
+            m = Mask(scale=0.1, softcap=0.0, slopes=None, window=window, prefix_lens=None, cu_q=4096, max_q=rows)
+            return size(ctypes.byref(c), ctypes.byref(m), rows, 28)
+
+        want = need(0)
+        assert want >= 0
+        for window in (width * 16, width * 16 + 1, 2**31 - 257, 2**31 - 1, 2**31, 2**62):
+            assert need(window) == want, window
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("window", [800, 2**31 - 1, 2**40])
+def test_windows_past_the_table(gpu, window):
+    from metal_native import paged
+
+    c = build(gpu, torch.float16, 28, 4, 128, 16, [790, 40, 513], [300, 40, 1], seed=9)
+    a, la = paged.attention(c["q"], c["k"], c["v"], c["table"], c["lens"], c["cu"], return_lse=True)
+    b, lb = paged.attention(c["q"], c["k"], c["v"], c["table"], c["lens"], c["cu"], window=window, return_lse=True)
+    assert torch.equal(a, b) and torch.equal(la, lb)
+    assert torch.equal(paged.attention_mass(c["q"], c["k"], c["table"], c["lens"], la, c["cu"]),
+                       paged.attention_mass(c["q"], c["k"], c["table"], c["lens"], la, c["cu"], window=window))
