@@ -11,6 +11,8 @@ the host and go to the device as one small copy a call.
 
 from __future__ import annotations
 
+from operator import index
+
 import torch
 
 from . import ops, paged
@@ -54,6 +56,12 @@ class PagedServer:
         idle = [s for s in range(len(self.lens)) if s not in self.last]
         if len(prompts) > len(idle) or any(not 0 < len(p) <= self.model.cfg.max_len for p in prompts):
             raise ValueError("PagedServer.start: more prompts than idle sequences, or one empty or past max_len")
+        try:   # the embedding is read on the GPU, where an index past its rows ends the process
+            prompts = [[index(t) for t in p] for p in prompts]
+        except TypeError as e:
+            raise ValueError(f"PagedServer.start: a token is not a whole number ({e})") from None
+        if any(not 0 <= t < self.model.cfg.vocab for p in prompts for t in p):
+            raise ValueError(f"PagedServer.start: a token outside the vocabulary of {self.model.cfg.vocab}")
         ids, at, out = idle[:len(prompts)], 0, {}
         try:
             while any(len(p) > at for p in prompts):
