@@ -34,6 +34,10 @@ class PagedServer:
         cfg = model.cfg
         if min(pages, batch, chunk) < 1 or (budget is not None and (budget < 1 or slack < 1)):
             raise ValueError("PagedServer: pages, batch, chunk, budget and slack must be positive")
+        if budget is not None and recent is not None and not 0 <= recent <= budget:
+            raise ValueError(f"PagedServer: recent must be 0 .. budget, got {recent} of {budget}")
+        if not 8 <= page_size <= 65536 or page_size & (page_size - 1):
+            raise ValueError(f"PagedServer: page_size must be a power of two from 8 to 65536, got {page_size}")
         self.model, self.page_size, self.chunk, self.budget, self.slack = model, page_size, chunk, budget, slack
         self.recent = budget // 2 if budget is not None and recent is None else recent
         most = cfg.max_len if budget is None else min(cfg.max_len, budget + slack + chunk)
