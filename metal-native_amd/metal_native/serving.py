@@ -138,8 +138,10 @@ class PagedServer:
             k, v = self.kv[li, 0], self.kv[li, 1]
             qkv = layer["qkv"](ops.add_rmsnorm(x, delta, layer["ln1"], m.cfg.eps))
             q = paged.rope_kv(qkv, m.cos, m.sin, pos, k, v, table, lens, cu)
-            a, lse = paged.attention(q, k, v, table, lens, cu, max_q=max_q, return_lse=True)
-            if self.mass is not None:
+            if self.mass is None:
+                a = paged.attention(q, k, v, table, lens, cu, max_q=max_q)
+            else:
+                a, lse = paged.attention(q, k, v, table, lens, cu, max_q=max_q, return_lse=True)
                 self.mass[li].index_add_(0, rows, paged.attention_mass(q, k, table, lens, lse, cu, max_q=max_q))
             o = layer["o"](a.reshape(a.shape[0], -1))
             delta = layer["down"](layer["gate_up"](ops.add_rmsnorm(x, o, layer["ln2"], m.cfg.eps), "swiglu"))

@@ -427,3 +427,18 @@ def test_windows_past_the_table(gpu, window):
     assert torch.equal(a, b) and torch.equal(la, lb)
     assert torch.equal(paged.attention_mass(c["q"], c["k"], c["table"], c["lens"], la, c["cu"]),
                        paged.attention_mass(c["q"], c["k"], c["table"], c["lens"], la, c["cu"], window=window))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("budget", [None, 20])
+def test_serving_asks_for_log_sums_only_where_it_cuts(gpu, monkeypatch, budget):
+    from metal_native import paged
+    from metal_native.serving import PagedServer
+    from test_serving import PROMPTS, model_of
+
+    asked, attention = [], paged.attention
+    monkeypatch.setattr(paged, "attention", lambda *a, **how: asked.append(bool(how.get("return_lse"))) or attention(*a, **how))
+    server = PagedServer(model_of(gpu), 24, 4, chunk=24, **({} if budget is None else dict(budget=budget, recent=6, slack=5)))
+    server.start(PROMPTS)
+    server.step()
+    assert set(asked) == {budget is not None}
