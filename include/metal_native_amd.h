@@ -316,6 +316,12 @@ MQ_API int mq_paged_attention(const mq_paged_cache* cache, const mq_paged_mask* 
                               int64_t q_head, int64_t rows, int32_t heads, void* out, float* lse, void* workspace,
                               int64_t workspace_bytes, void* stream);
 
+/* What such a call would launch on the current device, from the same host values:
+ * the rows of a workgroup's block (32 or 256: query heads of a kv_head times
+ * tokens) and the most parts that a block's slots are dealt out to.  Status. */
+MQ_API int mq_paged_attention_plan(const mq_paged_cache* cache, const mq_paged_mask* mask, int64_t rows, int32_t heads,
+                                   int32_t* block_rows, int32_t* parts);
+
 /* mass [batch, kv_heads, width * page_size]: the sum over the call's tokens and
  * the query heads of a key/value head of exp(x - lse), zero past lens.  Rows of
  * lse -inf add nothing.  v is not read. */

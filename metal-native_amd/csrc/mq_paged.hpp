@@ -140,6 +140,11 @@ struct PagedArgs {
   bool extra() const { return softcap != 0.f || slopes != nullptr; }
 };
 
+struct PagedPlan {
+  int block_rows;   // kRowsS or kRowsP of mq_pattn.hip
+  int64_t parts;
+};
+PagedPlan pattn_plan(const PagedArgs& a, int num_cus);
 size_t pattn_workspace(const PagedArgs& a, int num_cus);
 hipError_t pattn_launch(const PagedArgs& a, int num_cus, void* ws, hipStream_t s);
 size_t pmass_workspace(const PagedArgs& a, int num_cus);

@@ -178,6 +178,18 @@ MQ_API int64_t mq_paged_attention_workspace_size(const mq_paged_cache* c, const 
   return (int64_t)mq::pattn_workspace(a, mq::current_num_cus());
 }
 
+MQ_API int mq_paged_attention_plan(const mq_paged_cache* c, const mq_paged_mask* m, int64_t rows, int32_t heads,
+                                   int32_t* block_rows, int32_t* parts) {
+  const char* op = "paged.attention";
+  mq::PagedArgs a;
+  if (const char* bad = attn_args(a, c, m, rows, heads, true)) return refuse(op, bad);
+  if (!block_rows || !parts) return refuse(op, "null output");
+  const mq::PagedPlan plan = mq::pattn_plan(a, mq::current_num_cus());
+  *block_rows = plan.block_rows;
+  *parts = (int32_t)plan.parts;
+  return MQ_SUCCESS;
+}
+
 MQ_API int mq_paged_attention(const mq_paged_cache* c, const mq_paged_mask* m, const void* q, int64_t q_token,
                               int64_t q_head, int64_t rows, int32_t heads, void* out, float* lse, void* ws,
                               int64_t ws_bytes, void* stream) {

@@ -1064,6 +1064,11 @@ hipError_t launch(const PagedArgs& a, int num_cus, void* ws, hipStream_t s) {
 
 }  // namespace
 
+PagedPlan pattn_plan(const PagedArgs& a, int num_cus) {
+  if (many_rows(a)) return {kRowsP, rows_plan(a, num_cus).parts};
+  return {kRowsS, split_plan(a, num_cus).parts};
+}
+
 size_t pattn_workspace(const PagedArgs& a, int num_cus) {
   return many_rows(a) ? rows_plan(a, num_cus).ws_bytes : split_plan(a, num_cus).ws_bytes;
 }

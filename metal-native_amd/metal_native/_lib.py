@@ -84,6 +84,7 @@ SIGNATURES = {
     "mq_paged_rope_kv": (_i32, [_c_void_p, _c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64, _i64, _c_void_p, _i64, _i32,
                                 _c_void_p, _c_void_p, _i64, _i32, _c_void_p, _c_void_p]),
     "mq_paged_attention_workspace_size": (_i64, [_c_void_p, _c_void_p, _i64, _i32]),
+    "mq_paged_attention_plan": (_i32, [_c_void_p, _c_void_p, _i64, _i32, _c_void_p, _c_void_p]),
     "mq_paged_attention": (_i32, [_c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i64, _i32, _c_void_p, _c_void_p,
                                   _c_void_p, _i64, _c_void_p]),
     "mq_paged_attention_mass_workspace_size": (_i64, [_c_void_p, _c_void_p, _i64, _i32]),
