@@ -479,7 +479,8 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p, float* 
   // whether some page in reach is not one of the cache
   bool gaps = false;
   for (int range = 0; range < 2; ++range) {
-    const int from = range ? span.lo * TK : 0, to = min(range ? span.hi * TK : span.pre * TK, sq.len);
+    // the last tile may end past 2^31
+    const int from = range ? span.lo * TK : 0, to = (int)min((int64_t)(range ? span.hi : span.pre) * TK, (int64_t)sq.len);
     for (int x = (from >> p.shift) + threadIdx.x; (int64_t)x << p.shift < to; x += 512) gaps |= row[x] < 0 || row[x] >= p.pages;
   }
   // values of "tile -1", which tile 0's first phase multiplies by weights of zero:
@@ -567,7 +568,7 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs p, float* 
   if (!gaps) {
     auto clean = [&](int i) {
       const int t0 = tile_at(i) * TK;
-      return t0 + TK - 1 <= rw.first && t0 + TK <= sq.len && (p.window <= 0 || (int64_t)t0 > (int64_t)rw.last - p.window);
+      return t0 + TK - 1 <= rw.first && t0 <= sq.len - TK && (p.window <= 0 || (int64_t)t0 > (int64_t)rw.last - p.window);
     };
     // one run of tiles: before it lie those of the prefix and the window's edge,
     // after it those past the wave's first row or the sequence

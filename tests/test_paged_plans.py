@@ -90,3 +90,32 @@ def test_many_rows_masked(gpu, dtype, name):
     if "prefix" in how:
         how["prefix"] = torch.tensor(how["prefix"], dtype=torch.int32, device=gpu)
     check_attention(c, **how)
+
+
+@pytest.mark.gpu
+def test_absent_pages_at_the_end_of_the_longest_sequence(gpu):
+    """2^31 - 32 slots, whose last tile of 64 ends past 32 bits: 600 tokens that see the last 300 slots, one page of them absent."""
+    from metal_native import paged
+
+    H, D, ps, n, window, width = 16, 64, 32, 600, 300, 2**26 - 1
+    assert plan(n, H, 1, D, ps, 1, width, window=window)[0] == 256
+    g = torch.Generator(device=gpu)
+    g.manual_seed(2)
+    tail = 40   # pages whose slots these tokens may see
+    k, v = (torch.randn(tail, 1, ps, D, device=gpu, generator=g).half() for _ in range(2))
+    far = torch.zeros(1, width, dtype=torch.int32, device=gpu)
+    far[0, -tail:] = torch.arange(tail, device=gpu)
+    for absent in (None, 1, 2, 9):
+        near = torch.arange(tail, dtype=torch.int32, device=gpu)[None].clone()
+        far[0, -tail:] = near[0]
+        if absent:
+            near[0, -absent] = far[0, -absent] = -1
+        q = torch.randn(n, H, D, device=gpu, generator=g).half()
+        cu = torch.tensor([0, n], dtype=torch.int32, device=gpu)
+        end = torch.tensor([width * ps], dtype=torch.int32, device=gpu)
+        a, la = paged.attention(q, k, v, far, end, cu, window=window, return_lse=True)
+        b, lb = paged.attention(q, k, v, near, torch.tensor([tail * ps], dtype=torch.int32, device=gpu), cu, window=window, return_lse=True)
+        # the same slots in other tiles: two results, each within the bounds of one
+        e = torch.finfo(torch.float16).eps / 2
+        assert bool(((la - lb).abs() <= 2 * ((D + 4) * 60 + n) * 2.0**-24).all())
+        assert bool(((a - b).float().abs() <= 4 * e * v.float().abs().max()).all())
