@@ -36,7 +36,7 @@ constexpr float kAbove = 15.f, kBelow = 7.f;
 
 // What a wave knows of its 32 rows.
 struct Rows {
-  int pos;              // position of the lane's row; padding rows see nothing
+  int pos;              // position of the lane's row (a padding row's queries are zeros, its results go nowhere)
   int first, last;      // positions of the wave's first and last row (uniform)
   float slope2;         // slope * log2(e) of the lane's head
 };
@@ -355,12 +355,12 @@ __device__ __forceinline__ void clear_unused(int kv, int at) {
 // issue slots are free (beside the softmax the loads' address arithmetic took 230
 // of 1900 cycles), and waits for them before its products of tile t + 2.
 //
-// 4096 tokens of 28 heads over 4, 128 wide, fp16, behind 28672 slots: 1.63-1.71 ms,
+// 4096 tokens of 28 heads over 4, 128 wide, fp16, behind 28672 slots: 1.63-1.72 ms,
 // 1.05-1.11 PFLOP/s where a large matrix product reaches 1.35.  On the way: four
 // waves of 32 rows with two tiles in flight 2.30 ms; eight in two groups 1.79;
 // no maximum beforehand 1.69; three tiles ahead 1.63.  What bounds it then is the
 // count of workgroups: 448 on 256 CUs, one each, are two rounds of which the
-// second is three quarters full (rows_plan says why they are not split).  Seven prompts of 300 to 2048 tokens: 77 us for
+// second is three quarters full (rows_plan says why they are not split).  Seven prompts of 300 to 2048 tokens: 79 us for
 // 48 GFLOP, of which the longest workgroup's 32 tiles take 55.
 
 constexpr int kRowsP = 256, kTileP = 64, kPerMinP = 8;   // kPerMinP: fewest tiles of a part
@@ -972,11 +972,14 @@ int64_t most_slots(const PagedArgs& a, int rows, int tk) {   // that a row block
 // Whether the sequences' chunks fill half a block of 256 rows on average, and
 // there is work (rows by slots) enough for its longer start-up.  Single tokens
 // never do: a block would hold the g rows of one (1280 tokens of 32 heads over 8,
-// 500 slots: 1150 us, in blocks of 32 rows 440).  28 heads over 4, 128 wide, few-row
-// kernel and this one, us: 40 tokens over 600 slots (0.7 M) 15 and 27; 20 over 8192
-// (4.6 M) 34 and 33; 64 over 8192 59 and 35; 512 over 8192 191 and 77.  With caps and
-// biases, whose softmax weighs more here: 4 chunks of 160 over 1000 slots (18 M) 65 and
-// 70, 800 over 1000 (22 M) 70 and 71, 128 over 8192 (29 M) 110 and 67.
+// 500 slots: 1150 us, in blocks of 32 rows 440).  28 heads over 4, 128 wide, fp16, us
+// in blocks of 32 rows and in blocks of 256 with their parts: 40 tokens over 600 slots
+// (0.7 M) 15 and 27; 20 over 8192 (4.6 M) 33 and 32; 64 over 8192 57 and 38; 512 over
+// 8192 189 and 77.  With a cap and a bias, whose softmax weighs more here: 4 chunks of
+// 160 over 1000 slots (18 M) 63 and 67, 800 over 1000 (22 M) 66 and 67, 128 over 8192
+// (29 M) 100 and 62; a bias alone would pay from less (800 over 1000: 62 and 50).  The
+// average chunk decides, so a batch of single tokens and one chunk runs in one kind
+// of block.
 constexpr int64_t kWork = 4 << 20, kWorkExtra = 24 << 20;
 bool many_rows(const PagedArgs& a) {
   const int64_t slots = a.window > 0 ? std::min<int64_t>(a.cap, (int64_t)a.window + kRowsP) : a.cap;
@@ -989,8 +992,9 @@ bool many_rows(const PagedArgs& a) {
 // heads, 6 until the first tile has landed, a part's record written and read
 // again at the copy rate, 8 for the second launch; a tenth must be gained (4096
 // tokens behind 28672 slots in four parts, 1.75 rounds for 2: 1690 us for 1665, the
-// clock falls when all CUs work).  8192 slots, 28 heads over 4, one part and these:
-// 512 tokens 191 and 77 us, 1100 tokens 186 and 138.
+// clock falls when all CUs work).  The time of a tile is that without caps and biases.
+// 8192 slots, 28 heads over 4, blocks of 256 rows in one part and in these: 128 tokens
+// 184 and 41 us, 512 184 and 77, 1100 185 and 139.
 struct RowsPlan {
   int64_t blocks, parts;
   size_t ws_bytes;

@@ -15,7 +15,7 @@ namespace {
 // fp32, one rounding.  A thread takes eight frequencies of one token and walks
 // over heads with their cosines and sines in registers: one 16-byte load per
 // half head, and the tables are read once per thread instead of once per head.
-// Bound by memory: 6700 tokens of 28 heads over 4, bf16, three axes, 100 MB: 18.6 us
+// Bound by memory: 5262 tokens of 28 heads over 4, bf16, three axes, 100 MB: 18.6 us
 // (5.4 TB/s; a large copy 4.95), 22 with the launch; one token 3 us, the launch.
 template <typename T> struct V8 { typedef typename T::e v __attribute__((ext_vector_type(8))); };
 typedef float f8 __attribute__((ext_vector_type(8)));

@@ -14,9 +14,9 @@
 // 16 blocks, then all: fp32 throughout.
 //
 // Decode of 8 sequences of 2 to 16 thousand slots, 28 heads over 4, 54 MB of keys:
-// 16 us (11 at the copy rate), bound by start-up and one wave of loads.  A chunk of
-// 1500 tokens of each of two prompts of up to 8191 slots, bf16, 116 GFLOP: 250-256
-// us, 0.46 PFLOP/s.  Per block of 64 rows a wave spends about 3000 cycles on 1024 of
+// 16.5 us (11 at the copy rate), bound by start-up and one wave of loads.  A chunk of
+// 1500 tokens of each of two prompts of up to 8191 slots, bf16, 116 GFLOP: 258
+// us, 0.45 PFLOP/s.  Per block of 64 rows a wave spends about 3000 cycles on 1024 of
 // matrix work, the exponentials and the sums, and 1200 on the next block's loads and
 // row data; eight waves per CU do not hide one another's.  Keeping the scores of
 // one block in flight over the weights of the last gave 223 us but 22 for the

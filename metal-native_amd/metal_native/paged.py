@@ -211,6 +211,10 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, tab
     [heads] * distance``.  A row at position p sees slot j where ``j <= p``, with
     a ``window`` only the last ``window`` of those, and always the first
     ``prefix_lens [batch]`` slots.  A row that sees nothing gives zeros and -inf.
+    Sums and log sums are held in 32 bits; the weights are rounded to the cache's
+    type for their product with the values (half a step of it, next to the
+    output's own rounding), and an infinite value under a weight that rounds to
+    zero gives NaN where a whole tile of slots is seen.
     ``max_q``: the longest chunk where it is known (it sizes launches, no more).
     """
     op = "paged.attention"
