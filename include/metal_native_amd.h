@@ -322,6 +322,43 @@ MQ_API int mq_paged_attention(const mq_paged_cache* cache, const mq_paged_mask* 
 MQ_API int mq_paged_attention_plan(const mq_paged_cache* cache, const mq_paged_mask* mask, int64_t rows, int32_t heads,
                                    int32_t* block_rows, int32_t* parts);
 
+/* ---- trees of drafted tokens ----
+ *
+ * The call's tokens of a sequence are the nodes of a tree, in order the newest
+ * slots of its cache; parents[row] is the number of a node's parent in the chunk,
+ * smaller than its own (anything else: it has none).
+ *
+ * tree [rows, words]: bit i of a row is set where node i of its sequence is the
+ * row's own or one of its ancestors; nodes from 64 * words on have no bit.  Rows
+ * that belong to no sequence get zeros. */
+MQ_API int mq_paged_ancestors(const int32_t* parents, const int32_t* cu_q, int64_t batch, int64_t rows, int64_t words,
+                              int64_t* tree, void* stream);
+
+/* Attention of such nodes: a row sees the slots in front of the chunk and those of
+ * the chunk whose bits are set in its row of tree [rows, words] (row stride
+ * ld_tree words; any bits, whether a tree's or not).  It stands (number of its
+ * bits) - 1 slots past the chunk's first one, and the distance to a slot of the
+ * chunk is the number of its bits above it; the mask's window and slopes go by
+ * these, its prefix by the slots in front of the chunk. */
+MQ_API int64_t mq_paged_tree_attention_workspace_size(const mq_paged_cache* cache, const mq_paged_mask* mask,
+                                                      int64_t rows, int32_t heads);
+MQ_API int mq_paged_tree_attention(const mq_paged_cache* cache, const mq_paged_mask* mask, const int64_t* tree,
+                                   int64_t ld_tree, int64_t words, const void* q, int64_t q_token, int64_t q_head,
+                                   int64_t rows, int32_t heads, void* out, float* lse, void* workspace,
+                                   int64_t workspace_bytes, void* stream);
+
+/* The path of a tree that was drawn: from node 0 to the child (the first, where
+ * several are alike) whose drafted token is the one drawn behind its parent, and
+ * on, for at most `steps` nodes.  path [batch, steps]: the nodes, and tokens
+ * [batch, steps] what was drawn behind each, -1 past the path; count [batch] its
+ * length, new_lens [batch] lens less the nodes that are not on it.  In every one
+ * of `layers` caches (strides k_layer, v_layer from the first) the path's slots
+ * move to the chunk's first ones. */
+MQ_API int mq_paged_accept(const mq_paged_cache* cache, int64_t layers, int64_t k_layer, int64_t v_layer,
+                           const int64_t* drawn, const int64_t* drafted, const int32_t* parents, const int32_t* cu_q,
+                           int64_t rows, int64_t steps, int32_t* path, int64_t* tokens, int32_t* count,
+                           int32_t* new_lens, void* stream);
+
 /* mass [batch, kv_heads, width * page_size]: the sum over the call's tokens and
  * the query heads of a key/value head of exp(x - lse), zero past lens.  Rows of
  * lse -inf add nothing.  v is not read. */
@@ -340,6 +377,33 @@ MQ_API int mq_paged_attention_mass(const mq_paged_cache* cache, const mq_paged_m
 MQ_API int mq_paged_evict(const mq_paged_cache* cache, const float* mass, int64_t mass_batch, int64_t mass_head,
                           const int32_t* to, int64_t ld_to, int64_t to_width, int64_t budget, int64_t recent,
                           int32_t* kept, int32_t* new_lens, float* left, void* stream);
+
+/* ---- drawing tokens from logits (no reference counterpart) ----
+ *
+ * A row's tokens are ordered by logit, the largest first, ties by index; NaN
+ * counts as -inf, which is never drawn.  Weights are w = exp((x - largest) /
+ * temperature).  Of that order stay the first top_k tokens (0 or less: all); of
+ * those with the sum S of their weights the tokens before which less than top_p *
+ * S has gone (1 or more: all; 0 or less: the first); of those the ones of w >=
+ * min_p (1 where it is more).  Drawn is, in order of index, the first of them with which their
+ * running sum passes u times their sum.  temperature 0 or less, or
+ * NaN: the first token; another setting's NaN cuts nothing.
+ * u outside [0, 1) is cut to it.
+ *
+ * Each setting is one value, or where its pointer is not NULL an array of `rows`
+ * in device memory.  logprob (or NULL): the log of the drawn token's share of the
+ * sum.  A row without a logit above -inf gives token -1 and -inf. */
+enum mq_sample_dtype { MQ_SAMPLE_F16 = 0, MQ_SAMPLE_BF16 = 1, MQ_SAMPLE_F32 = 2 };
+typedef struct mq_sampling {
+  const float *temperatures, *top_ps, *min_ps;
+  const int32_t* top_ks;
+  float temperature, top_p, min_p;
+  int32_t top_k;
+} mq_sampling;
+MQ_API int64_t mq_sample_workspace_size(int64_t rows, int64_t vocab, int32_t dtype, const mq_sampling* how);
+MQ_API int mq_sample(const void* logits, int64_t ld, int64_t rows, int64_t vocab, int32_t dtype, const float* u,
+                     const mq_sampling* how, int64_t* token, float* logprob, void* workspace, int64_t workspace_bytes,
+                     void* stream);
 
 /* Read probe: a measurement aid with no reference counterpart.  Reads the
  * `bytes` (< 2^31) bytes at p once, in one launch, the fastest way found on

@@ -23,8 +23,8 @@ FRONT_NAME = "_mq_torch.so"
 BUILD_DIR = os.path.join(HERE, "_build")
 
 SOURCES = ["mq_capi.cpp", "mq_gemv.hip", "mq_rows.hip", "mq_rstream.hip", "mq_gemmw.hip", "mq_gemm16.hip", "mq_gemmn.hip", "mq_tiled.hip", "mq_misc.hip", "mq_quant.hip", "mq_glue.hip", "mq_vecmat32.hip",
-           "mq_paged_capi.cpp", "mq_pattn.hip", "mq_pmass.hip", "mq_pcache.hip"]
-FRONT_SOURCES = ["mq_torch.cpp", "mq_torch_paged.cpp"]
+           "mq_paged_capi.cpp", "mq_pattn.hip", "mq_ptattn.hip", "mq_pmass.hip", "mq_pcache.hip", "mq_ptree.hip", "mq_sample_capi.cpp", "mq_sample.hip"]
+FRONT_SOURCES = ["mq_torch.cpp", "mq_torch_paged.cpp", "mq_torch_sample.cpp"]
 
 HIP_FLAGS = [
     "-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950",
@@ -36,7 +36,7 @@ HIP_FLAGS = [
 ]
 # MFMA results in ordinary registers wherever they fit: the softmax reads them,
 # and from accumulation registers each read is an instruction of its own
-SOURCE_FLAGS = {s: ["-mllvm", "-amdgpu-mfma-vgpr-form=true"] for s in ("mq_pattn.hip", "mq_pmass.hip")}
+SOURCE_FLAGS = {s: ["-mllvm", "-amdgpu-mfma-vgpr-form=true"] for s in ("mq_pattn.hip", "mq_ptattn.hip", "mq_pmass.hip")}
 
 
 def _hipcc() -> str:

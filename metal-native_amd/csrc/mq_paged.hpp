@@ -97,6 +97,16 @@ MQ_HD PagedRange paged_rows(int j0, int slots, const PagedSeq& s, int window, in
   return a < b ? PagedRange{(int)(a * g), (int)(b * g)} : PagedRange{0, 0};
 }
 
+// Bits d .. d + 63 of a row of `words` words; zeros outside them.
+MQ_HD uint64_t paged_tree_bits(const uint64_t* row, int words, int64_t d) {
+  if (d <= -64 || d >= (int64_t)words * 64) return 0;
+  const int64_t w = d < 0 ? -1 : d >> 6;   // the word that holds bit d
+  const int sh = (int)(d & 63);
+  const uint64_t lo = w >= 0 ? row[w] >> sh : 0;
+  const uint64_t hi = sh && w + 1 < words ? row[w + 1] << (64 - sh) : 0;
+  return lo | hi;
+}
+
 // Page that holds slot j, or -1 where there is none.
 MQ_HD int paged_page(const int32_t* row, int j, int len, int shift, int pages) {
   if (j < 0 || j >= len) return -1;
@@ -137,6 +147,9 @@ struct PagedArgs {
   void* out;              // [rows, heads, dim] contiguous
   float* lse;             // [rows, heads] or null (attention); given (mass)
   float* mass;            // [b, kv_heads, width << shift]
+  const uint64_t* tree;   // [rows, tree_words] ancestor bits of a tree's nodes, or null: a chunk in order
+  int64_t ld_tree;
+  int tree_words;
   bool extra() const { return softcap != 0.f || slopes != nullptr; }
 };
 
@@ -147,6 +160,7 @@ struct PagedPlan {
 PagedPlan pattn_plan(const PagedArgs& a, int num_cus);
 size_t pattn_workspace(const PagedArgs& a, int num_cus);
 hipError_t pattn_launch(const PagedArgs& a, int num_cus, void* ws, hipStream_t s);
+hipError_t ptattn_launch(const PagedArgs& a, int num_cus, void* ws, hipStream_t s);   // a.tree set
 size_t pmass_workspace(const PagedArgs& a, int num_cus);
 hipError_t pmass_launch(const PagedArgs& a, int num_cus, void* ws, hipStream_t s);
 
@@ -186,6 +200,31 @@ struct PagedEvictArgs {
   float* left;            // [b, KVH, to_width << shift]
 };
 hipError_t pevict_launch(const PagedEvictArgs& a, int num_cus, hipStream_t s);
+
+// A tree's nodes are the rows of its sequence's chunk; parents[row] is a node's
+// number in it, smaller than the row's own, anything else no parent.
+struct AncestorsArgs {
+  const int32_t *parents, *cu;   // cu null: one row per sequence
+  int b, rows, words;
+  uint64_t* tree;   // [rows, words]
+};
+hipError_t pancestors_launch(const AncestorsArgs& a, hipStream_t s);
+
+struct AcceptArgs {
+  PagedCache k, v;
+  int64_t k_layer, v_layer;   // strides of the caches' layers
+  int layers;
+  const int32_t* table;
+  int64_t ld_table;
+  int width, pages, shift, cap;
+  const int32_t *lens, *cu;
+  int b, rows, KVH, D, steps;
+  const int64_t *drawn, *drafted;   // [rows]
+  const int32_t* parents;           // [rows]
+  int32_t *path, *count, *new_lens;   // [b, steps], [b], [b]
+  int64_t* tokens;                    // [b, steps]
+};
+hipError_t paccept_launch(const AcceptArgs& a, hipStream_t s);
 
 }  // namespace mq
 #endif

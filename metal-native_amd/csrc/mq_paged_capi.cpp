@@ -100,6 +100,18 @@ const char* attn_args(mq::PagedArgs& a, const mq_paged_cache* c, const mq_paged_
   a.out = nullptr;
   a.lse = nullptr;
   a.mass = nullptr;
+  a.tree = nullptr;
+  a.ld_tree = a.tree_words = 0;
+  return nullptr;
+}
+
+// The bits of a tree's rows; null, or what is wrong
+const char* tree_rows(mq::PagedArgs& a, const int64_t* tree, int64_t ld_tree, int64_t words) {
+  if (!tree || ((uintptr_t)tree & 7)) return "the tree's bits must be there, 8-byte aligned";
+  if (words < 1 || words > INT_MAX / 64 || ld_tree < 0) return "the tree needs 1 to 2^25 words a row, and a stride that is not negative";
+  a.tree = (const uint64_t*)tree;
+  a.ld_tree = ld_tree;
+  a.tree_words = (int)words;
   return nullptr;
 }
 
@@ -206,6 +218,79 @@ MQ_API int mq_paged_attention(const mq_paged_cache* c, const mq_paged_mask* m, c
   if (need && (!ws || !aligned16(ws) || ws_bytes < (int64_t)need)) return refuse(op, "workspace too small or not 16-byte aligned");
   const hipError_t e = mq::pattn_launch(a, cus, ws, (hipStream_t)stream);
   return e == hipSuccess ? MQ_SUCCESS : mq::hip_fail_with(e, "paged.attention: kernel launch failed");
+}
+
+MQ_API int mq_paged_ancestors(const int32_t* parents, const int32_t* cu_q, int64_t batch, int64_t rows, int64_t words,
+                              int64_t* tree, void* stream) {
+  const char* op = "paged.ancestors";
+  if (batch < 1 || batch > INT_MAX - 1 || rows < 0 || rows > INT_MAX - 256) return refuse(op, "batch must be positive, rows not negative, both below 2^31");
+  if (words < 1 || words > INT_MAX / 64) return refuse(op, "1 to 2^25 words a row");
+  if (!cu_q && rows != batch) return refuse(op, "without cu_q there must be one row per sequence");
+  if (rows == 0) return MQ_SUCCESS;
+  if (!parents || !tree || ((uintptr_t)tree & 7)) return refuse(op, "null pointer argument, or bits that are not 8-byte aligned");
+  const hipError_t e = mq::pancestors_launch({parents, cu_q, (int)batch, (int)rows, (int)words, (uint64_t*)tree}, (hipStream_t)stream);
+  return e == hipSuccess ? MQ_SUCCESS : mq::hip_fail_with(e, "paged.ancestors: kernel launch failed");
+}
+
+MQ_API int64_t mq_paged_tree_attention_workspace_size(const mq_paged_cache* c, const mq_paged_mask* m, int64_t rows,
+                                                      int32_t heads) {
+  mq::PagedArgs a;
+  const char* bad = attn_args(a, c, m, rows, heads, true);
+  const int64_t any = 0;
+  if (!bad) bad = tree_rows(a, &any, 1, 1);   // whichever they are
+  if (bad) {
+    refuse("paged.tree_attention", bad);
+    return -1;
+  }
+  return (int64_t)mq::pattn_workspace(a, mq::current_num_cus());
+}
+
+MQ_API int mq_paged_tree_attention(const mq_paged_cache* c, const mq_paged_mask* m, const int64_t* tree, int64_t ld_tree,
+                                   int64_t words, const void* q, int64_t q_token, int64_t q_head, int64_t rows,
+                                   int32_t heads, void* out, float* lse, void* ws, int64_t ws_bytes, void* stream) {
+  const char* op = "paged.tree_attention";
+  mq::PagedArgs a;
+  if (const char* bad = attn_args(a, c, m, rows, heads, true)) return refuse(op, bad);
+  if (rows == 0) return MQ_SUCCESS;
+  if (const char* bad = tree_rows(a, tree, ld_tree, words)) return refuse(op, bad);
+  if (const char* bad = query(a, q, q_token, q_head)) return refuse(op, bad);
+  if (!out || !aligned16(out)) return refuse(op, "the output must be 16-byte aligned");
+  a.out = out;
+  a.lse = lse;
+  const int cus = mq::current_num_cus();
+  const size_t need = mq::pattn_workspace(a, cus);
+  if (need && (!ws || !aligned16(ws) || ws_bytes < (int64_t)need)) return refuse(op, "workspace too small or not 16-byte aligned");
+  const hipError_t e = mq::ptattn_launch(a, cus, ws, (hipStream_t)stream);
+  return e == hipSuccess ? MQ_SUCCESS : mq::hip_fail_with(e, "paged.tree_attention: kernel launch failed");
+}
+
+MQ_API int mq_paged_accept(const mq_paged_cache* c, int64_t layers, int64_t k_layer, int64_t v_layer, const int64_t* drawn,
+                           const int64_t* drafted, const int32_t* parents, const int32_t* cu_q, int64_t rows,
+                           int64_t steps, int32_t* path, int64_t* tokens, int32_t* count, int32_t* new_lens, void* stream) {
+  const char* op = "paged.accept";
+  if (const char* bad = bad_cache(c, true)) return refuse(op, bad);
+  if (layers < 1 || layers > INT_MAX / 2 || k_layer < 0 || v_layer < 0 || k_layer % 8 || v_layer % 8)
+    return refuse(op, "layers must be positive, their strides multiples of 8");
+  if (rows < 0 || rows > INT_MAX || steps < 1 || steps > INT_MAX - 64) return refuse(op, "rows must not be negative, steps positive, both below 2^31");
+  if (!cu_q && rows != c->batch) return refuse(op, "without cu_q there must be one row per sequence");
+  if (!path || !tokens || !count || !new_lens || (rows > 0 && (!drawn || !drafted || !parents))) return refuse(op, "null pointer argument");
+  mq::AcceptArgs a{};
+  fill_cache(a, c);
+  a.k_layer = k_layer;
+  a.v_layer = v_layer;
+  a.layers = (int)layers;
+  a.cu = cu_q;
+  a.rows = (int)rows;
+  a.steps = (int)steps;
+  a.drawn = drawn;
+  a.drafted = drafted;
+  a.parents = parents;
+  a.path = path;
+  a.tokens = tokens;
+  a.count = count;
+  a.new_lens = new_lens;
+  const hipError_t e = mq::paccept_launch(a, (hipStream_t)stream);
+  return e == hipSuccess ? MQ_SUCCESS : mq::hip_fail_with(e, "paged.accept: kernel launch failed");
 }
 
 MQ_API int64_t mq_paged_attention_mass_workspace_size(const mq_paged_cache* c, const mq_paged_mask* m, int64_t rows,

@@ -1,0 +1,126 @@
+// Trees of drafted tokens over a paged cache: ancestor bits, and the accepted
+// path with its slots moved together.
+#include "mq_paged_dev.hpp"
+
+namespace mq {
+namespace {
+
+// One thread walks from its row's node to the root; parents have smaller numbers
+// (anything else is no parent), so the walk ends, and words are written from the
+// highest down.
+__global__ __launch_bounds__(256) void ancestors_kernel(AncestorsArgs a) {
+  const int row = blockIdx.x * 256 + threadIdx.x;
+  if (row >= a.rows) return;
+  int start = row, i = 0;
+  if (a.cu) {   // the last sequence that begins at or before the row
+    int lo = 0, hi = a.b;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (a.cu[mid] <= row) lo = mid;
+      else hi = mid;
+    }
+    start = max(a.cu[lo], 0);
+    i = row >= start && row < a.cu[lo + 1] ? row - start : -1;
+  }
+  uint64_t* out = a.tree + (int64_t)row * a.words;
+  uint64_t bits = 0;
+  int w = a.words - 1;
+  while (i >= 0) {
+    const int at = i >> 6;
+    for (; w > at; --w) {
+      out[w] = bits;
+      bits = 0;
+    }
+    if (at < a.words) bits |= 1ull << (i & 63);
+    const int up = a.parents[start + i];
+    i = up < i ? up : -1;
+  }
+  for (; w >= 0; --w) {
+    out[w] = bits;
+    bits = 0;
+  }
+}
+
+// A thread moves one 16-byte piece of a slot, of one layer, cache and head,
+// through all of the path; every wave walks the path for itself.  Node i of the
+// path goes to the i-th slot of the chunk, which is never behind its own: what a
+// store overwrites is a slot that has been moved before, or by the same thread's
+// loads in front of it.
+__global__ __launch_bounds__(256) void accept_kernel(AcceptArgs a) {
+  const int s = blockIdx.y, lane = threadIdx.x & 63;
+  const PagedSeq sq = paged_seq(s, a.cu ? a.cu[s] : 0, a.cu ? a.cu[s + 1] : 0, a.cu != nullptr, a.lens[s], 0, a.rows, a.cap);
+  const int off = sq.len - sq.n, per = a.D / 8, mask = (1 << a.shift) - 1;
+  const int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const bool have = x < (int64_t)a.layers * 2 * a.KVH * per;
+  int64_t y = x / per;
+  const int piece = (int)(x - y * per), head = (int)(y % a.KVH);
+  y /= a.KVH;
+  const PagedCache c = y & 1 ? a.v : a.k;
+  u4* const base = (u4*)((uint16_t*)c.ptr + (y >> 1) * (y & 1 ? a.v_layer : a.k_layer) + head * c.head) + piece;
+  const int32_t *row = a.table + (int64_t)s * a.ld_table, *parents = a.parents + sq.start;
+  const int64_t *drawn = a.drawn + sq.start, *drafted = a.drafted + sq.start;
+  const bool tells = blockIdx.x == 0 && threadIdx.x < 64;
+  int cur = sq.n > 0 ? 0 : -1, done = 0;
+  while (cur >= 0 && done < a.steps) {
+    int mine = 0, m = 0;   // the path's next nodes: lane i the i-th
+    while (cur >= 0 && m < 64 && done + m < a.steps) {
+      if (lane == m) mine = cur;
+      ++m;
+      const int64_t want = drawn[cur];
+      int next = -1;
+      for (int i0 = cur + 1; i0 < sq.n && next < 0; i0 += 64) {
+        const int i = i0 + lane;
+        const uint64_t hit = __ballot(i < sq.n && parents[i] == cur && drafted[i] == want);
+        if (hit) next = i0 + __ffsll((unsigned long long)hit) - 1;
+      }
+      cur = next;
+    }
+    if (tells && lane < m) {
+      a.path[(int64_t)s * a.steps + done + lane] = mine;
+      a.tokens[(int64_t)s * a.steps + done + lane] = drawn[mine];
+    }
+    const int from = off + mine, to = off + done + lane;
+    const int page0 = lane < m && from != to ? paged_page(row, from, sq.len, a.shift, a.pages) : -1;
+    const int page1 = page0 >= 0 ? paged_page(row, to, sq.len, a.shift, a.pages) : -1;
+    for (int k0 = 0; k0 < m; k0 += 8) {
+      u4 v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (__builtin_amdgcn_readlane(page1, k0 + k) >= 0 && have)
+          v[k] = base[((int64_t)__builtin_amdgcn_readlane(page0, k0 + k) * c.page +
+                       (int64_t)(__builtin_amdgcn_readlane(from, k0 + k) & mask) * c.slot) / 8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int page = __builtin_amdgcn_readlane(page1, k0 + k);
+        if (page >= 0 && have) base[((int64_t)page * c.page + (int64_t)((off + done + k0 + k) & mask) * c.slot) / 8] = v[k];
+      }
+    }
+    done += m;
+  }
+  if (!tells) return;
+  for (int i = done + lane; i < a.steps; i += 64) {
+    a.path[(int64_t)s * a.steps + i] = -1;
+    a.tokens[(int64_t)s * a.steps + i] = -1;
+  }
+  if (lane == 0) {
+    a.count[s] = done;
+    a.new_lens[s] = max(off + done, 0);
+  }
+}
+
+}  // namespace
+
+hipError_t pancestors_launch(const AncestorsArgs& a, hipStream_t s) {
+  ancestors_kernel<<<(a.rows + 255) / 256, 256, 0, s>>>(a);
+  return hipGetLastError();
+}
+
+hipError_t paccept_launch(const AcceptArgs& a, hipStream_t s) {
+  const int64_t pieces = (int64_t)a.layers * 2 * a.KVH * (a.D / 8);
+  const int64_t blocks = (pieces + 255) / 256;
+  if (blocks > 0x7fffffff) return hipErrorInvalidValue;
+  accept_kernel<<<dim3((unsigned)blocks, a.b), 256, 0, s>>>(a);
+  return hipGetLastError();
+}
+
+}  // namespace mq

@@ -155,6 +155,10 @@ PyMethodDef kMethods[] = {
     {"paged_attention", (PyCFunction)(void (*)(void))mq_front::paged_attention, METH_FASTCALL, nullptr},
     {"paged_attention_mass", (PyCFunction)(void (*)(void))mq_front::paged_attention_mass, METH_FASTCALL, nullptr},
     {"paged_evict", (PyCFunction)(void (*)(void))mq_front::paged_evict, METH_FASTCALL, nullptr},
+    {"paged_ancestors", (PyCFunction)(void (*)(void))mq_front::paged_ancestors, METH_FASTCALL, nullptr},
+    {"paged_tree_attention", (PyCFunction)(void (*)(void))mq_front::paged_tree_attention, METH_FASTCALL, nullptr},
+    {"paged_accept", (PyCFunction)(void (*)(void))mq_front::paged_accept, METH_FASTCALL, nullptr},
+    {"sample", (PyCFunction)(void (*)(void))mq_front::sample, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_mq_torch", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

@@ -7,12 +7,8 @@
 #include "mq_torch.hpp"
 
 #include <algorithm>
-#include <initializer_list>
 #include <utility>
 
-#include <c10/core/DeviceGuard.h>
-#include <c10/core/GradMode.h>
-#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -28,13 +24,10 @@ bool index_rows(const at::Tensor& t, c10::Device dev) {
   return t.device() == dev && t.scalar_type() == at::kInt && t.dim() == 2 && (t.size(1) <= 1 || t.stride(1) == 1) &&
          (t.size(0) <= 1 || t.stride(0) >= t.size(1));
 }
-bool vec(const at::Tensor* t, c10::Device dev, at::ScalarType ty, int64_t n) {
-  return t && t->device() == dev && t->scalar_type() == ty && t->dim() == 1 && t->size(0) == n && t->is_contiguous();
-}
-
 // no two elements share memory: each stride reaches past all smaller dimensions
 bool distinct(const at::Tensor& t) {
-  std::pair<int64_t, int64_t> d[4];
+  if (t.dim() > 8) return false;
+  std::pair<int64_t, int64_t> d[8];
   int n = 0;
   for (int64_t i = 0; i < t.dim(); ++i)
     if (t.size(i) > 1) d[n++] = {t.stride(i), t.size(i)};
@@ -62,7 +55,11 @@ struct Cache {
   }
   // v null: keys alone
   bool take(PyObject* ko, PyObject* vo, PyObject* table, PyObject* lens, bool write) {
-    const at::Tensor *k = plain(ko), *v = vo ? plain(vo) : k, *t = plain(table), *l = plain(lens);
+    const at::Tensor* k = plain(ko);
+    return take(k, vo ? plain(vo) : k, table, lens, write);
+  }
+  bool take(const at::Tensor* k, const at::Tensor* v, PyObject* table, PyObject* lens, bool write) {
+    const at::Tensor *t = plain(table), *l = plain(lens);
     if (!k || !v || !t || !l) return false;
     dev = k->device();
     ty = k->scalar_type();
@@ -87,21 +84,6 @@ struct Cache {
   }
 };
 
-bool as_int(PyObject* o, int64_t* v) {
-  if (!PyLong_CheckExact(o)) return false;
-  int over = 0;
-  *v = PyLong_AsLongLongAndOverflow(o, &over);
-  return !over;
-}
-bool as_float(PyObject* o, float* v) {
-  if (!PyFloat_CheckExact(o) && !PyLong_CheckExact(o)) return false;
-  *v = (float)PyFloat_AsDouble(o);
-  if (PyErr_Occurred()) {
-    PyErr_Clear();
-    return false;
-  }
-  return true;
-}
 bool chunks(PyObject* o, const Cache& k, int64_t rows, const int32_t** cu) {
   *cu = nullptr;
   if (o == Py_None) return rows == k.c.batch;
@@ -148,33 +130,10 @@ bool mask(PyObject* const* a, const Cache& k, const Query& q, mq_paged_mask* m) 
   return as_int(a[6], &m->max_q);
 }
 
-// Device of a call, and dispatch below Python's modes: what is allocated here
-// is launched on at once and has to be memory.
-struct Call {
-  c10::DeviceGuard device;
-  c10::impl::ExcludeDispatchKeyGuard modes;
-  explicit Call(c10::Device d)
-      : device(d), modes(c10::DispatchKeySet({c10::DispatchKey::Python, c10::DispatchKey::PythonTLSSnapshot})) {}
-};
-
-// whether autograd follows one of them (null: not given); paged.py then marks
-// the outputs as having no gradient
-bool tracked(std::initializer_list<const at::Tensor*> ts) {
-  if (!c10::GradMode::is_enabled()) return false;
-  for (const at::Tensor* t : ts)
-    if (t && t->requires_grad()) return true;
-  return false;
-}
 // a cache that the call wrote
 void written(PyObject* o) {
   const at::Tensor& t = THPVariable_Unpack(o);
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-}
-
-PyObject* status(int rc) { return PyLong_FromLong(rc); }
-PyObject* wrong_count(const char* what) {
-  PyErr_SetString(PyExc_TypeError, what);
-  return nullptr;
 }
 
 }  // namespace
@@ -270,6 +229,110 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Py_DECREF(o);
   Py_DECREF(l);
   return r;
+  END_HANDLE_TH_ERRORS
+}
+
+// (parents, cu, words, stream)
+PyObject* paged_ancestors(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 4) return wrong_count("paged_ancestors: 4 arguments");
+  const at::Tensor *p = plain(a[0]), *cu = a[1] == Py_None ? nullptr : plain(a[1]);
+  int64_t words;
+  if (!p || p->dim() != 1 || !vec(p, p->device(), at::kInt, p->size(0)) || !as_int(a[2], &words) || words < 1 || words > INT32_MAX / 64)
+    return decline();
+  if (a[1] != Py_None && (!cu || cu->dim() != 1 || cu->size(0) < 2 || !vec(cu, p->device(), at::kInt, cu->size(0)))) return decline();
+  const int64_t rows = p->size(0);
+  void* stream = PyLong_AsVoidPtr(a[3]);
+  if (PyErr_Occurred()) return nullptr;
+  HANDLE_TH_ERRORS
+  const Call guard(p->device());
+  at::Tensor out = at::empty({rows, words}, p->options().dtype(at::kLong));
+  if (rows == 0) return THPVariable_Wrap(std::move(out));
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = mq_paged_ancestors(p->const_data_ptr<int32_t>(), cu ? cu->const_data_ptr<int32_t>() : nullptr, cu ? cu->size(0) - 1 : rows,
+                          rows, words, out.mutable_data_ptr<int64_t>(), stream);
+  Py_END_ALLOW_THREADS
+  return rc == MQ_SUCCESS ? THPVariable_Wrap(std::move(out)) : status(rc);
+  END_HANDLE_TH_ERRORS
+}
+
+// (q, k, v, table, lens, tree, cu, scale, softcap, slopes, window, prefix_lens, max_q, return_lse, stream)
+PyObject* paged_tree_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 15) return wrong_count("paged_tree_attention: 15 arguments");
+  Cache k;
+  Query q;
+  mq_paged_mask m{};
+  const at::Tensor* bits = plain(a[5]);
+  if (!bits || !k.take(a[1], a[2], a[3], a[4], false) || !q.take(a[0], k) || !mask(a + 6, k, q, &m) ||
+      tracked({q.t, plain(a[1]), plain(a[2]), plain(a[9])}))
+    return decline();
+  if (bits->device() != k.dev || bits->scalar_type() != at::kLong || bits->dim() != 2 || bits->size(0) != q.rows || bits->size(1) < 1 ||
+      bits->size(1) > INT32_MAX / 64 || (bits->size(1) > 1 && bits->stride(1) != 1) || bits->stride(0) < 0)
+    return decline();
+  const int want_lse = PyObject_IsTrue(a[13]);
+  if (want_lse < 0) return nullptr;
+  void* stream = PyLong_AsVoidPtr(a[14]);
+  if (PyErr_Occurred()) return nullptr;
+  HANDLE_TH_ERRORS
+  const Call guard(k.dev);
+  const int64_t wsb = mq_paged_tree_attention_workspace_size(&k.c, &m, q.rows, (int32_t)q.heads);
+  if (wsb < 0) return status(MQ_INVALID_ARGUMENT);
+  at::Tensor out = at::empty({q.rows, q.heads, q.t->size(2)}, q.t->options());
+  at::Tensor lse, ws;
+  if (want_lse) lse = at::empty({q.rows, q.heads}, q.t->options().dtype(at::kFloat));
+  if (wsb) ws = at::empty({wsb}, q.t->options().dtype(at::kByte));
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = mq_paged_tree_attention(&k.c, &m, bits->const_data_ptr<int64_t>(), bits->stride(0), bits->size(1), q.t->const_data_ptr(), q.s_t,
+                               q.s_h, q.rows, (int32_t)q.heads, out.mutable_data_ptr(),
+                               want_lse ? lse.mutable_data_ptr<float>() : nullptr, wsb ? ws.mutable_data_ptr() : nullptr, wsb, stream);
+  Py_END_ALLOW_THREADS
+  if (rc != MQ_SUCCESS) return status(rc);
+  return want_lse ? packed({out, lse}) : THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// (k, v, table, lens, drawn, drafted, parents, cu, steps, stream); k and v with or without a dimension of layers
+PyObject* paged_accept(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 10) return wrong_count("paged_accept: 10 arguments");
+  Cache k;
+  const at::Tensor *kt = plain(a[0]), *vt = plain(a[1]), *drawn = plain(a[4]), *drafted = plain(a[5]), *parents = plain(a[6]);
+  int64_t steps;
+  if (!kt || !vt || !drawn || drawn->dim() != 1 || !as_int(a[8], &steps) || steps < 1 || steps > INT32_MAX - 64 || tracked({kt, vt}))
+    return decline();
+  const int64_t rows = drawn->size(0);
+  const int32_t* cu;
+  int64_t layers = 1, kl = 0, vl = 0;
+  void* stream = PyLong_AsVoidPtr(a[9]);
+  if (PyErr_Occurred()) return nullptr;
+  HANDLE_TH_ERRORS
+  const Call guard(kt->device());
+  if (kt->dim() == 5) {
+    if (vt->dim() != 5 || kt->size(0) < 1 || kt->size(0) != vt->size(0) || !distinct(*kt) || !distinct(*vt)) return decline();
+    layers = kt->size(0);
+    kl = layers > 1 ? kt->stride(0) : 0;
+    vl = layers > 1 ? vt->stride(0) : 0;
+    if (kl % 8 || vl % 8 || kl < 0 || vl < 0) return decline();
+    const at::Tensor k0 = kt->select(0, 0), v0 = vt->select(0, 0);
+    if (!k.take(&k0, &v0, a[2], a[3], true)) return decline();
+  } else if (!k.take(kt, vt, a[2], a[3], true)) {
+    return decline();
+  }
+  if (!vec(drawn, k.dev, at::kLong, rows) || !vec(drafted, k.dev, at::kLong, rows) || !vec(parents, k.dev, at::kInt, rows) ||
+      !chunks(a[7], k, rows, &cu))
+    return decline();
+  const auto ints = drawn->options().dtype(at::kInt);
+  at::Tensor path = at::empty({k.c.batch, steps}, ints), tokens = at::empty({k.c.batch, steps}, drawn->options());
+  at::Tensor count = at::empty({k.c.batch}, ints), lens = at::empty({k.c.batch}, ints);
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = mq_paged_accept(&k.c, layers, kl, vl, drawn->const_data_ptr<int64_t>(), drafted->const_data_ptr<int64_t>(),
+                       parents->const_data_ptr<int32_t>(), cu, rows, steps, path.mutable_data_ptr<int32_t>(),
+                       tokens.mutable_data_ptr<int64_t>(), count.mutable_data_ptr<int32_t>(), lens.mutable_data_ptr<int32_t>(), stream);
+  Py_END_ALLOW_THREADS
+  if (rc != MQ_SUCCESS) return status(rc);
+  written(a[0]), written(a[1]);
+  return packed({path, tokens, count, lens});
   END_HANDLE_TH_ERRORS
 }
 

@@ -92,6 +92,16 @@ SIGNATURES = {
                                        _c_void_p, _i64, _c_void_p]),
     "mq_paged_evict": (_i32, [_c_void_p, _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _i64, _i64, _c_void_p,
                               _c_void_p, _c_void_p, _c_void_p]),
+    "mq_paged_ancestors": (_i32, [_c_void_p, _c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p]),
+    "mq_paged_tree_attention_workspace_size": (_i64, [_c_void_p, _c_void_p, _i64, _i32]),
+    "mq_paged_tree_attention": (_i32, [_c_void_p, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _i64, _i32,
+                                       _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p]),
+    "mq_paged_accept": (_i32, [_c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64,
+                               _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
+    # struct mq_sampling goes by address
+    "mq_sample_workspace_size": (_i64, [_i64, _i64, _i32, _c_void_p]),
+    "mq_sample": (_i32, [_c_void_p, _i64, _i64, _i64, _i32, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64,
+                         _c_void_p]),
     "mq_release_workspaces": (_i32, []),
     "mq_set_option": (_i32, [ctypes.c_char_p, _i64]),
     "mq_last_path": (_i32, []),

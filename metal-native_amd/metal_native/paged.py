@@ -1,7 +1,9 @@
 """Serving from a paged key/value cache: rotary positions, attention, the
-attention weight that keys gathered, eviction by it.  No reference counterpart.
+attention weight that keys gathered, eviction by it; for drafted tokens the
+ancestors of a tree's nodes, attention of a tree, and the accepted path.  No
+reference counterpart.
 
-Shapes, for all four operators:
+Shapes, for all operators:
 
 * caches ``k_cache``, ``v_cache``: ``[pages, kv_heads, page_size, head_dim]``,
   Float16 or BFloat16, ``page_size`` a power of two from 8, ``head_dim`` 64 or
@@ -15,7 +17,13 @@ Shapes, for all four operators:
   ``cu[s]:cu[s + 1]`` are the newest of sequence ``s``; ``None``: one token per
   sequence.  Tokens before ``cu[0]`` or past ``cu[batch]`` (a batch padded for a
   graph) belong to no sequence: ``rope_kv`` turns their queries and writes no
-  slot, ``attention`` gives zeros and -inf, ``attention_mass`` counts none.
+  slot, ``attention`` gives zeros and -inf, ``attention_mass`` counts none;
+* a tree of drafted tokens is a sequence's chunk: node i is its token ``cu[s] +
+  i``, node 0 the root, the newest token that is settled; ``parents`` int32
+  ``[rows]`` names each node's parent by its number in the chunk, smaller than
+  the node's own (anything else, -1 for one: it has none).  Its slots are in the
+  order of the nodes; the position that a node has in the text, which is what
+  turns it by rotary tables, is its depth past the slots in front of the chunk.
 
 The index tensors are device memory that no call looks at on the host, so a
 step of a decode loop is capturable in a graph.  Whatever they hold, no kernel
@@ -36,7 +44,7 @@ import torch
 
 from .ops import _check, _invalid, _mq_torch, _raw_stream, _require_cuda
 
-__all__ = ["rope_kv", "attention", "attention_mass", "evict"]
+__all__ = ["rope_kv", "attention", "attention_mass", "evict", "ancestors", "tree_attention", "accept"]
 
 
 def _plain(*tensors):
@@ -320,3 +328,122 @@ def evict(k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor, len
         r = _mq_torch.paged_evict(k_cache, v_cache, table, lens, mass.contiguous(), to.contiguous(), budget, recent,
                                   _raw_stream(k_cache.get_device()))
     return _finish(op, r, tracked)
+
+
+def ancestors(parents: torch.Tensor, cu: torch.Tensor | None = None, max_q: int | None = None) -> torch.Tensor:
+    """What every node of its tree descends from, as ``tree_attention`` reads it:
+    int64 ``[rows, ceil(max_q / 64)]``, bit ``i % 64`` of word ``i // 64`` set where
+    node i is the row's own node or an ancestor of it.  ``max_q``: the most nodes
+    of a tree (default: rows); nodes past these words have no bit.  Rows of no
+    sequence get zeros.
+    """
+    op = "paged.ancestors"
+    if max_q is None:
+        max_q = parents.shape[0] if isinstance(parents, torch.Tensor) and parents.dim() else 1
+    max_q = int(max_q)
+    if not 0 <= max_q <= 2**31 - 64:
+        _invalid(f"{op}: max_q must be the most nodes of a tree, got {max_q}")
+    words = max(1, -(-max_q // 64))
+    if type(parents) is torch.Tensor and parents.is_cuda:
+        r = _mq_torch.paged_ancestors(parents, cu, words, _raw_stream(parents.get_device()))
+        if r is not None:
+            return _finish(op, r)
+    parents, cu = _plain(parents, cu)
+    _require_cuda(parents, "parents", op)
+    if parents.dtype != torch.int32 or parents.dim() != 1:
+        _invalid(f"{op}: parents must be Int32 [rows]")
+    if cu is not None:
+        _require_cuda(cu, "cu", op)
+        if cu.dtype != torch.int32 or cu.dim() != 1 or cu.shape[0] < 2 or cu.device != parents.device:
+            _invalid(f"{op}: cu must be Int32 [batch + 1] on the parents' device")
+        cu = cu.contiguous()
+    with torch.cuda.device(parents.device):
+        return _finish(op, _mq_torch.paged_ancestors(parents.contiguous(), cu, words, _raw_stream(parents.get_device())))
+
+
+def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
+                   tree: torch.Tensor, cu: torch.Tensor | None = None, *, scale: float | None = None, softcap: float = 0.0,
+                   slopes: torch.Tensor | None = None, window: int = 0, prefix_lens: torch.Tensor | None = None,
+                   max_q: int | None = None, return_lse: bool = False):
+    """``attention`` of the nodes of a tree: a row sees every slot in front of its
+    chunk, and of the chunk's those whose bits are set in its row of ``tree`` (int64
+    ``[rows, words]``, as ``ancestors`` gives it; any bits do, and nodes past the
+    words are not seen).
+
+    With ``window``, ``slopes`` and ``prefix_lens`` a row with n bits stands n - 1
+    slots past the chunk's first; its distance to a slot of the chunk is the number
+    of its bits above that slot's; a prefix ends where the chunk begins.
+    Everything else is as in ``attention``.
+    """
+    op = "paged.tree_attention"
+    if scale is None:
+        scale = q.shape[-1] ** -0.5 if isinstance(q, torch.Tensor) and q.dim() and q.shape[-1] else 1.0
+    if max_q is None:
+        max_q = 0
+    if type(q) is torch.Tensor and q.is_cuda:
+        r = _mq_torch.paged_tree_attention(q, k_cache, v_cache, table, lens, tree, cu, scale, softcap, slopes, window, prefix_lens,
+                                           max_q, return_lse, _raw_stream(q.get_device()))
+        if r is not None:
+            return _finish(op, r)
+    q, k_cache, v_cache, table, lens, tree, cu, slopes, prefix_lens = _plain(q, k_cache, v_cache, table, lens, tree, cu, slopes,
+                                                                             prefix_lens)
+    table, lens = _cache(op, k_cache, v_cache, table, lens)
+    tracked = _tracked(op, (q, k_cache, v_cache, slopes))
+    how = _mask(op, q, k_cache, table, cu, scale, softcap, slopes, window, prefix_lens, max_q)
+    _require_cuda(tree, "tree", op)
+    if tree.dtype != torch.int64 or tree.dim() != 2 or tree.shape[0] != q.shape[0] or tree.shape[1] < 1 or tree.device != q.device:
+        _invalid(f"{op}: tree must be Int64 [rows, words] = [{q.shape[0]}, words] on the queries' device")
+    with torch.no_grad(), torch.cuda.device(q.device):
+        for copied in (False, True):   # as it is, then laid out anew
+            r = _mq_torch.paged_tree_attention(q.clone(memory_format=torch.contiguous_format) if copied else q, k_cache, v_cache,
+                                               table, lens, tree.contiguous(), *how, bool(return_lse), _raw_stream(q.get_device()))
+            if r is not None:
+                break
+    return _finish(op, r, tracked)
+
+
+def accept(k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, drawn: torch.Tensor,
+           drafted: torch.Tensor, parents: torch.Tensor, cu: torch.Tensor | None = None, *, steps: int):
+    """Keeps of every tree the path that was drawn.  It begins at node 0 and goes on
+    to the child (the first, where several are alike) whose token in ``drafted``
+    is the one in ``drawn`` (both int64 ``[rows]``; drawn: behind that node) of its
+    parent, for at most ``steps`` nodes.  Its slots move, in their order, to the
+    first slots of the chunk, in the caches of all layers where they have a
+    dimension of layers in front (``[layers, pages, kv_heads, page_size,
+    head_dim]``; one table for all of them).
+
+    Returns ``(path, tokens, count, lens)``: the nodes, int32 ``[batch, steps]``, and
+    the tokens drawn behind them, int64 ``[batch, steps]``, both -1 past the path;
+    its length, int32 ``[batch]``; the lengths without the nodes that are not on it.
+    The last of the tokens has no slot yet: it is the next tree's root.  The pages
+    of a chunk may be in no other sequence's table.
+    """
+    op = "paged.accept"
+    if type(drawn) is torch.Tensor and drawn.is_cuda:
+        r = _mq_torch.paged_accept(k_cache, v_cache, table, lens, drawn, drafted, parents, cu, steps, _raw_stream(drawn.get_device()))
+        if r is not None:
+            return _finish(op, r)
+    k_cache, v_cache, table, lens, drawn, drafted, parents, cu = _plain(k_cache, v_cache, table, lens, drawn, drafted, parents, cu)
+    for t, what in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        _require_cuda(t, what, op)
+    k0, v0 = k_cache, v_cache
+    if k_cache.dim() == 5:
+        if v_cache.shape != k_cache.shape or k_cache.numel() == 0:
+            _invalid(f"{op}: k_cache and v_cache must have the same shape, [layers, pages, kv_heads, page_size, head_dim]")
+        if any(t.shape[0] > 1 and (t.stride(0) % 8 or t.stride(0) < 0) for t in (k_cache, v_cache)):
+            _invalid(f"{op}: layers of the caches must be 16-byte aligned")
+        k0, v0 = k_cache.detach()[0], v_cache.detach()[0]
+    table, lens = _cache(op, k0, v0, table, lens)
+    for t, what, dtype in ((drawn, "drawn", torch.int64), (drafted, "drafted", torch.int64), (parents, "parents", torch.int32)):
+        _require_cuda(t, what, op)
+        if t.dtype != dtype or t.dim() != 1 or t.shape != drawn.shape or t.device != k_cache.device:
+            _invalid(f"{op}: {what} must be {'Int64' if dtype == torch.int64 else 'Int32'} [rows] on the cache's device")
+    cu = _chunks(op, cu, table, drawn.shape[0])
+    steps = int(steps)
+    if not 1 <= steps <= 2**31 - 65:
+        _invalid(f"{op}: steps must be positive, got {steps}")
+    _tracked(op, (), (k_cache, v_cache))
+    with torch.no_grad(), torch.cuda.device(k_cache.device):
+        r = _mq_torch.paged_accept(k_cache, v_cache, table, lens, drawn.contiguous(), drafted.contiguous(), parents.contiguous(), cu,
+                                   steps, _raw_stream(k_cache.get_device()))
+    return _finish(op, r)

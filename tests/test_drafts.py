@@ -1,0 +1,374 @@
+"""Operators for trees of drafted tokens against their definitions: ancestor bits, tree attention (bounds in
+paged_ref), accepted paths."""
+
+import math
+import random
+
+import numpy as np
+import pytest
+import torch
+
+import draft_ref as ref
+from paged_ref import half_step
+from test_paged import DT, HEADS, build
+
+pytestmark = pytest.mark.gpu
+
+
+def random_tree(rng, n, kind="mixed"):
+    if kind == "chain":
+        return list(range(-1, n - 1))
+    if kind == "star":
+        return ([-1] + [0] * (n - 1))[:n]
+    return ([-1] + [rng.randrange(i) if rng.random() < 0.3 else max(0, i - 1 - int(rng.expovariate(0.7))) for i in range(1, n)])[:n]
+
+
+def trees(gpu, counts, seed=0, kind="mixed"):
+    rng = random.Random(seed)
+    parents = [random_tree(rng, n, kind) for n in counts]
+    cu = torch.tensor([sum(counts[:i]) for i in range(len(counts) + 1)], dtype=torch.int32, device=gpu)
+    flat = torch.tensor([p for t in parents for p in t], dtype=torch.int32, device=gpu)
+    return parents, flat, cu
+
+
+# ---- ancestors ----
+@pytest.mark.parametrize("kind", ["mixed", "chain", "star"])
+@pytest.mark.parametrize("counts", [[1], [64], [65, 1, 0, 63], [16, 130, 3, 300], [0, 0, 5], [1000, 2, 2500]])
+def test_ancestors(gpu, kind, counts):
+    from metal_native import paged
+
+    parents, flat, cu = trees(gpu, counts, len(counts), kind)
+    most = max(counts)
+    for max_q in {most, most + 64, max(1, most // 2), 1}:
+        words = -(-max_q // 64)
+        want = torch.cat([ref.pack(ref.closure(p), words) for p in parents])
+        got = paged.ancestors(flat, cu, max_q)
+        assert got.dtype == torch.int64 and torch.equal(got.cpu(), want)
+    assert paged.ancestors(flat, cu).shape == (sum(counts), -(-sum(counts) // 64))
+
+
+def test_ancestors_of_odd_parents_and_rows_of_no_sequence(gpu):
+    from metal_native import paged
+
+    flat = torch.tensor([9, 9, -1, 0, 7, 1, -(2**31), 2**31 - 1, 3, 4, 5, 5], dtype=torch.int32, device=gpu)
+    cu = torch.tensor([2, 6, 6, 10], dtype=torch.int32, device=gpu)   # two rows before the first tree, two past the last
+    want = torch.zeros(12, 1, dtype=torch.int64)
+    for s in range(3):
+        a, b = int(cu[s]), int(cu[s + 1])
+        if b > a:
+            want[a:b] = ref.pack(ref.closure(flat[a:b].tolist()), 1)
+    assert torch.equal(paged.ancestors(flat, cu, 4).cpu(), want)
+    assert torch.equal(paged.ancestors(flat).cpu()[:, 0], torch.ones(12, dtype=torch.int64))   # one token for each sequence
+    for wild in ([-5, 3, 10**6, 10**6], [7, 3, 1, 12], [2**31 - 1, -(2**31), 5, 6]):   # any offsets: nothing past the rows
+        assert paged.ancestors(flat, torch.tensor(wild, dtype=torch.int32, device=gpu), 64).shape == (12, 1)
+    assert paged.ancestors(flat[::2], cu // 2, 4).shape == (6, 1)
+    assert paged.ancestors(flat[:0], torch.zeros(2, dtype=torch.int32, device=gpu), 8).shape == (0, 1)
+
+
+# ---- attention ----
+def check_tree(c, families, bits, *, scale=None, softcap=0.0, slopes=None, window=0, prefix=None, max_q=None):
+    from metal_native import paged
+
+    s = scale or 1.0 / math.sqrt(c["q"].shape[2])
+    out, lse = paged.tree_attention(c["q"], c["k"], c["v"], c["table"], c["lens"], bits, c["cu"], scale=s, softcap=softcap, slopes=slopes,
+                                    window=window, prefix_lens=prefix, max_q=max_q, return_lse=True)
+    o, l, ob, lb = ref.tree_attention(c["q"], c["k"], c["v"], c["table"], c["lens"], families, c["cu"], scale=s, softcap=softcap,
+                                      slopes=slopes, window=window, prefix=prefix)
+    got, gl = out.double().cpu(), lse.double().cpu()
+    assert bool((torch.isnan(got) == torch.isnan(o)).all())
+    fin = ~torch.isnan(o)
+    assert bool(((got == o) | ((got - o).abs() <= ob))[fin].all()), float(((got - o).abs() / ob)[fin].nan_to_num().max())
+    assert bool(((gl == l) | (torch.isnan(gl) & torch.isnan(l)) | ((gl - l).abs() <= lb)).all())
+    return out, lse
+
+
+def tree_case(gpu, dt, H, KVH, D, ps, lens, counts, seed=0, kind="mixed", words=None, **how):
+    parents, flat, cu = trees(gpu, counts, seed, kind)
+    c = build(gpu, dt, H, KVH, D, ps, lens, counts, seed=seed, **how)
+    families = [ref.closure(p) for p in parents]
+    words = words or max(1, -(-max(counts) // 64))
+    bits = torch.cat([ref.pack(f, words) for f in families]).to(gpu)
+    return c, families, bits
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("H,KVH,D", HEADS)
+@pytest.mark.parametrize("ps", [8, 64])
+def test_trees(gpu, dtype, H, KVH, D, ps):
+    lens, counts = [1, 40, 0, 64, 300, 129, 77, 33], [1, 3, 0, 64, 65, 0, 30, 33]
+    c, families, bits = tree_case(gpu, DT[dtype], H, KVH, D, ps, lens, counts, seed=D + ps)
+    check_tree(c, families, bits)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("masked", [False, True])
+def test_trees_in_blocks_of_256_rows(gpu, dtype, D, masked):
+    """Enough rows for the other kernel, in one part and (one long sequence) in several."""
+    for lens, counts in (([700, 240, 513, 1, 200, 0], [140, 200, 90, 1, 70, 0]), ([4000], [65])):
+        c, families, bits = tree_case(gpu, DT[dtype], 32, 4, D, 16, lens, counts, seed=D)
+        how = {}
+        if masked:
+            how = dict(softcap=15.0, slopes=torch.rand(32, device=gpu, generator=c["gen"]) * 0.1, window=150,
+                       prefix=torch.tensor([90, 3, 0, 0, 10**6, 1][:len(lens)], dtype=torch.int32, device=gpu))
+        check_tree(c, families, bits, **how)
+
+
+@pytest.mark.parametrize("window,prefix", [(0, True), (1, False), (3, True), (7, False), (64, True), (100, False), (1000, True)])
+@pytest.mark.parametrize("softcap,bias", [(0.0, False), (0.0, True), (20.0, True)])
+@pytest.mark.parametrize("kind", ["mixed", "chain"])
+def test_tree_masks_and_scores(gpu, window, prefix, softcap, bias, kind):
+    lens, counts = [200, 75, 330, 1, 128], [9, 65, 130, 1, 20]
+    c, families, bits = tree_case(gpu, torch.float16, 14, 2, 64, 32, lens, counts, seed=window, kind=kind, amp=2.0)
+    slopes = torch.rand(14, device=gpu, generator=c["gen"]) if bias else None
+    pre = torch.tensor([0, 70, 33, 5, 500], dtype=torch.int32, device=gpu) if prefix else None
+    check_tree(c, families, bits, softcap=softcap, slopes=slopes, window=window, prefix=pre)
+
+
+@pytest.mark.parametrize("H,KVH,D", [(28, 4, 128), (14, 2, 64)])
+def test_a_chain_is_a_chunk_in_order(gpu, H, KVH, D):
+    """The same masks as attention's: the same numbers, but for where a window or a bias takes another way to them."""
+    from metal_native import paged
+
+    lens, counts = [300, 70, 5], [70, 64, 5]
+    c, families, bits = tree_case(gpu, torch.float16, H, KVH, D, 16, lens, counts, kind="chain")
+    out, lse = check_tree(c, families, bits)
+    a, la = paged.attention(c["q"], c["k"], c["v"], c["table"], c["lens"], c["cu"], return_lse=True)
+    u = half_step(torch.float16)
+    assert float((out.float() - a.float()).abs().max()) <= 8 * u * float(c["v"][c["v"].isfinite()].abs().max())
+    assert float((lse - la).abs().max()) <= 1e-4
+
+
+@pytest.mark.parametrize("n", [40, 300])
+@pytest.mark.parametrize("window", [0, 11])
+def test_any_bits(gpu, n, window):
+    """Bits of no tree: later nodes, not the row's own, none at all, set past the chunk; fewer words than nodes; a row
+    that sees nothing."""
+    rng = np.random.default_rng(n)
+    lens, counts = [n + 100, n, 7], [n, n, 7]
+    c = build(gpu, torch.bfloat16, 8, 2, 64, 16, lens, counts, seed=n)
+    words = -(-n // 64)
+    families = [rng.random((m, 64 * words)) < 0.2 for m in counts]
+    families[0][3] = families[1][5] = families[2][0] = False
+    families[1][6] = True
+    bits = torch.cat([ref.pack(f, words) for f in families]).to(gpu)
+    slopes = torch.rand(8, device=gpu) * 0.05
+    check_tree(c, families, bits, window=window, slopes=slopes)
+    out, lse = check_tree(c, families, bits, window=window)
+    assert float(out[n + 5].abs().max()) == 0 and bool((lse[n + 5] == -math.inf).all())
+    wide = torch.nn.functional.pad(bits, (0, 3), value=-1)[:, :words + 1]   # a row stride of its own; junk past the nodes
+    assert torch.equal(paged_tree(c, wide), paged_tree(c, bits))
+    if words > 1:
+        for f in families:
+            f[:, 64:] = False
+        check_tree(c, families, bits[:, :1], window=window)
+
+
+def paged_tree(c, bits, **how):
+    from metal_native import paged
+
+    return paged.tree_attention(c["q"], c["k"], c["v"], c["table"], c["lens"], bits, c["cu"], **how)
+
+
+@pytest.mark.parametrize("many", [False, True])
+def test_hidden_infinities_absent_pages_and_short_caches(gpu, many):
+    """What a row does not see leaves it alone, whatever it holds; what it sees is seen."""
+    H, KVH, lens, counts = (32, 4, [700, 300], [140, 60]) if many else (8, 2, [90, 50], [33, 20])
+    c, families, bits = tree_case(gpu, torch.float16, H, KVH, 64, 16, lens, counts, seed=2)
+    for s, node in ((0, 5), (0, 31), (1, 17)):
+        slot = lens[s] - counts[s] + node
+        page = c["table"][s, slot // 16].long()
+        c["v"][page, :, slot % 16, 3] = math.inf if node == 5 else math.nan
+    check_tree(c, families, bits)
+    t = c["table"]
+    t[0, 1], t[1, 0], t[0, (lens[0] - 3) // 16] = -1, 10**6, -(2**31)
+    check_tree(c, families, bits)
+    c["lens"][:] = torch.tensor([counts[0] - 7, 3], device=gpu)   # fewer slots than nodes
+    check_tree(c, families, bits, window=4, prefix=torch.tensor([2, 0], dtype=torch.int32, device=gpu))
+    t[1, :] = -1
+    check_tree(c, families, bits)
+
+
+def test_tree_layouts_and_rows_of_no_sequence(gpu):
+    from metal_native import paged
+
+    c, families, bits = tree_case(gpu, torch.float16, 8, 2, 64, 16, [50, 90], [12, 20], seed=7)
+    want = paged_tree(c, bits)
+    kv = torch.stack([c["k"], c["v"]], 1)
+    q2 = c["q"].transpose(0, 1).contiguous().transpose(0, 1)
+    assert torch.equal(paged.tree_attention(q2, kv[:, 0], kv[:, 1], c["table"], c["lens"], bits, c["cu"]), want)
+    odd = torch.empty(32, 8, 65, dtype=torch.float16, device=gpu)[..., 1:].copy_(c["q"])   # copied
+    assert torch.equal(paged.tree_attention(odd, c["k"], c["v"], c["table"], c["lens"], bits.t().contiguous().t(), c["cu"]), want)
+    pad = lambda x, v: torch.nn.functional.pad(x, (0, 0) * (x.dim() - 1) + (3, 5), value=v)  # noqa: E731
+    out, lse = paged.tree_attention(pad(c["q"], math.nan), c["k"], c["v"], c["table"], c["lens"], pad(bits, -1), c["cu"] + 3, return_lse=True)
+    assert torch.equal(out[3:-5], want) and float(out[:3].abs().max()) == 0 and float(out[-5:].abs().max()) == 0
+    assert bool((lse[:3] == -math.inf).all()) and bool((lse[-5:] == -math.inf).all())
+    one = paged.tree_attention(c["q"][:2], c["k"], c["v"], c["table"], c["lens"], bits[:2] * 0 + 1)
+    assert torch.equal(one, paged.attention(c["q"][:2], c["k"], c["v"], c["table"], c["lens"]))
+    assert paged.tree_attention(c["q"][:0], c["k"], c["v"], c["table"], c["lens"], bits[:0], c["cu"] * 0).shape == (0, 8, 64)
+
+
+# ---- accepted paths ----
+def accept_case(gpu, lens, counts, *, layers=None, KVH=2, D=64, ps=16, words=2, seed=0, kind="mixed", dtype=torch.float16):
+    parents, flat, cu = trees(gpu, counts, seed, kind)
+    c = build(gpu, dtype, KVH, KVH, D, ps, lens, counts, seed=seed, junk=7.0)
+    g = c["gen"]
+    shape = c["k"].shape if layers is None else (layers, *c["k"].shape)
+    k, v = (torch.randn(shape, device=gpu, generator=g).to(dtype) for _ in range(2))
+    drawn, drafted = (torch.randint(0, words, (sum(counts),), device=gpu, generator=g) for _ in range(2))
+    return dict(k=k, v=v, table=c["table"], lens=c["lens"], cu=cu, drawn=drawn, drafted=drafted, parents=flat, trees=parents, ps=ps)
+
+
+def check_accept(c, steps, k=None, v=None):
+    from metal_native import paged
+
+    k, v = c["k"] if k is None else k, c["v"] if v is None else v
+    want = [k.clone(), v.clone()]
+    b = len(c["trees"])
+    path, tokens = torch.full((b, steps), -1, dtype=torch.int32), torch.full((b, steps), -1)
+    count, new = torch.zeros(b, dtype=torch.int32), torch.zeros(b, dtype=torch.int32)
+    pages = k.shape[-4]
+    for s, tree in enumerate(c["trees"]):
+        a, n = int(c["cu"][s]), len(tree)
+        p, t = ref.accept(c["drawn"][a:a + n].tolist(), c["drafted"][a:a + n].tolist(), tree, steps)
+        path[s, :len(p)], tokens[s, :len(p)] = torch.tensor(p, dtype=torch.int32), torch.tensor(t, dtype=torch.int64)
+        count[s] = len(p)
+        off = int(c["lens"][s]) - n
+        new[s] = max(0, off + len(p))
+        for x, y in ((off + node, off + i) for i, node in enumerate(p)):
+            row = c["table"][s].tolist()
+            ids = [row[z // c["ps"]] if z >= 0 else -1 for z in (x, y)]
+            if x != y and all(0 <= z < pages for z in ids):
+                for cache, old in zip(want, (k, v)):
+                    cache[..., ids[1], :, y % c["ps"], :] = old[..., ids[0], :, x % c["ps"], :]
+    k, v = (x.clone(memory_format=torch.preserve_format) if x.is_contiguous() else x for x in (k, v))
+    got = paged.accept(k, v, c["table"], c["lens"], c["drawn"], c["drafted"], c["parents"], c["cu"], steps=steps)
+    assert torch.equal(got[0].cpu(), path) and torch.equal(got[1].cpu(), tokens)
+    assert torch.equal(got[2].cpu(), count) and torch.equal(got[3].cpu(), new)
+    assert torch.equal(k, want[0]) and torch.equal(v, want[1])
+    return path
+
+
+@pytest.mark.parametrize("layers", [None, 1, 5])
+@pytest.mark.parametrize("words,kind", [(1, "mixed"), (2, "mixed"), (2, "chain"), (1, "chain"), (3, "star"), (1000, "mixed")])
+def test_accept(gpu, layers, words, kind):
+    c = accept_case(gpu, [40, 70, 1, 90, 300, 20], [16, 64, 1, 0, 130, 20], layers=layers, words=words, kind=kind, seed=words)
+    for steps in (1, 3, 64, 70, 200):
+        check_accept(c, steps)
+
+
+@pytest.mark.parametrize("dtype,KVH,D,ps", [("bf16", 4, 128, 16), ("fp16", 1, 64, 8), ("fp16", 3, 128, 128)])
+def test_accept_layouts(gpu, dtype, KVH, D, ps):
+    c = accept_case(gpu, [100, 33], [40, 33], layers=3, KVH=KVH, D=D, ps=ps, words=1, dtype=DT[dtype])
+    check_accept(c, 20)
+    both = torch.stack([c["k"], c["v"]], 2)                       # [layers, pages, 2, ...]
+    check_accept(c, 20, both[:, :, 0], both[:, :, 1])
+    far = torch.stack([c["k"], c["v"]], 0)                        # and [2, layers, ...]
+    check_accept(c, 20, far[0], far[1])
+    turned = [x.transpose(2, 3).contiguous().transpose(2, 3) for x in (c["k"], c["v"])]
+    check_accept(c, 20, *turned)
+
+
+def test_accept_of_absent_pages_and_short_caches(gpu):
+    from metal_native import paged
+
+    c = accept_case(gpu, [100, 33, 60], [64, 33, 20], words=1, kind="chain", seed=1)
+    c["drawn"][10] = 5   # the chain breaks there
+    c["trees"][0][5:] = [p - 1 if p > 1 else 0 for p in c["trees"][0][5:]]
+    c["parents"][:64] = torch.tensor(c["trees"][0], dtype=torch.int32, device=gpu)
+    check_accept(c, 64)
+    t = c["table"]
+    t[0, 3], t[1, 0], t[2, 3] = -1, 10**6, -7
+    check_accept(c, 64)
+    c["lens"][:] = torch.tensor([50, 4, 1000], device=gpu)   # fewer slots than nodes; more than the table's width: cut to it
+    got = paged.accept(c["k"].clone(), c["v"].clone(), t, c["lens"], c["drawn"], c["drafted"], c["parents"], c["cu"], steps=64)
+    width = t.shape[1] * 16
+    assert got[3].tolist() == [max(0, 50 - 64 + int(got[2][0])), max(0, 4 - 33 + int(got[2][1])), width - 20 + int(got[2][2])]
+    for wild in ([-4, 3, 10**6, 5], [9, 2, 0, 117]):
+        got = paged.accept(c["k"].clone(), c["v"].clone(), t, c["lens"], c["drawn"], c["drafted"], c["parents"],
+                           torch.tensor(wild, dtype=torch.int32, device=gpu), steps=8)
+        assert got[0].shape == (3, 8)
+
+
+def test_accept_counts_its_writes_and_refuses_gradients(gpu):
+    from metal_native import MetalNativeError, paged
+
+    c = accept_case(gpu, [40], [16], layers=2, words=1)
+    call = lambda k: paged.accept(k, c["v"], c["table"], c["lens"], c["drawn"], c["drafted"], c["parents"], c["cu"], steps=4)  # noqa: E731
+    before = c["k"]._version
+    call(c["k"])
+    assert c["k"]._version == before + 1
+    with pytest.raises(MetalNativeError, match="requires a gradient"):
+        call(c["k"].clone().requires_grad_())
+    with pytest.raises(MetalNativeError):
+        call(c["k"][:1].expand(2, -1, -1, -1, -1))   # layers that share memory
+
+
+# ---- together ----
+def test_a_drafted_step_as_it_is_used(gpu):
+    """Chains hidden in trees: what the path's nodes saw is what the same tokens see in order, and the cache after the
+    step is the one that they leave."""
+    from metal_native import paged, sampling
+
+    H, KVH, D, ps, V = 8, 2, 64, 16, 50
+    lens, counts = [60, 33, 130], [21, 13, 40]
+    c, families, bits = tree_case(gpu, torch.float16, H, KVH, D, ps, lens, counts, seed=4)
+    parents, flat, cu = trees(gpu, counts, 4)
+    assert torch.equal(paged.ancestors(flat, cu, max(counts)), bits)
+    out = paged_tree(c, bits, max_q=max(counts))
+    logits = out.float().reshape(sum(counts), -1)[:, :V] * 10
+    drawn = sampling.sample(logits, torch.rand(sum(counts), device=gpu, generator=c["gen"]), temperature=0.7, top_k=9)
+    drafted = drawn[(cu[:-1].long().repeat_interleave(torch.tensor(counts, device=gpu)) + flat.clamp(min=0)).long()].clone()
+    drafted[::3] = V   # a third of the guesses is wrong
+    k, v = c["k"].clone(), c["v"].clone()
+    path, tokens, count, new = paged.accept(k, v, c["table"], c["lens"], drawn, drafted, flat, cu, steps=16)
+    assert int(count.max()) > 1
+    for s in range(3):
+        p = path[s, :int(count[s])].long()
+        rows = cu[s].long() + p
+        assert torch.equal(tokens[s, :len(p)], drawn[rows])
+        again = paged.attention(c["q"][rows], k, v, c["table"][s:s + 1], new[s:s + 1],
+                                torch.tensor([0, len(p)], dtype=torch.int32, device=gpu))
+        u = half_step(torch.float16)
+        assert float((again.float() - out[rows].float()).abs().max()) <= 8 * u * float(v[v.isfinite()].abs().max())
+
+
+def test_a_drafted_step_captured(gpu):
+    """Replayed between eager calls; the caches are put back before each turn."""
+    from metal_native import paged, sampling
+
+    counts, lens = [9, 30], [70, 200]
+    c, _, _ = tree_case(gpu, torch.float16, 8, 2, 64, 16, lens, counts, seed=6)
+    parents, flat, cu = trees(gpu, counts, 6)
+    u = torch.rand(39, device=gpu)
+    drafted = torch.randint(0, 3, (39,), device=gpu)
+    k0, v0 = c["k"].clone(), c["v"].clone()
+
+    def step():
+        bits = paged.ancestors(flat, cu, 30)
+        out = paged.tree_attention(c["q"], c["k"], c["v"], c["table"], c["lens"], bits, cu, max_q=30)
+        drawn = sampling.sample(out.reshape(39, -1)[:, :3], u, temperature=0.9, top_p=0.99)
+        return (bits, out, drawn, *paged.accept(c["k"], c["v"], c["table"], c["lens"], drawn, drafted, flat, cu, steps=8))
+
+    def reset(turn):
+        c["k"].copy_(k0)
+        c["v"].copy_(v0)
+        g = torch.Generator(device=gpu)
+        g.manual_seed(turn)
+        u.copy_(torch.rand(39, device=gpu, generator=g))
+        drafted.copy_(torch.randint(0, 3, (39,), device=gpu, generator=g))
+
+    reset(0)
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for turn in range(4):
+        reset(turn)
+        graph.replay()
+        kept = [t.clone() for t in got] + [c["k"].clone(), c["v"].clone()]
+        reset(turn)
+        want = [*step(), c["k"], c["v"]]
+        same = lambda a, b: torch.equal(a.nan_to_num(), b.nan_to_num()) if a.is_floating_point() else torch.equal(a, b)  # noqa: E731
+        assert all(same(a, b) for a, b in zip(kept, want))

@@ -1,0 +1,188 @@
+"""Operators for drafted tokens on the host: bits of a row, refused arguments."""
+
+import ctypes
+import os
+import shutil
+import subprocess
+
+import pytest
+import torch
+
+from test_paged_host import BAD_CACHE, BAD_MASK, BAD_QUERY, BAD_V, BIG, CACHE, CU, LIBRARY, MASK, P, ROOT, ROWS, V, Cache, Mask
+from test_paged_host import arguments as paged_arguments
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="needs g++")
+def test_bits_of_a_row(tmp_path):
+    """Every 64 of them, from in front of the row to past it, read inside it alone (bounds trapped)."""
+    src = tmp_path / "bits.cpp"
+    src.write_text('''
+#include <cstdio>
+#include <vector>
+#include "mq_paged.hpp"
+int main() {
+  long bad = 0;
+  for (int words = 1; words <= 4; ++words) {
+    std::vector<uint64_t> row(words);
+    for (int w = 0; w < words; ++w) row[w] = 0x9E3779B97F4A7C15ull * (w + 3) ^ (0xD1B54A32D192ED03ull >> w);
+    for (int64_t d = -200; d <= 64 * words + 200; ++d) {
+      uint64_t want = 0;
+      for (int i = 0; i < 64; ++i) {
+        const int64_t at = d + i;
+        if (at >= 0 && at < 64 * words) want |= (row[at / 64] >> (at % 64) & 1) << i;
+      }
+      bad += mq::paged_tree_bits(row.data(), words, d) != want;
+    }
+    for (int64_t d : {-(int64_t{1} << 40), int64_t{1} << 40, -(int64_t{1} << 31), int64_t{1} << 31}) bad += mq::paged_tree_bits(row.data(), words, d) != 0;
+  }
+  std::printf("bad %ld\\n", bad);
+}
+''')
+    exe = tmp_path / "bits"
+    subprocess.run(["g++", "-O1", "-std=c++17", "-fsanitize=undefined,address", "-fno-sanitize-recover=all",
+                    f"-I{os.path.join(ROOT, 'metal-native_amd', 'csrc')}", str(src), "-o", str(exe)], check=True, capture_output=True, timeout=300)
+    out = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300, env={k: v for k, v in os.environ.items() if k != "LD_PRELOAD"})
+    assert out.returncode == 0 and "bad 0" in out.stdout, out.stdout + out.stderr
+
+
+def arguments(dev):
+    h = paged_arguments(dev)["attention"]
+    i = dict(dtype=torch.int32, device=dev)
+    cache = {n: h[n] for n in ("k_cache", "v_cache", "table", "lens")}
+    return {
+        "ancestors": dict(parents=torch.zeros(ROWS, **i), cu=h["cu"], max_q=3),
+        "tree_attention": dict(h, tree=torch.ones(ROWS, 1, dtype=torch.int64, device=dev)),
+        "accept": dict(cache, drawn=torch.zeros(ROWS, dtype=torch.int64, device=dev), drafted=torch.zeros(ROWS, dtype=torch.int64, device=dev),
+                       parents=torch.zeros(ROWS, **i), cu=h["cu"], steps=2),
+    }
+
+
+INT64 = [None, lambda x: x.int(), lambda x: x[:-1], lambda x: x[None]]
+CHANGES = {
+    "ancestors": {"parents": [None, lambda x: x.long(), lambda x: x[None]], "cu": [lambda x: x[:1], lambda x: x.long(), lambda x: x[None]],
+                  "max_q": [lambda _: -1, lambda _: 2**31]},
+    "tree_attention": {**CACHE, **V, **CU, **MASK, "tree": [None, lambda x: x.int(), lambda x: x[:-1], lambda x: x[:, :0], lambda x: x[:, 0]]},
+    "accept": {**CACHE, **V, **CU, "drawn": INT64, "drafted": INT64, "parents": [None, lambda x: x.long(), lambda x: x[1:]],
+               "steps": [lambda _: 0, lambda _: -3, lambda _: 2**31]},
+}
+# the caches of accept may have a dimension of layers, in which case both have it
+LAYERS = [lambda k, v: (k[None], v), lambda k, v: (k, v[None]), lambda k, v: (k[None][:0], v[None][:0]), lambda k, v: (k.expand(2, -1, -1, -1, -1), v[None]),
+          lambda k, v: (k[None, None], v[None, None])]
+REFUSED = [(op, name, i) for op, by in CHANGES.items() for name, how in by.items() for i in range(len(how))]
+
+
+def call(op, name, i, dev):
+    from metal_native import paged
+
+    kw = arguments(dev)[op]
+    change = CHANGES[op][name][i]
+    value = None if change is None else change(kw.get(name))
+    kw[name] = value.to(dev) if isinstance(value, torch.Tensor) and value.device != dev and name in ("slopes", "prefix_lens") else value
+    return getattr(paged, op)(**kw)
+
+
+@pytest.fixture
+def stand_in(monkeypatch):
+    """CPU tensors stand in for the GPU's: no call gets past the checks."""
+    from metal_native import MetalNativeError, paged
+
+    def tensor(t, what, op):
+        if not isinstance(t, torch.Tensor):
+            raise MetalNativeError(f"{op}: {what} must be a torch.Tensor")
+
+    monkeypatch.setattr(paged, "_require_cuda", tensor)
+
+
+@pytest.mark.parametrize("op,name,i", [r for r in REFUSED if r[1] not in LIBRARY])
+def test_refused_before_the_library(op, name, i, stand_in):
+    from metal_native import MetalNativeError
+
+    with pytest.raises(MetalNativeError, match=f"paged.{op}: "):
+        call(op, name, i, torch.device("cpu"))
+
+
+@pytest.mark.parametrize("how", LAYERS)
+def test_layers_refused(how, stand_in):
+    from metal_native import MetalNativeError, paged
+
+    kw = arguments(torch.device("cpu"))["accept"]
+    kw["k_cache"], kw["v_cache"] = how(kw["k_cache"], kw["v_cache"])
+    with pytest.raises(MetalNativeError, match="paged.accept: "):
+        paged.accept(**kw)
+
+
+@pytest.mark.parametrize("op", list(CHANGES))
+def test_cpu_tensors_are_refused(op):
+    from metal_native import MetalNativeError, paged
+
+    with pytest.raises(MetalNativeError, match="GPU tensor"):
+        getattr(paged, op)(**arguments(torch.device("cpu"))[op])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op", list(CHANGES))
+def test_refused(gpu, op):
+    from metal_native import MetalNativeError, paged
+
+    getattr(paged, op)(**arguments(gpu)[op])
+    for name, how in CHANGES[op].items():
+        for i in range(len(how)):
+            with pytest.raises(MetalNativeError):
+                call(op, name, i, gpu)
+    for name in [n for n, x in arguments(gpu)[op].items() if isinstance(x, torch.Tensor)]:
+        with pytest.raises(MetalNativeError):   # one tensor on the host
+            getattr(paged, op)(**{n: x.cpu() if n == name else x for n, x in arguments(gpu)[op].items()})
+    if op == "accept":
+        for how in LAYERS:
+            kw = arguments(gpu)[op]
+            kw["k_cache"], kw["v_cache"] = how(kw["k_cache"], kw["v_cache"])
+            with pytest.raises(MetalNativeError):
+                paged.accept(**kw)
+        kw = arguments(gpu)[op]
+        kw["k_cache"] = kw["k_cache"][:, :1].expand(-1, 2, -1, -1)   # heads that share memory
+        with pytest.raises(MetalNativeError):
+            paged.accept(**kw)
+    getattr(paged, op)(**arguments(gpu)[op])
+
+
+# ---- the C entries: pointers that no refused call follows ----
+def c_call(op, cache=None, mask=None, **other):
+    from metal_native import _lib
+
+    L = _lib.load()
+    c = Cache(**{**dict(k=P, v=P, k_page=2048, k_head=1024, k_slot=64, v_page=2048, v_head=1024, v_slot=64, pages=6, kv_heads=2,
+                        page_size=16, head_dim=64, dtype=0, table=P, ld_table=3, width=3, batch=2, lens=P), **(cache or {})})
+    m = Mask(**{**dict(scale=0.125, softcap=0.0, slopes=None, window=0, prefix_lens=None, cu_q=P, max_q=0), **(mask or {})})
+    o = dict(q=P, q_token=512, q_head=64, rows=5, heads=8, out=P, lse=P, ws=None, ws_bytes=0, parents=P, cu=P, batch=2, words=1, tree=P,
+             ld_tree=1, layers=1, k_layer=0, v_layer=0, drawn=P, drafted=P, steps=4, path=P, tokens=P, count=P, new_lens=P)
+    assert set(other) <= set(o)
+    o.update(other)
+    names, first = {"ancestors": ("parents cu batch rows words tree", []),
+                    "tree_attention": ("tree ld_tree words q q_token q_head rows heads out lse ws ws_bytes", [ctypes.byref(c), ctypes.byref(m)]),
+                    "accept": ("layers k_layer v_layer drawn drafted parents cu rows steps path tokens count new_lens", [ctypes.byref(c)])}[op]
+    rc = getattr(L, f"mq_paged_{op}")(*first, *[o[n] for n in names.split()], None)
+    return rc, L.mq_last_error().decode()
+
+
+C_REFUSED = [("ancestors", b) for b in (dict(parents=None), dict(tree=None), dict(tree=P + 4), dict(batch=0), dict(batch=BIG), dict(rows=-1),
+                                        dict(rows=2**31 - 1), dict(words=0), dict(words=2**26), dict(cu=None))] + \
+    [(op, dict(cache=b)) for op in ("tree_attention", "accept") for b in BAD_CACHE + BAD_V] + \
+    [("tree_attention", dict(mask=b)) for b in BAD_MASK] + [("tree_attention", b) for b in BAD_QUERY] + \
+    [("tree_attention", b) for b in (dict(out=None), dict(out=P + 8), dict(tree=None), dict(tree=P + 4), dict(words=0), dict(words=BIG), dict(ld_tree=-1))] + \
+    [("accept", b) for b in (dict(layers=0), dict(layers=BIG), dict(k_layer=-8), dict(v_layer=-8), dict(k_layer=4), dict(v_layer=12), dict(drawn=None),
+                             dict(drafted=None), dict(parents=None), dict(cu=None), dict(rows=-1), dict(rows=2**31), dict(steps=0), dict(steps=BIG),
+                             dict(path=None), dict(tokens=None), dict(count=None), dict(new_lens=None))]
+
+
+@pytest.mark.parametrize("op,how", C_REFUSED, ids=lambda x: x if isinstance(x, str) else str(x))
+def test_c_entries_refuse(op, how):
+    rc, text = c_call(op, **how)
+    assert rc == 4 and text.startswith(f"paged.{op}: "), (rc, text)
+
+
+def test_c_entries_of_null_structs_and_no_rows():
+    from metal_native import _lib
+
+    assert _lib.load().mq_paged_tree_attention_workspace_size(None, None, 1, 1) == -1
+    assert c_call("tree_attention", rows=0, q=None, out=None)[0] == 0
+    assert c_call("ancestors", rows=0, parents=None, tree=None)[0] == 0
