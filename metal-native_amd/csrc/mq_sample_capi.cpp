@@ -19,7 +19,7 @@ int refuse(const char* what) {
 const char* sample_args(mq::SampleArgs& a, int64_t rows, int64_t vocab, int32_t dtype, const mq_sampling* how) {
   if (!how) return "null settings";
   if (dtype != MQ_SAMPLE_F16 && dtype != MQ_SAMPLE_BF16 && dtype != MQ_SAMPLE_F32) return "unknown dtype";
-  if (rows < 0 || rows > INT_MAX || vocab < 1 || vocab > 1 << 28) return "rows must be below 2^31, the vocabulary 1 to 2^28";
+  if (rows < 0 || rows > INT_MAX || vocab < 1 || vocab > 1 << 22) return "rows must be below 2^31, the vocabulary 1 to 2^22";
   a = mq::SampleArgs{};
   a.rows = (int)rows;
   a.vocab = (int)vocab;

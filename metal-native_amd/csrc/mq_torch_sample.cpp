@@ -24,7 +24,7 @@ bool setting(PyObject* o, const at::Tensor& x, float* one, const float** each) {
 PyObject* sample(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 8) return wrong_count("sample: 8 arguments");
   const at::Tensor *x = plain(a[0]), *u = plain(a[1]);
-  if (!x || x->dim() != 2 || x->size(1) < 1 || x->size(1) > 1 << 28 || (x->size(1) > 1 && x->stride(1) != 1) || x->stride(0) < 0) return decline();
+  if (!x || x->dim() != 2 || x->size(1) < 1 || x->size(1) > 1 << 22 || (x->size(1) > 1 && x->stride(1) != 1) || x->stride(0) < 0) return decline();
   const at::ScalarType ty = x->scalar_type();
   if ((ty != at::kHalf && ty != at::kBFloat16 && ty != at::kFloat) || !vec(u, x->device(), at::kFloat, x->size(0))) return decline();
   mq_sampling how{};

@@ -47,8 +47,8 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top_k=0, t
             return _finish(op, r)
     logits, u, temperature, top_k, top_p, min_p = _plain(logits, u, temperature, top_k, top_p, min_p)
     _require_cuda(logits, "logits", op)
-    if logits.dtype not in (torch.float16, torch.bfloat16, torch.float32) or logits.dim() != 2 or not 1 <= logits.shape[1] <= 2**28:
-        _invalid(f"{op}: logits must be Float16, BFloat16 or Float32 [rows, vocab], the vocabulary 1 to 2^28")
+    if logits.dtype not in (torch.float16, torch.bfloat16, torch.float32) or logits.dim() != 2 or not 1 <= logits.shape[1] <= 2**22:
+        _invalid(f"{op}: logits must be Float16, BFloat16 or Float32 [rows, vocab], the vocabulary 1 to 2^22")
     rows = logits.shape[0]
     _require_cuda(u, "u", op)
     if u.dtype != torch.float32 or tuple(u.shape) != (rows,) or u.device != logits.device:

@@ -4,6 +4,7 @@ paged_ref: its scores and sums are the same, only which slots a row sees and how
 far away they are is not."""
 
 import math
+from fractions import Fraction
 
 import numpy as np
 import torch
@@ -104,6 +105,12 @@ def accept(drawn, drafted, parents, steps):
     return path, [drawn[i] for i in path]
 
 
+def passes(w, n, u):
+    """Whether the first n weights add up to more than u times all of them, exactly."""
+    add = lambda a: sum(Fraction(float(v)) * int(m) for v, m in zip(*np.unique(a, return_counts=True)))  # noqa: E731
+    return add(w[:n]) > Fraction(u) * add(w)
+
+
 def sample(x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """(token, log of its share) of one row of float64 logits; settings as float32 holds them."""
     x = np.where(np.isnan(x), -np.inf, x.astype(np.float64))
@@ -133,4 +140,10 @@ def sample(x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     order, w, z = order[by], w[by], z[by]
     c = np.cumsum(w)
     i = int(np.searchsorted(c, u * c[-1], side="right"))
+    # A running sum that is the aim but for this sum's own rounding (few values: halves of a row that hold the same
+    # ones) is compared once more, as the fraction that its weights add up to.
+    while i > 0 and abs(c[i - 1] - u * c[-1]) < 1e-12 * c[-1] and passes(w, i, u):
+        i -= 1
+    while i + 1 < len(w) and abs(c[i] - u * c[-1]) < 1e-12 * c[-1] and not passes(w, i + 1, u):
+        i += 1
     return int(order[i]), float(z[i] - math.log(c[-1]))
