@@ -18,16 +18,19 @@
 // (a sub).  What a row needs follows from its settings, which the GPU alone may
 // know (Kind); the launches are the same for all of them:
 //   scan    of every part: its largest logit, and by kind its first token; the
-//           tokens that may be among the row's first top_k; the subs' sums; or how
-//           much weight and how many tokens each cell of a grid over the
-//           logits has.  Sums are relative to the part's own largest logit.
-//   gather  where the grid was filled, or min_p alone cuts: the cells in which the
-//           cuts fall, from all parts' grids; the subs' sums of what lies over
-//           them, and a list of the tokens in them.
-//   pick    the cuts among the listed tokens, the sub in which the running sum
-//           passes its aim, and the token in it.
-// A list that is too short (masses of equal logits at a cut) sends its row to
-// the long way: cuts found digit by digit by one workgroup, pass after pass.
+//           largest logit of each lane of a sub; the subs' sums; or how much weight
+//           and how many tokens lie, about, in each cell of a grid over the logits.
+//   bounds  where the grid was filled: from all parts' grids, the logits between
+//           which the cuts must fall.
+//   gather  there, or where min_p alone cuts: the subs' sums of what lies over these,
+//           and a list of the tokens between them.
+//   pick    the cuts among the listed tokens (or those of the lanes that may hold
+//           the first top_k), the sub in which the running sum passes its aim, and the
+//           token in it.
+// The grid only says where to look: that a cut falls among the listed tokens is
+// checked with exact sums.  Where it does not, or a list is too short (masses of
+// equal logits at a cut), the row goes the long way: cuts found digit by digit by
+// one workgroup, pass after pass.
 #include "mq_device.hpp"
 #include "mq_sample.hpp"
 
@@ -40,9 +43,8 @@ namespace {
 
 typedef unsigned long long ull;
 constexpr int kThreads = 1024, kWaves = kThreads / 64, kSub = 1024;
-constexpr int kListRow = 8192;              // list entries of a row, over all parts
-constexpr int kHeld = kListRow / kThreads;  // of them in a thread
-constexpr int kFewMost = 512;               // top_k up to which a row may be Few
+constexpr int kListRow = 4096;   // list entries of a row, over all parts
+constexpr int kFewMost = 512;    // top_k up to which a row may be kFew
 
 // Whole numbers in the order of the values: NaN counts as -inf, -0 as 0.
 __device__ __forceinline__ uint32_t order_of(float x) {
@@ -65,7 +67,7 @@ struct Settings {
   float u;
   int kind;
 };
-// few: the largest top_k that goes by the parts' first tokens
+// few: the largest top_k that goes by the lanes' largest logits
 __device__ __forceinline__ Settings settings_of(const SampleArgs& p, int row, int few) {
   Settings s;
   const float t = p.temperatures ? p.temperatures[row] : p.temperature;
@@ -115,22 +117,33 @@ constexpr double kUnit = 0x1p-44;
 __device__ __forceinline__ ull whole_of_list(double w) { return (ull)__double_as_longlong(w + 4.0) & ((1ull << 52) - 1); }
 constexpr double kListUnit = 0x1p-50;
 
-// ---- the grid: cells of 1/64 of a factor of two in weight, the same ones for all
-// parts of a row; 1536 under the largest logit's by themselves, the rest by
-// sixteens, what lies under all of these in the last one ----
-constexpr int kFine = 1536, kCoarse = 512, kCells = kFine + kCoarse;
-__device__ __forceinline__ float grid_scale(double inv_t) { return (float)fmin(steps_of(inv_t), 1e30); }
-__device__ __forceinline__ int grid_of(float x, float scale) {   // grows with x
-  const float g = fminf(fmaxf(floorf(x * scale), -0x1p29f), 0x1p29f);
-  return x == INFINITY ? 1 << 29 : (int)g;
+// ---- the grid: cells of 1/128 of a factor of two in weight, the same ones for all
+// parts of a row; kFine of them under the largest logit's (28 factors of two, further
+// than a cut by top_p can lie: weights of 2^-28 add up to less than it leaves out),
+// the rest by eights, what lies under all of these in the last one ----
+constexpr int kFine = 3584, kCoarse = 4608, kCells = kFine + kCoarse;
+constexpr float kEnd = 0x1p29f;   // the grid's ends
+// A cell's weights add up as whole multiples of 2^-9 of the weight at its lower edge (2^22 tokens fit 32
+// bits): each is off by 2^-10 of itself at most, and by the rounding of the product with the scale
+constexpr float kCellUnits = 512.f;
+__device__ __forceinline__ float grid_scale(double inv_t) { return (float)fmin(inv_t * (128 * 1.44269504088896340736), 1e30); }
+struct Place {
+  int g;
+  float part;   // of a cell, over its lower edge
+};
+__device__ __forceinline__ Place grid_of(float x, float scale) {   // g grows with x
+  const float t = x == INFINITY ? kEnd : fminf(fmaxf(x * scale, -kEnd), kEnd), low = floorf(t);
+  return {(int)low, t - low};
 }
-__device__ __forceinline__ int cell_of(int g, int top) {
-  const int d = top - g;
-  return d < kFine ? d : kFine + min(kCoarse - 1, (top >> 4) - (g >> 4));
+// The logit at a cell's lower edge, moved `way` by more than its roundings
+__device__ __forceinline__ float edge_of(int g, float scale, float way) {
+  if (scale < 0x1p-100f || fabsf((float)g) >= kEnd) return way * INFINITY;
+  const float x = (float)g / scale;
+  return x + way * (fabsf(x) * 0x1p-20f + 0x1p-20f / scale);
 }
 
-// ---- a workgroup's sums ----
-template <typename V, typename F> __device__ __forceinline__ V reduce(V v, V* lds, F&& f) {   // on every thread
+// ---- sums of the workgroup's first N waves (the others have gone, if there are any) ----
+template <int N, typename V, typename F> __device__ __forceinline__ V reduce(V v, V* lds, F&& f) {   // on every thread
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
 #pragma unroll
   for (int o = 32; o; o >>= 1) v = f(v, (V)__shfl_xor(v, o));
@@ -138,14 +151,21 @@ template <typename V, typename F> __device__ __forceinline__ V reduce(V v, V* ld
   if (lane == 0) lds[w] = v;
   __syncthreads();
   v = lds[0];
-  for (int i = 1; i < kWaves; ++i) v = f(v, lds[i]);
+#pragma unroll
+  for (int i = 1; i < N; ++i) v = f(v, lds[i]);
   return v;
 }
-template <typename V> __device__ __forceinline__ V add_up(V v, V* lds) {
-  return reduce<V>(v, lds, [](V a, V b) { return a + b; });
+template <int N, typename V> __device__ __forceinline__ V add_up(V v, V* lds) {
+  return reduce<N, V>(v, lds, [](V a, V b) { return a + b; });
+}
+template <int N> __device__ __forceinline__ ull least_of(ull v, ull* lds) {
+  return reduce<N, ull>(v, lds, [](ull a, ull b) { return a < b ? a : b; });
+}
+template <int N> __device__ __forceinline__ ull most_of(ull v, ull* lds) {
+  return reduce<N, ull>(v, lds, [](ull a, ull b) { return a > b ? a : b; });
 }
 // inclusive, and the sum of all
-template <typename V> __device__ __forceinline__ V scan(V v, V* lds, V& all) {
+template <int N, typename V> __device__ __forceinline__ V scan(V v, V* lds, V& all) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -157,20 +177,21 @@ template <typename V> __device__ __forceinline__ V scan(V v, V* lds, V& all) {
   __syncthreads();
   V before = 0;
   all = 0;
-  for (int i = 0; i < kWaves; ++i) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
     if (i < w) before += lds[i];
     all += lds[i];
   }
   return v + before;
 }
-// of 32-bit counts that are the same on a wave's lanes; one barrier, by turns in two halves of lds
-__device__ __forceinline__ uint32_t count_up(uint32_t n, uint32_t* lds, int& turn) {
+// of counts that are the same on a wave's lanes; one barrier, by turns in two halves of lds
+template <int N> __device__ __forceinline__ uint32_t count_up(uint32_t n, uint32_t* lds, int& turn) {
   turn ^= kWaves;
   if ((threadIdx.x & 63) == 0) lds[turn + (threadIdx.x >> 6)] = n;
   __syncthreads();
   uint32_t s = 0;
 #pragma unroll
-  for (int i = 0; i < kWaves; ++i) s += lds[turn + i];
+  for (int i = 0; i < N; ++i) s += lds[turn + i];
   return s;
 }
 
@@ -182,8 +203,8 @@ template <typename E> struct Row {
   __device__ __forceinline__ Row(const SampleArgs& p, int row) : x((const E*)p.logits + (int64_t)row * p.ld), V(p.vocab), aligned(((uintptr_t)x & 15) == 0) {}
   static constexpr int kPer = 16 / sizeof(E);
   // the lane's j-th: index within the sub, growing with j
-  __device__ __forceinline__ int at(int j) const {
-    const int lane = threadIdx.x & 63;
+  __device__ __forceinline__ int at(int j) const { return at(j, threadIdx.x & 63); }
+  __device__ __forceinline__ int at(int j, int lane) const {
     return aligned ? j / kPer * (64 * kPer) + lane * kPer + j % kPer : j * 64 + lane;
   }
   __device__ __forceinline__ void load(int sub, float (&v)[16]) const {   // -inf past the row
@@ -207,62 +228,68 @@ template <typename E> struct Row {
 
 // ---- what the launches hand on ----
 struct Part {
-  float top;       // largest logit
-  uint32_t listed; // tokens that asked for a place in the list; past its length: it is not whole
-  uint32_t first;  // kGreedy: the first token of that logit
-  uint32_t pad;
-  double tail;     // kGrid: weights that are in no cell
+  float top;        // largest logit
+  uint32_t first;   // kGreedy: the first token of that logit
+  uint32_t far;     // kGrid, without counts: tokens under the fine cells
+  uint32_t listed;  // tokens that asked for a place in the list; past its length: it is not whole
+  uint32_t over_n;  // kGrid: tokens from Bounds::k_hi on
+  uint32_t cells;   // kGrid: the last cell that holds a token, and one
+  double over_k, over_p;   // kGrid: weight from k_hi on (of all tokens where top_k does not cut), from p_hi on
 };
-struct RowCut {   // by gather, for pick
-  int cell_k, cell_p0, cell_p1;   // the cut of top_k falls in cell_k, that of top_p in cell_p0 .. cell_p1 (kCells: there is none)
-  uint32_t before_n;              // tokens before cell_k
-  double before_k, before_p;      // weight before cell_k, cell_p0
-  double sum;                     // of all tokens
+struct Bounds {   // by gather, for pick: the cut of top_k falls among logits of k_lo <= x < k_hi, that of top_p between p_lo and p_hi
+  float k_lo, k_hi, p_lo, p_hi;   // -inf where there is none
+  int cut_k, cut_p;
+  __device__ __forceinline__ float sure() const { return cut_p ? p_hi : k_hi; }   // tokens from here on stay, but for min_p
 };
 struct Work {
   Part* part;       // [rows, parts]
-  RowCut* cut;      // [rows]
+  Bounds* bounds;   // [rows]
   double* sub;      // [rows, subs]
+  float* most;      // [rows, subs, 64]: of each lane
   uint32_t* list;   // [rows, parts, places]
-  ull* weight;      // [rows, parts, kCells]
+  uint32_t* weight; // [rows, parts, kCells]
   uint32_t* number; // [rows, parts, kCells]
   int row0, parts, subs, places, few;
-  __device__ __forceinline__ int first_sub(int part) const { return (int)((int64_t)subs * part / parts); }
+  int part_subs;   // of a part; fewer of the last
+  __device__ __forceinline__ int first_sub(int part) const { return min(part * part_subs, subs); }
 };
 
 template <typename E> __global__ __launch_bounds__(kThreads) void sample_scan_kernel(SampleArgs p, Work ws) {
   __shared__ double table[64];
-  __shared__ union {
-    ull weight[kCells];
-    ull red[kWaves];
-    uint32_t count[2 * kWaves];
-  } sh;
-  __shared__ uint32_t number[kCells], places;
+  __shared__ ull red[kWaves];
+  __shared__ uint32_t cells[2 * kCells];   // weights, then numbers
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int r = blockIdx.x / ws.parts, part = blockIdx.x - r * ws.parts, row = ws.row0 + r;
   const Settings st = settings_of(p, row, ws.few);
   const Row<E> x(p, row);
   const int s0 = ws.first_sub(part) + w, s1 = ws.first_sub(part + 1);
-  fill_table(table);
-  if (tid == 0) places = 0;
+  const bool count = st.top_k < p.vocab;
   float v[16], mine = -INFINITY;
   for (int s = s0; s < s1; s += kWaves) {
     x.load(s, v);
+    float m = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) mine = fmaxf(mine, v[j]);   // the number of the two, where one is NaN
+    for (int j = 0; j < 16; ++j) m = fmaxf(m, v[j]);   // the number of the two, where one is NaN
+    if (st.kind == kFew) ws.most[((int64_t)r * ws.subs + s) * 64 + lane] = m;
+    mine = fmaxf(mine, m);
   }
-  const float M = __uint_as_float((uint32_t)reduce<ull>(__float_as_uint(mine), sh.red, [](ull a, ull b) {
-    return (ull)__float_as_uint(fmaxf(__uint_as_float((uint32_t)a), __uint_as_float((uint32_t)b)));
-  }));
+  if (st.kind == kAll) fill_table(table);
+  if (st.kind == kGrid)
+    for (int i = tid; i < (count ? 2 * kCells : kFine); i += kThreads) cells[i] = 0;
+#pragma unroll
+  for (int o = 32; o; o >>= 1) mine = fmaxf(mine, __shfl_xor(mine, o));
+  if (lane == 0) ((float*)red)[w] = mine;
+  __syncthreads();
+  float M = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) M = fmaxf(M, ((float*)red)[i]);
+  __syncthreads();   // red is read
   Part& out = ws.part[(int64_t)r * ws.parts + part];
-  if (tid == 0) out.top = M;
-  __syncthreads();   // sh.red is read
-  if (M == -INFINITY) {
-    if (tid == 0) out.listed = 0;
-    return;
+  if (tid == 0) {
+    out.top = M;
+    out.cells = 0;
   }
-  const Weights weight{table, steps_of(st.inv_t), M};
-  double* sub = ws.sub + (int64_t)r * ws.subs;
+  if (M == -INFINITY || st.kind == kFew || st.kind == kFloor) return;
   if (st.kind == kGreedy) {
     uint32_t first = ~0u;
     for (int s = s0; s < s1 && first == ~0u; s += kWaves) {
@@ -270,9 +297,11 @@ template <typename E> __global__ __launch_bounds__(kThreads) void sample_scan_ke
 #pragma unroll
       for (int j = 15; j >= 0; --j) first = v[j] == M ? s * kSub + x.at(j) : first;
     }
-    first = (uint32_t)reduce<ull>(first, sh.red, [](ull a, ull b) { return a < b ? a : b; });
+    first = (uint32_t)least_of<kWaves>(first, red);
     if (tid == 0) out.first = first;
   } else if (st.kind == kAll) {
+    const Weights weight{table, steps_of(st.inv_t), M};
+    double* sub = ws.sub + (int64_t)r * ws.subs;
     for (int s = s0; s < s1; s += kWaves) {
       x.load(s, v);
       double sum = 0;
@@ -282,84 +311,209 @@ template <typename E> __global__ __launch_bounds__(kThreads) void sample_scan_ke
       for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
       if (lane == 0) sub[s] = sum;
     }
-  } else if (st.kind == kFew) {
-    // At least top_k of the threads hold a token as large as the top_k-th
-    // largest of what each holds at most, so all of the row's first top_k in
-    // this part are as large; about top_k tokens are, while it is half the threads or less.
-    const uint32_t key = order_of(mine) >> kLow<E>;
-    uint32_t least = 0;
-    int turn = 0;
-#pragma unroll 1
-    for (int bit = 31 - kLow<E>; bit >= 0; --bit) {
-      const uint32_t t = least | 1u << bit;
-      if (count_up(__popcll(__ballot(key >= t)), sh.count, turn) >= (uint32_t)st.top_k) least = t;
-    }
-    uint32_t* list = ws.list + ((int64_t)r * ws.parts + part) * ws.places;
-    const float low = value_of(least << kLow<E> | ((least >> (31 - kLow<E>)) & 1 ? 0 : (1u << kLow<E>) - 1));
-    for (int s = s0; s < s1; s += kWaves) {
-      x.load(s, v);
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const bool take = v[j] >= low && v[j] > -INFINITY;
-        const uint64_t all = __ballot(take);
-        if (!all) continue;
-        uint32_t at = 0;
-        if (lane == 0) at = atomicAdd(&places, (uint32_t)__popcll(all));
-        at = __builtin_amdgcn_readfirstlane(at) + __popcll(all & ((1ull << lane) - 1));
-        if (take && at < (uint32_t)ws.places) list[at] = s * kSub + x.at(j);
-      }
-    }
-    __syncthreads();
-    if (tid == 0) out.listed = places;
-  } else if (st.kind == kGrid) {
-    const bool count = st.top_k < p.vocab;
+  } else {
     const float scale = grid_scale(st.inv_t);
-    const int top = grid_of(M, scale);
-    // Of tokens under (1 - top_p) / 2 V of the part's largest weight, all of them
-    // together are less than the cut leaves out: where nothing counts them they
-    // need no cell
-    const double least = count ? -1.0 : (1.0 - st.top_p) / (2.0 * p.vocab);
-    for (int i = tid; i < kCells; i += kThreads) sh.weight[i] = 0, number[i] = 0;
-    __syncthreads();
-    double tail = 0;
+    const int top = grid_of(M, scale).g;
+    // 2^(y / 128) for y in 0 .. 1, in a cell's units
+    constexpr float kLn = 0.69314718f / 128, kA = kCellUnits * kLn, kB = kCellUnits * kLn * kLn / 2;
+    uint32_t far = 0;
     for (int s = s0; s < s1; s += kWaves) {
       x.load(s, v);
+      if (!count) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const Place at = grid_of(v[j], scale);
+          const int d = top - at.g;
+          if (d < kFine && v[j] > -INFINITY)
+            atomicAdd(&cells[d], (uint32_t)__builtin_fmaf(__builtin_fmaf(kB, at.part, kA), at.part, kCellUnits + 0.5f));
+          else
+            far += v[j] > -INFINITY;
+        }
+      } else {
 #pragma unroll 4
-      for (int j = 0; j < 16; ++j) {
-        const double wt = weight(v[j]);
-        if (wt < least) {
-          tail += wt;
-        } else if (v[j] > -INFINITY) {
-          const int cell = cell_of(grid_of(v[j], scale), top);
-          atomicAdd(&sh.weight[cell], whole(wt));
-          if (count) atomicAdd(&number[cell], 1u);
+        for (int j = 0; j < 16; ++j) {
+          const Place at = grid_of(v[j], scale);
+          if (!(v[j] > -INFINITY)) continue;
+          const int d = top - at.g;
+          const bool fine = d < kFine;
+          const int cell = fine ? d : kFine + min(kCoarse - 1, (top >> 3) - (at.g >> 3));
+          const float y = at.part + (fine ? 0 : at.g & 7);
+          atomicAdd(&cells[cell], (uint32_t)(kCellUnits * exp2f(y * (1.f / 128)) + 0.5f));
+          atomicAdd(&cells[kCells + cell], 1u);
         }
       }
     }
     __syncthreads();
-    ull* weights = ws.weight + ((int64_t)r * ws.parts + part) * kCells;
-    for (int i = tid; i < kCells; i += kThreads) weights[i] = sh.weight[i];
-    if (count) {
-      uint32_t* numbers = ws.number + ((int64_t)r * ws.parts + part) * kCells;
-      for (int i = tid; i < kCells; i += kThreads) numbers[i] = number[i];
+    uint32_t* weights = ws.weight + ((int64_t)r * ws.parts + part) * kCells;
+    uint32_t* numbers = ws.number + ((int64_t)r * ws.parts + part) * kCells;
+    uint32_t end = 0;
+    for (int i = tid; i < (count ? kCells : kFine); i += kThreads) {
+      const uint32_t c = cells[i];
+      weights[i] = c;
+      if (count) numbers[i] = cells[kCells + i];
+      if (c) end = i + 1;
     }
-    __syncthreads();
-    tail = add_up<double>(tail, (double*)sh.red);
-    if (tid == 0) out.tail = tail;
+    end = (uint32_t)most_of<kWaves>(end, red);
+    far = (uint32_t)add_up<kWaves, ull>(far, red);
+    if (tid == 0) {
+      out.cells = end;
+      out.far = far;
+    }
   }
 }
 
-// The row's largest logit, over its parts
+// The row's largest logit, over its parts (at most kPartsMost: one to a lane)
+constexpr int kPartsMost = 16;
 __device__ __forceinline__ float top_of(const Part* part, int parts) {
-  float M = -INFINITY;
-  for (int i = 0; i < parts; ++i) M = fmaxf(M, part[i].top);
+  const int i = threadIdx.x & (kPartsMost - 1);
+  float M = i < parts ? part[i].top : -INFINITY;
+#pragma unroll
+  for (int o = kPartsMost / 2; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
   return M;
 }
 
-// Grids are laid over each other: a cell of a part's grid is one of the row's.
+// All parts' grids laid over each other: a part's cell, from its own largest logit
+// down, is one of the row's.  Then between which logits the cuts fall; a workgroup
+// for each row.
+__global__ __launch_bounds__(kThreads) void sample_bounds_kernel(SampleArgs p, Work ws) {
+  __shared__ uint32_t weights[kCells], numbers[kCells];
+  __shared__ double red[kWaves];
+  __shared__ uint32_t far_of;
+  __shared__ int cell[3];
+  const int tid = threadIdx.x, r = blockIdx.x, row = ws.row0 + r;
+  const Settings st = settings_of(p, row, ws.few);
+  if (st.kind != kGrid) return;
+  const Part* parts = ws.part + (int64_t)r * ws.parts;
+  const float M = top_of(parts, ws.parts);
+  if (M == -INFINITY) return;
+  const bool count = st.top_k < p.vocab;
+  const int cells = count ? kCells : kFine;
+  const float scale = grid_scale(st.inv_t);
+  const int top = grid_of(M, scale).g;
+  for (int i = tid; i < cells; i += kThreads) weights[i] = numbers[i] = 0;
+  if (tid == 0) far_of = 0;
+  __syncthreads();
+  uint32_t far = 0;   // tokens under the row's fine cells, or more
+  // as many threads to each part: a power of two
+  int lanes = kThreads;
+  while (lanes * ws.parts > kThreads) lanes >>= 1;
+  const int of = tid / lanes;
+  if (of < ws.parts) {
+    const Part& q = parts[of];
+    const int end = (int)q.cells, mt = grid_of(q.top, scale).g, down = top - mt;
+    const uint32_t* pw = ws.weight + ((int64_t)r * ws.parts + of) * kCells;
+    const uint32_t* pn = ws.number + ((int64_t)r * ws.parts + of) * kCells;
+    if ((tid & (lanes - 1)) == 0 && !count && end) far += q.far;
+    constexpr int kStep = 8;   // loads of a thread on their way
+    for (int d0 = tid & (lanes - 1); d0 < end; d0 += kStep * lanes) {
+      uint32_t wt[kStep], n[kStep];
+#pragma unroll
+      for (int k = 0; k < kStep; ++k) {
+        const int d = d0 + k * lanes;
+        wt[k] = d < end ? pw[d] : 0;
+        n[k] = count && d < end ? pn[d] : 0;
+      }
+#pragma unroll
+      for (int k = 0; k < kStep; ++k) {
+        if (wt[k] == 0) continue;
+        const int d = d0 + k * lanes;
+        if (d < kFine && d + down < kFine) {
+          atomicAdd(&weights[d + down], wt[k]);
+          if (count) atomicAdd(&numbers[d + down], n[k]);
+        } else if (!count) {
+          far += wt[k] / (uint32_t)kCellUnits;   // no token has less
+        } else if (d < kFine) {   // to the lower edge of a coarse cell
+          const int g = mt - d, c = kFine + min(kCoarse - 1, (top >> 3) - (g >> 3));
+          atomicAdd(&weights[c], (uint32_t)((float)wt[k] * exp2f((g & 7) * (1.f / 128))));
+          atomicAdd(&numbers[c], n[k]);
+        } else {
+          const int c = kFine + min(kCoarse - 1, d - kFine + (top >> 3) - (mt >> 3));
+          atomicAdd(&weights[c], wt[k]);
+          atomicAdd(&numbers[c], n[k]);
+        }
+      }
+    }
+  }
+  if (far) atomicAdd(&far_of, far);
+  if (tid == 0) cell[0] = cell[1] = cell[2] = cells;
+  __syncthreads();
+  constexpr int N = kCells / kThreads;
+  const int per = count ? N : (kFine + kThreads - 1) / kThreads, b0 = per * tid;   // the thread's cells
+  double wt[N], mine = 0;
+  uint32_t n[N], mine_n = 0;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int b = b0 + k;
+    const bool have = k < per && b < cells;
+    const int down = b < kFine ? b : top - 8 * ((top >> 3) - (b - kFine));   // of the lower edge, from the top cell's
+    wt[k] = have ? (double)weights[have ? b : 0] * exp2((double)-down * (1.0 / 128)) : 0;
+    n[k] = have && count ? numbers[b] : 0;
+    mine += wt[k];
+    mine_n += n[k];
+  }
+  double all;
+  const double before = scan<kWaves, double>(mine, red, all) - mine;
+  if (count) {
+    uint32_t all_n, at = scan<kWaves, uint32_t>(mine_n, (uint32_t*)red, all_n) - mine_n;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      if (at < (uint32_t)st.top_k && at + n[k] >= (uint32_t)st.top_k) cell[0] = b0 + k;   // one thread
+      at += n[k];
+    }
+  }
+  __syncthreads();
+  const int cell_k = cell[0];
+  if (st.top_p < 1.0) {
+    // What is known: sums of cells to e of themselves; what lies under the fine cells, from nothing to
+    // 2^-28 a token; of cell_k, some part
+    const double e = 1.2e-3 + fabs((double)top) * 0x1p-28, share = fmax(st.top_p, 0.0);
+    double upto = all, in_k = 0;
+    if (cell_k < cells) {
+      double run = before;
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        run += wt[k];
+        if (b0 + k == cell_k && k < per) red[0] = run, red[1] = wt[k];
+      }
+      __syncthreads();
+      upto = red[0];
+      in_k = red[1];
+    }
+    const double under = count ? 0 : far_of * 0x1p-28 * kCellUnits;
+    const double lo = (upto - in_k) * (1 - e), hi = upto * (1 + e) + under;   // of what top_p is a share of
+    double run = before;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      run += wt[k];
+      const int b = b0 + k;
+      if (b > cell_k || wt[k] == 0) continue;
+      const double rest = fmax(upto - run, 0.0);   // weight past the cell, with all of cell_k
+      const bool may = run * (1 + e) >= share * lo && fmax(rest - in_k, 0.0) * (1 - e) <= (1 - share) * hi;
+      const bool must = run * (1 - e) >= share * hi || rest * (1 + e) + under <= (1 - share) * upto * (1 - e);
+      if (may) atomicMin(&cell[1], b);
+      if (must) atomicMin(&cell[2], b);
+    }
+    __syncthreads();
+  }
+  if (tid) return;
+  auto lower = [&](int c) { return c < kFine ? top - c : 8 * ((top >> 3) - (c - kFine)); };   // smallest g of a cell
+  auto upper = [&](int c) { return c < kFine ? top - c : min(8 * ((top >> 3) - (c - kFine)) + 7, top - kFine); };
+  Bounds b{-INFINITY, -INFINITY, -INFINITY, -INFINITY, cell_k < cells, st.top_p < 1.0};
+  if (b.cut_k) {
+    b.k_hi = edge_of(upper(cell_k) + 1, scale, 1.f);
+    b.k_lo = cell_k == kCells - 1 ? -INFINITY : edge_of(lower(cell_k), scale, -1.f);
+  }
+  if (b.cut_p) {
+    const int p1 = cell[2], p0 = min(cell[1], min(p1, cells - 1));
+    b.p_hi = edge_of(upper(p0) + 1, scale, 1.f);
+    b.p_lo = p1 >= cells || p1 == kCells - 1 ? b.k_lo : edge_of(lower(p1), scale, -1.f);
+  }
+  ws.bounds[r] = b;
+}
+
 template <typename E> __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleArgs p, Work ws) {
   __shared__ double table[64], red[kWaves];
-  __shared__ RowCut cut;
   __shared__ uint32_t places;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int r = blockIdx.x / ws.parts, part = blockIdx.x - r * ws.parts, row = ws.row0 + r;
@@ -369,137 +523,74 @@ template <typename E> __global__ __launch_bounds__(kThreads) void sample_gather_
   const float M = top_of(parts, ws.parts);
   if (M == -INFINITY) return;
   fill_table(table);
-  if (tid == 0) {
-    places = 0;
-    cut.cell_k = cut.cell_p0 = cut.cell_p1 = kCells;
-    cut.before_n = 0;
-    cut.before_k = cut.before_p = cut.sum = 0;
-  }
+  if (tid == 0) places = 0;
   __syncthreads();
   const Weights weight{table, steps_of(st.inv_t), M};
-  const bool count = st.top_k < p.vocab;
-  const float scale = grid_scale(st.inv_t);
-  const int top = grid_of(M, scale);
-  if (st.kind == kGrid) {
-    const int b0 = 2 * tid;   // the thread's two cells
-    double wt[2] = {0, 0}, tail = 0;
-    uint32_t n[2] = {0, 0};
-    for (int i = 0; i < ws.parts; ++i) {
-      const float m = parts[i].top;
-      if (m == -INFINITY) continue;
-      const double f = weight(m);
-      if (!count) tail += f * parts[i].tail;
-      const int mt = grid_of(m, scale);
-      const ull* pw = ws.weight + ((int64_t)r * ws.parts + i) * kCells;
-      const uint32_t* pn = ws.number + ((int64_t)r * ws.parts + i) * kCells;
-      auto take = [&](int k, int c) {
-        wt[k] += f * kUnit * (double)pw[c];
-        if (count) n[k] += pn[c];
-      };
-      if (b0 < kFine) {
-        const int l = b0 - (top - mt);
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-          if (l + k >= 0 && l + k < kFine) take(k, l + k);
-      } else {
-        for (int k = 0; k < 2; ++k) {
-          const int c = b0 + k - kFine, cell = (top >> 4) - c;   // values g with g >> 4 == cell, for the last c also the ones under it
-          const bool last = c == kCoarse - 1;
-          const int from = max((mt >> 4) - cell, 0), to = last ? kCoarse - 1 : min((mt >> 4) - cell, kCoarse - 1);
-          for (int q = from; q <= to; ++q) take(k, kFine + q);
-          // its fine cells that are not the row's
-          const int lo = max(max(mt - (cell * 16 + 15), mt - top + kFine), 0), hi = last ? kFine - 1 : min(mt - cell * 16, kFine - 1);
-          for (int q = lo; q <= hi; ++q) take(k, q);
-        }
-      }
-    }
-    double all, sum0 = scan<double>(wt[0] + wt[1], red, all) - (wt[0] + wt[1]);   // before the first
-    const double sums[3] = {sum0, sum0 + wt[0], sum0 + wt[0] + wt[1]};
-    uint32_t alln = 0, num0 = 0;
-    if (count) num0 = scan<uint32_t>(n[0] + n[1], (uint32_t*)red, alln) - n[0] - n[1];
-    const uint32_t nums[3] = {num0, num0 + n[0], num0 + n[0] + n[1]};
-    __syncthreads();
-    if (count)
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-        if (nums[k] < (uint32_t)st.top_k && nums[k + 1] >= (uint32_t)st.top_k) {
-          cut.cell_k = b0 + k;
-          cut.before_n = nums[k];
-          cut.before_k = sums[k];
-          cut.sum = sums[k + 1];   // with all of the cell
-        }
-    __syncthreads();
-    if (tid == 0 && cut.cell_k == kCells) cut.sum = all + tail;
-    __syncthreads();
-    if (st.top_p < 1.0) {
-      // what top_p is taken of is known but for cell_k
-      const double lo = cut.cell_k < kCells ? cut.before_k : cut.sum, hi = cut.sum;
-      const double aim0 = fmax(st.top_p, 0.0) * lo * (1 - 1e-9), aim1 = fmax(st.top_p, 0.0) * hi * (1 + 1e-9);
-      const int end = min(cut.cell_k, kCells - 1);
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-        if (b0 + k <= end && sums[k + 1] > sums[k]) {
-          if (sums[k + 1] >= aim0) atomicMin(&cut.cell_p0, b0 + k);
-          if (sums[k + 1] >= aim1) atomicMin(&cut.cell_p1, b0 + k);
-        }
-      __syncthreads();
-      if (tid == 0) {
-        cut.cell_p0 = min(cut.cell_p0, end);
-        cut.cell_p1 = min(cut.cell_p1, end);
-      }
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-        if (b0 + k == cut.cell_p0) cut.before_p = sums[k];
-      __syncthreads();
-    }
-    if (part == 0 && tid == 0) ws.cut[r] = cut;
-  }
-  const int cell_k = cut.cell_k, p0 = cut.cell_p0, p1 = cut.cell_p1, sure = min(cell_k, p0);
-  const int past = max(sure - 1, max(cell_k < kCells ? cell_k : 0, p1 < kCells ? p1 : 0));   // the last cell that counts
   const Row<E> x(p, row);
   const int s0 = ws.first_sub(part) + w, s1 = ws.first_sub(part + 1);
   double* sub = ws.sub + (int64_t)r * ws.subs;
-  uint32_t* list = ws.list + ((int64_t)r * ws.parts + part) * ws.places;
   float v[16];
-  // weights under min_p, as logits, with a margin for the division by T
-  const double span = (log(st.min_p) - 1e-9) / st.inv_t;
-  const double low = st.min_p > 0 ? (double)M + span - 1e-9 * fabs(span) : -INFINITY;
-  for (int s = s0; s < s1; s += kWaves) {
-    x.load(s, v);
-    double sum = 0;
-    if (st.kind == kFloor) {
+  if (st.kind == kFloor) {
+    // weights under min_p, as logits, with a margin for the division by T
+    const double span = (log(st.min_p) - 1e-9) / st.inv_t, low = (double)M + span - 1e-9 * fabs(span);
+    for (int s = s0; s < s1; s += kWaves) {
+      x.load(s, v);
+      double sum = 0;
 #pragma unroll 4
       for (int j = 0; j < 16; ++j)
         if (v[j] == M || (double)v[j] >= low) {
           const double wt = weight(v[j]);
           sum += wt >= st.min_p ? wt : 0.0;
         }
-    } else {
+#pragma unroll
+      for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+      if (lane == 0) sub[s] = sum;
+    }
+    return;
+  }
+  const Bounds b = ws.bounds[r];
+  const bool cut_k = b.cut_k, cut_p = b.cut_p;
+  const float sure = b.sure();
+  uint32_t* list = ws.list + ((int64_t)r * ws.parts + part) * ws.places;
+  double over_k = 0, over_p = 0;
+  uint32_t over_n = 0;
+  for (int s = s0; s < s1; s += kWaves) {
+    x.load(s, v);
+    double kept = 0;
+    uint32_t take = 0;
 #pragma unroll 4
-      for (int j = 0; j < 16; ++j) {
-        const int cell = v[j] > -INFINITY ? cell_of(grid_of(v[j], scale), top) : kCells;
-        if (!__any(cell <= past)) continue;
-        if (cell < sure) {
-          const double wt = weight(v[j]);
-          sum += wt >= st.min_p ? wt : 0.0;
-        }
-        const bool take = cell < kCells && ((cell >= p0 && cell <= p1) || cell == cell_k);
-        const uint64_t all = __ballot(take);
-        if (all) {
-          uint32_t at = 0;
-          if (lane == 0) at = atomicAdd(&places, (uint32_t)__popcll(all));
-          at = __builtin_amdgcn_readfirstlane(at) + __popcll(all & ((1ull << lane) - 1));
-          if (take && at < (uint32_t)ws.places) list[at] = s * kSub + x.at(j);
-        }
-      }
+    for (int j = 0; j < 16; ++j) {
+      const bool in_k = cut_k && v[j] >= b.k_lo && v[j] < b.k_hi, in_p = cut_p && v[j] >= b.p_lo && v[j] < b.p_hi;
+      take |= (uint32_t)((in_k || in_p) && v[j] > -INFINITY) << j;
+      if (cut_k && !__any(v[j] >= b.k_hi)) continue;
+      const double wt = weight(v[j]);
+      const bool of_k = !cut_k || v[j] >= b.k_hi;
+      over_k += of_k ? wt : 0.0;
+      over_n += of_k && cut_k;
+      const double top_part = v[j] >= sure ? wt : 0.0;
+      over_p += top_part;
+      kept += top_part >= st.min_p ? top_part : 0.0;
     }
 #pragma unroll
-    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
-    if (lane == 0) sub[s] = sum;
+    for (int o = 32; o; o >>= 1) kept += __shfl_xor(kept, o);
+    if (lane == 0) sub[s] = kept;
+    while (take) {
+      const int j = __builtin_ctz(take);
+      take &= take - 1;
+      const uint32_t at = atomicAdd(&places, 1u);
+      if (at < (uint32_t)ws.places) list[at] = s * kSub + x.at(j);
+    }
   }
-  __syncthreads();
-  if (tid == 0) parts[part].listed = places;
+  over_k = add_up<kWaves, double>(over_k, red);
+  over_p = add_up<kWaves, double>(over_p, red);
+  const ull n = add_up<kWaves, ull>(over_n, (ull*)red);
+  if (tid == 0) {
+    Part& out = parts[part];
+    out.listed = places;
+    out.over_n = (uint32_t)n;
+    out.over_k = over_k;
+    out.over_p = over_p;
+  }
 }
 
 struct LongWay {
@@ -519,7 +610,7 @@ __device__ __forceinline__ void tell(const SampleArgs& p, int row, int token, do
   if (p.logprob) p.logprob[row] = (float)log_share;
 }
 template <typename E>
-__device__ __noinline__ void long_way(const SampleArgs& p, int row, const Settings& st, const Weights& weigh, LongWay& sh) {
+__device__ __forceinline__ void long_way(const SampleArgs& p, int row, const Settings& st, const Weights& weigh, LongWay& sh) {
   uint32_t* const cnt = sh.cnt;
   ull *const wt = sh.wt, *const red = sh.red;
   auto& found = sh.found;
@@ -557,8 +648,8 @@ __device__ __noinline__ void long_way(const SampleArgs& p, int row, const Settin
       const int d0 = 2047 - 2 * tid, d1 = d0 - 1;
       const ull c0 = cnt[d0], c1 = cnt[d1], w0 = wt[d0], w1 = wt[d1];
       ull all;
-      const ull cs = scan<ull>(c0 + c1, red, all) - c0 - c1 + c.before_n, end_n = all + c.before_n;
-      const ull ws = scan<ull>(w0 + w1, red, all) - w0 - w1 + c.before_w, end_w = all + c.before_w;
+      const ull cs = scan<kWaves, ull>(c0 + c1, red, all) - c0 - c1 + c.before_n, end_n = all + c.before_n;
+      const ull ws = scan<kWaves, ull>(w0 + w1, red, all) - w0 - w1 + c.before_w, end_w = all + c.before_w;
       const ull aim = by_count ? min(n, end_n) : min(n, end_w);   // some group reaches it
       auto mine = [&](ull bn, ull bw, ull dn, ull dw) {
         const ull b = by_count ? bn : bw, d = by_count ? dn : dw;
@@ -598,7 +689,7 @@ __device__ __noinline__ void long_way(const SampleArgs& p, int row, const Settin
       ull sum = 0;
       for (int i = tid; i < V; i += kThreads)
         if (const uint32_t k = key(i); k > kNone) sum += whole(k);
-      scan<ull>(sum, red, kept_w);
+      scan<kWaves, ull>(sum, red, kept_w);
     }
     const ull aim = max((ull)1, (ull)ceil(fmax(st.top_p, 0.0) * (double)kept_w));
     const Cut c = find(false, aim);
@@ -615,7 +706,7 @@ __device__ __noinline__ void long_way(const SampleArgs& p, int row, const Settin
       const int i = i0 + tid;
       const bool tie = i < V && key(i) == at;
       ull all;
-      const ull r = scan<ull>(tie, red, all) + seen;
+      const ull r = scan<kWaves, ull>(tie, red, all) + seen;
       if (tie && r == ties) found.bin = i;
       seen += all;
       if (seen >= ties) break;
@@ -631,16 +722,16 @@ __device__ __noinline__ void long_way(const SampleArgs& p, int row, const Settin
   };
   double sum = 0;
   for (int i = tid; i < V; i += kThreads) sum += weight(i);
-  const double total = add_up<double>(sum, (double*)red), aim = (double)st.u * total;
+  const double total = add_up<kWaves, double>(sum, (double*)red), aim = (double)st.u * total;
   double before = 0;
   for (int i0 = 0; i0 < V; i0 += kThreads) {
     const int i = i0 + tid;
     const double w = i < V ? weight(i) : 0;
     double all;
-    const double r = scan<double>(w, (double*)red, all) + before;
+    const double r = scan<kWaves, double>(w, (double*)red, all) + before;
     // what rounding leaves under the aim at the row's end goes to the last token
-    const ull pick = w > 0 && r > aim ? (ull)i : ~0ull, best = reduce<ull>(pick, red, [](ull a, ull b) { return a < b ? a : b; });
-    const ull back = reduce<ull>(w > 0 ? (ull)i + 1 : 0, red, [](ull a, ull b) { return a > b ? a : b; });
+    const ull pick = w > 0 && r > aim ? (ull)i : ~0ull, best = least_of<kWaves>(pick, red);
+    const ull back = most_of<kWaves>(w > 0 ? (ull)i + 1 : 0, red);
     if (back) sh.found.bin = (uint32_t)back - 1;
     if (best != ~0ull) {
       sh.found.bin = (uint32_t)best;
@@ -652,139 +743,158 @@ __device__ __noinline__ void long_way(const SampleArgs& p, int row, const Settin
   if (tid == 0) tell(p, row, (int)sh.found.bin, log(weigh((float)x[sh.found.bin]) / total));
 }
 
-// ---- the last launch: a workgroup for each row ----
-struct Held {   // list entries in registers; key 0: none
-  uint32_t key[kHeld], idx[kHeld];
+// ---- the last launch: a workgroup for each row, of which four waves do the work
+// (their barriers are short) unless the row goes the long way ----
+constexpr int kNear = 4, kNearThreads = 64 * kNear;
+constexpr int kFewRoom = 1024;   // places for the tokens of kFew that are as large as the top_k-th largest of the lanes'
+
+struct List {
+  uint32_t key[kListRow], idx[kListRow];   // order_of without its low bits
+  ull units[kListRow];                     // weights in kListUnit
 };
-// The n-th largest key of those that are true to `of`, as bits from kLow on, among
-// `bits` of them under a common head; one barrier a bit
-template <int LOW, typename F>
-__device__ __forceinline__ uint32_t nth_key(const Held& h, uint32_t n, uint32_t head, int bits, uint32_t* lds, int& turn, F&& of) {
+
+// Of the entries that are true to `of`, the n-th largest key, among `bits` of them
+// under a common head; one barrier a bit
+template <typename F>
+__device__ __forceinline__ uint32_t nth_key(int held, uint32_t n, uint32_t head, int bits, const uint32_t* key, uint32_t* lds, int& turn, F&& of) {
   uint32_t least = head;
 #pragma unroll 1
   for (int bit = bits - 1; bit >= 0; --bit) {
     const uint32_t t = least | 1u << bit;
     uint32_t c = 0;
-#pragma unroll
-    for (int j = 0; j < kHeld; ++j) c += __popcll(__ballot(of(j) && h.key[j] >> LOW >= t));
-    if (count_up(c, lds, turn) >= n) least = t;
+    for (int i = threadIdx.x; i < (held + 63 & ~63); i += kNearThreads) c += __popcll(__ballot(i < held && key[i] >= t && of(i)));
+    if (count_up<kNear>(c, lds, turn) >= n) least = t;
   }
   return least;
 }
-// The n-th smallest index of those that are true to `of`
+template <typename F> __device__ __forceinline__ uint32_t number_of(int held, uint32_t* lds, int& turn, F&& of) {
+  uint32_t c = 0;
+  for (int i = threadIdx.x; i < (held + 63 & ~63); i += kNearThreads) c += __popcll(__ballot(i < held && of(i)));
+  return count_up<kNear>(c, lds, turn);
+}
+// The n-th smallest index of them
 template <typename F>
-__device__ __forceinline__ uint32_t nth_index(const Held& h, uint32_t n, int vocab, uint32_t* lds, int& turn, F&& of) {
+__device__ __forceinline__ uint32_t nth_index(int held, uint32_t n, int vocab, const uint32_t* idx, uint32_t* lds, int& turn, F&& of) {
   uint32_t most = 0;   // fewer than n lie under it
 #pragma unroll 1
   for (int bit = 31 - __clz(vocab); bit >= 0; --bit) {
     const uint32_t t = most | 1u << bit;
-    uint32_t c = 0;
-#pragma unroll
-    for (int j = 0; j < kHeld; ++j) c += __popcll(__ballot(of(j) && h.idx[j] < t));
-    if (count_up(c, lds, turn) < n) most = t;
+    if (number_of(held, lds, turn, [&](int i) { return of(i) && idx[i] < t; }) < n) most = t;
   }
   return most;
 }
-template <typename F> __device__ __forceinline__ uint32_t number_of(uint32_t* lds, int& turn, F&& of) {
-  uint32_t c = 0;
-#pragma unroll
-  for (int j = 0; j < kHeld; ++j) c += __popcll(__ballot(of(j)));
-  return count_up(c, lds, turn);
-}
 
-template <typename E> __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs p, Work ws) {
-  __shared__ double table[64], red[kWaves];
-  __shared__ uint32_t count[2 * kWaves], place;
-  __shared__ union {
+struct PickShared {
+  double table[64], red[kWaves];
+  uint2 count2[2 * kWaves];
+  uint32_t count[2 * kWaves], place, spots, at[kPartsMost + 1];
+  union {
     LongWay far;
+    List list;
     struct {
-      ull key[kFewMost];   // order_of and the index turned round: a larger one comes first
+      uint32_t lane[kFewRoom];
+      ull key[kFewRoom];   // order_of and the index turned round: a larger one comes first
       ull sorted[kFewMost];
       double w[kFewMost];
     } few;
-    ull sub[4096 + 1];
-  } sh;
-  const int tid = threadIdx.x, row = ws.row0 + blockIdx.x, r = blockIdx.x, V = p.vocab;
-  const Settings st = settings_of(p, row, ws.few);
-  const Part* parts = ws.part + (int64_t)r * ws.parts;
-  const float M = top_of(parts, ws.parts);
-  if (M == -INFINITY) {
-    if (tid == 0) tell(p, row, -1, -INFINITY);
-    return;
-  }
-  if (st.kind == kGreedy) {
-    if (tid == 0) {
-      int i = 0;
-      while (parts[i].top != M) ++i;
-      tell(p, row, (int)parts[i].first, 0);
+  };
+};
+
+// The largest t that n of the threads' keys reach, two bits a barrier
+__device__ __forceinline__ uint32_t reached_by(uint32_t key, uint32_t n, double* red, uint2* count) {
+  const ull both = reduce<kWaves, ull>((ull)key << 32 | ~key, (ull*)red, [](ull a, ull b) { return a & b; });
+  const uint32_t same = (uint32_t)(both >> 32) | (uint32_t)both;   // bits that all keys share
+  int bit = same == ~0u ? 0 : 32 - __clz(~same), turn = 0;
+  bit += bit & 1;
+  uint32_t t = bit >= 32 ? 0 : (uint32_t)(both >> 32) >> bit << bit;
+  for (bit -= 2; bit >= 0; bit -= 2) {
+    const uint32_t c1 = __popcll(__ballot(key >= (t | 1u << bit))), c2 = __popcll(__ballot(key >= (t | 2u << bit))),
+                   c3 = __popcll(__ballot(key >= (t | 3u << bit)));
+    turn ^= kWaves;
+    if ((threadIdx.x & 63) == 0) count[turn + (threadIdx.x >> 6)] = {c1 | c2 << 16, c3};
+    __syncthreads();
+    uint32_t s12 = 0, s3 = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+      const uint2 c = count[turn + i];
+      s12 += c.x;
+      s3 += c.y;
     }
-    return;
+    t |= (s3 >= n ? 3u : (s12 >> 16 >= n ? 2u : ((s12 & 0xffff) >= n ? 1u : 0u))) << bit;
   }
-  fill_table(table);
-  if (tid == 0) place = 0;
-  __syncthreads();
-  const Weights weight{table, steps_of(st.inv_t), M};
+  return t;
+}
+
+// True, on all threads, where the row has to go the long way.
+template <typename E>
+__device__ __forceinline__ bool pick(const SampleArgs& p, const Work& ws, const Settings& st, const Weights& weight, PickShared& sh,
+                                     ull* sub_units) {
+  double* const red = sh.red;
+  uint32_t* const count = sh.count;
+  const int tid = threadIdx.x, row = ws.row0 + blockIdx.x, r = blockIdx.x, V = p.vocab;
+  const Part* parts = ws.part + (int64_t)r * ws.parts;
   const Row<E> x(p, row);
   constexpr int LOW = kLow<E>;
-  int turn = 0;
   const double aim_share = (double)st.u;
+  int turn = 0;
 
-  // ---- the listed tokens ----
-  Held h;
-  uint32_t held = 0;
-  bool whole_list = true;
-  if (st.kind == kFew || st.kind == kGrid) {
-    for (int i = 0; i < ws.parts; ++i) {
-      whole_list &= parts[i].listed <= (uint32_t)ws.places;
-      held += parts[i].listed;
-    }
-    if (!whole_list) {
-      long_way<E>(p, row, st, weight, sh.far);
-      return;
-    }
-#pragma unroll
-    for (int j = 0; j < kHeld; ++j) {
-      uint32_t e = tid + j * kThreads;
-      h.key[j] = h.idx[j] = 0;
-      if (e < held) {
-        int i = 0;
-        while (e >= parts[i].listed) e -= parts[i++].listed;
-        h.idx[j] = ws.list[((int64_t)r * ws.parts + i) * ws.places + e];
-        h.key[j] = order_of((float)x.x[h.idx[j]]);
-      }
-    }
-  }
   if (st.kind == kFew) {
-    // the first top_k of the list, by its keys and where they are equal by index
-    const uint32_t k = min((uint32_t)st.top_k, held);
-    auto any = [&](int j) { return h.key[j] != 0; };
-    const uint32_t at = nth_key<LOW>(h, k, 0, 32 - LOW, count, turn, any);
-    const uint32_t over = number_of(count, turn, [&](int j) { return h.key[j] >> LOW > at; });
-    auto tie = [&](int j) { return h.key[j] >> LOW == at && h.key[j] != 0; };
-    const uint32_t ties = number_of(count, turn, tie);
-    const uint32_t last = ties > k - over ? nth_index(h, k - over, V, count, turn, tie) : ~0u;
+    // At least top_k threads hold a token as large as the top_k-th largest of what
+    // each holds at most, so the row's first top_k are among the tokens that are as
+    // large: those of a little over top_k lanes, 16 each, and a few more than top_k of these.
+    const int lanes = ws.subs * 64;
+    const float* most = ws.most + (int64_t)r * lanes;
+    constexpr int kStep = 16;   // loads on their way; kept, for rows of up to 2^18
+    float m[kStep], mine_most = -INFINITY;
+    for (int i0 = (lanes - 1) / (kStep * kThreads) * (kStep * kThreads); i0 >= 0; i0 -= kStep * kThreads) {
 #pragma unroll
-    for (int j = 0; j < kHeld; ++j)
-      if (h.key[j] >> LOW > at || (tie(j) && h.idx[j] <= last))
-        sh.few.key[atomicAdd(&place, 1u)] = (ull)h.key[j] << 32 | (uint32_t)~h.idx[j];
+      for (int k = 0; k < kStep; ++k) {
+        const int i = i0 + k * kThreads + tid;
+        m[k] = i < lanes ? most[i] : -INFINITY;
+      }
+#pragma unroll
+      for (int k = 0; k < kStep; ++k) mine_most = fmaxf(mine_most, m[k]);
+    }
+    const uint32_t mine_key = order_of(mine_most) >> LOW;
+    const uint32_t least = reached_by(mine_key, st.top_k, red, sh.count2);
+    if (mine_key >= least) {
+      auto take = [&](int i, float v) {
+        if (const uint32_t k = order_of(v); k >> LOW >= least && k > kNone)
+          if (const uint32_t at = atomicAdd(&sh.spots, 1u); at < kFewRoom) sh.few.lane[at] = i;
+      };
+#pragma unroll
+      for (int k = 0; k < kStep; ++k) take(k * kThreads + tid, m[k]);
+      for (int i = kStep * kThreads + tid; i < lanes; i += kThreads) take(i, most[i]);
+    }
     __syncthreads();
-    ull mine = 0;
-    if (tid < (int)k) {
-      mine = sh.few.key[tid];
+    const uint32_t n = sh.spots;
+    for (uint32_t i = tid; i < min(n, (uint32_t)kFewRoom) * 16; i += kThreads) {
+      const int lane = sh.few.lane[i / 16], at = lane / 64 * kSub + x.at(i % 16, lane % 64);
+      const uint32_t k = order_of(at < V ? (float)x.x[at] : -INFINITY);
+      if (k >> LOW >= least && k > kNone)
+        if (const uint32_t to = atomicAdd(&sh.place, 1u); to < kFewRoom) sh.few.key[to] = (ull)k << 32 | (uint32_t)~at;
+    }
+    __syncthreads();
+    const uint32_t held = sh.place;
+    if (n > kFewRoom || held > kFewRoom) return true;
+    // the first top_k of them in their order
+    const uint32_t k = min((uint32_t)st.top_k, held);
+    if (tid < (int)held) {
+      const ull mine = sh.few.key[tid];
       uint32_t rank = 0;
-      for (uint32_t i = 0; i < k; ++i) rank += sh.few.key[i] > mine;
-      sh.few.sorted[rank] = mine;
+      for (uint32_t i = 0; i < held; ++i) rank += sh.few.key[i] > mine;
+      if (rank < k) sh.few.sorted[rank] = mine;
     }
     __syncthreads();
     double w = 0;
     uint32_t idx = 0;
     if (tid < (int)k) {
-      mine = sh.few.sorted[tid];
+      const ull mine = sh.few.sorted[tid];
       idx = ~(uint32_t)mine;
       w = weight(value_of((uint32_t)(mine >> 32)));
     }
     double sum;
-    const double before = scan<double>(w, red, sum) - w;
+    const double before = scan<kWaves, double>(w, red, sum) - w;
     if (st.top_p < 1.0 && tid > 0 && !(before < st.top_p * sum)) w = 0;
     if (w < st.min_p) w = 0;
     if (tid < (int)k) sh.few.w[tid] = w;
@@ -797,112 +907,159 @@ template <typename E> __global__ __launch_bounds__(kThreads) void sample_pick_ke
         upto += ~(uint32_t)sh.few.sorted[i] <= idx ? t : 0.0;
       }
     }
-    const bool hit = w > 0 && upto > aim_share * total;
-    const ull first = reduce<ull>(hit ? (ull)idx << 32 | tid : ~0ull, (ull*)red, [](ull a, ull b) { return a < b ? a : b; });
-    if (first != ~0ull ? tid == (int)(uint32_t)first : tid == 0) tell(p, row, (int)idx, log(w / total));
-    return;
+    // (the last one's sum is the total, which the aim is less than)
+    const ull first = least_of<kWaves>(w > 0 && upto > aim_share * total ? (ull)idx << 32 | tid : ~0ull, (ull*)red);
+    if (tid == (int)(uint32_t)first) tell(p, row, (int)idx, log(w / total));
+    return false;
   }
 
   // ---- the cuts: tokens stay whose key is over `key`, or just it with an index up to `idx` ----
   struct Cut {
     uint32_t key, idx;
-    __device__ __forceinline__ bool keeps(uint32_t k, uint32_t i) const { return k > key || (k == key && i <= idx); }
-  } cut_k{0, ~0u}, cut_p{0, ~0u};
-  RowCut rc{};
-  const float scale = grid_scale(st.inv_t);
-  const int top = grid_of(M, scale);
-  int sure = kCells;
-  auto cell = [&](uint32_t key) { return cell_of(grid_of(value_of(key), scale), top); };
+    __device__ __forceinline__ bool keeps(uint32_t k, uint32_t i) const { return (k > key) | ((k == key) & (i <= idx)); }
+  } by_k{0, ~0u}, by_p{0, ~0u};
+  Bounds b{-INFINITY, -INFINITY, -INFINITY, -INFINITY, 0, 0};
+  uint32_t held = 0;
+  double over_k = 0, over_p = 0;
+  uint32_t over_n = 0;
   if (st.kind == kGrid) {
-    rc = ws.cut[r];
-    sure = min(rc.cell_k, rc.cell_p0);
-    ull units[kHeld];
-    bool of_k[kHeld];
+    b = ws.bounds[r];
+    const int l = tid & 63;
+    const bool mine = l < ws.parts;
+    const uint32_t listed = mine ? parts[l].listed : 0;
+    double ok = mine ? parts[l].over_k : 0, op = mine ? parts[l].over_p : 0;
+    uint32_t on = mine ? parts[l].over_n : 0, upto = listed;
 #pragma unroll
-    for (int j = 0; j < kHeld; ++j) {
-      units[j] = h.key[j] ? whole_of_list(weight(value_of(h.key[j]))) : 0;
-      of_k[j] = h.key[j] && cell(h.key[j]) == rc.cell_k;
+    for (int o = 1; o < kPartsMost; o <<= 1) {
+      ok += __shfl_xor(ok, o);
+      op += __shfl_xor(op, o);
+      on += __shfl_xor(on, o);
+      const uint32_t t = __shfl_up(upto, o);
+      if (l >= o) upto += t;
     }
+    over_k = __shfl(ok, 0);
+    over_p = __shfl(op, 0);
+    over_n = __shfl(on, 0);
+    held = __shfl(upto, kPartsMost - 1);
+    if (__any(listed > (uint32_t)ws.places)) return true;
+    if (tid < kPartsMost) sh.at[tid + 1] = upto;
+    if (tid == 0) sh.at[0] = 0;
+    __syncthreads();
+    for (uint32_t e = tid; e < held; e += kThreads) {
+      int i = 0;
+#pragma unroll
+      for (int k = 1; k < kPartsMost; ++k) i += e >= sh.at[k];
+      const uint32_t idx = ws.list[((int64_t)r * ws.parts + i) * ws.places + e - sh.at[i]];
+      const float v = (float)x.x[idx];
+      sh.list.key[e] = order_of(v) >> LOW;
+      sh.list.idx[e] = idx;
+      sh.list.units[e] = whole_of_list(weight(v));
+    }
+  }
+  const bool cut_k = b.cut_k, cut_p = b.cut_p;
+  auto value = [&](uint32_t key) { return value_of(key << LOW | (key >> (31 - LOW) & 1 ? 0 : (1u << LOW) - 1)); };
+  auto of_k = [&](int i) {
+    const float v = value(sh.list.key[i]);
+    return cut_k && v >= b.k_lo && v < b.k_hi;
+  };
+  auto of_p = [&](int i) {
+    const float v = value(sh.list.key[i]);
+    return cut_p && v >= b.p_lo && v < b.p_hi;
+  };
+  __syncthreads();
+  // Whether the cut of top_k is among the listed, and how much weight stays by it:
+  // what must hold for the four waves to go on is the same for all threads.
+  const uint32_t* const key = sh.list.key;
+  const uint32_t* const index = sh.list.idx;
+  if (cut_k) {   // too few tokens in the row: no cut; the grid's counts said that there is one
+    const ull n = add_up<kWaves, ull>([&] {
+      ull c = 0;
+      for (int i = tid; i < (int)held; i += kThreads) c += of_k(i);
+      return c;
+    }(), (ull*)red);
+    if (!(over_n < (uint32_t)st.top_k && over_n + n >= (uint32_t)st.top_k)) return true;
+  }
+  if (cut_p) {
+    // with all or nothing of the window of top_k: the aim lies between these two
+    ull in_k = 0, in_p = 0;
+    for (int i = tid; i < (int)held; i += kThreads) {
+      if (of_k(i)) in_k += sh.list.units[i];
+      if (of_p(i)) in_p += sh.list.units[i];
+    }
+    in_k = add_up<kWaves, ull>(in_k, (ull*)red);
+    in_p = add_up<kWaves, ull>(in_p, (ull*)red);
+    const double lo = st.top_p * over_k, hi = st.top_p * (over_k + kListUnit * (double)in_k);
+    // a window that ends with the tokens that top_k may leave needs no lower end of its own
+    if (!((over_p < lo || over_p == 0) && (over_p + kListUnit * (double)in_p >= hi || (cut_k && b.p_lo <= b.k_lo)))) return true;
+  }
+  if (tid >= kNearThreads) return false;
+
+  if (cut_k || cut_p) {
     // the keys' common head
     uint32_t ones = ~0u, zeros = ~0u;
-#pragma unroll
-    for (int j = 0; j < kHeld; ++j)
-      if (h.key[j]) ones &= h.key[j] >> LOW, zeros &= ~(h.key[j] >> LOW);
-    const ull both = reduce<ull>((ull)ones << 32 | zeros, (ull*)red, [](ull a, ull b) { return a & b; });
+    for (int i = tid; i < (int)held; i += kNearThreads) ones &= key[i], zeros &= ~key[i];
+    const ull both = reduce<kNear, ull>((ull)ones << 32 | zeros, (ull*)red, [](ull a, ull b) { return a & b; });
     const uint32_t same = (uint32_t)(both >> 32) | (uint32_t)both;
     const int bits = same == ~0u ? 0 : 32 - __clz(~same);
     const uint32_t head = bits == 32 ? 0 : (uint32_t)(both >> 32) >> bits << bits;
-    double sum = rc.sum;
-    if (rc.cell_k < kCells) {
-      const uint32_t n = st.top_k - rc.before_n;
-      auto of = [&](int j) { return of_k[j]; };
-      cut_k.key = nth_key<LOW>(h, n, head, bits, count, turn, of);
-      const uint32_t over = number_of(count, turn, [&](int j) { return of_k[j] && h.key[j] >> LOW > cut_k.key; });
-      auto tie = [&](int j) { return of_k[j] && h.key[j] >> LOW == cut_k.key; };
-      if (number_of(count, turn, tie) > n - over) cut_k.idx = nth_index(h, n - over, V, count, turn, tie);
+    double sum = over_k;
+    if (cut_k) {
+      const uint32_t n = st.top_k - over_n;
+      by_k.key = nth_key(held, n, head, bits, key, count, turn, of_k);
+      const uint32_t over = number_of(held, count, turn, [&](int i) { return key[i] > by_k.key && of_k(i); });
+      auto tie = [&](int i) { return key[i] == by_k.key; };
+      if (number_of(held, count, turn, tie) > n - over) by_k.idx = nth_index(held, n - over, V, index, count, turn, tie);
       ull mine = 0;
-#pragma unroll
-      for (int j = 0; j < kHeld; ++j) mine += of_k[j] && cut_k.keeps(h.key[j] >> LOW, h.idx[j]) ? units[j] : 0;
-      sum = rc.before_k + kListUnit * (double)add_up<ull>(mine, (ull*)red);
+      for (int i = tid; i < (int)held; i += kNearThreads)
+        if (of_k(i) && by_k.keeps(key[i], index[i])) mine += sh.list.units[i];
+      sum += kListUnit * (double)add_up<kNear, ull>(mine, (ull*)red);
     }
-    if (rc.cell_p0 < kCells) {
+    if (cut_p) {
       const double aim = fmax(st.top_p * sum, 0x1p-1000);   // the first token stays
-      bool of_p[kHeld];
-#pragma unroll
-      for (int j = 0; j < kHeld; ++j) {
-        const int c = h.key[j] ? cell(h.key[j]) : -1;
-        of_p[j] = c >= rc.cell_p0 && c <= rc.cell_p1;
-      }
       auto over = [&](uint32_t t) {   // the weight before key t's tokens
         ull mine = 0;
-#pragma unroll
-        for (int j = 0; j < kHeld; ++j) mine += of_p[j] && h.key[j] >> LOW > t ? units[j] : 0;
-        return rc.before_p + kListUnit * (double)add_up<ull>(mine, (ull*)red);
+        for (int i = tid; i < (int)held; i += kNearThreads)
+          if (key[i] > t && of_p(i)) mine += sh.list.units[i];
+        return over_p + kListUnit * (double)add_up<kNear, ull>(mine, (ull*)red);
       };
       // the smallest key before which the aim is not reached: tokens of it stay
       uint32_t t = head | (bits == 32 ? ~0u : (1u << bits) - 1);
 #pragma unroll 1
       for (int bit = bits - 1; bit >= 0; --bit)
         if (over(t & ~(1u << bit)) < aim) t &= ~(1u << bit);
-      cut_p.key = t;
-      auto tie = [&](int j) { return of_p[j] && h.key[j] >> LOW == t; };
-      const uint32_t ties = number_of(count, turn, tie);
+      by_p.key = t;
+      auto tie = [&](int i) { return key[i] == t; };
+      const uint32_t ties = number_of(held, count, turn, tie);
       if (ties > 0) {
-        const double w = weight(value_of(t << LOW | (((t >> (31 - LOW)) & 1) ? 0 : (1u << LOW) - 1)));
-        const double n = fmax(ceil((aim - over(t)) / w), 1.0);
-        if (n < (double)ties) cut_p.idx = nth_index(h, (uint32_t)n, V, count, turn, tie);
+        const double n = fmax(ceil((aim - over(t)) / weight(value(t))), 1.0);
+        if (n < (double)ties) by_p.idx = nth_index(held, (uint32_t)n, V, index, count, turn, tie);
       }
     }
   }
-  auto stays = [&](float v, uint32_t i) {   // a token in no cell over the cuts
-    const uint32_t k = order_of(v) >> LOW;
-    return (rc.cell_k == kCells || st.kind != kGrid || cut_k.keeps(k, i)) && (rc.cell_p0 == kCells || st.kind != kGrid || cut_p.keeps(k, i));
-  };
+  // {0, ~0u}, what a cut that there is not keeps, is everything
+  auto stays = [&](uint32_t k, uint32_t i) { return by_k.keeps(k, i) & by_p.keeps(k, i); };
 
   // ---- the sub ----
   const double* sub = ws.sub + (int64_t)r * ws.subs;
+  for (int s = tid; s < ws.subs; s += kNearThreads) sub_units[s] = 0;
   __syncthreads();
-  for (int s = tid; s < ws.subs; s += kThreads) sh.sub[s] = 0;
+  const float sure = b.sure();
+  for (int i = tid; i < (int)held; i += kNearThreads)
+    if (stays(key[i], index[i])) {
+      const double w = weight(value(key[i]));
+      if (w >= st.min_p) atomicAdd(&sub_units[index[i] / kSub], sh.list.units[i]);
+    }
   __syncthreads();
-  if (st.kind == kGrid)
-#pragma unroll
-    for (int j = 0; j < kHeld; ++j)
-      if (h.key[j] && stays(value_of(h.key[j]), h.idx[j])) {
-        const double w = weight(value_of(h.key[j]));
-        if (w >= st.min_p) atomicAdd(&sh.sub[h.idx[j] / kSub], whole_of_list(w));
-      }
-  __syncthreads();
-  const int per = (ws.subs + kThreads - 1) / kThreads, f0 = tid * per;
+  const int per = (ws.subs + kNearThreads - 1) / kNearThreads, f0 = tid * per;
   auto sum_of = [&](int s) {
-    if (st.kind != kAll) return sub[s] + kListUnit * (double)sh.sub[s];
-    int i = 0;
-    while (s >= ws.first_sub(i + 1)) ++i;
-    return parts[i].top == -INFINITY ? 0.0 : sub[s] * weight(parts[i].top);
+    if (st.kind != kAll) return sub[s] + kListUnit * (double)sub_units[s];
+    const float m = parts[s / ws.part_subs].top;
+    return m == -INFINITY ? 0.0 : sub[s] * weight(m);
   };
   double mine = 0;
   for (int s = f0; s < min(f0 + per, ws.subs); ++s) mine += sum_of(s);
   double total;
-  double before = scan<double>(mine, red, total) - mine;
+  double before = scan<kNear, double>(mine, red, total) - mine;
   const double aim = aim_share * total;
   ull found = ~0ull, back = 0;
   double found_before = 0, back_before = 0;
@@ -918,8 +1075,7 @@ template <typename E> __global__ __launch_bounds__(kThreads) void sample_pick_ke
     }
     before += w;
   }
-  const ull first = reduce<ull>(found, (ull*)red, [](ull a, ull b) { return a < b ? a : b; });
-  const ull end = reduce<ull>(back, (ull*)red, [](ull a, ull b) { return a > b ? a : b; });
+  const ull first = least_of<kNear>(found, (ull*)red), end = most_of<kNear>(back, (ull*)red);
   const int s = first != ~0ull ? (int)first : (int)end - 1;   // rounding may leave the sum under its aim
   __syncthreads();
   if (first != ~0ull ? found == first : back == end) red[0] = first != ~0ull ? found_before : back_before;
@@ -927,41 +1083,92 @@ template <typename E> __global__ __launch_bounds__(kThreads) void sample_pick_ke
   const double left = aim - red[0];
   __syncthreads();
 
-  // ---- the token ----
-  const int i = s * kSub + tid;
-  const float v = i < V ? (float)x.x[i] : -INFINITY;
-  double w = weight(v);
-  if (w < st.min_p) w = 0;
-  if (st.kind == kGrid && w > 0 && cell_of(grid_of(v, scale), top) >= sure && !stays(v, i)) w = 0;
-  double all;
-  const double upto = scan<double>(w, red, all);
-  const ull hit = reduce<ull>(w > 0 && upto > left ? (ull)tid : ~0ull, (ull*)red, [](ull a, ull b) { return a < b ? a : b; });
-  const ull stop = reduce<ull>(w > 0 ? (ull)tid + 1 : 0, (ull*)red, [](ull a, ull b) { return a > b ? a : b; });
-  if (tid == (hit != ~0ull ? (int)hit : (int)stop - 1)) tell(p, row, i, log(w / total));
+  // ---- the token: four in a row to a thread ----
+  constexpr int kIn = kSub / kNearThreads;
+  double w[kIn], sums = 0;
+  const int i0 = s * kSub + tid * kIn;
+#pragma unroll
+  for (int j = 0; j < kIn; ++j) {
+    const int i = i0 + j;
+    const float v = i < V ? (float)x.x[i] : -INFINITY;
+    const double t = weight(v);
+    // without branches: with them this compiler loses the zeros of all but the first
+    w[j] = (t >= st.min_p) & ((v >= sure) | stays(order_of(v) >> LOW, i)) ? t : 0.0;
+    sums += w[j];
+  }
+  double all, upto = scan<kNear, double>(sums, red, all) - sums;
+  ull hit = ~0ull, stop = 0;
+#pragma unroll
+  for (int j = 0; j < kIn; ++j) {
+    upto += w[j];
+    if (w[j] > 0) {
+      stop = tid * kIn + j + 1;
+      if (hit == ~0ull && upto > left) hit = tid * kIn + j;
+    }
+  }
+  const ull one = least_of<kNear>(hit, (ull*)red), last = most_of<kNear>(stop, (ull*)red);
+  const int at = one != ~0ull ? (int)one : (int)last - 1;
+  if (at >= 0 && at / kIn == tid) tell(p, row, s * kSub + at, log(weight((float)x.x[s * kSub + at]) / total));
+  return false;
+}
+
+template <typename E> __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs p, Work ws) {
+  __shared__ PickShared sh;
+  extern __shared__ ull sub_units[];   // [subs]
+  const int tid = threadIdx.x, row = ws.row0 + blockIdx.x;
+  const Settings st = settings_of(p, row, ws.few);
+  const Part* parts = ws.part + (int64_t)blockIdx.x * ws.parts;
+  const float M = top_of(parts, ws.parts);
+  if (M == -INFINITY) {
+    if (tid == 0) tell(p, row, -1, -INFINITY);
+    return;
+  }
+  if (st.kind == kGreedy) {
+    const uint64_t of = __ballot((tid & 63) < ws.parts && parts[(tid & 63) < ws.parts ? tid & 63 : 0].top == M);
+    if (tid == 0) tell(p, row, (int)parts[__builtin_ctzll(of)].first, 0);
+    return;
+  }
+  fill_table(sh.table);
+  if (tid == 0) sh.place = sh.spots = 0;
+  __syncthreads();
+  const Weights weight{sh.table, steps_of(st.inv_t), M};
+  if (pick<E>(p, ws, st, weight, sh, sub_units)) {
+    __syncthreads();
+    long_way<E>(p, row, st, weight, sh.far);
+  }
 }
 
 // ---- launches ----
-// Parts of a row: enough workgroups for four to a CU, of 16 subs at least (one to a wave), 2^18 tokens at most
+// Parts of a row: enough workgroups for four to a CU, of 16 subs at least (one to a
+// wave), 2^18 tokens at most; of a few numbers the one whose waves have most even work.
 struct Plan {
-  int parts, subs, places, few;
+  int parts, subs, part_subs, places, few;
   int64_t rows;   // of a launch
-  bool gather;    // some row may need it
-  size_t part_at, cut_at, sub_at, list_at, weight_at, number_at, bytes;
+  bool grid, gather, counts;    // some row may need it
+  size_t part_at, bounds_at, sub_at, most_at, list_at, weight_at, number_at, bytes;
 };
 Plan plan_of(const SampleArgs& a, int num_cus) {
   Plan pl;
   pl.subs = (a.vocab + kSub - 1) / kSub;
   pl.rows = std::min<int64_t>(a.rows, 1024);
-  const int64_t want = (4 * (int64_t)num_cus + pl.rows - 1) / std::max<int64_t>(pl.rows, 1);
-  pl.parts = (int)std::max<int64_t>(1, std::min<int64_t>({want, 16, (pl.subs + kWaves - 1) / kWaves}));
+  const int most = std::min(kPartsMost, (pl.subs + kWaves - 1) / kWaves);
+  const int want = (int)std::max<int64_t>(1, std::min<int64_t>((4 * (int64_t)num_cus + pl.rows - 1) / pl.rows, most));
+  pl.parts = want;
+  auto rounds = [&](int parts) { return ((pl.subs + parts - 1) / parts + kWaves - 1) / kWaves; };
+  for (int n = want + 1; n <= std::min(most, want + 3); ++n)
+    if (n * rounds(n) < pl.parts * rounds(pl.parts)) pl.parts = n;
   pl.parts = std::max(pl.parts, (int)(((int64_t)a.vocab + (1 << 18) - 1) >> 18));
+  pl.part_subs = (pl.subs + pl.parts - 1) / pl.parts;
+  pl.parts = (pl.subs + pl.part_subs - 1) / pl.part_subs;
   pl.places = kListRow / pl.parts;
-  const int least = pl.subs / pl.parts;   // subs of the smallest part
-  pl.few = std::min({kFewMost, 32 * std::min(least, kWaves), pl.places / 2});
+  pl.few = std::min(kFewMost, 32 * pl.subs);
   const bool greedy = !a.temperatures && !(a.temperature > 0.f);
   const bool cuts = a.top_ks || (a.top_k > pl.few && a.top_k < a.vocab);                       // by number, with a grid
   const bool shares = !(!a.top_ks && a.top_k >= 1 && a.top_k <= pl.few) && (a.top_ps || a.min_ps || a.top_p < 1.f || a.min_p > 0.f);
   pl.gather = !greedy && (cuts || shares);
+  pl.counts = !greedy && cuts;
+  pl.grid = pl.counts || (pl.gather && (a.top_ps || a.top_p < 1.f));
+  const bool some = !greedy && (a.top_ks || (a.top_k > 1 && a.top_k <= pl.few));               // kFew
   size_t at = 0;
   auto take = [&](size_t n) {
     const size_t was = at;
@@ -970,11 +1177,12 @@ Plan plan_of(const SampleArgs& a, int num_cus) {
   };
   const size_t rp = (size_t)pl.rows * pl.parts;
   pl.part_at = take(rp * sizeof(Part));
-  pl.cut_at = take(pl.rows * sizeof(RowCut));
+  pl.bounds_at = take(pl.rows * sizeof(Bounds));
   pl.sub_at = take((size_t)pl.rows * pl.subs * sizeof(double));
-  pl.list_at = take(rp * pl.places * sizeof(uint32_t));
-  pl.weight_at = take(pl.gather ? rp * kCells * sizeof(ull) : 0);
-  pl.number_at = take(pl.gather ? rp * kCells * sizeof(uint32_t) : 0);
+  pl.most_at = take(some ? (size_t)pl.rows * pl.subs * 64 * sizeof(float) : 0);
+  pl.list_at = take(pl.gather ? rp * pl.places * sizeof(uint32_t) : 0);
+  pl.weight_at = take(pl.grid ? rp * kCells * sizeof(uint32_t) : 0);
+  pl.number_at = take(pl.counts ? rp * kCells * sizeof(uint32_t) : 0);
   pl.bytes = at;
   return pl;
 }
@@ -982,21 +1190,24 @@ Plan plan_of(const SampleArgs& a, int num_cus) {
 template <typename E> hipError_t launch(const SampleArgs& a, const Plan& pl, char* ws, hipStream_t s) {
   Work w;
   w.part = (Part*)(ws + pl.part_at);
-  w.cut = (RowCut*)(ws + pl.cut_at);
+  w.bounds = (Bounds*)(ws + pl.bounds_at);
   w.sub = (double*)(ws + pl.sub_at);
+  w.most = (float*)(ws + pl.most_at);
   w.list = (uint32_t*)(ws + pl.list_at);
-  w.weight = (ull*)(ws + pl.weight_at);
+  w.weight = (uint32_t*)(ws + pl.weight_at);
   w.number = (uint32_t*)(ws + pl.number_at);
   w.parts = pl.parts;
   w.subs = pl.subs;
+  w.part_subs = pl.part_subs;
   w.places = pl.places;
   w.few = pl.few;
   for (int64_t row0 = 0; row0 < a.rows; row0 += pl.rows) {
     w.row0 = (int)row0;
     const int rows = (int)std::min<int64_t>(pl.rows, a.rows - row0);
     sample_scan_kernel<E><<<rows * pl.parts, kThreads, 0, s>>>(a, w);
+    if (pl.grid) sample_bounds_kernel<<<rows, kThreads, 0, s>>>(a, w);
     if (pl.gather) sample_gather_kernel<E><<<rows * pl.parts, kThreads, 0, s>>>(a, w);
-    sample_pick_kernel<E><<<rows, kThreads, 0, s>>>(a, w);
+    sample_pick_kernel<E><<<rows, kThreads, pl.subs * sizeof(ull), s>>>(a, w);
   }
   return hipGetLastError();
 }
