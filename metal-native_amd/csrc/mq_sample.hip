@@ -18,8 +18,8 @@
 // (a sub).  What a row needs follows from its settings, which the GPU alone may
 // know (Kind); the launches are the same for all of them:
 //   scan    of every part: its largest logit, and by kind its first token; the
-//           largest logit of each lane of a sub; the subs' sums; or how much weight
-//           and how many tokens lie, about, in each cell of a grid over the logits.
+//           largest logit of each lane of a sub; the subs' sums; or how many tokens
+//           lie in each cell of a grid over the logits.
 //   bounds  where the grid was filled: from all parts' grids, the logits between
 //           which the cuts must fall.
 //   gather  there, or where min_p alone cuts: the subs' sums of what lies over these,
@@ -123,21 +123,16 @@ constexpr double kListUnit = 0x1p-50;
 // the rest by eights, what lies under all of these in the last one ----
 constexpr int kFine = 3584, kCoarse = 4608, kCells = kFine + kCoarse;
 constexpr float kEnd = 0x1p29f;   // the grid's ends
-// A cell's weights add up as whole multiples of 2^-9 of the weight at its lower edge (2^22 tokens fit 32
-// bits): each is off by 2^-10 of itself at most, and by the rounding of the product with the scale
-constexpr float kCellUnits = 512.f;
-__device__ __forceinline__ float grid_scale(double inv_t) { return (float)fmin(inv_t * (128 * 1.44269504088896340736), 1e30); }
-struct Place {
-  int g;
-  float part;   // of a cell, over its lower edge
-};
-__device__ __forceinline__ Place grid_of(float x, float scale) {   // g grows with x
-  const float t = x == INFINITY ? kEnd : fminf(fmaxf(x * scale, -kEnd), kEnd), low = floorf(t);
-  return {(int)low, t - low};
+__device__ __forceinline__ float grid_scale(double inv_t) {
+  return (float)fmin(fmax(inv_t * (128 * 1.44269504088896340736), 1e-30), 1e30);
 }
+__device__ __forceinline__ int grid_of(float x, float scale) {   // grows with x
+  return (int)floorf(__builtin_amdgcn_fmed3f(x * scale, -kEnd, kEnd));
+}
+__device__ __forceinline__ int coarse_of(int g, int top) { return kFine + min(kCoarse - 1, (top >> 3) - (g >> 3)); }
 // The logit at a cell's lower edge, moved `way` by more than its roundings
 __device__ __forceinline__ float edge_of(int g, float scale, float way) {
-  if (scale < 0x1p-100f || fabsf((float)g) >= kEnd) return way * INFINITY;
+  if (fabsf((float)g) >= kEnd) return way * INFINITY;
   const float x = (float)g / scale;
   return x + way * (fabsf(x) * 0x1p-20f + 0x1p-20f / scale);
 }
@@ -230,9 +225,9 @@ template <typename E> struct Row {
 struct Part {
   float top;        // largest logit
   uint32_t first;   // kGreedy: the first token of that logit
-  uint32_t far;     // kGrid, without counts: tokens under the fine cells
+  uint32_t far;     // kGrid, where top_k does not cut: tokens under the fine cells, and what is no number
   uint32_t listed;  // tokens that asked for a place in the list; past its length: it is not whole
-  uint32_t over_n;  // kGrid: tokens from Bounds::k_hi on
+  uint32_t over_n;  // kGrid, where top_k cuts: tokens from Bounds::k_hi on
   uint32_t cells;   // kGrid: the last cell that holds a token, and one
   double over_k, over_p;   // kGrid: weight from k_hi on (of all tokens where top_k does not cut), from p_hi on
 };
@@ -247,8 +242,7 @@ struct Work {
   double* sub;      // [rows, subs]
   float* most;      // [rows, subs, 64]: of each lane
   uint32_t* list;   // [rows, parts, places]
-  uint32_t* weight; // [rows, parts, kCells]
-  uint32_t* number; // [rows, parts, kCells]
+  uint32_t* cells;  // [rows, parts, kCells]
   int row0, parts, subs, places, few;
   int part_subs;   // of a part; fewer of the last
   __device__ __forceinline__ int first_sub(int part) const { return min(part * part_subs, subs); }
@@ -257,7 +251,7 @@ struct Work {
 template <typename E> __global__ __launch_bounds__(kThreads) void sample_scan_kernel(SampleArgs p, Work ws) {
   __shared__ double table[64];
   __shared__ ull red[kWaves];
-  __shared__ uint32_t cells[2 * kCells];   // weights, then numbers
+  __shared__ uint32_t cells[kCells];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int r = blockIdx.x / ws.parts, part = blockIdx.x - r * ws.parts, row = ws.row0 + r;
   const Settings st = settings_of(p, row, ws.few);
@@ -275,7 +269,7 @@ template <typename E> __global__ __launch_bounds__(kThreads) void sample_scan_ke
   }
   if (st.kind == kAll) fill_table(table);
   if (st.kind == kGrid)
-    for (int i = tid; i < (count ? 2 * kCells : kFine); i += kThreads) cells[i] = 0;
+    for (int i = tid; i < (count ? kCells : kFine); i += kThreads) cells[i] = 0;
 #pragma unroll
   for (int o = 32; o; o >>= 1) mine = fmaxf(mine, __shfl_xor(mine, o));
   if (lane == 0) ((float*)red)[w] = mine;
@@ -313,48 +307,36 @@ template <typename E> __global__ __launch_bounds__(kThreads) void sample_scan_ke
     }
   } else {
     const float scale = grid_scale(st.inv_t);
-    const int top = grid_of(M, scale).g;
-    // 2^(y / 128) for y in 0 .. 1, in a cell's units
-    constexpr float kLn = 0.69314718f / 128, kA = kCellUnits * kLn, kB = kCellUnits * kLn * kLn / 2;
+    const int top = grid_of(M, scale);
     uint32_t far = 0;
     for (int s = s0; s < s1; s += kWaves) {
       x.load(s, v);
       if (!count) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-          const Place at = grid_of(v[j], scale);
-          const int d = top - at.g;
-          if (d < kFine && v[j] > -INFINITY)
-            atomicAdd(&cells[d], (uint32_t)__builtin_fmaf(__builtin_fmaf(kB, at.part, kA), at.part, kCellUnits + 0.5f));
-          else
-            far += v[j] > -INFINITY;
+          const int d = top - grid_of(v[j], scale);
+          const bool fine = d < kFine;
+          far += 64 - __popcll(__ballot(fine));   // of the wave
+          if (fine) atomicAdd(&cells[d], 1u);
         }
       } else {
-#pragma unroll 4
+#pragma unroll
         for (int j = 0; j < 16; ++j) {
-          const Place at = grid_of(v[j], scale);
-          if (!(v[j] > -INFINITY)) continue;
-          const int d = top - at.g;
-          const bool fine = d < kFine;
-          const int cell = fine ? d : kFine + min(kCoarse - 1, (top >> 3) - (at.g >> 3));
-          const float y = at.part + (fine ? 0 : at.g & 7);
-          atomicAdd(&cells[cell], (uint32_t)(kCellUnits * exp2f(y * (1.f / 128)) + 0.5f));
-          atomicAdd(&cells[kCells + cell], 1u);
+          const int g = grid_of(v[j], scale), d = top - g;
+          if (v[j] > -INFINITY) atomicAdd(&cells[d < kFine ? d : coarse_of(g, top)], 1u);
         }
       }
     }
     __syncthreads();
-    uint32_t* weights = ws.weight + ((int64_t)r * ws.parts + part) * kCells;
-    uint32_t* numbers = ws.number + ((int64_t)r * ws.parts + part) * kCells;
+    uint32_t* to = ws.cells + ((int64_t)r * ws.parts + part) * kCells;
     uint32_t end = 0;
     for (int i = tid; i < (count ? kCells : kFine); i += kThreads) {
       const uint32_t c = cells[i];
-      weights[i] = c;
-      if (count) numbers[i] = cells[kCells + i];
+      to[i] = c;
       if (c) end = i + 1;
     }
     end = (uint32_t)most_of<kWaves>(end, red);
-    far = (uint32_t)add_up<kWaves, ull>(far, red);
+    far = (uint32_t)add_up<kWaves, ull>(lane == 0 ? far : 0, red);
     if (tid == 0) {
       out.cells = end;
       out.far = far;
@@ -376,10 +358,10 @@ __device__ __forceinline__ float top_of(const Part* part, int parts) {
 // down, is one of the row's.  Then between which logits the cuts fall; a workgroup
 // for each row.
 __global__ __launch_bounds__(kThreads) void sample_bounds_kernel(SampleArgs p, Work ws) {
-  __shared__ uint32_t weights[kCells], numbers[kCells];
+  __shared__ uint32_t numbers[kCells];
   __shared__ double red[kWaves];
   __shared__ uint32_t far_of;
-  __shared__ int cell[3];
+  __shared__ int cell;
   const int tid = threadIdx.x, r = blockIdx.x, row = ws.row0 + r;
   const Settings st = settings_of(p, row, ws.few);
   if (st.kind != kGrid) return;
@@ -389,66 +371,58 @@ __global__ __launch_bounds__(kThreads) void sample_bounds_kernel(SampleArgs p, W
   const bool count = st.top_k < p.vocab;
   const int cells = count ? kCells : kFine;
   const float scale = grid_scale(st.inv_t);
-  const int top = grid_of(M, scale).g;
-  for (int i = tid; i < cells; i += kThreads) weights[i] = numbers[i] = 0;
-  if (tid == 0) far_of = 0;
+  const int top = grid_of(M, scale);
+  for (int i = tid; i < cells; i += kThreads) numbers[i] = 0;
+  if (tid == 0) {
+    far_of = 0;
+    cell = cells;
+  }
   __syncthreads();
-  uint32_t far = 0;   // tokens under the row's fine cells, or more
+  uint32_t far = 0;   // tokens under the row's fine cells
   // as many threads to each part: a power of two
   int lanes = kThreads;
   while (lanes * ws.parts > kThreads) lanes >>= 1;
   const int of = tid / lanes;
   if (of < ws.parts) {
     const Part& q = parts[of];
-    const int end = (int)q.cells, mt = grid_of(q.top, scale).g, down = top - mt;
-    const uint32_t* pw = ws.weight + ((int64_t)r * ws.parts + of) * kCells;
-    const uint32_t* pn = ws.number + ((int64_t)r * ws.parts + of) * kCells;
+    const int end = (int)q.cells, mt = grid_of(q.top, scale), down = top - mt;
+    const uint32_t* from = ws.cells + ((int64_t)r * ws.parts + of) * kCells;
     if ((tid & (lanes - 1)) == 0 && !count && end) far += q.far;
     constexpr int kStep = 8;   // loads of a thread on their way
     for (int d0 = tid & (lanes - 1); d0 < end; d0 += kStep * lanes) {
-      uint32_t wt[kStep], n[kStep];
+      uint32_t n[kStep];
 #pragma unroll
       for (int k = 0; k < kStep; ++k) {
         const int d = d0 + k * lanes;
-        wt[k] = d < end ? pw[d] : 0;
-        n[k] = count && d < end ? pn[d] : 0;
+        n[k] = d < end ? from[d] : 0;
       }
 #pragma unroll
       for (int k = 0; k < kStep; ++k) {
-        if (wt[k] == 0) continue;
         const int d = d0 + k * lanes;
-        if (d < kFine && d + down < kFine) {
-          atomicAdd(&weights[d + down], wt[k]);
-          if (count) atomicAdd(&numbers[d + down], n[k]);
-        } else if (!count) {
-          far += wt[k] / (uint32_t)kCellUnits;   // no token has less
-        } else if (d < kFine) {   // to the lower edge of a coarse cell
-          const int g = mt - d, c = kFine + min(kCoarse - 1, (top >> 3) - (g >> 3));
-          atomicAdd(&weights[c], (uint32_t)((float)wt[k] * exp2f((g & 7) * (1.f / 128))));
-          atomicAdd(&numbers[c], n[k]);
-        } else {
-          const int c = kFine + min(kCoarse - 1, d - kFine + (top >> 3) - (mt >> 3));
-          atomicAdd(&weights[c], wt[k]);
-          atomicAdd(&numbers[c], n[k]);
-        }
+        int to = d + down;
+        if (d >= kFine) to = kFine + min(kCoarse - 1, d - kFine + (top >> 3) - (mt >> 3));
+        else if (to >= kFine) to = count ? coarse_of(mt - d, top) : -1;
+        if (to < 0) far += n[k];
+        else if (n[k]) atomicAdd(&numbers[to], n[k]);
       }
     }
   }
   if (far) atomicAdd(&far_of, far);
-  if (tid == 0) cell[0] = cell[1] = cell[2] = cells;
   __syncthreads();
   constexpr int N = kCells / kThreads;
   const int per = count ? N : (kFine + kThreads - 1) / kThreads, b0 = per * tid;   // the thread's cells
-  double wt[N], mine = 0;
+  double wt[N], mine = 0, low = 0;
   uint32_t n[N], mine_n = 0;
 #pragma unroll
   for (int k = 0; k < N; ++k) {
     const int b = b0 + k;
     const bool have = k < per && b < cells;
-    const int down = b < kFine ? b : top - 8 * ((top >> 3) - (b - kFine));   // of the lower edge, from the top cell's
-    wt[k] = have ? (double)weights[have ? b : 0] * exp2((double)-down * (1.0 / 128)) : 0;
-    n[k] = have && count ? numbers[b] : 0;
+    // the weight at a fine cell's middle, a coarse one's lower edge; the top cell's is 1
+    const float down = b < kFine ? (float)b : (float)(top - 8 * ((top >> 3) - (b - kFine))) + 0.5f;
+    n[k] = have ? numbers[have ? b : 0] : 0;
+    wt[k] = (double)((float)n[k] * exp2f(down * (-1.f / 128)));
     mine += wt[k];
+    low += b < kFine ? 0 : wt[k];
     mine_n += n[k];
   }
   double all;
@@ -457,16 +431,19 @@ __global__ __launch_bounds__(kThreads) void sample_bounds_kernel(SampleArgs p, W
     uint32_t all_n, at = scan<kWaves, uint32_t>(mine_n, (uint32_t*)red, all_n) - mine_n;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      if (at < (uint32_t)st.top_k && at + n[k] >= (uint32_t)st.top_k) cell[0] = b0 + k;   // one thread
+      if (at < (uint32_t)st.top_k && at + n[k] >= (uint32_t)st.top_k) cell = b0 + k;   // one thread
       at += n[k];
     }
   }
   __syncthreads();
-  const int cell_k = cell[0];
+  const int cell_k = cell;
+  int cell_p0 = cells, cell_p1 = cells;
   if (st.top_p < 1.0) {
-    // What is known: sums of cells to e of themselves; what lies under the fine cells, from nothing to
-    // 2^-28 a token; of cell_k, some part
-    const double e = 1.2e-3 + fabs((double)top) * 0x1p-28, share = fmax(st.top_p, 0.0);
+    // What is known: sums of fine cells to e of themselves (half a cell's width, and the rounding of the product
+    // with the scale); coarse ones to 7 / 128 of a factor of two; what lies under the fine cells from nothing to
+    // 2^-28 a token; of cell_k some part.
+    const double e = 2.8e-3 + fabs((double)top) * 0x1p-28, share = fmax(st.top_p, 0.0);
+    const double slack = count ? 0.045 * add_up<kWaves, double>(low, red) : far_of * 0x1p-28;
     double upto = all, in_k = 0;
     if (cell_k < cells) {
       double run = before;
@@ -480,21 +457,21 @@ __global__ __launch_bounds__(kThreads) void sample_bounds_kernel(SampleArgs p, W
       upto = red[0];
       in_k = red[1];
     }
-    const double under = count ? 0 : far_of * 0x1p-28 * kCellUnits;
-    const double lo = (upto - in_k) * (1 - e), hi = upto * (1 + e) + under;   // of what top_p is a share of
+    const double lo = (upto - in_k) * (1 - e), hi = upto * (1 + e) + slack;   // of what top_p is a share of
     double run = before;
+    ull may = cells, must = cells;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       run += wt[k];
       const int b = b0 + k;
-      if (b > cell_k || wt[k] == 0) continue;
       const double rest = fmax(upto - run, 0.0);   // weight past the cell, with all of cell_k
-      const bool may = run * (1 + e) >= share * lo && fmax(rest - in_k, 0.0) * (1 - e) <= (1 - share) * hi;
-      const bool must = run * (1 - e) >= share * hi || rest * (1 + e) + under <= (1 - share) * upto * (1 - e);
-      if (may) atomicMin(&cell[1], b);
-      if (must) atomicMin(&cell[2], b);
+      if (b <= cell_k && wt[k] > 0) {
+        if (run * (1 + e) + slack >= share * lo && fmax(rest - in_k, 0.0) * (1 - e) <= (1 - share) * hi) may = min(may, (ull)b);
+        if (run * (1 - e) >= share * hi || rest * (1 + e) + slack <= (1 - share) * upto * (1 - e)) must = min(must, (ull)b);
+      }
     }
-    __syncthreads();
+    cell_p1 = (int)least_of<kWaves>(must, (ull*)red);
+    cell_p0 = (int)least_of<kWaves>(may, (ull*)red);
   }
   if (tid) return;
   auto lower = [&](int c) { return c < kFine ? top - c : 8 * ((top >> 3) - (c - kFine)); };   // smallest g of a cell
@@ -505,9 +482,8 @@ __global__ __launch_bounds__(kThreads) void sample_bounds_kernel(SampleArgs p, W
     b.k_lo = cell_k == kCells - 1 ? -INFINITY : edge_of(lower(cell_k), scale, -1.f);
   }
   if (b.cut_p) {
-    const int p1 = cell[2], p0 = min(cell[1], min(p1, cells - 1));
-    b.p_hi = edge_of(upper(p0) + 1, scale, 1.f);
-    b.p_lo = p1 >= cells || p1 == kCells - 1 ? b.k_lo : edge_of(lower(p1), scale, -1.f);
+    b.p_hi = edge_of(upper(min(cell_p0, min(cell_p1, cells - 1))) + 1, scale, 1.f);
+    b.p_lo = cell_p1 >= cells || cell_p1 == kCells - 1 ? b.k_lo : edge_of(lower(cell_p1), scale, -1.f);
   }
   ws.bounds[r] = b;
 }
@@ -554,31 +530,57 @@ template <typename E> __global__ __launch_bounds__(kThreads) void sample_gather_
   uint32_t* list = ws.list + ((int64_t)r * ws.parts + part) * ws.places;
   double over_k = 0, over_p = 0;
   uint32_t over_n = 0;
-  for (int s = s0; s < s1; s += kWaves) {
-    x.load(s, v);
-    double kept = 0;
-    uint32_t take = 0;
-#pragma unroll 4
-    for (int j = 0; j < 16; ++j) {
-      const bool in_k = cut_k && v[j] >= b.k_lo && v[j] < b.k_hi, in_p = cut_p && v[j] >= b.p_lo && v[j] < b.p_hi;
-      take |= (uint32_t)((in_k || in_p) && v[j] > -INFINITY) << j;
-      if (cut_k && !__any(v[j] >= b.k_hi)) continue;
-      const double wt = weight(v[j]);
-      const bool of_k = !cut_k || v[j] >= b.k_hi;
-      over_k += of_k ? wt : 0.0;
-      over_n += of_k && cut_k;
-      const double top_part = v[j] >= sure ? wt : 0.0;
-      over_p += top_part;
-      kept += top_part >= st.min_p ? top_part : 0.0;
-    }
-#pragma unroll
-    for (int o = 32; o; o >>= 1) kept += __shfl_xor(kept, o);
-    if (lane == 0) sub[s] = kept;
+  auto enlist = [&](int s, uint32_t take) {   // bit j: the lane's j-th token
     while (take) {
       const int j = __builtin_ctz(take);
       take &= take - 1;
       const uint32_t at = atomicAdd(&places, 1u);
       if (at < (uint32_t)ws.places) list[at] = s * kSub + x.at(j);
+    }
+  };
+  if (!cut_k && st.min_p == 0) {   // top_p alone
+    for (int s = s0; s < s1; s += kWaves) {
+      x.load(s, v);
+      double kept = 0;
+      uint32_t take = 0;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const double wt = weight(v[j]);
+        const bool stays = v[j] >= sure;
+        over_k += wt;
+        kept += stays ? wt : 0.0;
+        take |= (!stays & (v[j] >= b.p_lo) & (v[j] > -INFINITY)) << j;
+      }
+      over_p += kept;
+#pragma unroll
+      for (int o = 32; o; o >>= 1) kept += __shfl_xor(kept, o);
+      if (lane == 0) sub[s] = kept;
+      enlist(s, take);
+    }
+  } else {
+    // where top_k cuts, what lies under both windows has no part in anything
+    const float least = cut_k ? (cut_p ? fminf(b.k_lo, b.p_lo) : b.k_lo) : -INFINITY;
+    for (int s = s0; s < s1; s += kWaves) {
+      x.load(s, v);
+      double kept = 0;
+      uint32_t take = 0;
+#pragma unroll 4
+      for (int j = 0; j < 16; ++j) {
+        if (!__any(v[j] >= least)) continue;
+        const bool in_k = cut_k & (v[j] >= b.k_lo) & (v[j] < b.k_hi), in_p = cut_p & (v[j] >= b.p_lo) & (v[j] < b.p_hi);
+        take |= ((in_k | in_p) & (v[j] > -INFINITY)) << j;
+        const double wt = weight(v[j]);
+        const bool of_k = !cut_k | (v[j] >= b.k_hi);
+        over_k += of_k ? wt : 0.0;
+        over_n += of_k;
+        const double stays = v[j] >= sure ? wt : 0.0;
+        over_p += stays;
+        kept += stays >= st.min_p ? stays : 0.0;
+      }
+#pragma unroll
+      for (int o = 32; o; o >>= 1) kept += __shfl_xor(kept, o);
+      if (lane == 0) sub[s] = kept;
+      enlist(s, take);
     }
   }
   over_k = add_up<kWaves, double>(over_k, red);
@@ -971,26 +973,28 @@ __device__ __forceinline__ bool pick(const SampleArgs& p, const Work& ws, const 
   // what must hold for the four waves to go on is the same for all threads.
   const uint32_t* const key = sh.list.key;
   const uint32_t* const index = sh.list.idx;
-  if (cut_k) {   // too few tokens in the row: no cut; the grid's counts said that there is one
-    const ull n = add_up<kWaves, ull>([&] {
-      ull c = 0;
-      for (int i = tid; i < (int)held; i += kThreads) c += of_k(i);
-      return c;
-    }(), (ull*)red);
-    if (!(over_n < (uint32_t)st.top_k && over_n + n >= (uint32_t)st.top_k)) return true;
-  }
-  if (cut_p) {
-    // with all or nothing of the window of top_k: the aim lies between these two
-    ull in_k = 0, in_p = 0;
+  if (cut_k || cut_p) {
+    // tokens of the window of top_k; the weights of both.  With all or nothing of the
+    // former in the sum that top_p takes its share of, the aim lies between these two.
+    ull n = 0, in_k = 0, in_p = 0;
     for (int i = tid; i < (int)held; i += kThreads) {
-      if (of_k(i)) in_k += sh.list.units[i];
-      if (of_p(i)) in_p += sh.list.units[i];
+      const ull units = sh.list.units[i];
+      const bool k = of_k(i);
+      n += k;
+      in_k += k ? units : 0;
+      in_p += of_p(i) ? units : 0;
     }
-    in_k = add_up<kWaves, ull>(in_k, (ull*)red);
-    in_p = add_up<kWaves, ull>(in_p, (ull*)red);
-    const double lo = st.top_p * over_k, hi = st.top_p * (over_k + kListUnit * (double)in_k);
-    // a window that ends with the tokens that top_k may leave needs no lower end of its own
-    if (!((over_p < lo || over_p == 0) && (over_p + kListUnit * (double)in_p >= hi || (cut_k && b.p_lo <= b.k_lo)))) return true;
+    if (cut_k) {
+      n = add_up<kWaves, ull>(n, (ull*)red);
+      in_k = add_up<kWaves, ull>(in_k, (ull*)red);
+      if (!(over_n < (uint32_t)st.top_k && over_n + n >= (uint32_t)st.top_k)) return true;
+    }
+    if (cut_p) {
+      in_p = add_up<kWaves, ull>(in_p, (ull*)red);
+      const double lo = st.top_p * over_k, hi = st.top_p * (over_k + kListUnit * (double)in_k);
+      // a window that ends with the tokens that top_k may leave needs no lower end of its own
+      if (!((over_p < lo || over_p == 0) && (over_p + kListUnit * (double)in_p >= hi || (cut_k && b.p_lo <= b.k_lo)))) return true;
+    }
   }
   if (tid >= kNearThreads) return false;
 
@@ -1144,8 +1148,8 @@ template <typename E> __global__ __launch_bounds__(kThreads) void sample_pick_ke
 struct Plan {
   int parts, subs, part_subs, places, few;
   int64_t rows;   // of a launch
-  bool grid, gather, counts;    // some row may need it
-  size_t part_at, bounds_at, sub_at, most_at, list_at, weight_at, number_at, bytes;
+  bool grid, gather;   // some row may need it
+  size_t part_at, bounds_at, sub_at, most_at, list_at, cells_at, bytes;
 };
 Plan plan_of(const SampleArgs& a, int num_cus) {
   Plan pl;
@@ -1166,8 +1170,7 @@ Plan plan_of(const SampleArgs& a, int num_cus) {
   const bool cuts = a.top_ks || (a.top_k > pl.few && a.top_k < a.vocab);                       // by number, with a grid
   const bool shares = !(!a.top_ks && a.top_k >= 1 && a.top_k <= pl.few) && (a.top_ps || a.min_ps || a.top_p < 1.f || a.min_p > 0.f);
   pl.gather = !greedy && (cuts || shares);
-  pl.counts = !greedy && cuts;
-  pl.grid = pl.counts || (pl.gather && (a.top_ps || a.top_p < 1.f));
+  pl.grid = (!greedy && cuts) || (pl.gather && (a.top_ps || a.top_p < 1.f));
   const bool some = !greedy && (a.top_ks || (a.top_k > 1 && a.top_k <= pl.few));               // kFew
   size_t at = 0;
   auto take = [&](size_t n) {
@@ -1181,8 +1184,7 @@ Plan plan_of(const SampleArgs& a, int num_cus) {
   pl.sub_at = take((size_t)pl.rows * pl.subs * sizeof(double));
   pl.most_at = take(some ? (size_t)pl.rows * pl.subs * 64 * sizeof(float) : 0);
   pl.list_at = take(pl.gather ? rp * pl.places * sizeof(uint32_t) : 0);
-  pl.weight_at = take(pl.grid ? rp * kCells * sizeof(uint32_t) : 0);
-  pl.number_at = take(pl.counts ? rp * kCells * sizeof(uint32_t) : 0);
+  pl.cells_at = take(pl.grid ? rp * kCells * sizeof(uint32_t) : 0);
   pl.bytes = at;
   return pl;
 }
@@ -1194,8 +1196,7 @@ template <typename E> hipError_t launch(const SampleArgs& a, const Plan& pl, cha
   w.sub = (double*)(ws + pl.sub_at);
   w.most = (float*)(ws + pl.most_at);
   w.list = (uint32_t*)(ws + pl.list_at);
-  w.weight = (uint32_t*)(ws + pl.weight_at);
-  w.number = (uint32_t*)(ws + pl.number_at);
+  w.cells = (uint32_t*)(ws + pl.cells_at);
   w.parts = pl.parts;
   w.subs = pl.subs;
   w.part_subs = pl.part_subs;
