@@ -137,13 +137,51 @@ __device__ __forceinline__ float edge_of(int g, float scale, float way) {
   return x + way * (fabsf(x) * 0x1p-20f + 0x1p-20f / scale);
 }
 
-// ---- sums of the workgroup's first N waves (the others have gone, if there are any) ----
+// ---- sums over a wave, then over the workgroup's first N waves (the others have gone, if there are any) ----
+template <typename V> __device__ __forceinline__ V from_lane(V v, int b) {   // of lane ^ b, without the LDS unit
+  if constexpr (sizeof(V) == 4) {
+    return __builtin_bit_cast(V, xor_lane(__builtin_bit_cast(float, v), b));
+  } else {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    const f2 h = __builtin_bit_cast(f2, v);
+    return __builtin_bit_cast(V, (f2){xor_lane(h[0], b), xor_lane(h[1], b)});
+  }
+}
+template <typename V, typename F> __device__ __forceinline__ V wave_reduce(V v, F&& f) {   // on every lane
+  v = f(v, from_lane(v, 1));
+  v = f(v, from_lane(v, 2));
+  v = f(v, from_lane(v, 4));
+  v = f(v, from_lane(v, 8));
+  v = f(v, from_lane(v, 16));
+  return f(v, from_lane(v, 32));
+}
+template <typename V> __device__ __forceinline__ V wave_sum(V v) {
+  return wave_reduce(v, [](V a, V b) { return a + b; });
+}
+// zero where the lane has no source
+template <int CTRL, int ROWS, typename V> __device__ __forceinline__ V shifted(V v) {
+  if constexpr (sizeof(V) == 4) {
+    return __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xF, false));
+  } else {
+    typedef int i2 __attribute__((ext_vector_type(2)));
+    const i2 h = __builtin_bit_cast(i2, v);
+    return __builtin_bit_cast(V, (i2){__builtin_amdgcn_update_dpp(0, h[0], CTRL, ROWS, 0xF, false),
+                                      __builtin_amdgcn_update_dpp(0, h[1], CTRL, ROWS, 0xF, false)});
+  }
+}
+template <typename V> __device__ __forceinline__ V wave_scan(V v) {   // inclusive
+  v += shifted<0x111, 0xF>(v);   // row_shr 1, 2, 4, 8
+  v += shifted<0x112, 0xF>(v);
+  v += shifted<0x114, 0xF>(v);
+  v += shifted<0x118, 0xF>(v);
+  v += shifted<0x142, 0xA>(v);   // row_bcast 15, 31
+  v += shifted<0x143, 0xC>(v);
+  return v;
+}
 template <int N, typename V, typename F> __device__ __forceinline__ V reduce(V v, V* lds, F&& f) {   // on every thread
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-#pragma unroll
-  for (int o = 32; o; o >>= 1) v = f(v, (V)__shfl_xor(v, o));
+  v = wave_reduce(v, f);
   __syncthreads();
-  if (lane == 0) lds[w] = v;
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
   __syncthreads();
   v = lds[0];
 #pragma unroll
@@ -161,21 +199,18 @@ template <int N> __device__ __forceinline__ ull most_of(ull v, ull* lds) {
 }
 // inclusive, and the sum of all
 template <int N, typename V> __device__ __forceinline__ V scan(V v, V* lds, V& all) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const V t = __shfl_up(v, o);
-    if (lane >= o) v += t;
-  }
+  const int w = threadIdx.x >> 6;
+  v = wave_scan(v);
   __syncthreads();
-  if (lane == 63) lds[w] = v;
+  if ((threadIdx.x & 63) == 63) lds[w] = v;
   __syncthreads();
   V before = 0;
   all = 0;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    if (i < w) before += lds[i];
-    all += lds[i];
+    const V t = lds[i];
+    before += i < w ? t : V(0);
+    all += t;
   }
   return v + before;
 }
@@ -270,8 +305,7 @@ template <typename E> __global__ __launch_bounds__(kThreads) void sample_scan_ke
   if (st.kind == kAll) fill_table(table);
   if (st.kind == kGrid)
     for (int i = tid; i < (count ? kCells : kFine); i += kThreads) cells[i] = 0;
-#pragma unroll
-  for (int o = 32; o; o >>= 1) mine = fmaxf(mine, __shfl_xor(mine, o));
+  mine = wave_reduce(mine, [](float a, float b) { return fmaxf(a, b); });
   if (lane == 0) ((float*)red)[w] = mine;
   __syncthreads();
   float M = -INFINITY;
@@ -301,8 +335,7 @@ template <typename E> __global__ __launch_bounds__(kThreads) void sample_scan_ke
       double sum = 0;
 #pragma unroll 4
       for (int j = 0; j < 16; ++j) sum += weight(v[j]);
-#pragma unroll
-      for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+      sum = wave_sum(sum);
       if (lane == 0) sub[s] = sum;
     }
   } else {
@@ -350,7 +383,7 @@ __device__ __forceinline__ float top_of(const Part* part, int parts) {
   const int i = threadIdx.x & (kPartsMost - 1);
   float M = i < parts ? part[i].top : -INFINITY;
 #pragma unroll
-  for (int o = kPartsMost / 2; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
+  for (int o = kPartsMost / 2; o; o >>= 1) M = fmaxf(M, from_lane(M, o));
   return M;
 }
 
@@ -388,22 +421,23 @@ __global__ __launch_bounds__(kThreads) void sample_bounds_kernel(SampleArgs p, W
     const int end = (int)q.cells, mt = grid_of(q.top, scale), down = top - mt;
     const uint32_t* from = ws.cells + ((int64_t)r * ws.parts + of) * kCells;
     if ((tid & (lanes - 1)) == 0 && !count && end) far += q.far;
-    constexpr int kStep = 8;   // loads of a thread on their way
-    for (int d0 = tid & (lanes - 1); d0 < end; d0 += kStep * lanes) {
-      uint32_t n[kStep];
+    constexpr int kStep = 8;   // loads of a thread on their way, four cells each (the last ones past end: zeros)
+    for (int d0 = 4 * (tid & (lanes - 1)); d0 < end; d0 += 4 * kStep * lanes) {
+      u4 n4[kStep];
 #pragma unroll
       for (int k = 0; k < kStep; ++k) {
-        const int d = d0 + k * lanes;
-        n[k] = d < end ? from[d] : 0;
+        const int d = d0 + 4 * k * lanes;
+        n4[k] = d < end ? *(const u4*)(from + d) : (u4){0u, 0u, 0u, 0u};
       }
 #pragma unroll
-      for (int k = 0; k < kStep; ++k) {
-        const int d = d0 + k * lanes;
+      for (int k = 0; k < 4 * kStep; ++k) {
+        const int d = d0 + 4 * (k / 4) * lanes + k % 4;
+        const uint32_t n = n4[k / 4][k % 4];
         int to = d + down;
         if (d >= kFine) to = kFine + min(kCoarse - 1, d - kFine + (top >> 3) - (mt >> 3));
         else if (to >= kFine) to = count ? coarse_of(mt - d, top) : -1;
-        if (to < 0) far += n[k];
-        else if (n[k]) atomicAdd(&numbers[to], n[k]);
+        if (to < 0) far += n;
+        else if (n) atomicAdd(&numbers[to], n);
       }
     }
   }
@@ -518,8 +552,7 @@ template <typename E> __global__ __launch_bounds__(kThreads) void sample_gather_
           const double wt = weight(v[j]);
           sum += wt >= st.min_p ? wt : 0.0;
         }
-#pragma unroll
-      for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+      sum = wave_sum(sum);
       if (lane == 0) sub[s] = sum;
     }
     return;
@@ -552,8 +585,7 @@ template <typename E> __global__ __launch_bounds__(kThreads) void sample_gather_
         take |= (!stays & (v[j] >= b.p_lo) & (v[j] > -INFINITY)) << j;
       }
       over_p += kept;
-#pragma unroll
-      for (int o = 32; o; o >>= 1) kept += __shfl_xor(kept, o);
+      kept = wave_sum(kept);
       if (lane == 0) sub[s] = kept;
       enlist(s, take);
     }
@@ -577,8 +609,7 @@ template <typename E> __global__ __launch_bounds__(kThreads) void sample_gather_
         over_p += stays;
         kept += stays >= st.min_p ? stays : 0.0;
       }
-#pragma unroll
-      for (int o = 32; o; o >>= 1) kept += __shfl_xor(kept, o);
+      kept = wave_sum(kept);
       if (lane == 0) sub[s] = kept;
       enlist(s, take);
     }
