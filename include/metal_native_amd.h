@@ -392,7 +392,8 @@ MQ_API int mq_paged_evict(const mq_paged_cache* cache, const float* mass, int64_
  *
  * Each setting is one value, or where its pointer is not NULL an array of `rows`
  * in device memory.  logprob (or NULL): the log of the drawn token's share of the
- * sum.  A row without a logit above -inf gives token -1 and -inf. */
+ * sum.  A row without a logit above -inf gives token -1 and -inf.  Weights under
+ * 2^-45 of the largest are never drawn.  Rows below 2^31, vocab 1 to 2^22. */
 enum mq_sample_dtype { MQ_SAMPLE_F16 = 0, MQ_SAMPLE_BF16 = 1, MQ_SAMPLE_F32 = 2 };
 typedef struct mq_sampling {
   const float *temperatures, *top_ps, *min_ps;

@@ -10,20 +10,21 @@
 //
 // A token is a whole number: between two that border on each other in the running
 // sum nothing is half right, and 150 thousand borders lie in a row.  Weights are
-// therefore taken in 64 bits (to 4e-14 of themselves), and sums in 64 bits too:
-// as whole multiples of 2^-44 wherever atomics or a list's order would change
-// what is added to what.
+// therefore taken in 64 bits (to 4e-14 of themselves), and what is drawn goes by
+// their sums as whole multiples of 2^-44 (less for rows of more than 2^18): whole
+// numbers add up to the same in any order, and halves of a row that hold the same
+// logits to the same half.  Tokens of less than half of that are never drawn.
 //
 // A row is dealt out to `parts` workgroups, a wave taking 1024 tokens at a time
 // (a sub).  What a row needs follows from its settings, which the GPU alone may
 // know (Kind); the launches are the same for all of them:
 //   scan    of every part: its largest logit, and by kind its first token; the
-//           largest logit of each lane of a sub; the subs' sums; or how many tokens
-//           lie in each cell of a grid over the logits.
+//           largest logit of each lane of a sub; or how many tokens lie in each cell
+//           of a grid over the logits.
 //   bounds  where the grid was filled: from all parts' grids, the logits between
 //           which the cuts must fall.
-//   gather  there, or where min_p alone cuts: the subs' sums of what lies over these,
-//           and a list of the tokens between them.
+//   gather  the subs' sums of what lies over these (where nothing but min_p cuts, of
+//           all), and a list of the tokens between them.
 //   pick    the cuts among the listed tokens (or those of the lanes that may hold
 //           the first top_k), the sub in which the running sum passes its aim, and the
 //           token in it.
@@ -59,7 +60,7 @@ template <typename E> constexpr int kLow = 0;
 template <> constexpr int kLow<_Float16> = 13;
 template <> constexpr int kLow<__bf16> = 16;
 
-enum Kind { kGreedy, kFew, kGrid, kFloor, kAll };
+enum Kind { kGreedy, kFew, kGrid, kFloor };   // kFloor: nothing, or min_p alone, cuts
 
 struct Settings {
   double inv_t, top_p, min_p;
@@ -80,7 +81,7 @@ __device__ __forceinline__ Settings settings_of(const SampleArgs& p, int row, in
   s.u = u > 0.f ? fminf(u, 0x1.fffffep-1f) : 0.f;
   s.kind = !(t > 0.f) || s.top_k == 1 ? kGreedy
            : s.top_k <= few           ? kFew
-           : s.top_k < p.vocab || s.top_p < 1.0 ? kGrid : (s.min_p > 0 ? kFloor : kAll);
+           : s.top_k < p.vocab || s.top_p < 1.0 ? kGrid : kFloor;
   return s;
 }
 
@@ -110,12 +111,17 @@ __device__ __forceinline__ double steps_of(double inv_t) { return inv_t * (64 * 
 __device__ __forceinline__ void fill_table(double* table) {   // before a barrier
   if (threadIdx.x < 64) table[threadIdx.x] = exp2(threadIdx.x / 64.0);
 }
-// w in 2^-44, to the nearest
-__device__ __forceinline__ ull whole(double w) { return (ull)__double_as_longlong(w + 256.0) & ((1ull << 52) - 1); }
-constexpr double kUnit = 0x1p-44;
+// w as a whole number of units, to the nearest; one = 2^52 units: 2^8 for 2^-44
+__device__ __forceinline__ ull whole(double w, double one) { return (ull)(__double_as_longlong(w + one) - __double_as_longlong(one)); }
 // of a list's tokens, no more than kListRow of them, in 2^-50
-__device__ __forceinline__ ull whole_of_list(double w) { return (ull)__double_as_longlong(w + 4.0) & ((1ull << 52) - 1); }
+__device__ __forceinline__ ull whole_of_list(double w) { return whole(w, 4.0); }
 constexpr double kListUnit = 0x1p-50;
+// floor(u n): a whole number passes u n where it passes this
+__device__ __forceinline__ ull share_of(float u, ull n) {
+  const uint32_t b = __float_as_uint(u), down = 150 - (b >> 23);   // u = m 2^-down < 1
+  if (b >> 23 == 0 || down > 100) return 0;
+  return (ull)((unsigned __int128)((b & 0x7fffff) | 0x800000) * n >> down);
+}
 
 // ---- the grid: cells of 1/128 of a factor of two in weight, the same ones for all
 // parts of a row; kFine of them under the largest logit's (28 factors of two, further
@@ -178,52 +184,62 @@ template <typename V> __device__ __forceinline__ V wave_scan(V v) {   // inclusi
   v += shifted<0x143, 0xC>(v);
   return v;
 }
-template <int N, typename V, typename F> __device__ __forceinline__ V reduce(V v, V* lds, F&& f) {   // on every thread
-  v = wave_reduce(v, f);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = lds[0];
-#pragma unroll
-  for (int i = 1; i < N; ++i) v = f(v, lds[i]);
-  return v;
-}
-template <int N, typename V> __device__ __forceinline__ V add_up(V v, V* lds) {
-  return reduce<N, V>(v, lds, [](V a, V b) { return a + b; });
-}
-template <int N> __device__ __forceinline__ ull least_of(ull v, ull* lds) {
-  return reduce<N, ull>(v, lds, [](ull a, ull b) { return a < b ? a : b; });
-}
-template <int N> __device__ __forceinline__ ull most_of(ull v, ull* lds) {
-  return reduce<N, ull>(v, lds, [](ull a, ull b) { return a > b ? a : b; });
-}
-// inclusive, and the sum of all
-template <int N, typename V> __device__ __forceinline__ V scan(V v, V* lds, V& all) {
-  const int w = threadIdx.x >> 6;
-  v = wave_scan(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 63) lds[w] = v;
-  __syncthreads();
-  V before = 0;
-  all = 0;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const V t = lds[i];
-    before += i < w ? t : V(0);
-    all += t;
+// What the waves exchange, by turns in two halves: one barrier a sum, since who is
+// past it has read the half that the next one but one writes.
+struct Group {
+  ull* lds;   // [2 * kWaves]
+  int half = 0;
+  // every wave's value, of wave i on the lanes of i % N
+  template <int N, typename V> __device__ __forceinline__ V of_waves(V v, int from = 0) {
+    half ^= kWaves;
+    if ((int)(threadIdx.x & 63) == from) *(V*)(lds + half + (threadIdx.x >> 6)) = v;
+    __syncthreads();
+    return *(const V*)(lds + half + (threadIdx.x & (N - 1)));
   }
-  return v + before;
-}
-// of counts that are the same on a wave's lanes; one barrier, by turns in two halves of lds
-template <int N> __device__ __forceinline__ uint32_t count_up(uint32_t n, uint32_t* lds, int& turn) {
-  turn ^= kWaves;
-  if ((threadIdx.x & 63) == 0) lds[turn + (threadIdx.x >> 6)] = n;
-  __syncthreads();
-  uint32_t s = 0;
+  template <int N, typename V, typename F> __device__ __forceinline__ V reduce(V v, F&& f) {   // on every thread
+    v = of_waves<N>(wave_reduce(v, f));
 #pragma unroll
-  for (int i = 0; i < N; ++i) s += lds[turn + i];
-  return s;
-}
+    for (int o = 1; o < N; o <<= 1) v = f(v, from_lane(v, o));
+    return v;
+  }
+  template <int N, typename V> __device__ __forceinline__ V sum(V v) {
+    return reduce<N>(v, [](V a, V b) { return a + b; });
+  }
+  template <int N, typename V> __device__ __forceinline__ V least(V v) {
+    return reduce<N>(v, [](V a, V b) { return a < b ? a : b; });
+  }
+  template <int N, typename V> __device__ __forceinline__ V most(V v) {
+    return reduce<N>(v, [](V a, V b) { return a > b ? a : b; });
+  }
+  // of numbers that are the same on a wave's lanes
+  template <int N> __device__ __forceinline__ uint32_t sum_of_waves(uint32_t n) {
+    n = of_waves<N>(n);
+#pragma unroll
+    for (int o = 1; o < N; o <<= 1) n += from_lane(n, o);
+    return n;
+  }
+  // inclusive, and the sum of all
+  template <int N, typename V> __device__ __forceinline__ V scan(V v, V& all) {
+    v = wave_scan(v);
+    V t = of_waves<N>(v, 63);   // N waves' sums, again and again
+    t += shifted<0x111, 0xF>(t);
+    t += shifted<0x112, 0xF>(t);
+    if constexpr (N > 4) t += shifted<0x114, 0xF>(t);
+    if constexpr (N > 8) t += shifted<0x118, 0xF>(t);
+    all = at_lane(t, N - 1);
+    return v + at_lane(shifted<0x111, 0xF>(t), (int)(threadIdx.x >> 6));   // of the waves before
+  }
+  template <typename V> static __device__ __forceinline__ V at_lane(V v, int lane) {
+    lane = __builtin_amdgcn_readfirstlane(lane);
+    if constexpr (sizeof(V) == 4) {
+      return __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+    } else {
+      typedef int i2 __attribute__((ext_vector_type(2)));
+      const i2 h = __builtin_bit_cast(i2, v);
+      return __builtin_bit_cast(V, (i2){__builtin_amdgcn_readlane(h[0], lane), __builtin_amdgcn_readlane(h[1], lane)});
+    }
+  }
+};
 
 // ---- a wave's 1024 tokens ----
 template <typename E> struct Row {
@@ -274,18 +290,19 @@ struct Bounds {   // by gather, for pick: the cut of top_k falls among logits of
 struct Work {
   Part* part;       // [rows, parts]
   Bounds* bounds;   // [rows]
-  double* sub;      // [rows, subs]
+  ull* sub;         // [rows, subs]
   float* most;      // [rows, subs, 64]: of each lane
   uint32_t* list;   // [rows, parts, places]
   uint32_t* cells;  // [rows, parts, kCells]
   int row0, parts, subs, places, few;
+  double one;      // 2^52 of the units of sub
   int part_subs;   // of a part; fewer of the last
   __device__ __forceinline__ int first_sub(int part) const { return min(part * part_subs, subs); }
 };
 
 template <typename E> __global__ __launch_bounds__(kThreads) void sample_scan_kernel(SampleArgs p, Work ws) {
-  __shared__ double table[64];
-  __shared__ ull red[kWaves];
+  __shared__ ull lds[2 * kWaves];
+  Group grp{lds};
   __shared__ uint32_t cells[kCells];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int r = blockIdx.x / ws.parts, part = blockIdx.x - r * ws.parts, row = ws.row0 + r;
@@ -302,16 +319,9 @@ template <typename E> __global__ __launch_bounds__(kThreads) void sample_scan_ke
     if (st.kind == kFew) ws.most[((int64_t)r * ws.subs + s) * 64 + lane] = m;
     mine = fmaxf(mine, m);
   }
-  if (st.kind == kAll) fill_table(table);
   if (st.kind == kGrid)
     for (int i = tid; i < (count ? kCells : kFine); i += kThreads) cells[i] = 0;
-  mine = wave_reduce(mine, [](float a, float b) { return fmaxf(a, b); });
-  if (lane == 0) ((float*)red)[w] = mine;
-  __syncthreads();
-  float M = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < kWaves; ++i) M = fmaxf(M, ((float*)red)[i]);
-  __syncthreads();   // red is read
+  const float M = grp.reduce<kWaves>(mine, [](float a, float b) { return fmaxf(a, b); });
   Part& out = ws.part[(int64_t)r * ws.parts + part];
   if (tid == 0) {
     out.top = M;
@@ -325,19 +335,8 @@ template <typename E> __global__ __launch_bounds__(kThreads) void sample_scan_ke
 #pragma unroll
       for (int j = 15; j >= 0; --j) first = v[j] == M ? s * kSub + x.at(j) : first;
     }
-    first = (uint32_t)least_of<kWaves>(first, red);
+    first = (uint32_t)grp.least<kWaves, ull>(first);
     if (tid == 0) out.first = first;
-  } else if (st.kind == kAll) {
-    const Weights weight{table, steps_of(st.inv_t), M};
-    double* sub = ws.sub + (int64_t)r * ws.subs;
-    for (int s = s0; s < s1; s += kWaves) {
-      x.load(s, v);
-      double sum = 0;
-#pragma unroll 4
-      for (int j = 0; j < 16; ++j) sum += weight(v[j]);
-      sum = wave_sum(sum);
-      if (lane == 0) sub[s] = sum;
-    }
   } else {
     const float scale = grid_scale(st.inv_t);
     const int top = grid_of(M, scale);
@@ -368,8 +367,8 @@ template <typename E> __global__ __launch_bounds__(kThreads) void sample_scan_ke
       to[i] = c;
       if (c) end = i + 1;
     }
-    end = (uint32_t)most_of<kWaves>(end, red);
-    far = (uint32_t)add_up<kWaves, ull>(lane == 0 ? far : 0, red);
+    end = (uint32_t)grp.most<kWaves, ull>(end);
+    far = (uint32_t)grp.sum<kWaves, ull>(lane == 0 ? far : 0);
     if (tid == 0) {
       out.cells = end;
       out.far = far;
@@ -392,7 +391,9 @@ __device__ __forceinline__ float top_of(const Part* part, int parts) {
 // for each row.
 __global__ __launch_bounds__(kThreads) void sample_bounds_kernel(SampleArgs p, Work ws) {
   __shared__ uint32_t numbers[kCells];
-  __shared__ double red[kWaves];
+  __shared__ ull lds[2 * kWaves];
+  Group grp{lds};
+  __shared__ double at_k[2];
   __shared__ uint32_t far_of;
   __shared__ int cell;
   const int tid = threadIdx.x, r = blockIdx.x, row = ws.row0 + r;
@@ -430,14 +431,22 @@ __global__ __launch_bounds__(kThreads) void sample_bounds_kernel(SampleArgs p, W
         n4[k] = d < end ? *(const u4*)(from + d) : (u4){0u, 0u, 0u, 0u};
       }
 #pragma unroll
-      for (int k = 0; k < 4 * kStep; ++k) {
-        const int d = d0 + 4 * (k / 4) * lanes + k % 4;
-        const uint32_t n = n4[k / 4][k % 4];
-        int to = d + down;
-        if (d >= kFine) to = kFine + min(kCoarse - 1, d - kFine + (top >> 3) - (mt >> 3));
-        else if (to >= kFine) to = count ? coarse_of(mt - d, top) : -1;
-        if (to < 0) far += n;
-        else if (n) atomicAdd(&numbers[to], n);
+      for (int k = 0; k < kStep; ++k) {
+        const int d = d0 + 4 * k * lanes;
+        if (d + down + 3 < kFine && d + 3 < kFine) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) atomicAdd(&numbers[d + down + c], n4[k][c]);
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const uint32_t n = n4[k][c];
+            int to = d + c + down;
+            if (d >= kFine) to = kFine + min(kCoarse - 1, d + c - kFine + (top >> 3) - (mt >> 3));
+            else if (to >= kFine) to = count ? coarse_of(mt - d - c, top) : -1;
+            if (to < 0) far += n;
+            else if (n) atomicAdd(&numbers[to], n);
+          }
+        }
       }
     }
   }
@@ -460,9 +469,9 @@ __global__ __launch_bounds__(kThreads) void sample_bounds_kernel(SampleArgs p, W
     mine_n += n[k];
   }
   double all;
-  const double before = scan<kWaves, double>(mine, red, all) - mine;
+  const double before = grp.scan<kWaves, double>(mine, all) - mine;   // to a few steps of the sum
   if (count) {
-    uint32_t all_n, at = scan<kWaves, uint32_t>(mine_n, (uint32_t*)red, all_n) - mine_n;
+    uint32_t all_n, at = grp.scan<kWaves, uint32_t>(mine_n, all_n) - mine_n;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       if (at < (uint32_t)st.top_k && at + n[k] >= (uint32_t)st.top_k) cell = b0 + k;   // one thread
@@ -477,19 +486,18 @@ __global__ __launch_bounds__(kThreads) void sample_bounds_kernel(SampleArgs p, W
     // with the scale); coarse ones to 7 / 128 of a factor of two; what lies under the fine cells from nothing to
     // 2^-28 a token; of cell_k some part.
     const double e = 2.8e-3 + fabs((double)top) * 0x1p-28, share = fmax(st.top_p, 0.0);
-    const double slack = count ? 0.045 * add_up<kWaves, double>(low, red) : far_of * 0x1p-28;
+    const double slack = count ? 0.045 * grp.sum<kWaves, double>(low) : far_of * 0x1p-28;
     double upto = all, in_k = 0;
     if (cell_k < cells) {
       double run = before;
-      __syncthreads();
 #pragma unroll
       for (int k = 0; k < N; ++k) {
         run += wt[k];
-        if (b0 + k == cell_k && k < per) red[0] = run, red[1] = wt[k];
+        if (b0 + k == cell_k && k < per) at_k[0] = run, at_k[1] = wt[k];
       }
       __syncthreads();
-      upto = red[0];
-      in_k = red[1];
+      upto = at_k[0];
+      in_k = at_k[1];
     }
     const double lo = (upto - in_k) * (1 - e), hi = upto * (1 + e) + slack;   // of what top_p is a share of
     double run = before;
@@ -504,8 +512,8 @@ __global__ __launch_bounds__(kThreads) void sample_bounds_kernel(SampleArgs p, W
         if (run * (1 - e) >= share * hi || rest * (1 + e) + slack <= (1 - share) * upto * (1 - e)) must = min(must, (ull)b);
       }
     }
-    cell_p1 = (int)least_of<kWaves>(must, (ull*)red);
-    cell_p0 = (int)least_of<kWaves>(may, (ull*)red);
+    cell_p1 = (int)grp.least<kWaves, ull>(must);
+    cell_p0 = (int)grp.least<kWaves, ull>(may);
   }
   if (tid) return;
   auto lower = [&](int c) { return c < kFine ? top - c : 8 * ((top >> 3) - (c - kFine)); };   // smallest g of a cell
@@ -523,7 +531,9 @@ __global__ __launch_bounds__(kThreads) void sample_bounds_kernel(SampleArgs p, W
 }
 
 template <typename E> __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleArgs p, Work ws) {
-  __shared__ double table[64], red[kWaves];
+  __shared__ double table[64];
+  __shared__ ull lds[2 * kWaves];
+  Group grp{lds};
   __shared__ uint32_t places;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int r = blockIdx.x / ws.parts, part = blockIdx.x - r * ws.parts, row = ws.row0 + r;
@@ -538,19 +548,20 @@ template <typename E> __global__ __launch_bounds__(kThreads) void sample_gather_
   const Weights weight{table, steps_of(st.inv_t), M};
   const Row<E> x(p, row);
   const int s0 = ws.first_sub(part) + w, s1 = ws.first_sub(part + 1);
-  double* sub = ws.sub + (int64_t)r * ws.subs;
+  ull* sub = ws.sub + (int64_t)r * ws.subs;
   float v[16];
+  const double one = ws.one;
   if (st.kind == kFloor) {
     // weights under min_p, as logits, with a margin for the division by T
-    const double span = (log(st.min_p) - 1e-9) / st.inv_t, low = (double)M + span - 1e-9 * fabs(span);
+    const double span = (log(st.min_p) - 1e-9) / st.inv_t, low = st.min_p > 0 ? (double)M + span - 1e-9 * fabs(span) : -INFINITY;
     for (int s = s0; s < s1; s += kWaves) {
       x.load(s, v);
-      double sum = 0;
+      ull sum = 0;
 #pragma unroll 4
       for (int j = 0; j < 16; ++j)
         if (v[j] == M || (double)v[j] >= low) {
           const double wt = weight(v[j]);
-          sum += wt >= st.min_p ? wt : 0.0;
+          sum += whole(wt >= st.min_p ? wt : 0.0, one);
         }
       sum = wave_sum(sum);
       if (lane == 0) sub[s] = sum;
@@ -562,6 +573,7 @@ template <typename E> __global__ __launch_bounds__(kThreads) void sample_gather_
   const float sure = b.sure();
   uint32_t* list = ws.list + ((int64_t)r * ws.parts + part) * ws.places;
   double over_k = 0, over_p = 0;
+  ull kept_all = 0;
   uint32_t over_n = 0;
   auto enlist = [&](int s, uint32_t take) {   // bit j: the lane's j-th token
     while (take) {
@@ -574,17 +586,17 @@ template <typename E> __global__ __launch_bounds__(kThreads) void sample_gather_
   if (!cut_k && st.min_p == 0) {   // top_p alone
     for (int s = s0; s < s1; s += kWaves) {
       x.load(s, v);
-      double kept = 0;
+      ull kept = 0;
       uint32_t take = 0;
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         const double wt = weight(v[j]);
         const bool stays = v[j] >= sure;
         over_k += wt;
-        kept += stays ? wt : 0.0;
+        kept += stays ? whole(wt, one) : 0;
         take |= (!stays & (v[j] >= b.p_lo) & (v[j] > -INFINITY)) << j;
       }
-      over_p += kept;
+      kept_all += kept;
       kept = wave_sum(kept);
       if (lane == 0) sub[s] = kept;
       enlist(s, take);
@@ -594,7 +606,7 @@ template <typename E> __global__ __launch_bounds__(kThreads) void sample_gather_
     const float least = cut_k ? (cut_p ? fminf(b.k_lo, b.p_lo) : b.k_lo) : -INFINITY;
     for (int s = s0; s < s1; s += kWaves) {
       x.load(s, v);
-      double kept = 0;
+      ull kept = 0;
       uint32_t take = 0;
 #pragma unroll 4
       for (int j = 0; j < 16; ++j) {
@@ -607,16 +619,17 @@ template <typename E> __global__ __launch_bounds__(kThreads) void sample_gather_
         over_n += of_k;
         const double stays = v[j] >= sure ? wt : 0.0;
         over_p += stays;
-        kept += stays >= st.min_p ? stays : 0.0;
+        kept += whole(stays >= st.min_p ? stays : 0.0, one);
       }
       kept = wave_sum(kept);
       if (lane == 0) sub[s] = kept;
       enlist(s, take);
     }
   }
-  over_k = add_up<kWaves, double>(over_k, red);
-  over_p = add_up<kWaves, double>(over_p, red);
-  const ull n = add_up<kWaves, ull>(over_n, (ull*)red);
+  over_p += (double)kept_all * (one * 0x1p-52);
+  over_k = grp.sum<kWaves, double>(over_k);
+  over_p = grp.sum<kWaves, double>(over_p);
+  const ull n = grp.sum<kWaves, ull>(over_n);
   if (tid == 0) {
     Part& out = parts[part];
     out.listed = places;
@@ -628,7 +641,7 @@ template <typename E> __global__ __launch_bounds__(kThreads) void sample_gather_
 
 struct LongWay {
   uint32_t cnt[2048];
-  ull wt[2048], red[kWaves];
+  ull wt[2048];
   struct {
     uint32_t bin;
     ull above_n, above_w;
@@ -643,16 +656,15 @@ __device__ __forceinline__ void tell(const SampleArgs& p, int row, int token, do
   if (p.logprob) p.logprob[row] = (float)log_share;
 }
 template <typename E>
-__device__ __forceinline__ void long_way(const SampleArgs& p, int row, const Settings& st, const Weights& weigh, LongWay& sh) {
+__device__ __forceinline__ void long_way(const SampleArgs& p, int row, const Settings& st, const Weights& weigh, double one, LongWay& sh, Group& grp) {
   uint32_t* const cnt = sh.cnt;
-  ull *const wt = sh.wt, *const red = sh.red;
+  ull* const wt = sh.wt;
   auto& found = sh.found;
   const int tid = threadIdx.x, V = p.vocab;
   const E* x = (const E*)p.logits + (int64_t)row * p.ld;
-  const int spare = max(14 - __clz(V), 0);   // sums of V weights below 2^63
   auto key = [&](int i) { return order_of((float)x[i]); };
   auto real = [&](uint32_t k) { return weigh(value_of(k)); };
-  auto whole = [&](uint32_t k) { return mq::whole(real(k)) >> spare; };
+  auto whole = [&](uint32_t k) { return mq::whole(real(k), one); };
 
   // The key in whose group the n-th token (by_count) or the weight n lies, as
   // counted from the largest; how many tokens and how much weight come before the
@@ -681,8 +693,8 @@ __device__ __forceinline__ void long_way(const SampleArgs& p, int row, const Set
       const int d0 = 2047 - 2 * tid, d1 = d0 - 1;
       const ull c0 = cnt[d0], c1 = cnt[d1], w0 = wt[d0], w1 = wt[d1];
       ull all;
-      const ull cs = scan<kWaves, ull>(c0 + c1, red, all) - c0 - c1 + c.before_n, end_n = all + c.before_n;
-      const ull ws = scan<kWaves, ull>(w0 + w1, red, all) - w0 - w1 + c.before_w, end_w = all + c.before_w;
+      const ull cs = grp.scan<kWaves, ull>(c0 + c1, all) - c0 - c1 + c.before_n, end_n = all + c.before_n;
+      const ull ws = grp.scan<kWaves, ull>(w0 + w1, all) - w0 - w1 + c.before_w, end_w = all + c.before_w;
       const ull aim = by_count ? min(n, end_n) : min(n, end_w);   // some group reaches it
       auto mine = [&](ull bn, ull bw, ull dn, ull dw) {
         const ull b = by_count ? bn : bw, d = by_count ? dn : dw;
@@ -722,7 +734,7 @@ __device__ __forceinline__ void long_way(const SampleArgs& p, int row, const Set
       ull sum = 0;
       for (int i = tid; i < V; i += kThreads)
         if (const uint32_t k = key(i); k > kNone) sum += whole(k);
-      scan<kWaves, ull>(sum, red, kept_w);
+      grp.scan<kWaves, ull>(sum, kept_w);
     }
     const ull aim = max((ull)1, (ull)ceil(fmax(st.top_p, 0.0) * (double)kept_w));
     const Cut c = find(false, aim);
@@ -739,7 +751,7 @@ __device__ __forceinline__ void long_way(const SampleArgs& p, int row, const Set
       const int i = i0 + tid;
       const bool tie = i < V && key(i) == at;
       ull all;
-      const ull r = scan<kWaves, ull>(tie, red, all) + seen;
+      const ull r = grp.scan<kWaves, ull>(tie, all) + seen;
       if (tie && r == ties) found.bin = i;
       seen += all;
       if (seen >= ties) break;
@@ -747,38 +759,30 @@ __device__ __forceinline__ void long_way(const SampleArgs& p, int row, const Set
     __syncthreads();
     last = (int)found.bin;
   }
-  auto weight = [&](int i) {
+  auto weight = [&](int i) -> ull {
     const uint32_t k = key(i);
-    if (k <= kNone || (cut && (k < at || (k == at && i > last)))) return 0.0;
-    const double w = real(k);
-    return w >= st.min_p ? w : 0.0;
+    if (k <= kNone || (cut && (k < at || (k == at && i > last))) || real(k) < st.min_p) return 0;
+    return whole(k);
   };
-  double sum = 0;
+  ull sum = 0, total;
   for (int i = tid; i < V; i += kThreads) sum += weight(i);
-  const double total = add_up<kWaves, double>(sum, (double*)red), aim = (double)st.u * total;
-  double before = 0;
+  total = grp.sum<kWaves, ull>(sum);
+  const ull aim = share_of(st.u, total);
+  ull before = 0;
   for (int i0 = 0; i0 < V; i0 += kThreads) {
     const int i = i0 + tid;
-    const double w = i < V ? weight(i) : 0;
-    double all;
-    const double r = scan<kWaves, double>(w, (double*)red, all) + before;
-    // what rounding leaves under the aim at the row's end goes to the last token
-    const ull pick = w > 0 && r > aim ? (ull)i : ~0ull, best = least_of<kWaves>(pick, red);
-    const ull back = most_of<kWaves>(w > 0 ? (ull)i + 1 : 0, red);
-    if (back) sh.found.bin = (uint32_t)back - 1;
-    if (best != ~0ull) {
-      sh.found.bin = (uint32_t)best;
-      break;
-    }
+    const ull w = i < V ? weight(i) : 0;
+    ull all;
+    const ull r = grp.scan<kWaves, ull>(w, all) + before;
+    if (w && r > aim && r - w <= aim) tell(p, row, i, log(real(key(i)) / ((double)total * (one * 0x1p-52))));
     before += all;
+    if (before > aim) break;
   }
-  __syncthreads();
-  if (tid == 0) tell(p, row, (int)sh.found.bin, log(weigh((float)x[sh.found.bin]) / total));
 }
 
-// ---- the last launch: a workgroup for each row, of which four waves do the work
-// (their barriers are short) unless the row goes the long way ----
-constexpr int kNear = 4, kNearThreads = 64 * kNear;
+// ---- the last launch: a workgroup for each row, of which eight waves do the work
+// (their barriers are shorter) unless the row goes the long way ----
+constexpr int kNear = 8, kNearThreads = 64 * kNear;
 constexpr int kFewRoom = 1024;   // places for the tokens of kFew that are as large as the top_k-th largest of the lanes'
 
 struct List {
@@ -786,74 +790,81 @@ struct List {
   ull units[kListRow];                     // weights in kListUnit
 };
 
+// How many of n numbers (a zero behind them) are larger than mine
+__device__ __forceinline__ uint32_t rank_of(ull mine, const ull* of, int n) {
+  typedef ull ull2 __attribute__((ext_vector_type(2)));
+  uint32_t rank = 0;
+#pragma unroll 4
+  for (int i = 0; i < (n + 1) / 2; ++i) {
+    const ull2 q = ((const ull2*)of)[i];
+    rank += (q[0] > mine) + (q[1] > mine);
+  }
+  return rank;
+}
+
 // Of the entries that are true to `of`, the n-th largest key, among `bits` of them
 // under a common head; one barrier a bit
 template <typename F>
-__device__ __forceinline__ uint32_t nth_key(int held, uint32_t n, uint32_t head, int bits, const uint32_t* key, uint32_t* lds, int& turn, F&& of) {
+__device__ __forceinline__ uint32_t nth_key(int held, uint32_t n, uint32_t head, int bits, const uint32_t* key, Group& grp, F&& of) {
   uint32_t least = head;
 #pragma unroll 1
   for (int bit = bits - 1; bit >= 0; --bit) {
     const uint32_t t = least | 1u << bit;
     uint32_t c = 0;
     for (int i = threadIdx.x; i < (held + 63 & ~63); i += kNearThreads) c += __popcll(__ballot(i < held && key[i] >= t && of(i)));
-    if (count_up<kNear>(c, lds, turn) >= n) least = t;
+    if (grp.sum_of_waves<kNear>(c) >= n) least = t;
   }
   return least;
 }
-template <typename F> __device__ __forceinline__ uint32_t number_of(int held, uint32_t* lds, int& turn, F&& of) {
+template <typename F> __device__ __forceinline__ uint32_t number_of(int held, Group& grp, F&& of) {
   uint32_t c = 0;
   for (int i = threadIdx.x; i < (held + 63 & ~63); i += kNearThreads) c += __popcll(__ballot(i < held && of(i)));
-  return count_up<kNear>(c, lds, turn);
+  return grp.sum_of_waves<kNear>(c);
 }
 // The n-th smallest index of them
 template <typename F>
-__device__ __forceinline__ uint32_t nth_index(int held, uint32_t n, int vocab, const uint32_t* idx, uint32_t* lds, int& turn, F&& of) {
+__device__ __forceinline__ uint32_t nth_index(int held, uint32_t n, int vocab, const uint32_t* idx, Group& grp, F&& of) {
   uint32_t most = 0;   // fewer than n lie under it
 #pragma unroll 1
   for (int bit = 31 - __clz(vocab); bit >= 0; --bit) {
     const uint32_t t = most | 1u << bit;
-    if (number_of(held, lds, turn, [&](int i) { return of(i) && idx[i] < t; }) < n) most = t;
+    if (number_of(held, grp, [&](int i) { return of(i) && idx[i] < t; }) < n) most = t;
   }
   return most;
 }
 
 struct PickShared {
-  double table[64], red[kWaves];
-  uint2 count2[2 * kWaves];
-  uint32_t count[2 * kWaves], place, spots, at[kPartsMost + 1];
+  double table[64];
+  ull before, lds[2 * kWaves];
+  uint32_t place, spots, at[kPartsMost + 1];
+  uint32_t cut[2];
   union {
     LongWay far;
     List list;
     struct {
       uint32_t lane[kFewRoom];
-      ull key[kFewRoom];   // order_of and the index turned round: a larger one comes first
+      alignas(16) ull key[kFewRoom + 1];   // order_of and the index turned round: a larger one comes first
       ull sorted[kFewMost];
+      alignas(16) ull idx[kFewMost + 1];
       double w[kFewMost];
     } few;
   };
 };
 
 // The largest t that n of the threads' keys reach, two bits a barrier
-__device__ __forceinline__ uint32_t reached_by(uint32_t key, uint32_t n, double* red, uint2* count) {
-  const ull both = reduce<kWaves, ull>((ull)key << 32 | ~key, (ull*)red, [](ull a, ull b) { return a & b; });
+__device__ __forceinline__ uint32_t reached_by(uint32_t key, uint32_t n, Group& grp) {
+  const ull both = grp.reduce<kWaves, ull>((ull)key << 32 | ~key, [](ull a, ull b) { return a & b; });
   const uint32_t same = (uint32_t)(both >> 32) | (uint32_t)both;   // bits that all keys share
-  int bit = same == ~0u ? 0 : 32 - __clz(~same), turn = 0;
+  int bit = same == ~0u ? 0 : 32 - __clz(~same);
   bit += bit & 1;
   uint32_t t = bit >= 32 ? 0 : (uint32_t)(both >> 32) >> bit << bit;
   for (bit -= 2; bit >= 0; bit -= 2) {
-    const uint32_t c1 = __popcll(__ballot(key >= (t | 1u << bit))), c2 = __popcll(__ballot(key >= (t | 2u << bit))),
-                   c3 = __popcll(__ballot(key >= (t | 3u << bit)));
-    turn ^= kWaves;
-    if ((threadIdx.x & 63) == 0) count[turn + (threadIdx.x >> 6)] = {c1 | c2 << 16, c3};
-    __syncthreads();
-    uint32_t s12 = 0, s3 = 0;
+    const ull c1 = __popcll(__ballot(key >= (t | 1u << bit))), c2 = __popcll(__ballot(key >= (t | 2u << bit))),
+              c3 = __popcll(__ballot(key >= (t | 3u << bit)));
+    ull c = grp.of_waves<kWaves>(c1 | c2 << 16 | c3 << 32);
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-      const uint2 c = count[turn + i];
-      s12 += c.x;
-      s3 += c.y;
-    }
-    t |= (s3 >= n ? 3u : (s12 >> 16 >= n ? 2u : ((s12 & 0xffff) >= n ? 1u : 0u))) << bit;
+    for (int o = 1; o < kWaves; o <<= 1) c += from_lane(c, o);
+    t |= ((uint32_t)(c >> 32) >= n ? 3u : ((uint32_t)(c >> 16 & 0xffff) >= n ? 2u : ((uint32_t)(c & 0xffff) >= n ? 1u : 0u))) << bit;
   }
   return t;
 }
@@ -861,15 +872,11 @@ __device__ __forceinline__ uint32_t reached_by(uint32_t key, uint32_t n, double*
 // True, on all threads, where the row has to go the long way.
 template <typename E>
 __device__ __forceinline__ bool pick(const SampleArgs& p, const Work& ws, const Settings& st, const Weights& weight, PickShared& sh,
-                                     ull* sub_units) {
-  double* const red = sh.red;
-  uint32_t* const count = sh.count;
+                                     Group& grp, ull* sub_units) {
   const int tid = threadIdx.x, row = ws.row0 + blockIdx.x, r = blockIdx.x, V = p.vocab;
   const Part* parts = ws.part + (int64_t)r * ws.parts;
   const Row<E> x(p, row);
   constexpr int LOW = kLow<E>;
-  const double aim_share = (double)st.u;
-  int turn = 0;
 
   if (st.kind == kFew) {
     // At least top_k threads hold a token as large as the top_k-th largest of what
@@ -889,7 +896,7 @@ __device__ __forceinline__ bool pick(const SampleArgs& p, const Work& ws, const 
       for (int k = 0; k < kStep; ++k) mine_most = fmaxf(mine_most, m[k]);
     }
     const uint32_t mine_key = order_of(mine_most) >> LOW;
-    const uint32_t least = reached_by(mine_key, st.top_k, red, sh.count2);
+    const uint32_t least = reached_by(mine_key, st.top_k, grp);
     if (mine_key >= least) {
       auto take = [&](int i, float v) {
         if (const uint32_t k = order_of(v); k >> LOW >= least && k > kNone)
@@ -912,10 +919,11 @@ __device__ __forceinline__ bool pick(const SampleArgs& p, const Work& ws, const 
     if (n > kFewRoom || held > kFewRoom) return true;
     // the first top_k of them in their order
     const uint32_t k = min((uint32_t)st.top_k, held);
+    if (tid == 0) sh.few.key[held] = 0;
+    __syncthreads();
     if (tid < (int)held) {
       const ull mine = sh.few.key[tid];
-      uint32_t rank = 0;
-      for (uint32_t i = 0; i < held; ++i) rank += sh.few.key[i] > mine;
+      const uint32_t rank = rank_of(mine, sh.few.key, held);
       if (rank < k) sh.few.sorted[rank] = mine;
     }
     __syncthreads();
@@ -925,24 +933,25 @@ __device__ __forceinline__ bool pick(const SampleArgs& p, const Work& ws, const 
       const ull mine = sh.few.sorted[tid];
       idx = ~(uint32_t)mine;
       w = weight(value_of((uint32_t)(mine >> 32)));
+      sh.few.idx[tid] = ~idx;   // larger for the first
     }
+    if (tid == (int)k) sh.few.idx[k] = 0;
     double sum;
-    const double before = scan<kWaves, double>(w, red, sum) - w;
+    const double before = grp.scan<kWaves, double>(w, sum) - w;
     if (st.top_p < 1.0 && tid > 0 && !(before < st.top_p * sum)) w = 0;
     if (w < st.min_p) w = 0;
-    if (tid < (int)k) sh.few.w[tid] = w;
-    __syncthreads();
-    double upto = 0, total = 0;
+    // now by index
     if (tid < (int)k) {
-      for (uint32_t i = 0; i < k; ++i) {
-        const double t = sh.few.w[i];
-        total += t;
-        upto += ~(uint32_t)sh.few.sorted[i] <= idx ? t : 0.0;
-      }
+      const uint32_t rank = rank_of((uint32_t)~idx, sh.few.idx, k);
+      sh.few.w[rank] = w;
+      sh.few.key[rank] = idx;
     }
-    // (the last one's sum is the total, which the aim is less than)
-    const ull first = least_of<kWaves>(w > 0 && upto > aim_share * total ? (ull)idx << 32 | tid : ~0ull, (ull*)red);
-    if (tid == (int)(uint32_t)first) tell(p, row, (int)idx, log(w / total));
+    __syncthreads();
+    w = tid < (int)k ? sh.few.w[tid] : 0;
+    const ull units = whole_of_list(w);
+    ull total;
+    const ull upto = grp.scan<kWaves, ull>(units, total), aim = share_of(st.u, total);
+    if (upto > aim && upto - units <= aim) tell(p, row, (int)sh.few.key[tid], log(w / ((double)total * kListUnit)));
     return false;
   }
 
@@ -1016,12 +1025,12 @@ __device__ __forceinline__ bool pick(const SampleArgs& p, const Work& ws, const 
       in_p += of_p(i) ? units : 0;
     }
     if (cut_k) {
-      n = add_up<kWaves, ull>(n, (ull*)red);
-      in_k = add_up<kWaves, ull>(in_k, (ull*)red);
+      n = grp.sum<kWaves, ull>(n);
+      in_k = grp.sum<kWaves, ull>(in_k);
       if (!(over_n < (uint32_t)st.top_k && over_n + n >= (uint32_t)st.top_k)) return true;
     }
     if (cut_p) {
-      in_p = add_up<kWaves, ull>(in_p, (ull*)red);
+      in_p = grp.sum<kWaves, ull>(in_p);
       const double lo = st.top_p * over_k, hi = st.top_p * (over_k + kListUnit * (double)in_k);
       // a window that ends with the tokens that top_k may leave needs no lower end of its own
       if (!((over_p < lo || over_p == 0) && (over_p + kListUnit * (double)in_p >= hi || (cut_k && b.p_lo <= b.k_lo)))) return true;
@@ -1029,25 +1038,62 @@ __device__ __forceinline__ bool pick(const SampleArgs& p, const Work& ws, const 
   }
   if (tid >= kNearThreads) return false;
 
-  if (cut_k || cut_p) {
+  if ((cut_k || cut_p) && held < kNearThreads) {
+    // in their order, one to a thread: what stays is a first part of them
+    ull *const all = sh.list.units + 1024, *const order = all + 1024, *const units = order + 1024;
+    const ull mine = tid < (int)held ? (ull)key[tid] << 32 | (uint32_t)~index[tid] : 0;
+    all[tid] = mine;   // and at least one zero
+    if (tid == 0) sh.cut[0] = ~0u, sh.cut[1] = 0;   // none
+    __syncthreads();
+    if (tid < (int)held) {
+      const uint32_t rank = rank_of(mine, all, held);
+      order[rank] = mine;
+      units[rank] = sh.list.units[tid];
+    }
+    __syncthreads();
+    const ull own = tid < (int)held ? order[tid] : 0, unit = tid < (int)held ? units[tid] : 0;
+    const float v = value((uint32_t)(own >> 32));
+    const bool in_k = own && cut_k && v >= b.k_lo && v < b.k_hi, in_p = own && cut_p && v >= b.p_lo && v < b.p_hi;
+    bool stay = own != 0;
+    double sum = over_k;
+    if (cut_k) {
+      uint32_t n;
+      const uint32_t at = grp.scan<kNear, uint32_t>(in_k, n);
+      const bool first = in_k && at <= st.top_k - over_n;
+      sum += kListUnit * (double)grp.sum<kNear, ull>(first ? unit : 0);
+      stay &= first || v >= b.k_hi;
+    }
+    if (cut_p) {
+      ull n;
+      const ull at = grp.scan<kNear, ull>(in_p ? unit : 0, n);
+      stay &= in_p && over_p + kListUnit * (double)(at - unit) < fmax(st.top_p * sum, 0x1p-1000);   // the first token stays
+    }
+    const uint32_t n = grp.sum_of_waves<kNear>(__popcll(__ballot(stay)));
+    if (tid == (int)n - 1) {
+      sh.cut[0] = (uint32_t)(own >> 32);
+      sh.cut[1] = ~(uint32_t)own;
+    }
+    __syncthreads();
+    by_k = {sh.cut[0], sh.cut[1]};
+  } else if (cut_k || cut_p) {
     // the keys' common head
     uint32_t ones = ~0u, zeros = ~0u;
     for (int i = tid; i < (int)held; i += kNearThreads) ones &= key[i], zeros &= ~key[i];
-    const ull both = reduce<kNear, ull>((ull)ones << 32 | zeros, (ull*)red, [](ull a, ull b) { return a & b; });
+    const ull both = grp.reduce<kNear, ull>((ull)ones << 32 | zeros, [](ull a, ull b) { return a & b; });
     const uint32_t same = (uint32_t)(both >> 32) | (uint32_t)both;
     const int bits = same == ~0u ? 0 : 32 - __clz(~same);
     const uint32_t head = bits == 32 ? 0 : (uint32_t)(both >> 32) >> bits << bits;
     double sum = over_k;
     if (cut_k) {
       const uint32_t n = st.top_k - over_n;
-      by_k.key = nth_key(held, n, head, bits, key, count, turn, of_k);
-      const uint32_t over = number_of(held, count, turn, [&](int i) { return key[i] > by_k.key && of_k(i); });
+      by_k.key = nth_key(held, n, head, bits, key, grp, of_k);
+      const uint32_t over = number_of(held, grp, [&](int i) { return key[i] > by_k.key && of_k(i); });
       auto tie = [&](int i) { return key[i] == by_k.key; };
-      if (number_of(held, count, turn, tie) > n - over) by_k.idx = nth_index(held, n - over, V, index, count, turn, tie);
+      if (number_of(held, grp, tie) > n - over) by_k.idx = nth_index(held, n - over, V, index, grp, tie);
       ull mine = 0;
       for (int i = tid; i < (int)held; i += kNearThreads)
         if (of_k(i) && by_k.keeps(key[i], index[i])) mine += sh.list.units[i];
-      sum += kListUnit * (double)add_up<kNear, ull>(mine, (ull*)red);
+      sum += kListUnit * (double)grp.sum<kNear, ull>(mine);
     }
     if (cut_p) {
       const double aim = fmax(st.top_p * sum, 0x1p-1000);   // the first token stays
@@ -1055,7 +1101,7 @@ __device__ __forceinline__ bool pick(const SampleArgs& p, const Work& ws, const 
         ull mine = 0;
         for (int i = tid; i < (int)held; i += kNearThreads)
           if (key[i] > t && of_p(i)) mine += sh.list.units[i];
-        return over_p + kListUnit * (double)add_up<kNear, ull>(mine, (ull*)red);
+        return over_p + kListUnit * (double)grp.sum<kNear, ull>(mine);
       };
       // the smallest key before which the aim is not reached: tokens of it stay
       uint32_t t = head | (bits == 32 ? ~0u : (1u << bits) - 1);
@@ -1064,10 +1110,10 @@ __device__ __forceinline__ bool pick(const SampleArgs& p, const Work& ws, const 
         if (over(t & ~(1u << bit)) < aim) t &= ~(1u << bit);
       by_p.key = t;
       auto tie = [&](int i) { return key[i] == t; };
-      const uint32_t ties = number_of(held, count, turn, tie);
+      const uint32_t ties = number_of(held, grp, tie);
       if (ties > 0) {
         const double n = fmax(ceil((aim - over(t)) / weight(value(t))), 1.0);
-        if (n < (double)ties) by_p.idx = nth_index(held, (uint32_t)n, V, index, count, turn, tie);
+        if (n < (double)ties) by_p.idx = nth_index(held, (uint32_t)n, V, index, grp, tie);
       }
     }
   }
@@ -1075,52 +1121,35 @@ __device__ __forceinline__ bool pick(const SampleArgs& p, const Work& ws, const 
   auto stays = [&](uint32_t k, uint32_t i) { return by_k.keeps(k, i) & by_p.keeps(k, i); };
 
   // ---- the sub ----
-  const double* sub = ws.sub + (int64_t)r * ws.subs;
-  for (int s = tid; s < ws.subs; s += kNearThreads) sub_units[s] = 0;
+  const ull* sub = ws.sub + (int64_t)r * ws.subs;
+  for (int s = tid; s < ws.subs; s += kNearThreads) sub_units[s] = sub[s];
   __syncthreads();
   const float sure = b.sure();
+  const double one = ws.one;
   for (int i = tid; i < (int)held; i += kNearThreads)
     if (stays(key[i], index[i])) {
       const double w = weight(value(key[i]));
-      if (w >= st.min_p) atomicAdd(&sub_units[index[i] / kSub], sh.list.units[i]);
+      if (w >= st.min_p) atomicAdd(&sub_units[index[i] / kSub], whole(w, one));
     }
   __syncthreads();
-  const int per = (ws.subs + kNearThreads - 1) / kNearThreads, f0 = tid * per;
-  auto sum_of = [&](int s) {
-    if (st.kind != kAll) return sub[s] + kListUnit * (double)sub_units[s];
-    const float m = parts[s / ws.part_subs].top;
-    return m == -INFINITY ? 0.0 : sub[s] * weight(m);
-  };
-  double mine = 0;
-  for (int s = f0; s < min(f0 + per, ws.subs); ++s) mine += sum_of(s);
-  double total;
-  double before = scan<kNear, double>(mine, red, total) - mine;
-  const double aim = aim_share * total;
-  ull found = ~0ull, back = 0;
-  double found_before = 0, back_before = 0;
-  for (int s = f0; s < min(f0 + per, ws.subs); ++s) {
-    const double w = sum_of(s);
-    if (w > 0) {
-      back = s + 1;
-      back_before = before;
-      if (found == ~0ull && before + w > aim) {
-        found = s;
-        found_before = before;
-      }
-    }
-    before += w;
+  const int per = (ws.subs + kNearThreads - 1) / kNearThreads, f0 = tid * per, f1 = min(f0 + per, ws.subs);
+  ull mine = 0, total;
+  for (int s = f0; s < f1; ++s) mine += sub_units[s];
+  ull before = grp.scan<kNear, ull>(mine, total) - mine;
+  const ull aim = share_of(st.u, total);
+  if (before <= aim && before + mine > aim) {   // one thread
+    int s = f0;
+    for (; before + sub_units[s] <= aim; ++s) before += sub_units[s];
+    sh.cut[0] = s;
+    sh.before = before;
   }
-  const ull first = least_of<kNear>(found, (ull*)red), end = most_of<kNear>(back, (ull*)red);
-  const int s = first != ~0ull ? (int)first : (int)end - 1;   // rounding may leave the sum under its aim
   __syncthreads();
-  if (first != ~0ull ? found == first : back == end) red[0] = first != ~0ull ? found_before : back_before;
-  __syncthreads();
-  const double left = aim - red[0];
-  __syncthreads();
+  const int s = (int)sh.cut[0];
+  const ull left = aim - sh.before;
 
-  // ---- the token: four in a row to a thread ----
+  // ---- the token: some in a row to a thread ----
   constexpr int kIn = kSub / kNearThreads;
-  double w[kIn], sums = 0;
+  ull w[kIn], sums = 0;
   const int i0 = s * kSub + tid * kIn;
 #pragma unroll
   for (int j = 0; j < kIn; ++j) {
@@ -1128,22 +1157,15 @@ __device__ __forceinline__ bool pick(const SampleArgs& p, const Work& ws, const 
     const float v = i < V ? (float)x.x[i] : -INFINITY;
     const double t = weight(v);
     // without branches: with them this compiler loses the zeros of all but the first
-    w[j] = (t >= st.min_p) & ((v >= sure) | stays(order_of(v) >> LOW, i)) ? t : 0.0;
+    w[j] = whole((t >= st.min_p) & ((v >= sure) | stays(order_of(v) >> LOW, i)) ? t : 0.0, one);
     sums += w[j];
   }
-  double all, upto = scan<kNear, double>(sums, red, all) - sums;
-  ull hit = ~0ull, stop = 0;
+  ull all, upto = grp.scan<kNear, ull>(sums, all) - sums;
 #pragma unroll
   for (int j = 0; j < kIn; ++j) {
+    if (upto <= left && upto + w[j] > left) tell(p, row, i0 + j, log(weight((float)x.x[i0 + j]) / ((double)total * (one * 0x1p-52))));
     upto += w[j];
-    if (w[j] > 0) {
-      stop = tid * kIn + j + 1;
-      if (hit == ~0ull && upto > left) hit = tid * kIn + j;
-    }
   }
-  const ull one = least_of<kNear>(hit, (ull*)red), last = most_of<kNear>(stop, (ull*)red);
-  const int at = one != ~0ull ? (int)one : (int)last - 1;
-  if (at >= 0 && at / kIn == tid) tell(p, row, s * kSub + at, log(weight((float)x.x[s * kSub + at]) / total));
   return false;
 }
 
@@ -1167,9 +1189,10 @@ template <typename E> __global__ __launch_bounds__(kThreads) void sample_pick_ke
   if (tid == 0) sh.place = sh.spots = 0;
   __syncthreads();
   const Weights weight{sh.table, steps_of(st.inv_t), M};
-  if (pick<E>(p, ws, st, weight, sh, sub_units)) {
+  Group grp{sh.lds};
+  if (pick<E>(p, ws, st, weight, sh, grp, sub_units)) {
     __syncthreads();
-    long_way<E>(p, row, st, weight, sh.far);
+    long_way<E>(p, row, st, weight, ws.one, sh.far, grp);
   }
 }
 
@@ -1199,8 +1222,7 @@ Plan plan_of(const SampleArgs& a, int num_cus) {
   pl.few = std::min(kFewMost, 32 * pl.subs);
   const bool greedy = !a.temperatures && !(a.temperature > 0.f);
   const bool cuts = a.top_ks || (a.top_k > pl.few && a.top_k < a.vocab);                       // by number, with a grid
-  const bool shares = !(!a.top_ks && a.top_k >= 1 && a.top_k <= pl.few) && (a.top_ps || a.min_ps || a.top_p < 1.f || a.min_p > 0.f);
-  pl.gather = !greedy && (cuts || shares);
+  pl.gather = !greedy && (a.top_ks || a.top_k <= 0 || a.top_k > pl.few);
   pl.grid = (!greedy && cuts) || (pl.gather && (a.top_ps || a.top_p < 1.f));
   const bool some = !greedy && (a.top_ks || (a.top_k > 1 && a.top_k <= pl.few));               // kFew
   size_t at = 0;
@@ -1212,7 +1234,7 @@ Plan plan_of(const SampleArgs& a, int num_cus) {
   const size_t rp = (size_t)pl.rows * pl.parts;
   pl.part_at = take(rp * sizeof(Part));
   pl.bounds_at = take(pl.rows * sizeof(Bounds));
-  pl.sub_at = take((size_t)pl.rows * pl.subs * sizeof(double));
+  pl.sub_at = take((size_t)pl.rows * pl.subs * sizeof(ull));
   pl.most_at = take(some ? (size_t)pl.rows * pl.subs * 64 * sizeof(float) : 0);
   pl.list_at = take(pl.gather ? rp * pl.places * sizeof(uint32_t) : 0);
   pl.cells_at = take(pl.grid ? rp * kCells * sizeof(uint32_t) : 0);
@@ -1224,13 +1246,15 @@ template <typename E> hipError_t launch(const SampleArgs& a, const Plan& pl, cha
   Work w;
   w.part = (Part*)(ws + pl.part_at);
   w.bounds = (Bounds*)(ws + pl.bounds_at);
-  w.sub = (double*)(ws + pl.sub_at);
+  w.sub = (ull*)(ws + pl.sub_at);
   w.most = (float*)(ws + pl.most_at);
   w.list = (uint32_t*)(ws + pl.list_at);
   w.cells = (uint32_t*)(ws + pl.cells_at);
   w.parts = pl.parts;
   w.subs = pl.subs;
   w.part_subs = pl.part_subs;
+  w.one = 256.0;
+  while (a.vocab * (0x1p52 / w.one) > 0x1p62) w.one *= 2;
   w.places = pl.places;
   w.few = pl.few;
   for (int64_t row0 = 0; row0 < a.rows; row0 += pl.rows) {

@@ -38,7 +38,9 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top_k=0, t
     with nothing above -inf gives token -1 and -inf.
 
     Weights and their sums are held in 64 bits: a token is right or wrong, and rows
-    of 150 thousand have as many borders between two of them.
+    of 150 thousand have as many borders between two of them.  What is drawn goes by
+    whole multiples of 2^-44 of the largest weight; tokens of less than half of that
+    are never drawn.
     """
     op = "sampling.sample"
     if type(logits) is torch.Tensor and logits.is_cuda:
