@@ -37,6 +37,8 @@
 
 #include "../../include/metal_native_amd.h"
 
+#include <cfloat>
+
 #include <algorithm>
 
 namespace mq {
@@ -45,6 +47,7 @@ namespace {
 typedef unsigned long long ull;
 constexpr int kThreads = 1024, kWaves = kThreads / 64, kSub = 1024;
 constexpr int kListRow = 4096;   // list entries of a row, over all parts
+constexpr int kAtOnce = 4;       // weights that a lane takes at the same time: registers for eight waves on a SIMD
 constexpr int kFewMost = 512;    // top_k up to which a row may be kFew
 
 // Whole numbers in the order of the values: NaN counts as -inf, -0 as 0.
@@ -88,23 +91,33 @@ __device__ __forceinline__ Settings settings_of(const SampleArgs& p, int row, in
 // ---- weights ----
 // w = 2^(t / 64), t = (x - M) 64 log2(e) / T: the nearest whole number of t by
 // a table and the exponent's bits, the rest by its series to the fourth power,
-// (log(2) / 128)^5 / 120 = 4e-14 of w.  About 20 instructions where the library's exp takes
-// twice as many.  0 for NaN and -inf, and under 2^-1020.
+// (log(2) / 128)^5 / 120 = 4e-14 of w.  Some 20 instructions where the library's exp
+// takes twice as many.
 struct Weights {
   const double* table;   // 2^(i / 64)
   double c;
   float M;
+  // M finite; 2^-1020 for what is less, for -inf and NaN
+  __device__ __forceinline__ double finite(float x) const {
+    return at(__builtin_fmax(((double)x - (double)M) * c, -65280.0));
+  }
+  // 0 for NaN and -inf, and for what is under 2^-1020
   __device__ __forceinline__ double operator()(float x) const {
-    const double d = x == M ? 0.0 : (double)x - (double)M, t = d * c;
-    constexpr double kWhole = 0x1.8p52, kLn = 0.69314718055994530942 / 64;
-    const double n = t + kWhole, f = (t - (n - kWhole)) * kLn;
+    const double t = (x == M ? 0.0 : (double)x - (double)M) * c;
+    return t >= -65280.0 ? at(t) : 0.0;
+  }
+  __device__ __forceinline__ double at(double t) const {
+    constexpr double kWhole = 0x1.8p52, L = 0.69314718055994530942 / 64;
+    const double n = t + kWhole, f = t - (n - kWhole);
     const int i = (int)(uint32_t)__double_as_longlong(n);
-    double e = __builtin_fma(f, 1.0 / 24, 1.0 / 6);
-    e = __builtin_fma(f, e, 0.5);
-    e = __builtin_fma(f, e, 1.0) * f;
+    double e = __builtin_fma(f, L * L * L * L / 24, L * L * L / 6);
+    e = __builtin_fma(f, e, L * L / 2);
+    e = __builtin_fma(f, e, L) * f;
     const double w = table[i & 63];
-    const long long bits = __double_as_longlong(__builtin_fma(w, e, w)) + ((long long)(i >> 6) << 52);
-    return t >= -65280.0 ? __longlong_as_double(bits) : 0.0;
+    typedef int i2 __attribute__((ext_vector_type(2)));
+    i2 bits = __builtin_bit_cast(i2, __builtin_fma(w, e, w));
+    bits[1] += (i & ~63) << 14;   // i / 64 to the exponent
+    return __builtin_bit_cast(double, bits);
   }
 };
 __device__ __forceinline__ double steps_of(double inv_t) { return inv_t * (64 * 1.44269504088896340736); }
@@ -253,21 +266,50 @@ template <typename E> struct Row {
   __device__ __forceinline__ int at(int j, int lane) const {
     return aligned ? j / kPer * (64 * kPer) + lane * kPer + j % kPer : j * 64 + lane;
   }
-  __device__ __forceinline__ void load(int sub, float (&v)[16]) const {   // -inf past the row
+  struct Part {   // 16-bit tokens two to a register, however they came
+    uint32_t w[4 * sizeof(E)];
+    __device__ __forceinline__ float operator[](int j) const {
+      if constexpr (sizeof(E) == 4) {
+        return __uint_as_float(w[j]);
+      } else {
+        typedef E two __attribute__((ext_vector_type(2)));
+        return (float)__builtin_bit_cast(two, w[j / 2])[j % 2];
+      }
+    }
+  };
+  __device__ __forceinline__ void load(int sub, Part& p) const {   // -inf past the row
     const int base = sub * kSub, lane = threadIdx.x & 63;
     if (aligned && base + kSub <= V) {
-      typedef E vec __attribute__((ext_vector_type(kPer)));
-      vec t[16 / kPer];
 #pragma unroll
-      for (int i = 0; i < 16 / kPer; ++i) t[i] = *(const vec*)(x + base + (i * 64 + lane) * kPer);
+      for (int i = 0; i < 16 / kPer; ++i) {
+        const u4 t = *(const u4*)(x + base + (i * 64 + lane) * kPer);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) v[j] = (float)t[j / kPer][j % kPer];
-    } else {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const int i = base + at(j);
-        v[j] = i < V ? (float)x[i] : -INFINITY;
+        for (int k = 0; k < 4; ++k) p.w[4 * i + k] = t[k];
       }
+    } else {   // by distances from one place, which are constants
+      const E* from = x + (base + at(0));
+      const int left = V - base - at(0);
+      auto one = [&](int d) -> uint32_t {
+        if constexpr (sizeof(E) == 4) return __float_as_uint(d < left ? from[d] : -INFINITY);
+        else return __builtin_bit_cast(uint16_t, d < left ? from[d] : (E)-INFINITY);
+      };
+      auto all = [&](auto&& distance) {
+#pragma unroll
+        for (int i = 0; i < (int)(4 * sizeof(E)); ++i)
+          p.w[i] = sizeof(E) == 4 ? one(distance(i)) : one(distance(2 * i)) | one(distance(2 * i + 1)) << 16;
+      };
+      if (aligned) all([](int j) { return j / kPer * (64 * kPer) + j % kPer; });
+      else all([](int j) { return j * 64; });
+    }
+  }
+  // f(sub, its tokens) for the subs s0, s0 + kWaves .. before s1, the next one's loads on their way
+  template <typename F> __device__ __forceinline__ void each(int s0, int s1, F&& f) const {
+    Part next;
+    if (s0 < s1) load(s0, next);
+    for (int s = s0; s < s1; s += kWaves) {
+      const Part v = next;
+      if (s + kWaves < s1) load(s + kWaves, next);
+      f(s, v);
     }
   }
 };
@@ -300,7 +342,7 @@ struct Work {
   __device__ __forceinline__ int first_sub(int part) const { return min(part * part_subs, subs); }
 };
 
-template <typename E> __global__ __launch_bounds__(kThreads) void sample_scan_kernel(SampleArgs p, Work ws) {
+template <typename E> __global__ __launch_bounds__(kThreads, 8) void sample_scan_kernel(SampleArgs p, Work ws) {
   __shared__ ull lds[2 * kWaves];
   Group grp{lds};
   __shared__ uint32_t cells[kCells];
@@ -310,17 +352,17 @@ template <typename E> __global__ __launch_bounds__(kThreads) void sample_scan_ke
   const Row<E> x(p, row);
   const int s0 = ws.first_sub(part) + w, s1 = ws.first_sub(part + 1);
   const bool count = st.top_k < p.vocab;
-  float v[16], mine = -INFINITY;
-  for (int s = s0; s < s1; s += kWaves) {
-    x.load(s, v);
+  typedef typename Row<E>::Part Tokens;
+  float mine = -INFINITY;
+  x.each(s0, s1, [&](int s, const Tokens& v) {
     float m = -INFINITY;
 #pragma unroll
     for (int j = 0; j < 16; ++j) m = fmaxf(m, v[j]);   // the number of the two, where one is NaN
     if (st.kind == kFew) ws.most[((int64_t)r * ws.subs + s) * 64 + lane] = m;
     mine = fmaxf(mine, m);
-  }
+  });
   if (st.kind == kGrid)
-    for (int i = tid; i < (count ? kCells : kFine); i += kThreads) cells[i] = 0;
+    for (int i = tid; i < (count ? kCells : kFine + 64); i += kThreads) cells[i] = 0;
   const float M = grp.reduce<kWaves>(mine, [](float a, float b) { return fmaxf(a, b); });
   Part& out = ws.part[(int64_t)r * ws.parts + part];
   if (tid == 0) {
@@ -330,6 +372,7 @@ template <typename E> __global__ __launch_bounds__(kThreads) void sample_scan_ke
   if (M == -INFINITY || st.kind == kFew || st.kind == kFloor) return;
   if (st.kind == kGreedy) {
     uint32_t first = ~0u;
+    Tokens v;
     for (int s = s0; s < s1 && first == ~0u; s += kWaves) {
       x.load(s, v);
 #pragma unroll
@@ -340,16 +383,11 @@ template <typename E> __global__ __launch_bounds__(kThreads) void sample_scan_ke
   } else {
     const float scale = grid_scale(st.inv_t);
     const int top = grid_of(M, scale);
-    uint32_t far = 0;
-    for (int s = s0; s < s1; s += kWaves) {
-      x.load(s, v);
+    x.each(s0, s1, [&](int, const Tokens& v) {
       if (!count) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-          const int d = top - grid_of(v[j], scale);
-          const bool fine = d < kFine;
-          far += 64 - __popcll(__ballot(fine));   // of the wave
-          if (fine) atomicAdd(&cells[d], 1u);
+          atomicAdd(&cells[min(top - grid_of(v[j], scale), kFine + lane)], 1u);   // past the fine ones: one for each lane
         }
       } else {
 #pragma unroll
@@ -358,7 +396,7 @@ template <typename E> __global__ __launch_bounds__(kThreads) void sample_scan_ke
           if (v[j] > -INFINITY) atomicAdd(&cells[d < kFine ? d : coarse_of(g, top)], 1u);
         }
       }
-    }
+    });
     __syncthreads();
     uint32_t* to = ws.cells + ((int64_t)r * ws.parts + part) * kCells;
     uint32_t end = 0;
@@ -368,10 +406,10 @@ template <typename E> __global__ __launch_bounds__(kThreads) void sample_scan_ke
       if (c) end = i + 1;
     }
     end = (uint32_t)grp.most<kWaves, ull>(end);
-    far = (uint32_t)grp.sum<kWaves, ull>(lane == 0 ? far : 0);
+    const uint32_t far = wave_sum(cells[kFine + lane]);
     if (tid == 0) {
       out.cells = end;
-      out.far = far;
+      out.far = far;   // used where top_k does not cut
     }
   }
 }
@@ -530,7 +568,7 @@ __global__ __launch_bounds__(kThreads) void sample_bounds_kernel(SampleArgs p, W
   ws.bounds[r] = b;
 }
 
-template <typename E> __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleArgs p, Work ws) {
+template <typename E> __global__ __launch_bounds__(kThreads, 8) void sample_gather_kernel(SampleArgs p, Work ws) {
   __shared__ double table[64];
   __shared__ ull lds[2 * kWaves];
   Group grp{lds};
@@ -539,9 +577,10 @@ template <typename E> __global__ __launch_bounds__(kThreads) void sample_gather_
   const int r = blockIdx.x / ws.parts, part = blockIdx.x - r * ws.parts, row = ws.row0 + r;
   const Settings st = settings_of(p, row, ws.few);
   if (st.kind != kGrid && st.kind != kFloor) return;
+  typedef typename Row<E>::Part Tokens;
   Part* parts = ws.part + (int64_t)r * ws.parts;
   const float M = top_of(parts, ws.parts);
-  if (M == -INFINITY) return;
+  if (fabsf(M) == INFINITY) return;   // nothing to draw; or the long way
   fill_table(table);
   if (tid == 0) places = 0;
   __syncthreads();
@@ -549,23 +588,26 @@ template <typename E> __global__ __launch_bounds__(kThreads) void sample_gather_
   const Row<E> x(p, row);
   const int s0 = ws.first_sub(part) + w, s1 = ws.first_sub(part + 1);
   ull* sub = ws.sub + (int64_t)r * ws.subs;
-  float v[16];
   const double one = ws.one;
+  // 16 numbers of w + one as they are, less 16 of one: their units
+  const ull none = 16 * (ull)__double_as_longlong(one);
   if (st.kind == kFloor) {
     // weights under min_p, as logits, with a margin for the division by T
-    const double span = (log(st.min_p) - 1e-9) / st.inv_t, low = st.min_p > 0 ? (double)M + span - 1e-9 * fabs(span) : -INFINITY;
-    for (int s = s0; s < s1; s += kWaves) {
-      x.load(s, v);
+    const double span = (log(st.min_p) - 1e-9) / st.inv_t;
+    const float low = st.min_p > 0 ? (float)((double)M + span - 1e-9 * fabs(span)) : -INFINITY, least = low - fabsf(low) * 0x1p-22f;
+    x.each(s0, s1, [&](int s, const Tokens& v) {
       ull sum = 0;
-#pragma unroll 4
-      for (int j = 0; j < 16; ++j)
-        if (v[j] == M || (double)v[j] >= low) {
-          const double wt = weight(v[j]);
-          sum += whole(wt >= st.min_p ? wt : 0.0, one);
-        }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        if (j % kAtOnce == 0) __builtin_amdgcn_sched_barrier(0);
+        if (!__any(v[j] >= least)) continue;
+        const double wt = weight.finite(v[j]);
+        sum += whole(wt >= st.min_p ? wt : 0.0, one);
+        asm volatile("" : "+v"(sum));
+      }
       sum = wave_sum(sum);
       if (lane == 0) sub[s] = sum;
-    }
+    });
     return;
   }
   const Bounds b = ws.bounds[r];
@@ -584,47 +626,51 @@ template <typename E> __global__ __launch_bounds__(kThreads) void sample_gather_
     }
   };
   if (!cut_k && st.min_p == 0) {   // top_p alone
-    for (int s = s0; s < s1; s += kWaves) {
-      x.load(s, v);
+    const float lo = fmaxf(b.p_lo, -FLT_MAX);
+    x.each(s0, s1, [&](int s, const Tokens& v) {
       ull kept = 0;
       uint32_t take = 0;
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        const double wt = weight(v[j]);
+        if (j % kAtOnce == 0) __builtin_amdgcn_sched_barrier(0);
+        const double wt = weight.finite(v[j]);
         const bool stays = v[j] >= sure;
         over_k += wt;
-        kept += stays ? whole(wt, one) : 0;
-        take |= (!stays & (v[j] >= b.p_lo) & (v[j] > -INFINITY)) << j;
+        kept += (ull)__double_as_longlong((stays ? wt : 0.0) + one);
+        take |= ((v[j] >= lo) & !stays) << j;
+        if (j % kAtOnce == kAtOnce - 1) asm volatile("" : "+v"(over_k), "+v"(kept), "+v"(take));   // added up here, not at the end
       }
+      kept -= none;
       kept_all += kept;
       kept = wave_sum(kept);
       if (lane == 0) sub[s] = kept;
       enlist(s, take);
-    }
+    });
   } else {
     // where top_k cuts, what lies under both windows has no part in anything
     const float least = cut_k ? (cut_p ? fminf(b.k_lo, b.p_lo) : b.k_lo) : -INFINITY;
-    for (int s = s0; s < s1; s += kWaves) {
-      x.load(s, v);
+    x.each(s0, s1, [&](int s, const Tokens& v) {
       ull kept = 0;
       uint32_t take = 0;
-#pragma unroll 4
+#pragma unroll
       for (int j = 0; j < 16; ++j) {
+        if (j % kAtOnce == 0) __builtin_amdgcn_sched_barrier(0);
         if (!__any(v[j] >= least)) continue;
         const bool in_k = cut_k & (v[j] >= b.k_lo) & (v[j] < b.k_hi), in_p = cut_p & (v[j] >= b.p_lo) & (v[j] < b.p_hi);
         take |= ((in_k | in_p) & (v[j] > -INFINITY)) << j;
-        const double wt = weight(v[j]);
+        const double wt = weight.finite(v[j]);
         const bool of_k = !cut_k | (v[j] >= b.k_hi);
         over_k += of_k ? wt : 0.0;
         over_n += of_k;
         const double stays = v[j] >= sure ? wt : 0.0;
         over_p += stays;
         kept += whole(stays >= st.min_p ? stays : 0.0, one);
+        asm volatile("" : "+v"(over_k), "+v"(over_p), "+v"(kept), "+v"(take), "+v"(over_n));
       }
       kept = wave_sum(kept);
       if (lane == 0) sub[s] = kept;
       enlist(s, take);
-    }
+    });
   }
   over_p += (double)kept_all * (one * 0x1p-52);
   over_k = grp.sum<kWaves, double>(over_k);
@@ -1190,14 +1236,15 @@ template <typename E> __global__ __launch_bounds__(kThreads) void sample_pick_ke
   __syncthreads();
   const Weights weight{sh.table, steps_of(st.inv_t), M};
   Group grp{sh.lds};
-  if (pick<E>(p, ws, st, weight, sh, grp, sub_units)) {
+  if ((M == INFINITY && st.kind != kFew) || pick<E>(p, ws, st, weight, sh, grp, sub_units)) {
     __syncthreads();
     long_way<E>(p, row, st, weight, ws.one, sh.far, grp);
   }
 }
 
 // ---- launches ----
-// Parts of a row: enough workgroups for four to a CU, of 16 subs at least (one to a
+constexpr int kEnough = 2;
+// Parts of a row: enough workgroups for kEnough to a CU, of 16 subs at least (one to a
 // wave), 2^18 tokens at most; of a few numbers the one whose waves have most even work.
 struct Plan {
   int parts, subs, part_subs, places, few;
@@ -1210,7 +1257,7 @@ Plan plan_of(const SampleArgs& a, int num_cus) {
   pl.subs = (a.vocab + kSub - 1) / kSub;
   pl.rows = std::min<int64_t>(a.rows, 1024);
   const int most = std::min(kPartsMost, (pl.subs + kWaves - 1) / kWaves);
-  const int want = (int)std::max<int64_t>(1, std::min<int64_t>((4 * (int64_t)num_cus + pl.rows - 1) / pl.rows, most));
+  const int want = (int)std::max<int64_t>(1, std::min<int64_t>((kEnough * (int64_t)num_cus + pl.rows - 1) / pl.rows, most));
   pl.parts = want;
   auto rounds = [&](int parts) { return ((pl.subs + parts - 1) / parts + kWaves - 1) / kWaves; };
   for (int n = want + 1; n <= std::min(most, want + 3); ++n)
