@@ -342,6 +342,8 @@ MQ_API int mq_paged_ancestors(const int32_t* parents, const int32_t* cu_q, int64
  * these, its prefix by the slots in front of the chunk. */
 MQ_API int64_t mq_paged_tree_attention_workspace_size(const mq_paged_cache* cache, const mq_paged_mask* mask,
                                                       int64_t rows, int32_t heads);
+MQ_API int mq_paged_tree_attention_plan(const mq_paged_cache* cache, const mq_paged_mask* mask, int64_t rows,
+                                        int32_t heads, int32_t* block_rows, int32_t* parts);
 MQ_API int mq_paged_tree_attention(const mq_paged_cache* cache, const mq_paged_mask* mask, const int64_t* tree,
                                    int64_t ld_tree, int64_t words, const void* q, int64_t q_token, int64_t q_head,
                                    int64_t rows, int32_t heads, void* out, float* lse, void* workspace,

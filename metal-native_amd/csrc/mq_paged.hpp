@@ -154,12 +154,14 @@ struct PagedArgs {
 };
 
 struct PagedPlan {
-  int block_rows;   // kRowsS or kRowsP of mq_pattn.hip
+  int block_rows;   // kRowsS or kRowsP of mq_pattn_dev.hpp
   int64_t parts;
 };
 PagedPlan pattn_plan(const PagedArgs& a, int num_cus);
 size_t pattn_workspace(const PagedArgs& a, int num_cus);
 hipError_t pattn_launch(const PagedArgs& a, int num_cus, void* ws, hipStream_t s);
+PagedPlan ptattn_plan(const PagedArgs& a, int num_cus);
+size_t ptattn_workspace(const PagedArgs& a, int num_cus);
 hipError_t ptattn_launch(const PagedArgs& a, int num_cus, void* ws, hipStream_t s);   // a.tree set
 size_t pmass_workspace(const PagedArgs& a, int num_cus);
 hipError_t pmass_launch(const PagedArgs& a, int num_cus, void* ws, hipStream_t s);

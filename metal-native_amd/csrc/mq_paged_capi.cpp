@@ -242,7 +242,21 @@ MQ_API int64_t mq_paged_tree_attention_workspace_size(const mq_paged_cache* c, c
     refuse("paged.tree_attention", bad);
     return -1;
   }
-  return (int64_t)mq::pattn_workspace(a, mq::current_num_cus());
+  return (int64_t)mq::ptattn_workspace(a, mq::current_num_cus());
+}
+
+MQ_API int mq_paged_tree_attention_plan(const mq_paged_cache* c, const mq_paged_mask* m, int64_t rows, int32_t heads,
+                                        int32_t* block_rows, int32_t* parts) {
+  const char* op = "paged.tree_attention";
+  mq::PagedArgs a;
+  const int64_t any = 0;
+  if (const char* bad = attn_args(a, c, m, rows, heads, true)) return refuse(op, bad);
+  if (!block_rows || !parts) return refuse(op, "null output");
+  tree_rows(a, &any, 1, 1);
+  const mq::PagedPlan plan = mq::ptattn_plan(a, mq::current_num_cus());
+  *block_rows = plan.block_rows;
+  *parts = (int32_t)plan.parts;
+  return MQ_SUCCESS;
 }
 
 MQ_API int mq_paged_tree_attention(const mq_paged_cache* c, const mq_paged_mask* m, const int64_t* tree, int64_t ld_tree,
@@ -258,7 +272,7 @@ MQ_API int mq_paged_tree_attention(const mq_paged_cache* c, const mq_paged_mask*
   a.out = out;
   a.lse = lse;
   const int cus = mq::current_num_cus();
-  const size_t need = mq::pattn_workspace(a, cus);
+  const size_t need = mq::ptattn_workspace(a, cus);
   if (need && (!ws || !aligned16(ws) || ws_bytes < (int64_t)need)) return refuse(op, "workspace too small or not 16-byte aligned");
   const hipError_t e = mq::ptattn_launch(a, cus, ws, (hipStream_t)stream);
   return e == hipSuccess ? MQ_SUCCESS : mq::hip_fail_with(e, "paged.tree_attention: kernel launch failed");

@@ -964,23 +964,22 @@ __global__ __launch_bounds__(256, 2) void paged_split_kernel(PagedArgs p, float*
   }
 }
 
-// Adds up the parts of a row block, of 32 rows or (MANY) of 256.  SHARES = 1: a thread takes a piece of four
+// Adds up the parts of a row block of ROWS rows, its slots in tiles of TILE.  SHARES = 1: a thread takes a piece of four
 // outputs of its row through all parts, several rows to a workgroup; else each
 // of SHARES threads takes every SHARES-th part, one row to a workgroup, and the
 // shares are added up in their order.  16 shares take 10 us for the 128 parts of
 // 28 heads and four long sequences; a call of one part has no join at all.
-template <typename T, int D, int SHARES, bool MANY>
+template <typename T, int D, int SHARES, int ROWS, int TILE>
 __global__ __launch_bounds__(SHARES == 1 ? 256 : D / 4 * SHARES) void paged_join_kernel(PagedArgs p, const float* ws, int parts_max,
                                                                                      int per_min, int R) {
   constexpr int P4 = D / 4;   // pieces of a row
   PagedSeq sq;
   int block;
-  constexpr int ROWS = MANY ? kRowsP : kRowsS;
   const int seq = find_block(p, blockIdx.z, ROWS, sq, block), kv = blockIdx.y;
   if (seq < 0) return;
-  if (MANY) block = (int)(((int64_t)sq.n * p.g + ROWS - 1) / ROWS) - 1 - block;   // that kernel takes the last rows first
+  if (ROWS == kRowsP) block = (int)(((int64_t)sq.n * p.g + ROWS - 1) / ROWS) - 1 - block;   // that kernel takes the last rows first
   const int r0 = block * ROWS;
-  const int count = block_span(p, sq, r0, ROWS, MANY ? kTileP : kTileS).count(), per = tiles_per_part(count, parts_max, per_min);
+  const int count = block_span(p, sq, r0, ROWS, TILE).count(), per = tiles_per_part(count, parts_max, per_min);
   const int parts = (count + per - 1) / per;
   const int d4 = threadIdx.x % P4, share = SHARES == 1 ? 0 : threadIdx.x / P4;
   const int r = SHARES == 1 ? blockIdx.x * (256 / P4) + threadIdx.x / P4 : blockIdx.x;
@@ -1041,8 +1040,19 @@ int64_t most_slots(const PagedArgs& a, int rows, int tk) {   // that a row block
 // average chunk decides, so a batch of single tokens and one chunk runs in one kind
 // of block.
 constexpr int64_t kWork = 4 << 20, kWorkExtra = 24 << 20;
+// A few trees of fewer rows, behind long caches, too: in blocks of 32 rows each block
+// reads all of the cache again, and one block of 256 for the whole tree, its slots in
+// parts, is faster though most of its rows are empty (us, blocks of 32 and of 256): 4
+// trees of 5 nodes, 28 heads over 4, behind 32768 slots 88 and 70, 4 of 30, 32 over 8,
+// 233 and 151, 2 of 15, 8 over 1, behind 65000 56 and 44.  Of many trees the caches'
+// lengths differ, which parts as many for all do not suit: 8 of 14 behind 1600 to
+// 32768, 32 over 8, 98 and 191, 20 of 13, 28 over 4, behind 800 to 16384 107 and 136.
+constexpr int64_t kTreeSlots = 8192, kTreeUnits = 32;
 bool many_rows(const PagedArgs& a) {
   const int64_t slots = a.window > 0 ? std::min<int64_t>(a.cap, (int64_t)a.window + kRowsP) : a.cap;
+  if (a.tree && a.cu && !a.extra() && slots >= kTreeSlots && (int64_t)a.b * a.KVH <= kTreeUnits &&
+      (int64_t)a.rows * a.g > (int64_t)kRowsS * a.b)
+    return true;
   return ((int64_t)(a.rows - a.b) * a.g >= 128 * (int64_t)a.b && (int64_t)a.rows * a.H * slots >= (a.extra() ? kWorkExtra : kWork)) ||
          row_blocks(a, kRowsS) > 65535;   // the grid's z
 }
@@ -1064,11 +1074,13 @@ RowsPlan rows_plan(const PagedArgs& a, int num_cus) {
   s.blocks = row_blocks(a, kRowsP);
   s.parts = 1;
   if (a.cu && s.blocks <= 65535) {
-    const int64_t units = (((int64_t)a.rows * a.g + kRowsP - 1) / kRowsP + (a.b - 1) / 2) * a.KVH;   // half of each chunk's last block
+    int64_t units = (((int64_t)a.rows * a.g + kRowsP - 1) / kRowsP + (a.b - 1) / 2) * a.KVH;   // half of each chunk's last block
+    if (a.tree) units = std::max<int64_t>(units, (int64_t)a.b * a.KVH);   // a block at least of each, however empty
+    const int most = a.tree ? 64 : 16;
     const int64_t tiles = (most_slots(a, kRowsP, kTileP) + kTileP - 1) / kTileP;
     const double record = (double)units * kRowsP * (a.D + 2) * sizeof(float) * 2 / 4.9e6, tile = 1.7 * a.D / 128;
     double least = 0;
-    for (int parts = 1; parts <= 16 && (parts == 1 || parts * kPerMinP <= tiles); ++parts) {
+    for (int parts = 1; parts <= most && (parts == 1 || parts * kPerMinP <= tiles); ++parts) {
       const int64_t rounds = (units * parts + num_cus - 1) / num_cus;
       const double t = (double)rounds * ((double)tiles / parts * tile + 6) + (parts > 1 ? 8 + parts * record : 0);
       if (parts == 1 || t < 0.9 * least) {
@@ -1111,30 +1123,35 @@ hipError_t launch(const PagedArgs& a, int num_cus, void* ws, hipStream_t s) {
     const int64_t grid = rp.blocks * a.KVH * rp.parts;
     if (grid > 0x7fffffff) return hipErrorInvalidValue;
     paged_rows_kernel<T, D, EXTRA, TREE><<<(int)grid, 512, 0, s>>>(a, (float*)ws, (int)rp.parts);
-    if (rp.parts > 1)
-      paged_join_kernel<T, D, 1, true><<<dim3(kRowsP * D / 1024, a.KVH, (unsigned)rp.blocks), 256, 0, s>>>(a, (const float*)ws, (int)rp.parts, kPerMinP, kRowsP);
+    if (rp.parts > 16)
+      paged_join_kernel<T, D, 16, kRowsP, kTileP><<<dim3(kRowsP, a.KVH, (unsigned)rp.blocks), D / 4 * 16, 0, s>>>(a, (const float*)ws, (int)rp.parts, kPerMinP, kRowsP);
+    else if (rp.parts > 1)
+      paged_join_kernel<T, D, 1, kRowsP, kTileP><<<dim3(kRowsP * D / 1024, a.KVH, (unsigned)rp.blocks), 256, 0, s>>>(a, (const float*)ws, (int)rp.parts, kPerMinP, kRowsP);
     return hipGetLastError();
   }
   const SplitPlan sp = split_plan(a, num_cus);
   const dim3 grid((unsigned)sp.parts, a.KVH, (unsigned)sp.blocks);
   paged_split_kernel<T, D, EXTRA, TREE><<<grid, 256, 0, s>>>(a, (float*)ws, sp.per_min, sp.R);
   if (sp.parts > 16)
-    paged_join_kernel<T, D, 16, false><<<dim3(sp.R, a.KVH, (unsigned)sp.blocks), D / 4 * 16, 0, s>>>(a, (const float*)ws, (int)sp.parts, sp.per_min, sp.R);
+    paged_join_kernel<T, D, 16, kRowsS, kTileS><<<dim3(sp.R, a.KVH, (unsigned)sp.blocks), D / 4 * 16, 0, s>>>(a, (const float*)ws, (int)sp.parts, sp.per_min, sp.R);
   else if (sp.parts > 1)
-    paged_join_kernel<T, D, 1, false><<<dim3((sp.R + 1024 / D - 1) / (1024 / D), a.KVH, (unsigned)sp.blocks), 256, 0, s>>>(a, (const float*)ws, (int)sp.parts, sp.per_min, sp.R);
+    paged_join_kernel<T, D, 1, kRowsS, kTileS><<<dim3((sp.R + 1024 / D - 1) / (1024 / D), a.KVH, (unsigned)sp.blocks), 256, 0, s>>>(a, (const float*)ws, (int)sp.parts, sp.per_min, sp.R);
   return hipGetLastError();
 }
 
+// f(type, width) for the call's
+template <typename F> hipError_t by_type(const PagedArgs& a, F&& f) {
+  using D64 = std::integral_constant<int, 64>;
+  using D128 = std::integral_constant<int, 128>;
+  if (a.D == 128) return a.bf16 ? f(BF16{}, D128{}) : f(F16{}, D128{});
+  return a.bf16 ? f(BF16{}, D64{}) : f(F16{}, D64{});
+}
 template <bool TREE> hipError_t launch(const PagedArgs& a, int num_cus, void* ws, hipStream_t s) {
-  auto of = [&](auto type, auto dim) {
+  return by_type(a, [&](auto type, auto dim) {
     using T = decltype(type);
     constexpr int D = decltype(dim)::value;
     return a.extra() ? launch<T, D, true, TREE>(a, num_cus, ws, s) : launch<T, D, false, TREE>(a, num_cus, ws, s);
-  };
-  using D64 = std::integral_constant<int, 64>;
-  using D128 = std::integral_constant<int, 128>;
-  if (a.D == 128) return a.bf16 ? of(BF16{}, D128{}) : of(F16{}, D128{});
-  return a.bf16 ? of(BF16{}, D64{}) : of(F16{}, D64{});
+  });
 }
 
 }  // namespace

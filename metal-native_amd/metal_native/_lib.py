@@ -94,6 +94,7 @@ SIGNATURES = {
                               _c_void_p, _c_void_p, _c_void_p]),
     "mq_paged_ancestors": (_i32, [_c_void_p, _c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p]),
     "mq_paged_tree_attention_workspace_size": (_i64, [_c_void_p, _c_void_p, _i64, _i32]),
+    "mq_paged_tree_attention_plan": (_i32, [_c_void_p, _c_void_p, _i64, _i32, _c_void_p, _c_void_p]),
     "mq_paged_tree_attention": (_i32, [_c_void_p, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _i64, _i64, _i64, _i32,
                                        _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p]),
     "mq_paged_accept": (_i32, [_c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64,
