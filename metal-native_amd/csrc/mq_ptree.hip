@@ -5,23 +5,10 @@
 namespace mq {
 namespace {
 
-// One thread walks from its row's node to the root; parents have smaller numbers
-// (anything else is no parent), so the walk ends, and words are written from the
-// highest down.
-__global__ __launch_bounds__(256) void ancestors_kernel(AncestorsArgs a) {
-  const int row = blockIdx.x * 256 + threadIdx.x;
-  if (row >= a.rows) return;
-  int start = row, i = 0;
-  if (a.cu) {   // the last sequence that begins at or before the row
-    int lo = 0, hi = a.b;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (a.cu[mid] <= row) lo = mid;
-      else hi = mid;
-    }
-    start = max(a.cu[lo], 0);
-    i = row >= start && row < a.cu[lo + 1] ? row - start : -1;
-  }
+// A row's node and its ancestors as bits, by a walk from it to the root: parents have
+// smaller numbers (anything else is no parent), so it ends, and words are written from
+// the highest down.  i < 0: a row of no sequence.
+__device__ __forceinline__ void walk(const AncestorsArgs& a, int row, int start, int i) {
   uint64_t* out = a.tree + (int64_t)row * a.words;
   uint64_t bits = 0;
   int w = a.words - 1;
@@ -39,6 +26,61 @@ __global__ __launch_bounds__(256) void ancestors_kernel(AncestorsArgs a) {
     out[w] = bits;
     bits = 0;
   }
+}
+
+// One token for each sequence: every row is a root.
+__global__ __launch_bounds__(256) void roots_kernel(AncestorsArgs a) {
+  const int row = blockIdx.x * 256 + threadIdx.x;
+  if (row < a.rows) walk(a, row, row, 0);
+}
+
+// One workgroup per tree.  Trees of up to 512 nodes, one to a thread, by doubling: a
+// node knows its ancestors up to some node, which knows its own up to another one, so
+// 9 rounds take every path to its root (trees of 100 to 512 nodes with paths of up to
+// 200: 6.5 us, by walks through memory 13.8).
+constexpr int kNodes = 512, kNodeWords = kNodes / 64;
+__global__ __launch_bounds__(kNodes) void ancestors_kernel(AncestorsArgs a) {
+  __shared__ uint64_t bits[kNodeWords][kNodes];
+  __shared__ int ups[kNodes];
+  const int s = blockIdx.x, tid = threadIdx.x;
+  const PagedSeq sq = paged_seq(s, a.cu[s], a.cu[s + 1], true, 0, 0, a.rows, 0);
+  // rows before the first tree and past the last: no bits
+  if (s == 0)
+    for (int r = tid; r < min(max(a.cu[0], 0), a.rows); r += kNodes) walk(a, r, r, -1);
+  if (s == a.b - 1)
+    for (int r = max(a.cu[a.b], 0) + tid; r < a.rows; r += kNodes) walk(a, r, r, -1);
+  if (sq.n > kNodes || a.words > kNodeWords) {
+    for (int i = tid; i < sq.n; i += kNodes) walk(a, sq.start + i, sq.start, i);
+    return;
+  }
+  uint64_t mine[kNodeWords];
+  int up = tid < sq.n ? a.parents[sq.start + tid] : -1;
+  up = up < tid && up >= 0 ? up : -1;
+#pragma unroll
+  for (int w = 0; w < kNodeWords; ++w) {
+    mine[w] = w == tid >> 6 ? 1ull << (tid & 63) : 0;
+    if (w < a.words) bits[w][tid] = mine[w];
+  }
+  ups[tid] = up;
+  for (int far = 1; far < sq.n; far *= 2) {
+    __syncthreads();
+    int next = -1;
+    if (up >= 0) {
+#pragma unroll
+      for (int w = 0; w < kNodeWords; ++w)
+        if (w < a.words) mine[w] |= bits[w][up];
+      next = ups[up];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kNodeWords; ++w)
+      if (w < a.words) bits[w][tid] = mine[w];
+    ups[tid] = up = next;
+  }
+  if (tid < sq.n)
+#pragma unroll
+    for (int w = 0; w < kNodeWords; ++w)
+      if (w < a.words) a.tree[(int64_t)(sq.start + tid) * a.words + w] = mine[w];
 }
 
 // A thread moves one 16-byte piece of a slot, of one layer, cache and head,
@@ -111,7 +153,8 @@ __global__ __launch_bounds__(256) void accept_kernel(AcceptArgs a) {
 }  // namespace
 
 hipError_t pancestors_launch(const AncestorsArgs& a, hipStream_t s) {
-  ancestors_kernel<<<(a.rows + 255) / 256, 256, 0, s>>>(a);
+  if (a.cu) ancestors_kernel<<<a.b, kNodes, 0, s>>>(a);
+  else roots_kernel<<<(a.rows + 255) / 256, 256, 0, s>>>(a);
   return hipGetLastError();
 }
 

@@ -45,12 +45,13 @@ struct Cache {
   c10::Device dev = c10::Device(c10::kCPU);
   at::ScalarType ty = at::kHalf;
 
-  bool one(const at::Tensor& t, int64_t* page, int64_t* head, int64_t* slot, bool write) const {
-    if (t.dim() != 4 || t.stride(3) != 1 || !aligned16(t)) return false;
-    *page = t.size(0) > 1 ? t.stride(0) : 0;
-    *head = t.size(1) > 1 ? t.stride(1) : 0;
-    *slot = t.stride(2);
-    return *page % 8 == 0 && *head % 8 == 0 && *slot % 8 == 0 && *page >= 0 && *head >= 0 && *slot >= t.size(3) &&
+  // l: dimensions in front of the pages'
+  bool one(const at::Tensor& t, int l, int64_t* page, int64_t* head, int64_t* slot, bool write) const {
+    if (t.dim() != l + 4 || t.stride(l + 3) != 1 || !aligned16(t)) return false;
+    *page = t.size(l) > 1 ? t.stride(l) : 0;
+    *head = t.size(l + 1) > 1 ? t.stride(l + 1) : 0;
+    *slot = t.stride(l + 2);
+    return *page % 8 == 0 && *head % 8 == 0 && *slot % 8 == 0 && *page >= 0 && *head >= 0 && *slot >= t.size(l + 3) &&
            (!write || distinct(t));
   }
   // v null: keys alone
@@ -58,28 +59,28 @@ struct Cache {
     const at::Tensor* k = plain(ko);
     return take(k, vo ? plain(vo) : k, table, lens, write);
   }
-  bool take(const at::Tensor* k, const at::Tensor* v, PyObject* table, PyObject* lens, bool write) {
-    const at::Tensor *t = plain(table), *l = plain(lens);
-    if (!k || !v || !t || !l) return false;
+  bool take(const at::Tensor* k, const at::Tensor* v, PyObject* table, PyObject* lens, bool write, int l = 0) {
+    const at::Tensor *t = plain(table), *n = plain(lens);
+    if (!k || !v || !t || !n) return false;
     dev = k->device();
     ty = k->scalar_type();
     if ((ty != at::kHalf && ty != at::kBFloat16) || v->scalar_type() != ty || v->device() != dev) return false;
-    if (!one(*k, &c.k_page, &c.k_head, &c.k_slot, write) || !one(*v, &c.v_page, &c.v_head, &c.v_slot, write)) return false;
-    if (k->sizes() != v->sizes() || !index_rows(*t, dev) || !vec(l, dev, at::kInt, t->size(0))) return false;
+    if (!one(*k, l, &c.k_page, &c.k_head, &c.k_slot, write) || !one(*v, l, &c.v_page, &c.v_head, &c.v_slot, write)) return false;
+    if (k->sizes() != v->sizes() || !index_rows(*t, dev) || !vec(n, dev, at::kInt, t->size(0))) return false;
     if (t->size(0) < 1 || t->size(1) < 1 || k->numel() == 0) return false;
-    if (k->size(1) > INT32_MAX || k->size(2) > INT32_MAX || k->size(3) > INT32_MAX) return false;
+    if (k->size(l + 1) > INT32_MAX || k->size(l + 2) > INT32_MAX || k->size(l + 3) > INT32_MAX) return false;
     c.k = const_cast<void*>(k->const_data_ptr());
     c.v = const_cast<void*>(v->const_data_ptr());
-    c.pages = k->size(0);
-    c.kv_heads = (int32_t)k->size(1);
-    c.page_size = (int32_t)k->size(2);
-    c.head_dim = (int32_t)k->size(3);
+    c.pages = k->size(l);
+    c.kv_heads = (int32_t)k->size(l + 1);
+    c.page_size = (int32_t)k->size(l + 2);
+    c.head_dim = (int32_t)k->size(l + 3);
     c.dtype = ty == at::kHalf ? MQ_PAGED_F16 : MQ_PAGED_BF16;
     c.table = t->const_data_ptr<int32_t>();
     c.ld_table = t->size(0) > 1 ? t->stride(0) : t->size(1);
     c.width = t->size(1);
     c.batch = t->size(0);
-    c.lens = l->const_data_ptr<int32_t>();
+    c.lens = n->const_data_ptr<int32_t>();
     return true;
   }
 };
@@ -307,16 +308,13 @@ PyObject* paged_accept(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (PyErr_Occurred()) return nullptr;
   HANDLE_TH_ERRORS
   const Call guard(kt->device());
-  if (kt->dim() == 5) {
-    if (vt->dim() != 5 || kt->size(0) < 1 || kt->size(0) != vt->size(0) || !distinct(*kt) || !distinct(*vt)) return decline();
+  const bool deep = kt->dim() == 5;
+  if (!k.take(kt, vt, a[2], a[3], true, deep)) return decline();
+  if (deep && kt->size(0) > 1) {
     layers = kt->size(0);
-    kl = layers > 1 ? kt->stride(0) : 0;
-    vl = layers > 1 ? vt->stride(0) : 0;
+    kl = kt->stride(0);
+    vl = vt->stride(0);
     if (kl % 8 || vl % 8 || kl < 0 || vl < 0) return decline();
-    const at::Tensor k0 = kt->select(0, 0), v0 = vt->select(0, 0);
-    if (!k.take(&k0, &v0, a[2], a[3], true)) return decline();
-  } else if (!k.take(kt, vt, a[2], a[3], true)) {
-    return decline();
   }
   if (!vec(drawn, k.dev, at::kLong, rows) || !vec(drafted, k.dev, at::kLong, rows) || !vec(parents, k.dev, at::kInt, rows) ||
       !chunks(a[7], k, rows, &cu))
