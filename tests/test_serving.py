@@ -126,3 +126,155 @@ def test_refusals_leave_the_server_as_it_was(gpu):
     with pytest.raises(ValueError, match="48 positions"):
         server.step()
     assert server.lens[0] == 48
+
+
+# ---- drawing and drafting ----
+def lines_of(server, prompts, n, drafted):
+    """n tokens behind every prompt, and how many passes they took."""
+    lines = {s: [t] for s, t in server.start(prompts).items()}
+    passes = 0
+    while server.last:
+        passes += 1
+        for s, t in (server.step_drafted() if drafted else server.step()).items():
+            lines[s] += t if drafted else [t]
+            if len(lines[s]) >= n:
+                server.finish(s)
+    return [lines[s][:n] for s in sorted(lines)], passes
+
+
+def exact(monkeypatch):
+    """Logits that depend on the row's token alone, so that how rows were grouped rounds nothing."""
+    from metal_native.serving import PagedServer
+
+    real = PagedServer._forward
+
+    def forward(self, flat, pos, rows, table, lens, cu, max_q, last, tree=None):
+        out = real(self, flat, pos, rows, table, lens, cu, max_q, last, tree)
+        flat = flat if last is None else flat[last]   # mostly one token behind another: text that repeats
+        x = torch.full(out.shape, -4.0, dtype=out.dtype, device=out.device)
+        for i, step in enumerate((7, 11, 30)):
+            x[torch.arange(len(flat), device=x.device), (flat * step + i) % 23] += (6.0, 4.0, 1.0)[i]
+        return x
+
+    monkeypatch.setattr(PagedServer, "_forward", forward)
+
+
+@pytest.mark.parametrize("settings", [dict(), dict(temperature=0.8, top_k=5, seed=3), dict(temperature=1.3, top_p=0.9, min_p=0.01)])
+def test_drafts_change_no_token(gpu, monkeypatch, settings):
+    from metal_native.serving import PagedServer
+
+    m = model_of(gpu)
+    exact(monkeypatch)
+    plain, _ = lines_of(PagedServer(m, 60, 4, chunk=32, **settings), PROMPTS, 60, False)
+    for draft in (1, 6, 40):
+        server = PagedServer(m, 60, 4, chunk=32, draft=draft, **settings)
+        got, passes = lines_of(server, PROMPTS, 60, True)
+        assert got == plain and passes < 59
+    other, _ = lines_of(PagedServer(m, 60, 4, chunk=32, **{**settings, "seed": 5}), PROMPTS, 60, False)
+    assert (other == plain) == (not settings)
+
+
+def test_a_sequence_draws_the_same_in_other_company(gpu, monkeypatch):
+    from metal_native.serving import PagedServer
+
+    m = model_of(gpu)
+    exact(monkeypatch)
+    how = dict(temperature=1.0, seed=9)
+    both, _ = lines_of(PagedServer(m, 40, 4, **how), PROMPTS[:2], 20, False)
+    one, _ = lines_of(PagedServer(m, 40, 4, **how), PROMPTS[:1], 20, False)
+    assert one[0] == both[0]
+
+
+def test_drafted_caches_and_logits(gpu, monkeypatch):
+    """After drafted steps the cache holds what the kept tokens leave when they run one at a time, and the logits of
+    the path are theirs."""
+    from metal_native import paged
+    from metal_native.serving import PagedServer
+
+    m = model_of(gpu)
+    server = PagedServer(m, 60, 4, chunk=32, draft=12)
+    logits, paths = [], []
+    real_forward, real_accept = PagedServer._forward, paged.accept
+    monkeypatch.setattr(PagedServer, "_forward", lambda self, *a: logits.append(real_forward(self, *a)) or logits[-1])
+
+    def agree(k, v, table, lens, drawn, drafted, parents, cu=None, *, steps):
+        """Takes a guess wherever there is one: random weights hardly repeat themselves."""
+        drawn = drawn.clone()
+        ends = [0, *range(1, len(drawn) + 1)] if cu is None else cu.tolist()
+        up, tokens = parents.tolist(), drafted.tolist()
+        for lo, hi in zip(ends, ends[1:]):
+            for i in range(hi - 1, lo, -1):
+                drawn[lo + up[i]] = tokens[i]
+        out = real_accept(k, v, table, lens, drawn, drafted, parents, cu, steps=steps)
+        paths.append((ends, out[0].tolist(), out[2].tolist()))
+        return out
+
+    monkeypatch.setattr(paged, "accept", agree)
+    prompts = [[3, 4, 5, 6] * 9, [5], [9, 8, 7, 9, 8, 1, 9, 8], list(range(16))]
+    lines = {s: p + [t] for (s, t), p in zip(server.start(prompts).items(), prompts)}
+    logits.clear()
+    firsts = {s: len(line) - 1 for s, line in lines.items()}
+    rows = {s: [] for s in lines}
+    for turn in range(5):
+        for s, t in server.step_drafted().items():
+            lines[s] += t
+        ends, path, count = paths[-1]
+        for s in lines:
+            rows[s] += [logits[-1][ends[s] + i] for i in path[s][:count[s]]]
+    assert max(max(c) for _, _, c in paths) > 3
+    for s, line in lines.items():
+        assert server.lens[s] == server.seen[s] == len(line) - 1 and server.last[s] == line[-1]
+        for i, t in enumerate(line[:-1]):
+            _, want = m.step(torch.tensor([t], device=gpu), torch.tensor([i], device=gpu), return_logits=True)
+            if i >= firsts[s]:   # both within 1e-2 + 1e-3 |x| of exact logits
+                got = rows[s][i - firsts[s]].float()
+                err = (got - want[0].float()).abs()
+                assert bool((err <= 2e-2 + 2e-3 * want[0].float().abs()).all()), (s, i, float(err.max()))
+        n = len(line) - 1
+        slots = torch.tensor([server.held[s][i // 16] * 16 + i % 16 for i in range(n)], device=gpu)
+        kv = server.kv.permute(0, 1, 3, 2, 4, 5).flatten(3, 4)[:, :, :, slots]
+        want = m.kv[:, :, :, :n]
+        assert bool(((kv.float() - want.float()).abs() <= 2e-2 + 2e-3 * want.float().abs()).all())
+
+
+def test_drafts_where_pages_and_positions_are_short(gpu, monkeypatch):
+    from metal_native.serving import PagedServer
+
+    m = model_of(gpu, max_len=48)
+    exact(monkeypatch)
+    prompts = [[1, 2, 3] * 5, [4, 5] * 7]
+    plain, _ = lines_of(PagedServer(m, 6, 2), prompts, 30, False)
+    server = PagedServer(m, 6, 2, draft=30)   # three pages a sequence: all that 48 positions need
+    got, _ = lines_of(server, prompts, 30, True)
+    assert got == plain
+    assert sorted(server.free) == list(range(6)) and not server.history
+
+    server = PagedServer(m, 3, 2, draft=30)
+    server.start([[1, 2, 3] * 5, [4]])   # 15 slots and 1: a page each, guesses take the third
+    before = dict(server.last)
+    server.step_drafted()
+    assert before.keys() == server.last.keys()
+    server.finish(1)
+    assert sum(len(h) for h in server.held) + len(server.free) == 3
+    while server.seen[0] < 48:
+        server.step_drafted()
+    with pytest.raises(ValueError, match="48 positions"):
+        server.step_drafted()
+
+
+def test_logits_with_nothing_to_draw(gpu, monkeypatch):
+    """The server stays as it was: the embedding has no row for -1."""
+    from metal_native.serving import PagedServer
+
+    m = model_of(gpu)
+    server = PagedServer(m, 40, 4, temperature=1.0, draft=3)
+    server.start(PROMPTS)
+    kept = dict(server.last), list(server.lens), list(server.seen)
+    real = PagedServer._forward
+    monkeypatch.setattr(PagedServer, "_forward", lambda self, *a: torch.full_like(real(self, *a), float("nan")))
+    for step in (server.step, server.step_drafted):
+        with pytest.raises(RuntimeError, match="nothing above"):
+            step()
+        assert (dict(server.last), list(server.lens), list(server.seen)) == kept
+    monkeypatch.setattr(PagedServer, "_forward", real)
+    assert server.step().keys() == kept[0].keys()
