@@ -114,6 +114,16 @@ def test_trees_in_blocks_of_256_rows(gpu, dtype, D, masked):
         check_tree(c, families, bits, **how)
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("H,KVH,D,lens,counts,width", [(28, 4, 128, [20003], [5], 2048), (14, 2, 64, [9000, 300, 17, 0], [14, 60, 17, 0], 1024),
+                                                       (32, 8, 128, [300, 9, 8192], [40, 9, 1], 512), (8, 1, 64, [30011, 64], [9, 64], 4096)])
+def test_few_trees_behind_tables_of_many_slots(gpu, dtype, H, KVH, D, lens, counts, width):
+    """Blocks of 256 rows, most of them empty, in up to 64 parts, most of those past the sequence."""
+    c, families, bits = tree_case(gpu, DT[dtype], H, KVH, D, 16, lens, counts, seed=width, width=width)
+    check_tree(c, families, bits)
+    check_tree(c, families, bits, prefix=torch.tensor([100, 3, 10**6, 0][:len(lens)], dtype=torch.int32, device=gpu), window=9000)
+
+
 @pytest.mark.parametrize("window,prefix", [(0, True), (1, False), (3, True), (7, False), (64, True), (100, False), (1000, True)])
 @pytest.mark.parametrize("softcap,bias", [(0.0, False), (0.0, True), (20.0, True)])
 @pytest.mark.parametrize("kind", ["mixed", "chain"])

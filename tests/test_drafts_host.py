@@ -186,3 +186,25 @@ def test_c_entries_of_null_structs_and_no_rows():
     assert _lib.load().mq_paged_tree_attention_workspace_size(None, None, 1, 1) == -1
     assert c_call("tree_attention", rows=0, q=None, out=None)[0] == 0
     assert c_call("ancestors", rows=0, parents=None, tree=None)[0] == 0
+
+
+def test_tree_plans():
+    """(rows of a block, most parts): few trees behind many slots in blocks of 256 rows, many or short ones as chunks are."""
+    from metal_native import _lib
+
+    def plan(rows, heads, kv_heads, dim, batch, slots, window=0, softcap=0.0, op="tree_attention"):
+        c = Cache(k=P, v=P, pages=1 << 20, kv_heads=kv_heads, page_size=16, head_dim=dim, dtype=0, table=P, ld_table=slots // 16, width=slots // 16,
+                  batch=batch, lens=P, **{f"{t}_{n}": x for t in "kv" for n, x in (("page", kv_heads * 16 * dim), ("head", 16 * dim), ("slot", dim))})
+        m = Mask(scale=0.1, softcap=softcap, slopes=None, window=window, prefix_lens=None, cu_q=P, max_q=0)
+        block, parts = ctypes.c_int32(), ctypes.c_int32()
+        assert getattr(_lib.load(), f"mq_paged_{op}_plan")(ctypes.byref(c), ctypes.byref(m), rows, heads, ctypes.byref(block), ctypes.byref(parts)) == 0
+        return block.value, parts.value
+
+    assert plan(5, 28, 4, 128, 1, 32768)[0] == 256 and 16 < plan(5, 28, 4, 128, 1, 32768)[1] <= 64
+    assert plan(14, 14, 2, 64, 2, 16384)[0] == 256 and plan(14, 14, 2, 64, 2, 16384, op="attention")[0] == 32
+    for other in (plan(4, 28, 4, 128, 1, 32768), plan(20, 28, 4, 128, 4, 8176), plan(100, 28, 4, 128, 9, 32768), plan(14, 14, 2, 64, 2, 16384, window=100),
+                  plan(14, 14, 2, 64, 2, 16384, softcap=2.0)):   # a block of 32 holds the tree; short; many; a window; a cap
+        assert other[0] == 32
+    assert plan(4096, 28, 4, 128, 1, 32768) == plan(4096, 28, 4, 128, 1, 32768, op="attention")
+    n = ctypes.c_int32()
+    assert _lib.load().mq_paged_tree_attention_plan(None, None, 1, 1, ctypes.byref(n), ctypes.byref(n)) == 4

@@ -127,6 +127,36 @@ def test_settings_at_their_ends(gpu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,V", [("fp16", 2**18), ("bf16", 2**18 + 1), ("fp32", 2**18 + 1027), ("bf16", 2**20 + 3), ("fp32", 2**22)])
+def test_large_vocabularies(gpu, dtype, V):
+    """A row's parts grow past 2^18 tokens in more than one workgroup's; 2^22 is the most."""
+    x, u = logits(gpu, 2, V, dtype, V, 1.0)
+    for s in ((0.9, 0, 0.9, 0.0), (1.1, 300, 1.0, 0.0), (1.0, 5000, 0.99, 0.0), (1.5, 0, 1.0, 0.0), (1.0, 0, 1.0, 0.01)):
+        check(x, u, *s)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [5, 700])
+def test_many_rows(gpu, V):
+    """More than a thousand rows go in several turns, settings of each row with them."""
+    x, u = logits(gpu, 2051, V, "fp16", V)
+    check(x, u, 0.9, 0, 0.9, 0.0)
+    every = [SETTINGS[r % len(SETTINGS)] for r in range(2051)]
+    check(x, u, *(list(c) for c in zip(*every)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("k", [63, 64, 65, 511, 512, 513, 1024, 1025])
+def test_borders_of_the_short_lists(gpu, k):
+    """Around the lengths at which lists change their place and way; nearly equal and many equal logits among them."""
+    for dtype, spread in (("bf16", 0.05), ("fp32", 1e-5), ("fp16", 3.0)):
+        x, u = logits(gpu, 3, 20000, dtype, k, spread)
+        for p, m in ((1.0, 0.0), (0.9, 0.0), (0.5, 1e-3)):
+            check(x, u, 0.8, k, p, m)
+            check(x, u, [0.8] * 3, [k, k, 1], [p] * 3, [m] * 3)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", list(DT))
 def test_strides_and_alignment(gpu, dtype):
     wide, _ = logits(gpu, 8, 6007, dtype, 1)
