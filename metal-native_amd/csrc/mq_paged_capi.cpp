@@ -223,7 +223,8 @@ MQ_API int mq_paged_attention(const mq_paged_cache* c, const mq_paged_mask* m, c
 MQ_API int mq_paged_ancestors(const int32_t* parents, const int32_t* cu_q, int64_t batch, int64_t rows, int64_t words,
                               int64_t* tree, void* stream) {
   const char* op = "paged.ancestors";
-  if (batch < 1 || batch > INT_MAX - 1 || rows < 0 || rows > INT_MAX - 256) return refuse(op, "batch must be positive, rows not negative, both below 2^31");
+  if (batch < 1 || (cu_q && batch > 65535)) return refuse(op, "batch must be positive, with cu_q at most 65535");
+  if (rows < 0 || rows > INT_MAX - 1024) return refuse(op, "rows must not be negative, and below 2^31 - 1024");
   if (words < 1 || words > INT_MAX / 64) return refuse(op, "1 to 2^25 words a row");
   if (!cu_q && rows != batch) return refuse(op, "without cu_q there must be one row per sequence");
   if (rows == 0) return MQ_SUCCESS;
@@ -285,7 +286,7 @@ MQ_API int mq_paged_accept(const mq_paged_cache* c, int64_t layers, int64_t k_la
   if (const char* bad = bad_cache(c, true)) return refuse(op, bad);
   if (layers < 1 || layers > INT_MAX / 2 || k_layer < 0 || v_layer < 0 || k_layer % 8 || v_layer % 8)
     return refuse(op, "layers must be positive, their strides multiples of 8");
-  if (rows < 0 || rows > INT_MAX || steps < 1 || steps > INT_MAX - 64) return refuse(op, "rows must not be negative, steps positive, both below 2^31");
+  if (rows < 0 || rows > INT_MAX - 1024 || steps < 1 || steps > INT_MAX - 64) return refuse(op, "rows must not be negative, steps positive, both below 2^31");
   if (!cu_q && rows != c->batch) return refuse(op, "without cu_q there must be one row per sequence");
   if (!path || !tokens || !count || !new_lens || (rows > 0 && (!drawn || !drafted || !parents))) return refuse(op, "null pointer argument");
   mq::AcceptArgs a{};

@@ -46,9 +46,9 @@ __global__ __launch_bounds__(kNodes) void ancestors_kernel(AncestorsArgs a) {
   const PagedSeq sq = paged_seq(s, a.cu[s], a.cu[s + 1], true, 0, 0, a.rows, 0);
   // rows before the first tree and past the last: no bits
   if (s == 0)
-    for (int r = tid; r < min(max(a.cu[0], 0), a.rows); r += kNodes) walk(a, r, r, -1);
+    for (int r = tid; r < min(a.cu[0], a.rows); r += kNodes) walk(a, r, r, -1);
   if (s == a.b - 1)
-    for (int r = max(a.cu[a.b], 0) + tid; r < a.rows; r += kNodes) walk(a, r, r, -1);
+    for (int r = min(max(a.cu[a.b], 0), a.rows) + tid; r < a.rows; r += kNodes) walk(a, r, r, -1);
   if (sq.n > kNodes || a.words > kNodeWords) {
     for (int i = tid; i < sq.n; i += kNodes) walk(a, sq.start + i, sq.start, i);
     return;

@@ -309,7 +309,7 @@ PyObject* paged_accept(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   const Call guard(kt->device());
   const bool deep = kt->dim() == 5;
-  if (!k.take(kt, vt, a[2], a[3], true, deep)) return decline();
+  if (!k.take(kt, vt, a[2], a[3], true, deep) || kt->const_data_ptr() == vt->const_data_ptr()) return decline();
   if (deep && kt->size(0) > 1) {
     layers = kt->size(0);
     kl = kt->stride(0);

@@ -434,6 +434,8 @@ def accept(k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor, le
             _invalid(f"{op}: layers of the caches must be 16-byte aligned")
         k0, v0 = k_cache.detach()[0], v_cache.detach()[0]
     table, lens = _cache(op, k0, v0, table, lens)
+    if k_cache.data_ptr() == v_cache.data_ptr():
+        _invalid(f"{op}: k_cache and v_cache must not be the same memory")
     for t, what, dtype in ((drawn, "drawn", torch.int64), (drafted, "drafted", torch.int64), (parents, "parents", torch.int32)):
         _require_cuda(t, what, op)
         if t.dtype != dtype or t.dim() != 1 or t.shape != drawn.shape or t.device != k_cache.device:

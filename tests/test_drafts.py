@@ -65,6 +65,29 @@ def test_ancestors_of_odd_parents_and_rows_of_no_sequence(gpu):
     assert paged.ancestors(flat[:0], torch.zeros(2, dtype=torch.int32, device=gpu), 8).shape == (0, 1)
 
 
+@pytest.mark.parametrize("n", [511, 512, 513, 577])
+def test_ancestors_around_512_nodes(gpu, n):
+    """Where trees no longer have a thread for each node; deep ones, wide ones, and words for fewer and more nodes."""
+    from metal_native import paged
+
+    for kind in ("mixed", "chain", "star"):
+        parents, flat, cu = trees(gpu, [n, 3, n], n, kind)
+        for max_q in (n, 512, 513, 64, 1000):
+            want = torch.cat([ref.pack(ref.closure(p), -(-max_q // 64)) for p in parents])
+            assert torch.equal(paged.ancestors(flat, cu, max_q).cpu(), want)
+
+
+def test_ancestors_of_any_offsets(gpu):
+    """The ends of what an offset can hold: rows of no tree have no bits, and nothing past the rows is touched."""
+    from metal_native import paged
+
+    flat = torch.arange(-1, 11, dtype=torch.int32, device=gpu)
+    big = 2**31 - 1
+    for cu, rows in (([0, 5, big], 12), ([3, 9, -big], 0), ([big, big, big], 0), ([-big, -5, -1], 0), ([-4, 12, big], 12), ([12, 12, 12], 0)):
+        got = paged.ancestors(flat, torch.tensor(cu, dtype=torch.int32, device=gpu), 64).cpu()
+        assert got.shape == (12, 1) and (int((got != 0).sum()) == rows or cu[0] == 3)
+
+
 # ---- attention ----
 def check_tree(c, families, bits, *, scale=None, softcap=0.0, slopes=None, window=0, prefix=None, max_q=None):
     from metal_native import paged
@@ -312,6 +335,8 @@ def test_accept_counts_its_writes_and_refuses_gradients(gpu):
         call(c["k"].clone().requires_grad_())
     with pytest.raises(MetalNativeError):
         call(c["k"][:1].expand(2, -1, -1, -1, -1))   # layers that share memory
+    with pytest.raises(MetalNativeError, match="same memory"):   # a slot would be moved twice
+        paged.accept(c["k"], c["k"], c["table"], c["lens"], c["drawn"], c["drafted"], c["parents"], c["cu"], steps=4)
 
 
 # ---- together ----
