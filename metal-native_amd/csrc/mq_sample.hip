@@ -829,6 +829,7 @@ __device__ __forceinline__ void long_way(const SampleArgs& p, int row, const Set
 // ---- the last launch: a workgroup for each row, of which eight waves do the work
 // (their barriers are shorter) unless the row goes the long way ----
 constexpr int kNear = 8, kNearThreads = 64 * kNear;
+constexpr uint32_t kRanked = 192;   // tokens that are put in order by their ranks; more by merging
 constexpr int kFewRoom = 1024;   // places for the tokens of kFew that are as large as the top_k-th largest of the lanes'
 
 struct List {
@@ -846,6 +847,31 @@ __device__ __forceinline__ uint32_t rank_of(ull mine, const ull* of, int n) {
     rank += (q[0] > mine) + (q[1] > mine);
   }
   return rank;
+}
+
+// The threads' numbers in falling order over the first N of them: runs that fall and rise
+// in turn are merged to longer ones, in a wave by lanes, over waves with one barrier a step.
+template <int N> __device__ __forceinline__ ull in_order(ull v, ull (*turn)[kThreads]) {
+  const int tid = threadIdx.x;
+  int half = 0;
+#pragma unroll
+  for (int run = 2; run <= N; run <<= 1)
+#pragma unroll
+    for (int by = run >> 1; by; by >>= 1) {
+      ull other;
+      if (by < 64) {
+        other = from_lane(v, by);
+      } else {
+        turn[half][tid] = v;
+        __syncthreads();
+        other = turn[half][tid ^ by];
+        half ^= 1;
+      }
+      const bool larger = ((tid & by) == 0) == ((tid & run) == 0);
+      v = (v > other) == larger ? v : other;
+    }
+  __syncthreads();   // `turn` may be used again
+  return v;
 }
 
 // Of the entries that are true to `of`, the n-th largest key, among `bits` of them
@@ -893,6 +919,7 @@ struct PickShared {
       ull sorted[kFewMost];
       alignas(16) ull idx[kFewMost + 1];
       double w[kFewMost];
+      ull turn[2][kThreads];
     } few;
   };
 };
@@ -967,16 +994,22 @@ __device__ __forceinline__ bool pick(const SampleArgs& p, const Work& ws, const 
     const uint32_t k = min((uint32_t)st.top_k, held);
     if (tid == 0) sh.few.key[held] = 0;
     __syncthreads();
-    if (tid < (int)held) {
-      const ull mine = sh.few.key[tid];
-      const uint32_t rank = rank_of(mine, sh.few.key, held);
-      if (rank < k) sh.few.sorted[rank] = mine;
+    ull own = tid < (int)held ? sh.few.key[tid] : 0;
+    const bool sorts = held > kRanked;
+    if (sorts) {
+      own = held <= 512 ? in_order<512>(own, sh.few.turn) : in_order<1024>(own, sh.few.turn);
+    } else {
+      if (tid < (int)held) {
+        const uint32_t rank = rank_of(own, sh.few.key, held);
+        if (rank < k) sh.few.sorted[rank] = own;
+      }
+      __syncthreads();
+      own = tid < (int)k ? sh.few.sorted[tid] : 0;
     }
-    __syncthreads();
     double w = 0;
     uint32_t idx = 0;
     if (tid < (int)k) {
-      const ull mine = sh.few.sorted[tid];
+      const ull mine = own;
       idx = ~(uint32_t)mine;
       w = weight(value_of((uint32_t)(mine >> 32)));
       sh.few.idx[tid] = ~idx;   // larger for the first
@@ -987,13 +1020,20 @@ __device__ __forceinline__ bool pick(const SampleArgs& p, const Work& ws, const 
     if (st.top_p < 1.0 && tid > 0 && !(before < st.top_p * sum)) w = 0;
     if (w < st.min_p) w = 0;
     // now by index
-    if (tid < (int)k) {
-      const uint32_t rank = rank_of((uint32_t)~idx, sh.few.idx, k);
-      sh.few.w[rank] = w;
-      sh.few.key[rank] = idx;
+    if (sorts) {
+      if (tid < (int)k) sh.few.w[tid] = w;
+      const ull to = in_order<512>(tid < (int)k ? (ull)~idx << 32 | tid : 0, sh.few.turn);
+      w = tid < (int)k ? sh.few.w[(uint32_t)to] : 0;
+      if (tid < (int)k) sh.few.key[tid] = ~(uint32_t)(to >> 32);
+    } else {
+      if (tid < (int)k) {
+        const uint32_t rank = rank_of((uint32_t)~idx, sh.few.idx, k);
+        sh.few.w[rank] = w;
+        sh.few.key[rank] = idx;
+      }
+      __syncthreads();
+      w = tid < (int)k ? sh.few.w[tid] : 0;
     }
-    __syncthreads();
-    w = tid < (int)k ? sh.few.w[tid] : 0;
     const ull units = whole_of_list(w);
     ull total;
     const ull upto = grp.scan<kWaves, ull>(units, total), aim = share_of(st.u, total);
