@@ -330,7 +330,7 @@ MQ_API int mq_paged_attention_plan(const mq_paged_cache* cache, const mq_paged_m
  *
  * tree [rows, words]: bit i of a row is set where node i of its sequence is the
  * row's own or one of its ancestors; nodes from 64 * words on have no bit.  Rows
- * that belong to no sequence get zeros. */
+ * that belong to no sequence get zeros.  At most 2^31 - 1024 rows. */
 MQ_API int mq_paged_ancestors(const int32_t* parents, const int32_t* cu_q, int64_t batch, int64_t rows, int64_t words,
                               int64_t* tree, void* stream);
 
@@ -339,7 +339,8 @@ MQ_API int mq_paged_ancestors(const int32_t* parents, const int32_t* cu_q, int64
  * ld_tree words; any bits, whether a tree's or not).  It stands (number of its
  * bits) - 1 slots past the chunk's first one, and the distance to a slot of the
  * chunk is the number of its bits above it; the mask's window and slopes go by
- * these, its prefix by the slots in front of the chunk. */
+ * these, its prefix by the slots in front of the chunk.  _plan: as that of
+ * mq_paged_attention. */
 MQ_API int64_t mq_paged_tree_attention_workspace_size(const mq_paged_cache* cache, const mq_paged_mask* mask,
                                                       int64_t rows, int32_t heads);
 MQ_API int mq_paged_tree_attention_plan(const mq_paged_cache* cache, const mq_paged_mask* mask, int64_t rows,
@@ -355,7 +356,8 @@ MQ_API int mq_paged_tree_attention(const mq_paged_cache* cache, const mq_paged_m
  * [batch, steps] what was drawn behind each, -1 past the path; count [batch] its
  * length, new_lens [batch] lens less the nodes that are not on it.  In every one
  * of `layers` caches (strides k_layer, v_layer from the first) the path's slots
- * move to the chunk's first ones. */
+ * move to the chunk's first ones.  The chunk's pages may be in no other sequence's
+ * table; keys and values may not be the same memory. */
 MQ_API int mq_paged_accept(const mq_paged_cache* cache, int64_t layers, int64_t k_layer, int64_t v_layer,
                            const int64_t* drawn, const int64_t* drafted, const int32_t* parents, const int32_t* cu_q,
                            int64_t rows, int64_t steps, int32_t* path, int64_t* tokens, int32_t* count,

@@ -1,5 +1,6 @@
 // Trees of drafted tokens over a paged cache: ancestor bits, and the accepted
-// path with its slots moved together.
+// path with its slots moved together.  Both are bound by latency: 64 trees of 100 to 512
+// nodes are 1.2 MB, 48 paths of 28 layers 34 MB (4 us at the copy rate, the launch takes 8.3).
 #include "mq_paged_dev.hpp"
 
 namespace mq {
@@ -87,7 +88,9 @@ __global__ __launch_bounds__(kNodes) void ancestors_kernel(AncestorsArgs a) {
 // through all of the path; every wave walks the path for itself.  Node i of the
 // path goes to the i-th slot of the chunk, which is never behind its own: what a
 // store overwrites is a slot that has been moved before, or by the same thread's
-// loads in front of it.
+// loads in front of it.  Eight of a thread's loads are on their way at a time; every wave
+// for itself needs no barrier and no second launch between the walk and the moves (one
+// tree of 16 nodes 8.3 us a call, 4.0 of the kernel, 48 trees of 20 to 64 8.3 and 5.9).
 __global__ __launch_bounds__(256) void accept_kernel(AcceptArgs a) {
   const int s = blockIdx.y, lane = threadIdx.x & 63;
   const PagedSeq sq = paged_seq(s, a.cu ? a.cu[s] : 0, a.cu ? a.cu[s + 1] : 0, a.cu != nullptr, a.lens[s], 0, a.rows, a.cap);
