@@ -36,7 +36,7 @@
 // Bound by the issue of instructions: a row is read twice, and 63 million weights of 20
 // instructions in 64 bits take longer than their bytes.  152064 logits, us of a call: one
 // row, top_k 50 and top_p 0.9, 14.6 (latency of some ten barriers and as many reads behind
-// one another); 416 rows of fp16, top_p 0.95, 168 (scan 45, bounds 25, gather 80, pick 24;
+// one another); 416 rows of fp16, top_p 0.95, 156 (scan 45, bounds 14, gather 80, pick 21;
 // read once they would take 25); 64 of bf16, settings of each, 69; 48 x 32003 in fp32,
 // min_p 0.05, 17.  The plain form (a sort, sums, searches) takes 410, 8700, 2000 and 620.
 #include "mq_device.hpp"
@@ -431,10 +431,11 @@ __device__ __forceinline__ float top_of(const Part* part, int parts) {
   return M;
 }
 
+// (Two workgroups to a CU, as pick: 416 rows 14 us where one takes 24.)
 // All parts' grids laid over each other: a part's cell, from its own largest logit
 // down, is one of the row's.  Then between which logits the cuts fall; a workgroup
 // for each row.
-__global__ __launch_bounds__(kThreads) void sample_bounds_kernel(SampleArgs p, Work ws) {
+__global__ __launch_bounds__(kThreads, 8) void sample_bounds_kernel(SampleArgs p, Work ws) {
   __shared__ uint32_t numbers[kCells];
   __shared__ ull lds[2 * kWaves];
   Group grp{lds};
@@ -467,7 +468,7 @@ __global__ __launch_bounds__(kThreads) void sample_bounds_kernel(SampleArgs p, W
     const int end = (int)q.cells, mt = grid_of(q.top, scale), down = top - mt;
     const uint32_t* from = ws.cells + ((int64_t)r * ws.parts + of) * kCells;
     if ((tid & (lanes - 1)) == 0 && !count && end) far += q.far;
-    constexpr int kStep = 8;   // loads of a thread on their way, four cells each (the last ones past end: zeros)
+    constexpr int kStep = 4;   // loads of a thread on their way, four cells each (the last ones past end: zeros)
     for (int d0 = 4 * (tid & (lanes - 1)); d0 < end; d0 += 4 * kStep * lanes) {
       u4 n4[kStep];
 #pragma unroll
@@ -500,18 +501,19 @@ __global__ __launch_bounds__(kThreads) void sample_bounds_kernel(SampleArgs p, W
   constexpr int N = kCells / kThreads;
   const int per = count ? N : (kFine + kThreads - 1) / kThreads, b0 = per * tid;   // the thread's cells
   double wt[N], mine = 0, low = 0;
-  uint32_t n[N], mine_n = 0;
+  uint32_t mine_n = 0;
 #pragma unroll
   for (int k = 0; k < N; ++k) {
     const int b = b0 + k;
-    const bool have = k < per && b < cells;
+    wt[k] = 0;
+    if (k >= per) continue;
+    const uint32_t n = b < cells ? numbers[b] : 0;
     // the weight at a fine cell's middle, a coarse one's lower edge; the top cell's is 1
     const float down = b < kFine ? (float)b : (float)(top - 8 * ((top >> 3) - (b - kFine))) + 0.5f;
-    n[k] = have ? numbers[have ? b : 0] : 0;
-    wt[k] = (double)((float)n[k] * exp2f(down * (-1.f / 128)));
+    wt[k] = (double)((float)n * exp2f(down * (-1.f / 128)));
     mine += wt[k];
     low += b < kFine ? 0 : wt[k];
-    mine_n += n[k];
+    mine_n += n;
   }
   double all;
   const double before = grp.scan<kWaves, double>(mine, all) - mine;   // to a few steps of the sum
@@ -519,8 +521,9 @@ __global__ __launch_bounds__(kThreads) void sample_bounds_kernel(SampleArgs p, W
     uint32_t all_n, at = grp.scan<kWaves, uint32_t>(mine_n, all_n) - mine_n;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      if (at < (uint32_t)st.top_k && at + n[k] >= (uint32_t)st.top_k) cell = b0 + k;   // one thread
-      at += n[k];
+      const uint32_t n = numbers[b0 + k];   // kCells are N to a thread
+      if (at < (uint32_t)st.top_k && at + n >= (uint32_t)st.top_k) cell = b0 + k;   // one thread
+      at += n;
     }
   }
   __syncthreads();
@@ -549,6 +552,7 @@ __global__ __launch_bounds__(kThreads) void sample_bounds_kernel(SampleArgs p, W
     ull may = cells, must = cells;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
+      if (k >= per) continue;
       run += wt[k];
       const int b = b0 + k;
       const double rest = fmax(upto - run, 0.0);   // weight past the cell, with all of cell_k
@@ -964,7 +968,7 @@ __device__ __forceinline__ bool pick(const SampleArgs& p, const Work& ws, const 
     // large: those of a little over top_k lanes, 16 each, and a few more than top_k of these.
     const int lanes = ws.subs * 64;
     const float* most = ws.most + (int64_t)r * lanes;
-    constexpr int kStep = 16;   // loads on their way; kept, for rows of up to 2^18
+    constexpr int kStep = 10;   // loads on their way; kept, for rows of up to 163840
     float m[kStep], mine_most = -INFINITY;
     for (int i0 = (lanes - 1) / (kStep * kThreads) * (kStep * kThreads); i0 >= 0; i0 -= kStep * kThreads) {
 #pragma unroll
@@ -1262,7 +1266,7 @@ __device__ __forceinline__ bool pick(const SampleArgs& p, const Work& ws, const 
   return false;
 }
 
-template <typename E> __global__ __launch_bounds__(kThreads) void sample_pick_kernel(SampleArgs p, Work ws) {
+template <typename E> __global__ __launch_bounds__(kThreads, 8) void sample_pick_kernel(SampleArgs p, Work ws) {
   __shared__ PickShared sh;
   extern __shared__ ull sub_units[];   // [subs]
   const int tid = threadIdx.x, row = ws.row0 + blockIdx.x;
