@@ -885,33 +885,41 @@ template <int N> __device__ __forceinline__ ull in_order(ull v, ull (*turn)[kThr
   return v;
 }
 
-// Of the entries that are true to `of`, the n-th largest key, among `bits` of them
-// under a common head; one barrier a bit
-template <typename F>
-__device__ __forceinline__ uint32_t nth_key(int held, uint32_t n, uint32_t head, int bits, const uint32_t* key, Group& grp, F&& of) {
-  uint32_t least = head;
-#pragma unroll 1
-  for (int bit = bits - 1; bit >= 0; --bit) {
-    const uint32_t t = least | 1u << bit;
-    uint32_t c = 0;
-    for (int i = threadIdx.x; i < (held + 63 & ~63); i += kNearThreads) c += __popcll(__ballot(i < held && key[i] >= t && of(i)));
-    if (grp.sum_of_waves<kNear>(c) >= n) least = t;
-  }
-  return least;
-}
 template <typename F> __device__ __forceinline__ uint32_t number_of(int held, Group& grp, F&& of) {
   uint32_t c = 0;
   for (int i = threadIdx.x; i < (held + 63 & ~63); i += kNearThreads) c += __popcll(__ballot(i < held && of(i)));
   return grp.sum_of_waves<kNear>(c);
 }
-// The n-th smallest index of them
+// For how many entries `of` is true to 1, to 2 and to 3, in 16 bits each
+template <typename F> __device__ __forceinline__ ull numbers_of(int held, Group& grp, F&& of) {
+  ull c = 0;
+  for (int i = threadIdx.x; i < (held + 63 & ~63); i += kNearThreads)
+    c += (ull)__popcll(__ballot(i < held && of(i, 1u))) | (ull)__popcll(__ballot(i < held && of(i, 2u))) << 16 |
+         (ull)__popcll(__ballot(i < held && of(i, 3u))) << 32;
+  c = grp.of_waves<kNear>(c);
+#pragma unroll
+  for (int o = 1; o < kNear; o <<= 1) c += from_lane(c, o);
+  return c;
+}
+// Of the entries that are true to `of`, the n-th largest key, among `bits` of them
+// under a common head, and the n-th smallest index: two bits a barrier
+template <typename F>
+__device__ __forceinline__ uint32_t nth_key(int held, uint32_t n, uint32_t head, int bits, const uint32_t* key, Group& grp, F&& of) {
+  uint32_t least = head;
+#pragma unroll 1
+  for (int bit = (bits - 1) & ~1; bit >= 0; bit -= 2) {
+    const ull c = numbers_of(held, grp, [&](int i, uint32_t d) { return key[i] >= (least | d << bit) && of(i); });
+    least |= ((uint32_t)(c >> 32) >= n ? 3u : ((uint32_t)(c >> 16 & 0xffff) >= n ? 2u : ((uint32_t)(c & 0xffff) >= n ? 1u : 0u))) << bit;
+  }
+  return least;
+}
 template <typename F>
 __device__ __forceinline__ uint32_t nth_index(int held, uint32_t n, int vocab, const uint32_t* idx, Group& grp, F&& of) {
   uint32_t most = 0;   // fewer than n lie under it
 #pragma unroll 1
-  for (int bit = 31 - __clz(vocab); bit >= 0; --bit) {
-    const uint32_t t = most | 1u << bit;
-    if (number_of(held, grp, [&](int i) { return of(i) && idx[i] < t; }) < n) most = t;
+  for (int bit = (31 - __clz(vocab)) & ~1; bit >= 0; bit -= 2) {
+    const ull c = numbers_of(held, grp, [&](int i, uint32_t d) { return idx[i] < (most | d << bit) && of(i); });
+    most |= ((uint32_t)(c >> 32) < n ? 3u : ((uint32_t)(c >> 16 & 0xffff) < n ? 2u : ((uint32_t)(c & 0xffff) < n ? 1u : 0u))) << bit;
   }
   return most;
 }
