@@ -1123,9 +1123,13 @@ hipError_t launch(const PagedArgs& a, int num_cus, void* ws, hipStream_t s) {
     const int64_t grid = rp.blocks * a.KVH * rp.parts;
     if (grid > 0x7fffffff) return hipErrorInvalidValue;
     paged_rows_kernel<T, D, EXTRA, TREE><<<(int)grid, 512, 0, s>>>(a, (float*)ws, (int)rp.parts);
-    if (rp.parts > 16)
-      paged_join_kernel<T, D, 16, kRowsP, kTileP><<<dim3(kRowsP, a.KVH, (unsigned)rp.blocks), D / 4 * 16, 0, s>>>(a, (const float*)ws, (int)rp.parts, kPerMinP, kRowsP);
-    else if (rp.parts > 1)
+    if constexpr (TREE) {
+      if (rp.parts > 16) {   // of chunks in order never
+        paged_join_kernel<T, D, 16, kRowsP, kTileP><<<dim3(kRowsP, a.KVH, (unsigned)rp.blocks), D / 4 * 16, 0, s>>>(a, (const float*)ws, (int)rp.parts, kPerMinP, kRowsP);
+        return hipGetLastError();
+      }
+    }
+    if (rp.parts > 1)
       paged_join_kernel<T, D, 1, kRowsP, kTileP><<<dim3(kRowsP * D / 1024, a.KVH, (unsigned)rp.blocks), 256, 0, s>>>(a, (const float*)ws, (int)rp.parts, kPerMinP, kRowsP);
     return hipGetLastError();
   }
