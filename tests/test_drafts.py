@@ -407,3 +407,35 @@ def test_a_drafted_step_captured(gpu):
         want = [*step(), c["k"], c["v"]]
         same = lambda a, b: torch.equal(a.nan_to_num(), b.nan_to_num()) if a.is_floating_point() else torch.equal(a, b)  # noqa: E731
         assert all(same(a, b) for a, b in zip(kept, want))
+
+
+def test_two_streams_at_once(gpu):
+    """Steps of two sets of sequences side by side, each with workspaces of its own stream."""
+    from metal_native import paged, sampling
+
+    sets = []
+    for seed, (lens, counts, width) in enumerate((([9000, 500], [40, 12], 1024), ([300, 77, 650], [100, 65, 200], None))):
+        c, _, bits = tree_case(gpu, torch.float16, 32, 8, 128, 16, lens, counts, seed=seed, width=width)
+        _, flat, cu = trees(gpu, counts, seed)
+        n = sum(counts)
+        sets.append((c, bits, flat, cu, torch.rand(n, device=gpu), torch.randint(0, 3, (n,), device=gpu)))
+
+    def step(c, bits, flat, cu, u, drafted):
+        k, v = c["k"].clone(), c["v"].clone()
+        out = paged.tree_attention(c["q"], k, v, c["table"], c["lens"], bits, c["cu"])
+        drawn = sampling.sample(out.reshape(len(u), -1)[:, :3], u, temperature=0.9, top_p=0.99)
+        wide = sampling.sample(out.reshape(len(u), -1), u, top_p=0.9)
+        return (out, drawn, wide, *paged.accept(k, v, c["table"], c["lens"], drawn, drafted, flat, cu, steps=8), k, v)
+
+    want = [step(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = []
+    for _ in range(6):
+        for stream, s in zip(streams, sets):
+            with torch.cuda.stream(stream):
+                got.append(step(*s))
+    torch.cuda.synchronize()
+    same = lambda a, b: torch.equal(a.nan_to_num(), b.nan_to_num()) if a.is_floating_point() else torch.equal(a, b)  # noqa: E731
+    for i, g in enumerate(got):
+        assert all(same(a, b) for a, b in zip(g, want[i % 2])), i
