@@ -37,12 +37,13 @@ __global__ __launch_bounds__(256) void roots_kernel(AncestorsArgs a) {
 
 // One workgroup per tree.  Trees of up to 512 nodes, one to a thread, by doubling: a
 // node knows its ancestors up to some node, which knows its own up to another one, so
-// 9 rounds take every path to its root (trees of 100 to 512 nodes with paths of up to
-// 200: 6.5 us, by walks through memory 13.8).
-constexpr int kNodes = 512, kNodeWords = kNodes / 64;
+// 9 rounds take every path to its root.  Rows are written from LDS, their words in a row
+// (64 trees of 100 to 512 nodes 6.9 us a call; each thread its own row 7.5; by walks
+// through memory 13.8).
+constexpr int kNodes = 512, kNodeWords = kNodes / 64, kRounds = 10;
 __global__ __launch_bounds__(kNodes) void ancestors_kernel(AncestorsArgs a) {
-  __shared__ uint64_t bits[kNodeWords][kNodes];
-  __shared__ int ups[kNodes];
+  __shared__ uint64_t bits[2][kNodeWords][kNodes];   // read and written in turn: one barrier a round
+  __shared__ int ups[2][kNodes], goes_on[kRounds];
   const int s = blockIdx.x, tid = threadIdx.x;
   const PagedSeq sq = paged_seq(s, a.cu[s], a.cu[s + 1], true, 0, 0, a.rows, 0);
   // rows before the first tree and past the last: no bits
@@ -54,34 +55,40 @@ __global__ __launch_bounds__(kNodes) void ancestors_kernel(AncestorsArgs a) {
     for (int i = tid; i < sq.n; i += kNodes) walk(a, sq.start + i, sq.start, i);
     return;
   }
+  const int words = min(a.words, (sq.n + 63) >> 6);   // those of the tree's own nodes; the others stay zero
   uint64_t mine[kNodeWords];
   int up = tid < sq.n ? a.parents[sq.start + tid] : -1;
   up = up < tid && up >= 0 ? up : -1;
 #pragma unroll
   for (int w = 0; w < kNodeWords; ++w) {
     mine[w] = w == tid >> 6 ? 1ull << (tid & 63) : 0;
-    if (w < a.words) bits[w][tid] = mine[w];
+    if (w < words) bits[0][w][tid] = mine[w];
   }
-  ups[tid] = up;
-  for (int far = 1; far < sq.n; far *= 2) {
+  ups[0][tid] = up;
+  if (tid < kRounds) goes_on[tid] = tid == 0;
+  int round = 0;
+  for (; round < kRounds - 1; ++round) {   // paths of up to 2^round nodes are whole
     __syncthreads();
-    int next = -1;
+    if (!goes_on[round]) break;
+    const int from = round & 1, to = from ^ 1;
     if (up >= 0) {
 #pragma unroll
       for (int w = 0; w < kNodeWords; ++w)
-        if (w < a.words) mine[w] |= bits[w][up];
-      next = ups[up];
+        if (w < words) mine[w] |= bits[from][w][up];
+      up = ups[from][up];
     }
-    __syncthreads();
 #pragma unroll
     for (int w = 0; w < kNodeWords; ++w)
-      if (w < a.words) bits[w][tid] = mine[w];
-    ups[tid] = up = next;
+      if (w < words) bits[to][w][tid] = mine[w];
+    ups[to][tid] = up;
+    if (up >= 0) goes_on[round + 1] = 1;
   }
-  if (tid < sq.n)
-#pragma unroll
-    for (int w = 0; w < kNodeWords; ++w)
-      if (w < a.words) a.tree[(int64_t)(sq.start + tid) * a.words + w] = mine[w];
+  if (round == kRounds - 1) __syncthreads();
+  uint64_t* out = a.tree + (int64_t)sq.start * a.words;
+  for (int i = tid; i < sq.n * a.words; i += kNodes) {
+    const int row = i / a.words, w = i - row * a.words;
+    out[i] = w < words ? bits[round & 1][w][row] : 0;
+  }
 }
 
 // A thread moves one 16-byte piece of a slot, of one layer, cache and head,
