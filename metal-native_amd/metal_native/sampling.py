@@ -65,10 +65,12 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top_k=0, t
             x = x.contiguous()
         else:
             try:
-                number = float(x)
-                if what == "top_k" and number != int(x):
-                    _invalid(f"{op}: top_k must be a whole number, got {x}")
-                x = int(x) if what == "top_k" else number
+                if what == "top_k":
+                    if int(x) != x:
+                        _invalid(f"{op}: top_k must be a whole number, got {x}")
+                    x = min(max(int(x), 0), 2**31 - 1)   # past any vocabulary
+                else:
+                    x = float(x)
             except (TypeError, ValueError, OverflowError):
                 _invalid(f"{op}: {what} must be a number or a tensor, got {x!r}")
         given.append(x)

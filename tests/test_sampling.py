@@ -236,6 +236,15 @@ def test_no_rows_subclasses_and_gradients(gpu):
         log.sum().backward()
 
 
+@pytest.mark.gpu
+def test_top_k_of_any_size(gpu):
+    from metal_native import sampling
+
+    x, u = logits(gpu, 3, 500, "fp16", 4)
+    for k, same in ((10**30, 0), (2**63, 0), (2**31, 0), (-(10**30), 0), (True, 1)):
+        assert torch.equal(sampling.sample(x, u, top_k=k), sampling.sample(x, u, top_k=same)), k
+
+
 def arguments(dev):
     return dict(logits=torch.zeros(3, 50, device=dev), u=torch.zeros(3, device=dev), temperature=torch.ones(3, device=dev),
                 top_k=torch.zeros(3, dtype=torch.int32, device=dev), top_p=torch.ones(3, device=dev), min_p=torch.zeros(3, device=dev))
