@@ -272,11 +272,8 @@ class PagedServer:
                 self.seen[s] += len(line)
             return out
         logits = self._forward(flat, pos, rows, table, lens, cu, max(new), ends.to(dev) - 1)
-        if self.settings["temperature"] == 0:
-            out = dict(zip(ids, logits.float().argmax(-1).tolist()))
-        else:
-            out = dict(zip(ids, self._draws(logits, ids, [self.seen[s] + n - 1 for s, n in zip(ids, new)]).tolist()))
-            self._drawn(out)
+        out = dict(zip(ids, self._draws(logits, ids, [self.seen[s] + n - 1 for s, n in zip(ids, new)]).tolist()))
+        self._drawn(out)
         for s, n in zip(ids, new):
             self.lens[s] += n
             self.seen[s] += n

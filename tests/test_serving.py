@@ -278,3 +278,29 @@ def test_logits_with_nothing_to_draw(gpu, monkeypatch):
         assert (dict(server.last), list(server.lens), list(server.seen)) == kept
     monkeypatch.setattr(PagedServer, "_forward", real)
     assert server.step().keys() == kept[0].keys()
+
+
+def test_greedy_steps_pass_over_nan(gpu, monkeypatch):
+    """A logit that is no number is never the largest, with drafts or without; a row of nothing else is refused."""
+    from metal_native.serving import PagedServer
+
+    m = model_of(gpu)
+    exact(monkeypatch)
+    even = PagedServer._forward
+
+    def forward(self, *a):
+        x = even(self, *a)
+        x[:, 5] = float("nan")
+        return x
+
+    monkeypatch.setattr(PagedServer, "_forward", forward)
+    plain, _ = lines_of(PagedServer(m, 60, 4, chunk=32), PROMPTS, 40, False)
+    assert not any(5 in line for line in plain)
+    assert lines_of(PagedServer(m, 60, 4, chunk=32, draft=6), PROMPTS, 40, True)[0] == plain
+    server = PagedServer(m, 60, 4, chunk=32)
+    server.start(PROMPTS)
+    kept = dict(server.last), list(server.lens), list(server.seen)
+    monkeypatch.setattr(PagedServer, "_forward", lambda self, *a: torch.full_like(even(self, *a), float("nan")))
+    with pytest.raises(RuntimeError, match="nothing above"):
+        server.step()
+    assert (dict(server.last), list(server.lens), list(server.seen)) == kept
