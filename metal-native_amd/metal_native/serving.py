@@ -144,6 +144,7 @@ class PagedServer:
                 part = {s: p[at:at + self.chunk] for s, p in zip(ids, prompts) if len(p) > at}
                 out.update(self._run(part))
                 at += self.chunk
+            self._drawn(out)
         except Exception:
             for s in ids:
                 self.finish(s)
@@ -273,7 +274,7 @@ class PagedServer:
             return out
         logits = self._forward(flat, pos, rows, table, lens, cu, max(new), ends.to(dev) - 1)
         out = dict(zip(ids, self._draws(logits, ids, [self.seen[s] + n - 1 for s, n in zip(ids, new)]).tolist()))
-        self._drawn(out)
+        self._drawn({s: t for s, t in out.items() if s in self.last})   # of a prompt only what its last chunk gives counts
         for s, n in zip(ids, new):
             self.lens[s] += n
             self.seen[s] += n

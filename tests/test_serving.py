@@ -304,3 +304,31 @@ def test_greedy_steps_pass_over_nan(gpu, monkeypatch):
     with pytest.raises(RuntimeError, match="nothing above"):
         server.step()
     assert (dict(server.last), list(server.lens), list(server.seen)) == kept
+
+
+@pytest.mark.parametrize("temperature", [0.0, 1.0])
+def test_logits_inside_a_prompt_draw_nothing(gpu, monkeypatch, temperature):
+    """What stands behind a chunk that is not a prompt's last may hold nothing above -inf."""
+    from metal_native.serving import PagedServer
+
+    m = model_of(gpu)
+    real, calls = PagedServer._forward, []
+
+    def forward(self, *a):
+        x = real(self, *a)
+        calls.append(len(calls))
+        return torch.full_like(x, -float("inf")) if calls[-1] < bad else x
+
+    monkeypatch.setattr(PagedServer, "_forward", forward)
+    bad = 0
+    want = PagedServer(m, 60, 4, chunk=16, temperature=temperature).start([PROMPTS[0], PROMPTS[2]])
+    calls.clear()
+    bad = 2   # of three chunks and of five
+    server = PagedServer(m, 60, 4, chunk=16, temperature=temperature)
+    assert server.start([PROMPTS[0], PROMPTS[2]]) == want
+    calls.clear()
+    bad = 3
+    server = PagedServer(m, 60, 4, chunk=16, temperature=temperature)
+    with pytest.raises(RuntimeError, match="nothing above"):
+        server.start([PROMPTS[0], PROMPTS[2]])
+    assert not server.last and sorted(server.free) == list(range(60)) and server.lens == [0] * 4
