@@ -357,7 +357,7 @@ MQ_API int mq_paged_tree_attention(const mq_paged_cache* cache, const mq_paged_m
  * length, new_lens [batch] lens less the nodes that are not on it.  In every one
  * of `layers` caches (strides k_layer, v_layer from the first) the path's slots
  * move to the chunk's first ones.  The chunk's pages may be in no other sequence's
- * table; keys and values may not be the same memory. */
+ * table; keys and values may share no memory. */
 MQ_API int mq_paged_accept(const mq_paged_cache* cache, int64_t layers, int64_t k_layer, int64_t v_layer,
                            const int64_t* drawn, const int64_t* drafted, const int32_t* parents, const int32_t* cu_q,
                            int64_t rows, int64_t steps, int32_t* path, int64_t* tokens, int32_t* count,

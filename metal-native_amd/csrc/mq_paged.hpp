@@ -107,6 +107,48 @@ MQ_HD uint64_t paged_tree_bits(const uint64_t* row, int words, int64_t d) {
   return lo | hi;
 }
 
+// Whether some i, lo <= i <= hi for each of n terms, gives sum of step * i = rest:
+// terms by falling steps (all positive), so that few i are left for each.  True too
+// where `tries` does not settle it.
+struct PagedTerm {
+  int64_t step, lo, hi;
+};
+inline bool paged_reaches(const PagedTerm* t, int n, __int128 rest, int* tries) {
+  if (n == 0) return rest == 0;
+  __int128 lo = 0, hi = 0;   // what the other terms add
+  for (int k = 1; k < n; ++k) {
+    lo += (__int128)t[k].step * t[k].lo;
+    hi += (__int128)t[k].step * t[k].hi;
+  }
+  const __int128 a = rest - hi, b = rest - lo, s = t[0].step;
+  __int128 i = a >= 0 ? (a + s - 1) / s : -(-a / s), end = b >= 0 ? b / s : -((-b + s - 1) / s);
+  if (i < t[0].lo) i = t[0].lo;
+  if (end > t[0].hi) end = t[0].hi;
+  for (; i <= end; ++i) {
+    if (--*tries < 0 || paged_reaches(t + 1, n - 1, rest - s * i, tries)) return true;
+  }
+  return false;
+}
+// Whether two arrays of up to 8 dimensions of these sizes, with strides x and y, the
+// second's first element `apart` elements behind the first's, may have one in common.
+inline bool paged_share(int dims, const int64_t* size, const int64_t* x, const int64_t* y, int64_t apart) {
+  PagedTerm t[16];
+  int n = 0;
+  auto add = [&](int64_t step, int64_t lo, int64_t hi) {
+    if (step == 0 || lo == hi) return;
+    int at = n++;
+    for (; at > 0 && t[at - 1].step < step; --at) t[at] = t[at - 1];
+    t[at] = {step, lo, hi};
+  };
+  for (int d = 0; d < dims; ++d) {
+    const int64_t most = size[d] - 1;
+    if (x[d] == y[d]) add(x[d], -most, most);
+    else add(x[d], 0, most), add(y[d], -most, 0);
+  }
+  int tries = 4096;
+  return paged_reaches(t, n, apart, &tries);
+}
+
 // Page that holds slot j, or -1 where there is none.
 MQ_HD int paged_page(const int32_t* row, int j, int len, int shift, int pages) {
   if (j < 0 || j >= len) return -1;

@@ -289,6 +289,10 @@ MQ_API int mq_paged_accept(const mq_paged_cache* c, int64_t layers, int64_t k_la
   if (rows < 0 || rows > INT_MAX - 1024 || steps < 1 || steps > INT_MAX - 64) return refuse(op, "rows must not be negative, steps positive, both below 2^31");
   if (!cu_q && rows != c->batch) return refuse(op, "without cu_q there must be one row per sequence");
   if (!path || !tokens || !count || !new_lens || (rows > 0 && (!drawn || !drafted || !parents))) return refuse(op, "null pointer argument");
+  const int64_t size[] = {layers, c->pages, c->kv_heads, c->page_size, c->head_dim};
+  const int64_t at_k[] = {k_layer, c->k_page, c->k_head, c->k_slot, 1}, at_v[] = {v_layer, c->v_page, c->v_head, c->v_slot, 1};
+  if (mq::paged_share(5, size, at_k, at_v, (int64_t)((intptr_t)c->v - (intptr_t)c->k) / 2))
+    return refuse(op, "keys and values must not share memory: a slot would be moved twice");
   mq::AcceptArgs a{};
   fill_cache(a, c);
   a.k_layer = k_layer;

@@ -416,7 +416,7 @@ def accept(k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor, le
     the tokens drawn behind them, int64 ``[batch, steps]``, both -1 past the path;
     its length, int32 ``[batch]``; the lengths without the nodes that are not on it.
     The last of the tokens has no slot yet: it is the next tree's root.  The pages
-    of a chunk may be in no other sequence's table.
+    of a chunk may be in no other sequence's table, and the caches may share no memory.
     """
     op = "paged.accept"
     if type(drawn) is torch.Tensor and drawn.is_cuda:

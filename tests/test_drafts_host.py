@@ -208,3 +208,82 @@ def test_tree_plans():
     assert plan(4096, 28, 4, 128, 1, 32768) == plan(4096, 28, 4, 128, 1, 32768, op="attention")
     n = ctypes.c_int32()
     assert _lib.load().mq_paged_tree_attention_plan(None, None, 1, 1, ctypes.byref(n), ctypes.byref(n)) == 4
+
+
+# ---- caches that share memory ----
+@pytest.mark.skipif(shutil.which("g++") is None, reason="needs g++")
+def test_whether_arrays_share_an_element(tmp_path):
+    """Against every element of both, for strides that nest, interleave, differ and overlap."""
+    src = tmp_path / "share.cpp"
+    src.write_text('''
+#include <cstdio>
+#include <random>
+#include <set>
+#include "mq_paged.hpp"
+int main() {
+  std::mt19937 rng(1);
+  long bad = 0, shared = 0, apart_ones = 0;
+  for (int turn = 0; turn < 60000; ++turn) {
+    const int dims = 1 + rng() % 4;
+    int64_t size[4], x[4], y[4];
+    for (int64_t* s : {x, y}) {   // nested, in an order of its own, with gaps
+      int order[4] = {0, 1, 2, 3};
+      if (s == x) for (int d = 0; d < dims; ++d) size[d] = 1 + rng() % 4;
+      if (s == x || turn % 3) for (int d = dims - 1; d > 0; --d) std::swap(order[d], order[rng() % (d + 1)]);
+      int64_t step = 1;
+      for (int d = 0; d < dims; ++d) {
+        s[order[d]] = step;
+        step *= size[order[d]] * (rng() % 3 ? 1 : 1 + rng() % 3);
+      }
+    }
+    if (turn % 2) for (int d = 0; d < dims; ++d) y[d] = x[d];
+    const int64_t apart = (int64_t)(rng() % 81) - 40;
+    auto all = [&](const int64_t* s, int64_t from) {
+      std::set<int64_t> r{from};
+      for (int d = 0; d < dims; ++d) {
+        std::set<int64_t> next;
+        for (int64_t v : r) for (int64_t i = 0; i < size[d]; ++i) next.insert(v + i * s[d]);
+        r = next;
+      }
+      return r;
+    };
+    bool want = false;
+    const auto a = all(x, 0), b = all(y, apart);
+    for (int64_t v : b) want |= a.count(v) != 0;
+    (want ? shared : apart_ones)++;
+    bad += mq::paged_share(dims, size, x, y, apart) != want;
+  }
+  // the largest there are: no overflow, and an end
+  const int64_t huge[5] = {INT64_C(1) << 30, INT64_C(1) << 31, 65535, 65536, 128}, s[5] = {INT64_C(1) << 61, INT64_C(1) << 30, 8, 128, 1}, z[5] = {8, 8, 8, 136, 1};
+  for (int64_t apart : {INT64_C(0), INT64_MAX / 2, INT64_MIN / 2, INT64_C(8)}) mq::paged_share(5, huge, s, z, apart), mq::paged_share(5, huge, s, s, apart);
+  std::printf("bad %ld of %ld and %ld\\n", bad, shared, apart_ones);
+  return shared < 10000 || apart_ones < 10000;
+}
+''')
+    exe = tmp_path / "share"
+    subprocess.run(["g++", "-O1", "-std=c++17", "-fsanitize=undefined,address", "-fno-sanitize-recover=all",
+                    f"-I{os.path.join(ROOT, 'metal-native_amd', 'csrc')}", str(src), "-o", str(exe)], check=True, capture_output=True, timeout=300)
+    out = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300, env={k: v for k, v in os.environ.items() if k != "LD_PRELOAD"})
+    assert out.returncode == 0 and "bad 0 " in out.stdout, out.stdout + out.stderr
+
+
+# a page is 2 heads of 16 slots of 64 halves: 4096 bytes; 6 pages a layer, one layer after the other
+@pytest.mark.parametrize("how", [dict(v=P), dict(v=P + 4096), dict(v=P + 5 * 4096), dict(v=P - 16), dict(v=P + 3 * 24576, layers=4), dict(v=P + 24576, layers=2),
+                                 dict(v=P + 64, k_slot=128, v_slot=128, k_head=2048, v_head=2048, k_page=4096, v_page=4096)])
+def test_keys_and_values_that_share_memory_are_refused(how):
+    layers = how.get("layers", 1)
+    rc, text = c_call("accept", cache={n: x for n, x in how.items() if n != "layers"}, layers=layers, k_layer=12288, v_layer=12288)
+    assert rc == 4 and text == "paged.accept: keys and values must not share memory: a slot would be moved twice", (rc, text)
+
+
+@pytest.mark.gpu
+def test_layers_shifted_by_one_are_refused(gpu):
+    from metal_native import MetalNativeError, paged
+
+    kw = arguments(gpu)["accept"]
+    both = kw["k_cache"].new_zeros(4, *kw["k_cache"].shape)
+    wide = kw["k_cache"].new_zeros(2, 9, *kw["k_cache"].shape[1:])
+    for k, v in ((both[:-1], both[1:]), (both[1:], both[:-1]), (wide[:, :6], wide[:, 3:])):
+        with pytest.raises(MetalNativeError, match="share memory"):
+            paged.accept(**{**kw, "k_cache": k, "v_cache": v})
+    paged.accept(**{**kw, "k_cache": both[::2], "v_cache": both[1::2]})   # layers in turn
