@@ -47,12 +47,12 @@ struct Call {
       : device(d), modes(c10::DispatchKeySet({c10::DispatchKey::Python, c10::DispatchKey::PythonTLSSnapshot})) {}
 };
 
-// whether autograd follows one of them (null: not given); the Python side then marks
-// the outputs as having no gradient
+// whether autograd follows one of them (null: not given), which has a tangent of forward
+// mode or requires a gradient; the Python side then refuses, or marks the outputs
 inline bool tracked(std::initializer_list<const at::Tensor*> ts) {
-  if (!c10::GradMode::is_enabled()) return false;
+  const bool backward = c10::GradMode::is_enabled();
   for (const at::Tensor* t : ts)
-    if (t && t->requires_grad()) return true;
+    if (t && ((backward && t->requires_grad()) || t->_fw_grad(0).defined())) return true;
   return false;
 }
 

@@ -33,14 +33,15 @@ width are cut to it, positions past the rotary tables to their last row.
 
 Every call launches HIP kernels of libmetal_native_amd.so on the current stream
 and returns without synchronising; workspaces come from torch's allocator on
-that stream.  None has a backward pass: where autograd follows an input, going
-back through the outputs raises, and a cache that is written may not require a
-gradient.
+that stream.  None has a derivative: where autograd follows an input, going
+back through the outputs raises, a cache that is written may not require a
+gradient, and tangents of forward mode are refused.
 """
 
 from __future__ import annotations
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from .ops import _check, _invalid, _mq_torch, _raw_stream, _require_cuda
 
@@ -112,8 +113,16 @@ class _NoGradient(torch.autograd.Function):
         _invalid(f"{ctx.op}: has no backward pass (call it under torch.no_grad(), or detach what goes in)")
 
 
+def _dual(t):
+    """Whether a tensor carries a tangent of forward-mode derivatives."""
+    return isinstance(t, torch.Tensor) and t.is_floating_point() and unpack_dual(t).tangent is not None
+
+
 def _tracked(op, read, written=()):
-    """The inputs that autograd follows; raises where one of them is written."""
+    """The inputs that autograd follows; raises where one of them is written, or
+    carries a tangent, which the outputs would not have."""
+    if any(_dual(t) for t in (*read, *written)):
+        _invalid(f"{op}: has no derivative, and a tangent would be lost (give the tensors of forward_ad.unpack_dual)")
     if not torch.is_grad_enabled():
         return []
     for t in written:

@@ -3,16 +3,18 @@
 The call launches HIP kernels of libmetal_native_amd.so on the current stream
 and returns without synchronising; workspaces come from torch's allocator on
 that stream, and no tensor is looked at on the host, so a step of a decode loop
-is capturable in a graph.  There is no backward pass: where autograd follows an
-input, going back through the outputs raises.
+is capturable in a graph.  There is no derivative: where autograd follows an
+input, going back through the outputs raises, and log shares refuse tangents of
+forward mode.
 """
 
 from __future__ import annotations
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from .ops import _invalid, _mq_torch, _raw_stream, _require_cuda
-from .paged import _finish, _plain, _tracked
+from .paged import _dual, _finish, _plain, _tracked
 
 __all__ = ["sample"]
 
@@ -74,6 +76,8 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top_k=0, t
             except (TypeError, ValueError, OverflowError):
                 _invalid(f"{op}: {what} must be a number or a tensor, got {x!r}")
         given.append(x)
+    if not return_logprob:   # a token has no tangent to lose
+        logits, u, *given = (unpack_dual(x).primal if _dual(x) else x for x in (logits, u, *given))
     tracked = _tracked(op, (logits, u, *given))
     with torch.no_grad(), torch.cuda.device(logits.device):
         for copied in (False, True):   # as it is, then laid out anew

@@ -287,3 +287,45 @@ def test_layers_shifted_by_one_are_refused(gpu):
         with pytest.raises(MetalNativeError, match="share memory"):
             paged.accept(**{**kw, "k_cache": k, "v_cache": v})
     paged.accept(**{**kw, "k_cache": both[::2], "v_cache": both[1::2]})   # layers in turn
+
+
+# ---- tangents of forward mode ----
+def every(dev):
+    return {**paged_arguments(dev), **arguments(dev)}
+
+
+def with_tangent(kw, name):
+    from torch.autograd import forward_ad
+
+    return {**kw, name: forward_ad.make_dual(kw[name], torch.ones_like(kw[name]))}
+
+
+FLOATS = [(op, name) for op, kw in every(torch.device("cpu")).items() for name, x in kw.items()
+          if isinstance(x, torch.Tensor) and x.is_floating_point()]
+
+
+@pytest.mark.parametrize("op,name", FLOATS)
+@pytest.mark.parametrize("grad", [True, False])
+def test_a_tangent_is_refused(op, name, grad, stand_in):
+    from torch.autograd import forward_ad
+
+    from metal_native import MetalNativeError, paged
+
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        with pytest.raises(MetalNativeError, match=f"paged.{op}: .*tangent"):
+            getattr(paged, op)(**with_tangent(every(torch.device("cpu"))[op], name))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op,name", FLOATS)
+def test_a_tangent_is_not_lost(gpu, op, name):
+    from torch.autograd import forward_ad
+
+    from metal_native import MetalNativeError, paged
+
+    kw = every(gpu)[op]
+    for grad in (True, False):
+        with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+            with pytest.raises(MetalNativeError, match=f"paged.{op}: .*tangent"):
+                getattr(paged, op)(**with_tangent(kw, name))
+    getattr(paged, op)(**kw)

@@ -245,6 +245,26 @@ def test_top_k_of_any_size(gpu):
         assert torch.equal(sampling.sample(x, u, top_k=k), sampling.sample(x, u, top_k=same)), k
 
 
+@pytest.mark.gpu
+def test_tangents(gpu):
+    """Lost by a log share, so refused; a token has none."""
+    from torch.autograd import forward_ad
+
+    from metal_native import MetalNativeError, sampling
+
+    kw = dict(arguments(gpu), logits=logits(gpu, 3, 50, "fp32", 6)[0])
+    want = sampling.sample(**kw)
+    for name, x in kw.items():
+        if x.is_floating_point():
+            for grad in (True, False):
+                with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+                    dual = {**kw, name: forward_ad.make_dual(x, torch.ones_like(x))}
+                    with pytest.raises(MetalNativeError, match="tangent"):
+                        sampling.sample(**dual, return_logprob=True)
+                    got = sampling.sample(**dual)
+                    assert torch.equal(got, want) and not got.requires_grad
+
+
 def arguments(dev):
     return dict(logits=torch.zeros(3, 50, device=dev), u=torch.zeros(3, device=dev), temperature=torch.ones(3, device=dev),
                 top_k=torch.zeros(3, dtype=torch.int32, device=dev), top_p=torch.ones(3, device=dev), min_p=torch.zeros(3, device=dev))
