@@ -1327,10 +1327,11 @@ Plan plan_of(const SampleArgs& a, int num_cus) {
   pl.places = kListRow / pl.parts;
   pl.few = std::min(kFewMost, 32 * pl.subs);
   const bool greedy = !a.temperatures && !(a.temperature > 0.f);
-  const bool cuts = a.top_ks || (a.top_k > pl.few && a.top_k < a.vocab);                       // by number, with a grid
-  pl.gather = !greedy && (a.top_ks || a.top_k <= 0 || a.top_k > pl.few);
+  const int k = a.top_k > 0 && a.top_k < a.vocab ? a.top_k : a.vocab;                          // as settings_of takes it
+  const bool cuts = a.top_ks || (k > pl.few && k < a.vocab);                                   // by number, with a grid
+  pl.gather = !greedy && (a.top_ks || k > pl.few);
   pl.grid = (!greedy && cuts) || (pl.gather && (a.top_ps || a.top_p < 1.f));
-  const bool some = !greedy && (a.top_ks || (a.top_k > 1 && a.top_k <= pl.few));               // kFew
+  const bool some = !greedy && (a.top_ks || (k > 1 && k <= pl.few));                           // kFew
   size_t at = 0;
   auto take = [&](size_t n) {
     const size_t was = at;

@@ -343,3 +343,37 @@ def test_c_entry_refuses():
     assert call(rows=0, logits=None)[0] == 0
     assert L.mq_sample_workspace_size(3, 0, 0, ctypes.byref(how)) == -1
     assert L.mq_sample_workspace_size(3, 100, 0, None) == -1
+
+
+def test_workspace_follows_what_top_k_leaves():
+    """Small vocabularies, whose rows go by the lanes' largest logits whether top_k says so or leaves all: the workspace
+    has a place for these."""
+    import ctypes
+
+    from metal_native import _lib
+
+    class Sampling(ctypes.Structure):
+        _fields_ = [("temperatures", ctypes.c_void_p), ("top_ps", ctypes.c_void_p), ("min_ps", ctypes.c_void_p), ("top_ks", ctypes.c_void_p),
+                    ("temperature", ctypes.c_float), ("top_p", ctypes.c_float), ("min_p", ctypes.c_float), ("top_k", ctypes.c_int32)]
+
+    def size(top_k, vocab, top_p=1.0):
+        return _lib.load().mq_sample_workspace_size(7, vocab, 0, ctypes.byref(Sampling(temperature=1.0, top_p=top_p, top_k=top_k)))
+
+    for vocab in (2, 20, 32):
+        assert size(vocab, vocab) >= 3 * 256 + 7 * 64 * 4   # of each part, of each row, the subs' sums; 64 lanes of each row
+        for top_k in (0, -5, vocab + 1, 1000, 2**31 - 1):
+            for top_p in (1.0, 0.9):
+                assert size(top_k, vocab, top_p) == size(vocab, vocab, top_p), (vocab, top_k, top_p)
+
+
+def test_the_largest_vocabulary_of_the_c_entry():
+    """One more than 2^22 is refused: shared memory and the number of parts go by it."""
+    import ctypes
+
+    from metal_native import _lib
+
+    how = (ctypes.c_char * 64)()
+    for vocab, refused in ((2**22, False), (2**22 + 1, True)):
+        size = _lib.load().mq_sample_workspace_size(1, vocab, 0, how)
+        assert (size == -1) == refused and (refused or size > 0)
+    assert _lib.load().mq_sample(4096, 2**22 + 1, 1, 2**22 + 1, 0, 4096, how, 4096, None, None, 0, None) == 4
