@@ -1040,13 +1040,22 @@ int64_t most_slots(const PagedArgs& a, int rows, int tk) {   // that a row block
 // average chunk decides, so a batch of single tokens and one chunk runs in one kind
 // of block.
 constexpr int64_t kWork = 4 << 20, kWorkExtra = 24 << 20;
-// A few trees of fewer rows, behind long caches, too: in blocks of 32 rows each block
-// reads all of the cache again, and one block of 256 for the whole tree, its slots in
+// A few trees of fewer rows in tables of many slots, too: in blocks of 32 rows each
+// block reads all of the cache again, and one block of 256 for the whole tree, its slots in
 // parts, is faster though most of its rows are empty (us, blocks of 32 and of 256): 4
 // trees of 5 nodes, 28 heads over 4, behind 32768 slots 88 and 70, 4 of 30, 32 over 8,
 // 233 and 151, 2 of 15, 8 over 1, behind 65000 56 and 44.  Of many trees the caches'
 // lengths differ, which parts as many for all do not suit: 8 of 14 behind 1600 to
 // 32768, 32 over 8, 98 and 191, 20 of 13, 28 over 4, behind 800 to 16384 107 and 136.
+// Only the table's width is known here, not how long the sequences are.  In one of 32768
+// slots, one tree of 16, 28 over 4: behind 528 slots 16 and 26, 2000 19 and 28, 4000
+// 24 and 27, 8000 30 and 28, 16000 35 and 30, 32000 56 and 41; of several trees the
+// larger blocks lose nothing where they are short (8 of 9 behind 708, 28 over 4, 26 and 25,
+// 4 of 9, 32 over 8, behind 2000 31 and 28, 16000 96 and 69).  So a caller that knows
+// the lengths gives no more columns than they need: 528 slots in as many 14 either way.
+// With a cap or a bias, whose tree build of 256 rows keeps 98 registers in memory (in
+// order: 8), more is lost than won (one of 16, 28 over 4, behind 600 18 and 40, 32000
+// 66 and 67; 4 of 30, 32 over 8, behind 600 26 and 40, 8000 89 and 80, 32000 292 and 241).
 constexpr int64_t kTreeSlots = 8192, kTreeUnits = 32;
 bool many_rows(const PagedArgs& a) {
   const int64_t slots = a.window > 0 ? std::min<int64_t>(a.cap, (int64_t)a.window + kRowsP) : a.cap;

@@ -382,7 +382,9 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     With ``window``, ``slopes`` and ``prefix_lens`` a row with n bits stands n - 1
     slots past the chunk's first; its distance to a slot of the chunk is the number
     of its bits above that slot's; a prefix ends where the chunk begins.
-    Everything else is as in ``attention``.
+    Everything else is as in ``attention``.  Kernels are chosen by the width of
+    ``table``: a short tree in a much wider one takes up to twice as long, so where
+    the longest sequence is known, give its columns alone (``table[:, :pages]``).
     """
     op = "paged.tree_attention"
     if scale is None:

@@ -260,6 +260,8 @@ class PagedServer:
         cu = None if single else torch.cat([ends.new_zeros(1), ends]).to(dev, torch.int32)
         flat = torch.tensor([t for part in tokens.values() for t in part], device=dev)
         if trees is not None:
+            # launches are sized by the table's width, not by lengths that only the device knows: no more columns than are used
+            table = table[:, :max(-(-(self.lens[s] + n) // ps) for s, n in zip(ids, new))]
             parents = torch.tensor([p for t in trees.values() for p in t[1]], dtype=torch.int32, device=dev)
             tree = paged.ancestors(parents, cu, max(new))
             logits = self._forward(flat, pos, rows, table, lens, cu, max(new), None, tree)

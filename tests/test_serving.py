@@ -332,3 +332,23 @@ def test_logits_inside_a_prompt_draw_nothing(gpu, monkeypatch, temperature):
     with pytest.raises(RuntimeError, match="nothing above"):
         server.start([PROMPTS[0], PROMPTS[2]])
     assert not server.last and sorted(server.free) == list(range(60)) and server.lens == [0] * 4
+
+
+def test_drafted_steps_are_sized_by_what_the_cache_holds(gpu, monkeypatch):
+    """The operators see the pages in use, not the widest table there can be: launches go by its width."""
+    from metal_native import paged
+    from metal_native.serving import PagedServer
+
+    m = model_of(gpu)
+    widths = []
+    real = paged.tree_attention
+    monkeypatch.setattr(paged, "tree_attention", lambda q, k, v, table, *a, **how: widths.append(table.shape[1]) or real(q, k, v, table, *a, **how))
+    server = PagedServer(m, 60, 4, draft=6)
+    server.start([[1, 2, 3] * 3, [4] * 20])
+    while server.seen[1] < 120:
+        widths.clear()
+        server.step_drafted()
+        assert len(set(widths)) == 1 and -(-max(server.seen) // 16) <= widths[0] <= max(len(h) for h in server.held)
+    server.finish(1)
+    server.step_drafted()
+    assert -(-server.seen[0] // 16) <= widths[-1] <= len(server.held[0])
