@@ -439,3 +439,83 @@ def test_two_streams_at_once(gpu):
     same = lambda a, b: torch.equal(a.nan_to_num(), b.nan_to_num()) if a.is_floating_point() else torch.equal(a, b)  # noqa: E731
     for i, g in enumerate(got):
         assert all(same(a, b) for a, b in zip(g, want[i % 2])), i
+
+
+# ---- offsets of any kind: where results and memory end ----
+WILD = [[-5, 3, 10**6, 10**6], [7, 3, 1, 12], [2**31 - 1, -(2**31), 5, 6], [3, 9, 9, -(2**31)], [0, 5, 2**31 - 1, 4], [-4, 12, 12, 2**31 - 1], [9, 2, 0, 11]]
+
+
+def c_entry(name, *args):
+    from metal_native import _lib
+
+    L = _lib.load()
+    args = [a.data_ptr() if isinstance(a, torch.Tensor) else a for a in args]
+    rc = getattr(L, name)(*args, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0, L.mq_last_error().decode()
+
+
+@pytest.mark.parametrize("wild", WILD)
+@pytest.mark.parametrize("words", [1, 9])
+def test_ancestors_of_wild_offsets(gpu, wild, words):
+    """A row has the bits of a tree that claims it, or none where rows of no tree begin; each row is written, and nothing
+    around them."""
+    rows = 12
+    flat = torch.tensor([9, 9, -1, 0, 7, 1, -(2**31), 2**31 - 1, 3, 4, 5, 5], dtype=torch.int32, device=gpu)
+    cu = torch.tensor(wild, dtype=torch.int32, device=gpu)
+    cut = lambda x: max(0, min(x, rows))  # noqa: E731
+    may = [set() for _ in range(rows)]
+    for r in range(rows):
+        if r < cut(wild[0]) or r >= cut(wild[-1]):
+            may[r].add((0,) * words)
+    for a, b in zip(wild, wild[1:]):
+        a, b = cut(a), cut(b)
+        for r, line in enumerate(ref.pack(ref.closure(flat[a:b].tolist()), words).tolist() if a < b else [], a):
+            may[r].add(tuple(line))
+    assert all(may)
+    out = torch.full((rows + 8, words), -7, dtype=torch.int64, device=gpu)
+    c_entry("mq_paged_ancestors", flat, cu, 3, rows, words, out[4:])
+    got = out.cpu()
+    assert bool((got[:4] == -7).all()) and bool((got[-4:] == -7).all())
+    assert all(tuple(x) in m for x, m in zip(got[4:-4].tolist(), may)), got[4:-4, 0]
+
+
+@pytest.mark.parametrize("wild", WILD)
+def test_accept_of_wild_offsets(gpu, wild):
+    """Slots move inside the pages of the tables alone, paths and tokens are a tree's, and nothing around the outputs is
+    written."""
+    import ctypes
+
+    from test_paged_host import Cache
+
+    steps, b, rows, ps, D, KVH, pages = 5, 3, 12, 16, 64, 2, 7
+    drawn, drafted = torch.ones(rows, dtype=torch.int64, device=gpu), torch.ones(rows, dtype=torch.int64, device=gpu)
+    parents = torch.tensor([-1, 0, 0, 1, 2, 2, 0, 5, 6, 2, 9, 1], dtype=torch.int32, device=gpu)
+    cu = torch.tensor(wild, dtype=torch.int32, device=gpu)
+    table = torch.tensor([[3, 4], [5, -1], [9, 6]], dtype=torch.int32, device=gpu)   # pages 3 to 6 of seven; 9 is none
+    lens = torch.tensor([20, 9, 32], dtype=torch.int32, device=gpu)
+    kv = torch.randn(2, pages + 2, KVH, ps, D, device=gpu).half()
+    before = kv.clone()
+    k, v = kv[0, 1:-1], kv[1, 1:-1]
+    path, count, new = (torch.full(n, -7, dtype=torch.int32, device=gpu) for n in ((b + 2, steps), (b + 2,), (b + 2,)))
+    tokens = torch.full((b + 2, steps), -7, dtype=torch.int64, device=gpu)
+    c = Cache(k=k.data_ptr(), v=v.data_ptr(), k_page=k.stride(0), k_head=k.stride(1), k_slot=k.stride(2), v_page=v.stride(0), v_head=v.stride(1),
+              v_slot=v.stride(2), pages=pages, kv_heads=KVH, page_size=ps, head_dim=D, dtype=0, table=table.data_ptr(), ld_table=2, width=2,
+              batch=b, lens=lens.data_ptr())
+    c_entry("mq_paged_accept", ctypes.byref(c), 1, 0, 0, drawn, drafted, parents, cu, rows, steps, path[1:], tokens[1:], count[1:], new[1:])
+    for out in (path, tokens, count, new):
+        assert bool((out[0] == -7).all()) and bool((out[-1] == -7).all())
+    cut = lambda x: max(0, min(x, rows))  # noqa: E731
+    want, at = before.clone(), [path[1:-1].tolist(), tokens[1:-1].tolist(), count[1:-1].tolist(), new[1:-1].tolist()]
+    for s, (a, e) in enumerate(zip(wild, wild[1:])):
+        a, e = cut(a), max(cut(a), cut(e))
+        n, row = e - a, table[s].tolist()
+        p, t = ref.accept([1] * n, [1] * n, parents[a:e].tolist(), steps)
+        assert at[0][s] == p + [-1] * (steps - len(p)) and at[1][s] == t + [-1] * (steps - len(p)) and at[2][s] == len(p)
+        off = int(lens[s]) - n
+        assert at[3][s] == max(0, off + len(p))
+        for i, node in enumerate(p):
+            x, y = off + node, off + i
+            ids = [row[z // ps] if z >= 0 else -1 for z in (x, y)]
+            if x != y and all(0 <= z < pages for z in ids):
+                want[:, 1 + ids[1], :, y % ps] = before[:, 1 + ids[0], :, x % ps]
+    assert torch.equal(kv, want)

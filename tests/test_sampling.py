@@ -265,6 +265,56 @@ def test_tangents(gpu):
                     assert torch.equal(got, want) and not got.requires_grad
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("V,top_k,unit", [(2, 0, -50), (32, 0, -50), (1000, 7, -50), (33, 0, -44), (1000, 600, -44), (2**18, 0, -44), (2**18 + 1, 0, -43),
+                                          (2**20 + 1, 0, -41), (2**22, 0, -40)])
+def test_the_smallest_weight_that_is_drawn(gpu, V, top_k, unit):
+    """Half of the unit that sums go by; u = 0 draws the first token that weighs one."""
+    from metal_native import sampling
+
+    x = torch.full((2, V), -math.inf, device=gpu)
+    x[:, 1] = 0.0
+    x[0, 0], x[1, 0] = (unit - 0.9) * math.log(2), (unit - 1.1) * math.log(2)
+    if top_k == 600:
+        x[:, 2:602] = -80.0
+    assert sampling.sample(x, torch.zeros(2, device=gpu), top_k=top_k).tolist() == [0, 1]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("first", [True, False])
+def test_a_cut_far_under_the_largest_weight(gpu, first):
+    """150 thousand weights around 2^-29 of the largest, of which top_p = 0.9999 leaves some two thirds: the cut lies under 2^-28.  Sums go by units
+    of 2^-44, half a unit off for each token, so the aim may lie that much beside a token's share; so may the cut."""
+    from metal_native import sampling
+
+    V, n = 152064, 48
+    g = torch.Generator(device=gpu)
+    g.manual_seed(11)
+    x = torch.randn(1, V, device=gpu, generator=g) * 0.3 - 20.0
+    top = 0 if first else V - 1
+    x[0, top] = 0.0
+    off = torch.linspace(2e-6, 1.9e-4, n, device=gpu)
+    u = 1 - off if first else off
+    got = sampling.sample(x.expand(n, -1), u, top_p=0.9999).tolist()
+    w = np.exp(x[0].double().cpu().numpy())
+    order = np.argsort(-w, kind="stable")
+    before = np.cumsum(w[order]) - w[order]
+    keep = order[:int((before < float(np.float32(0.9999)) * w.sum()).sum())]
+    err = V * 2.0**-45
+    assert 0.4 * V < len(keep) < 0.9 * V
+    least = w[keep].min()
+    assert least < 2.0**-28
+    kept = np.zeros(V)
+    kept[keep] = w[keep]
+    c = np.cumsum(kept)
+    for t, share in zip(got, u.double().tolist()):
+        aim, slack = share * c[-1], 2 * err + 2 * least
+        # a cut that lies `err` beside its place takes or leaves tokens of about the least weight that stays
+        assert w[t] >= least * 0.999
+        assert c[t] + slack > aim and c[t] - kept[t] - slack <= aim, (t, share)
+    assert len(set(got)) > n // 2
+
+
 def arguments(dev):
     return dict(logits=torch.zeros(3, 50, device=dev), u=torch.zeros(3, device=dev), temperature=torch.ones(3, device=dev),
                 top_k=torch.zeros(3, dtype=torch.int32, device=dev), top_p=torch.ones(3, device=dev), min_p=torch.zeros(3, device=dev))
