@@ -330,7 +330,9 @@ MQ_API int mq_paged_attention_plan(const mq_paged_cache* cache, const mq_paged_m
  *
  * tree [rows, words]: bit i of a row is set where node i of its sequence is the
  * row's own or one of its ancestors; nodes from 64 * words on have no bit.  Rows
- * that belong to no sequence get zeros.  At most 2^31 - 1024 rows. */
+ * that belong to no sequence get zeros.  At most 2^31 - 1024 rows.  Where cu_q
+ * decreases, a row that it gives to several sequences, or to one and to none, gets
+ * the bits of one of them. */
 MQ_API int mq_paged_ancestors(const int32_t* parents, const int32_t* cu_q, int64_t batch, int64_t rows, int64_t words,
                               int64_t* tree, void* stream);
 
@@ -396,8 +398,11 @@ MQ_API int mq_paged_evict(const mq_paged_cache* cache, const float* mass, int64_
  *
  * Each setting is one value, or where its pointer is not NULL an array of `rows`
  * in device memory.  logprob (or NULL): the log of the drawn token's share of the
- * sum.  A row without a logit above -inf gives token -1 and -inf.  Weights under
- * 2^-45 of the largest are never drawn.  Rows below 2^31, vocab 1 to 2^22. */
+ * sum.  A row without a logit above -inf gives token -1 and -inf.  Sums go by whole
+ * multiples of a unit, and weights under half of one are never drawn: 2^-44 of the
+ * largest weight up to 2^18 tokens, 2^-40 at 2^22; 2^-50 where top_k leaves at most
+ * 512 tokens (and 32 for each 1024 of the vocabulary).  Rows below 2^31, vocab 1 to
+ * 2^22. */
 enum mq_sample_dtype { MQ_SAMPLE_F16 = 0, MQ_SAMPLE_BF16 = 1, MQ_SAMPLE_F32 = 2 };
 typedef struct mq_sampling {
   const float *temperatures, *top_ps, *min_ps;

@@ -1,6 +1,7 @@
 // Trees of drafted tokens over a paged cache: ancestor bits, and the accepted
 // path with its slots moved together.  Both are bound by latency: 64 trees of 100 to 512
-// nodes are 1.2 MB, 48 paths of 28 layers 34 MB (4 us at the copy rate, the launch takes 8.3).
+// nodes are 1.2 MB, 48 paths of 28 layers and 4 heads of 128 move 5 MB (45 of 120 nodes
+// change their slot: 1 us at the copy rate, the call takes 8.3).
 #include "mq_paged_dev.hpp"
 
 namespace mq {
@@ -39,7 +40,9 @@ __global__ __launch_bounds__(256) void roots_kernel(AncestorsArgs a) {
 // node knows its ancestors up to some node, which knows its own up to another one, so
 // 9 rounds take every path to its root.  Rows are written from LDS, their words in a row
 // (64 trees of 100 to 512 nodes 6.9 us a call; each thread its own row 7.5; by walks
-// through memory 13.8).
+// through memory 13.8).  Larger trees, or rows of more words, go by these walks, a read
+// behind another one for every ancestor: one tree of 1000 nodes 116 us, a chain 304, of
+// 2500 643 and 1668.
 constexpr int kNodes = 512, kNodeWords = kNodes / 64, kRounds = 10;
 __global__ __launch_bounds__(kNodes) void ancestors_kernel(AncestorsArgs a) {
   __shared__ uint64_t bits[2][kNodeWords][kNodes];   // read and written in turn: one barrier a round

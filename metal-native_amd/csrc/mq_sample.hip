@@ -11,9 +11,13 @@
 // A token is a whole number: between two that border on each other in the running
 // sum nothing is half right, and 150 thousand borders lie in a row.  Weights are
 // therefore taken in 64 bits (to 4e-14 of themselves), and what is drawn goes by
-// their sums as whole multiples of 2^-44 (less for rows of more than 2^18): whole
-// numbers add up to the same in any order, and halves of a row that hold the same
-// logits to the same half.  Tokens of less than half of that are never drawn.
+// their sums as whole multiples of a unit: 2^-44, in rows of more than 2^18 tokens
+// coarser (2^-40 at 2^22), of a short top_k's list 2^-50.  Whole numbers add up to the
+// same in any order, and halves of a row that hold the same logits to the same half.
+// Tokens of less than half a unit are never drawn.  The sums by which top_p cuts are
+// floating ones of 64 bits (units where top_p alone cuts, and on the long way), grouped
+// by parts: how a row is dealt out can move a cut that lies within their rounding, and
+// nothing else.
 //
 // A row is dealt out to `parts` workgroups, a wave taking 1024 tokens at a time
 // (a sub).  What a row needs follows from its settings, which the GPU alone may
@@ -29,9 +33,12 @@
 //           the first top_k), the sub in which the running sum passes its aim, and the
 //           token in it.
 // The grid only says where to look: that a cut falls among the listed tokens is
-// checked with exact sums.  Where it does not, or a list is too short (masses of
-// equal logits at a cut), the row goes the long way: cuts found digit by digit by
-// one workgroup, pass after pass.
+// checked with the weights' sums.  Where it does not, or a list is too short, the row
+// goes the long way: cuts found digit by digit by one workgroup, pass after pass.  Such
+// rows are those with masses of equal logits at a cut (more of a part's than kListRow /
+// parts, or for a short top_k of more than kFewRoom lanes: a mask of the type's lowest
+// value that leaves fewer tokens than top_k, where one of -inf does not), those whose
+// cut by top_p lies under 2^-28 of the largest weight, and those of infinite logits.
 //
 // Bound by the issue of instructions: a row is read twice, and 63 million weights of 20
 // instructions in 64 bits take longer than their bytes.  152064 logits, us of a call: one
@@ -39,6 +46,9 @@
 // one another); 416 rows of fp16, top_p 0.95, 156 (scan 45, bounds 14, gather 80, pick 21;
 // read once they would take 25); 64 of bf16, settings of each, 69; 48 x 32003 in fp32,
 // min_p 0.05, 17.  The plain form (a sort, sums, searches) takes 410, 8700, 2000 and 620.
+// The long way, 1, 64 and 416 rows of fp16: 20 tokens over a mask of the lowest value,
+// top_k 50, 820, 827 and 1644 (masked by -inf 15, 18 and 42); all logits equal, top_p 0.5,
+// 988, 1107 and 2259; one token with nearly all of the weight, top_p 0.9999, 231, 265 and 555.
 #include "mq_device.hpp"
 #include "mq_sample.hpp"
 
@@ -144,9 +154,10 @@ __device__ __forceinline__ ull share_of(float u, ull n) {
 }
 
 // ---- the grid: cells of 1/128 of a factor of two in weight, the same ones for all
-// parts of a row; kFine of them under the largest logit's (28 factors of two, further
-// than a cut by top_p can lie: weights of 2^-28 add up to less than it leaves out),
-// the rest by eights, what lies under all of these in the last one ----
+// parts of a row; kFine of them under the largest logit's (28 factors of two: a cut by
+// top_p alone that lies further down is not found, as where 150 thousand weights of
+// 2^-28, 6e-4 of the largest, are more than top_p leaves out), the rest by eights, what
+// lies under all of these in the last one ----
 constexpr int kFine = 3584, kCoarse = 4608, kCells = kFine + kCoarse;
 constexpr float kEnd = 0x1p29f;   // the grid's ends
 __device__ __forceinline__ float grid_scale(double inv_t) {
@@ -331,7 +342,7 @@ struct Part {
   uint32_t cells;   // kGrid: the last cell that holds a token, and one
   double over_k, over_p;   // kGrid: weight from k_hi on (of all tokens where top_k does not cut), from p_hi on
 };
-struct Bounds {   // by gather, for pick: the cut of top_k falls among logits of k_lo <= x < k_hi, that of top_p between p_lo and p_hi
+struct Bounds {   // by bounds, for gather and pick: the cut of top_k falls among logits of k_lo <= x < k_hi, that of top_p between p_lo and p_hi
   float k_lo, k_hi, p_lo, p_hi;   // -inf where there is none
   int cut_k, cut_p;
   __device__ __forceinline__ float sure() const { return cut_p ? p_hi : k_hi; }   // tokens from here on stay, but for min_p
@@ -431,10 +442,9 @@ __device__ __forceinline__ float top_of(const Part* part, int parts) {
   return M;
 }
 
-// (Two workgroups to a CU, as pick: 416 rows 14 us where one takes 24.)
 // All parts' grids laid over each other: a part's cell, from its own largest logit
 // down, is one of the row's.  Then between which logits the cuts fall; a workgroup
-// for each row.
+// for each row, two to a CU (as pick: 416 rows 14 us where one takes 24).
 __global__ __launch_bounds__(kThreads, 8) void sample_bounds_kernel(SampleArgs p, Work ws) {
   __shared__ uint32_t numbers[kCells];
   __shared__ ull lds[2 * kWaves];
@@ -1115,7 +1125,7 @@ __device__ __forceinline__ bool pick(const SampleArgs& p, const Work& ws, const 
   };
   __syncthreads();
   // Whether the cut of top_k is among the listed, and how much weight stays by it:
-  // what must hold for the four waves to go on is the same for all threads.
+  // what must hold for the eight waves to go on is the same for all threads.
   const uint32_t* const key = sh.list.key;
   const uint32_t* const index = sh.list.idx;
   if (cut_k || cut_p) {

@@ -25,7 +25,7 @@ _MASK = 2**64 - 1
 
 
 def _mixed(x: int) -> int:
-    """64 bits in which every bit of ``x`` counts (xor-shifts and odd factors)."""
+    """64 bits in which every bit of ``x`` counts: the mixing function of SplitMix64 (Steele, Lea and Flood, 2014)."""
     x = (x ^ x >> 30) * 0xBF58476D1CE4E5B9 & _MASK
     x = (x ^ x >> 27) * 0x94D049BB133111EB & _MASK
     return x ^ x >> 31
